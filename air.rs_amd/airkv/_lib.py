@@ -112,6 +112,12 @@ SIGNATURES = {
     "air_paged_prefill": (_int, [_P, _P, _P, _i32, _i32, _P, _i32, _i32, _P, _P, _i32, _i32,
                                  ctypes.c_float, _P, _SZ, _P, _i32]),
     "air_paged_prefill_workspace_size": (_int, [_P, _i32, _i32, _i32, ctypes.POINTER(_SZ)]),
+    "air_paged_diff_decode_workspace_size": (_int, [_P, _i32, _i32, _i32, _i32, ctypes.POINTER(_SZ)]),
+    "air_paged_diff_decode": (_int, [_P, _P, _P, _i32, _i32, _P, _i32, _P, _P, _i32, _i32, ctypes.c_float, _i32,
+                                     _P, ctypes.c_float, ctypes.c_float, _P, _SZ, _P, _i32]),
+    "air_paged_diff_prefill_workspace_size": (_int, [_P, _i32, _i32, _i32, ctypes.POINTER(_SZ)]),
+    "air_paged_diff_prefill": (_int, [_P, _P, _P, _i32, _i32, _P, _i32, _P, _i32, _i32, _P, _P, _i32, _i32,
+                                      ctypes.c_float, _P, ctypes.c_float, ctypes.c_float, _P, _SZ, _P, _i32]),
     "air_kv_session_create": (_int, [_P, ctypes.POINTER(_P), _i32, ctypes.POINTER(_P)]),
     "air_kv_session_destroy": (_int, [_P]),
     "air_kv_session_fork": (_int, [_P, ctypes.POINTER(_P)]),
@@ -122,6 +128,7 @@ SIGNATURES = {
     "air_kv_session_load": (_int, [_P, _P, _i32, _P, _P, _i32]),
     "air_kv_session_clear": (_int, [_P]),
     "air_kv_session_truncate_to": (_int, [_P, _i64]),
+    "air_kv_session_compact": (_int, [_P, _P, _P, _i64]),
     "air_kv_session_memory_usage": (_int, [_P, ctypes.POINTER(_SZ)]),
     "air_kv_block_wire_bytes": (_int, [_P, ctypes.POINTER(_SZ)]),
     "air_kv_pack_blocks": (_int, [_P, _P, _P, _i32, _P]),
@@ -148,6 +155,7 @@ SIGNATURES = {
                                                ctypes.POINTER(ctypes.c_float), ctypes.POINTER(_P),
                                                ctypes.POINTER(_SZ)]),
     "air_kv_int8_payload_serialise_n": (_int, [_P, ctypes.c_uint16, _P, _P, _SZ, _i32, _P]),
+    "air_kv_compact": (_int, [_P, _P, _P, _P, _i32, _i32, _P, _P, _i32]),
     "air_kv_copy_blocks": (_int, [_P, _P, _P, _P, _i32]),
     "air_kv_read_blocks": (_int, [_P, _P, _pi32, _i32, _P]),
     "air_kv_write_blocks": (_int, [_P, _P, _pi32, _i32, _P]),

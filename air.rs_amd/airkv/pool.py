@@ -302,6 +302,133 @@ class KvPool:
         launch.workspace = ws
         return launch
 
+    # -- differential attention ---------------------------------------------------
+
+    def diff_decode_workspace_size(self, n_q_heads, batch, max_blocks, max_splits=64):
+        out = ctypes.c_size_t()
+        _lib.check(_lib.load().air_paged_diff_decode_workspace_size(self.handle, n_q_heads, batch, max_blocks,
+                                                                    max_splits, ctypes.byref(out)),
+                   "air_paged_diff_decode_workspace_size")
+        return out.value
+
+    def new_diff_workspace(self, n_q_heads, batch, max_blocks, max_splits=64):
+        torch = _torch()
+        n = self.diff_decode_workspace_size(n_q_heads, batch, max_blocks, max_splits)
+        return torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
+
+    def diff_prefill_workspace_size(self, n_q_heads, batch, max_q_len):
+        out = ctypes.c_size_t()
+        _lib.check(_lib.load().air_paged_diff_prefill_workspace_size(self.handle, n_q_heads, batch, max_q_len,
+                                                                     ctypes.byref(out)),
+                   "air_paged_diff_prefill_workspace_size")
+        return out.value
+
+    def new_diff_prefill_workspace(self, n_q_heads, batch, max_q_len):
+        torch = _torch()
+        n = self.diff_prefill_workspace_size(n_q_heads, batch, max_q_len)
+        return torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
+
+    def _diff_args(self, q, lam, out, norm_weight, norm_eps, out_scale):
+        """(q and lambda arguments, norm arguments, output arguments) of a differential call."""
+        torch = _torch()
+        rows, n_q, d = q.shape
+        if d != self.head_dim:
+            raise ValueError("q head_dim differs from the pool")
+        qt, ot = q.dtype, out.dtype
+        qdt, odt = self._act_dtypes(qt, ot)
+        q_at = _dev(q, qt, "q")
+        out_at = _dev(out, ot, "out", (rows, n_q // 2, 2 * d))
+        per_row = 1 if lam.dim() == 2 else 0
+        lam_at = _dev(lam, torch.float32, "lam", (rows, n_q // 2) if per_row else (n_q // 2,))
+        if norm_eps is None:
+            if norm_weight is not None:
+                raise ValueError("norm_weight needs norm_eps")
+            norm = (None, 0.0)
+        elif not norm_eps > 0:
+            raise ValueError("norm_eps must be positive (None: no norm)")
+        else:
+            norm = (None if norm_weight is None else _dev(norm_weight, torch.float32, "norm_weight", (2 * d,)), norm_eps)
+        return (q_at, qdt, n_q, lam_at, per_row), norm + (out_scale,), (out_at, odt)
+
+    def _diff_decode_args(self, q, lam, block_tables, seq_lens, out, norm_weight, norm_eps, out_scale, scale,
+                          max_splits, workspace, stream):
+        torch = _torch()
+        head, norm, tail = self._diff_args(q, lam, out, norm_weight, norm_eps, out_scale)
+        batch, n_q = q.shape[:2]
+        tables_at = _dev(block_tables, torch.int32, "block_tables")
+        rows, max_blocks = block_tables.shape
+        if rows != batch:
+            raise ValueError("block_tables rows differ from batch")
+        lens_at = _dev(seq_lens, torch.int32, "seq_lens", (batch,))
+        if workspace is None:
+            workspace = self.new_diff_workspace(n_q, batch, max_blocks, max_splits)
+        ws_at = _dev(workspace, workspace.dtype, "workspace")
+        return (self.handle, _stream_ptr(stream)) + head + (
+            tables_at, lens_at, batch, max_blocks, self._scale if scale is None else scale, max_splits) + norm + (
+            ws_at, workspace.nbytes) + tail, workspace
+
+    def paged_diff_decode(self, q, lam, block_tables, seq_lens, out, norm_weight=None, norm_eps=None, out_scale=1.0,
+                          scale=None, max_splits=64, workspace=None, stream=None):
+        """Differential attention of one token per sequence (air_paged_diff_decode):
+        K/V heads 2p and 2p + 1 are a pair, as are query heads 2h and 2h + 1, and
+        out[b, h] = out_scale * norm((P_0 - lam P_1) [V_2p | V_2p+1]).  q [batch,
+        n_q, d], out [batch, n_q / 2, 2 d]; lam float32 [n_q / 2] or [batch, n_q / 2];
+        norm_eps None leaves the norm out."""
+        args, _ws = self._diff_decode_args(q, lam, block_tables, seq_lens, out, norm_weight, norm_eps, out_scale,
+                                           scale, max_splits, workspace, stream)
+        _lib.check(_lib.load().air_paged_diff_decode(*args), "air_paged_diff_decode")
+        return out
+
+    def bind_diff_decode(self, q, lam, block_tables, seq_lens, out, norm_weight=None, norm_eps=None, out_scale=1.0,
+                         scale=None, max_splits=64, workspace=None, stream=None):
+        """Validate once, return a zero-argument launcher."""
+        args, ws = self._diff_decode_args(q, lam, block_tables, seq_lens, out, norm_weight, norm_eps, out_scale,
+                                          scale, max_splits, workspace, stream)
+        fn = _lib.load().air_paged_diff_decode
+        _lib.check(fn(*args), "air_paged_diff_decode")
+        return _launcher(fn, args, "air_paged_diff_decode",
+                         (q, lam, block_tables, seq_lens, out, norm_weight, ws, stream))
+
+    def _diff_prefill_args(self, q, lam, cu_q, block_tables, seq_lens, out, max_q_len, norm_weight, norm_eps,
+                           out_scale, scale, workspace, stream):
+        torch = _torch()
+        head, norm, tail = self._diff_args(q, lam, out, norm_weight, norm_eps, out_scale)
+        total_q, n_q = q.shape[:2]
+        tables_at = _dev(block_tables, torch.int32, "block_tables")
+        batch, max_blocks = block_tables.shape
+        lens_at = _dev(seq_lens, torch.int32, "seq_lens", (batch,))
+        cu_at = _dev(cu_q, torch.int32, "cu_q", (batch + 1,))
+        if max_q_len is None:
+            max_q_len = int((cu_q[1:] - cu_q[:-1]).max().item()) if batch else 0
+        if workspace is None:
+            workspace = self.new_diff_prefill_workspace(n_q, batch, max_q_len)
+        ws_at = _dev(workspace, workspace.dtype, "workspace")
+        return (self.handle, _stream_ptr(stream)) + head + (
+            cu_at, total_q, max_q_len, tables_at, lens_at, batch, max_blocks,
+            self._scale if scale is None else scale) + norm + (ws_at, workspace.nbytes) + tail, workspace
+
+    def paged_diff_prefill(self, q, lam, cu_q, block_tables, seq_lens, out, max_q_len=None, norm_weight=None,
+                           norm_eps=None, out_scale=1.0, scale=None, workspace=None, stream=None):
+        """Differential attention, causal, of each sequence's newest cu_q[b+1] -
+        cu_q[b] tokens over its pages (air_paged_diff_prefill); q [total_q, n_q, d],
+        out [total_q, n_q / 2, 2 d], lam float32 [n_q / 2] or [total_q, n_q / 2].
+        max_q_len defaults to the largest q_len (read back from cu_q, which
+        synchronises)."""
+        args, _ws = self._diff_prefill_args(q, lam, cu_q, block_tables, seq_lens, out, max_q_len, norm_weight,
+                                            norm_eps, out_scale, scale, workspace, stream)
+        _lib.check(_lib.load().air_paged_diff_prefill(*args), "air_paged_diff_prefill")
+        return out
+
+    def bind_diff_prefill(self, q, lam, cu_q, block_tables, seq_lens, out, max_q_len=None, norm_weight=None,
+                          norm_eps=None, out_scale=1.0, scale=None, workspace=None, stream=None):
+        """Validate once, return a zero-argument launcher."""
+        args, ws = self._diff_prefill_args(q, lam, cu_q, block_tables, seq_lens, out, max_q_len, norm_weight,
+                                           norm_eps, out_scale, scale, workspace, stream)
+        fn = _lib.load().air_paged_diff_prefill
+        _lib.check(fn(*args), "air_paged_diff_prefill")
+        return _launcher(fn, args, "air_paged_diff_prefill",
+                         (q, lam, cu_q, block_tables, seq_lens, out, norm_weight, ws, stream))
+
     def bind_append(self, k, v, slot_mapping, stream=None):
         """Validate once, return a zero-argument append launcher."""
         self.append(k, v, slot_mapping, stream)
@@ -331,6 +458,20 @@ class KvPool:
         dp = _dev(dst, torch.int32, "dst", (n,))
         _lib.check(_lib.load().air_kv_copy_blocks(self.handle, _stream_ptr(stream), sp, dp, n),
                    "air_kv_copy_blocks")
+
+    def compact(self, block_tables, seq_lens, keep, cu_keep, stream=None):
+        """Move the kept tokens of each sequence -- positions keep[cu_keep[b] :
+        cu_keep[b + 1]], ascending -- to its first positions, inside its own pages
+        (air_kv_compact).  The blocks written belong to that sequence alone; shorten
+        the sequence afterwards (SequenceManager.truncate)."""
+        torch = _torch()
+        tables_at = _dev(block_tables, torch.int32, "block_tables")
+        batch, max_blocks = block_tables.shape
+        lens_at = _dev(seq_lens, torch.int32, "seq_lens", (batch,))
+        keep_at = _dev(keep, torch.int32, "keep", (keep.shape[0],))
+        cu_at = _dev(cu_keep, torch.int32, "cu_keep", (batch + 1,))
+        _lib.check(_lib.load().air_kv_compact(self.handle, _stream_ptr(stream), tables_at, lens_at, batch, max_blocks,
+                                              keep_at, cu_at, keep.shape[0]), "air_kv_compact")
 
     # -- host copies ------------------------------------------------------------
 

@@ -18,11 +18,14 @@ operations keep their meaning:
                         src/kv_cache.rs:364-383); blocks past pos are released
 
 plus append(layer, k_new, v_new) (the reshape-and-cache that replaces the
-Tensor::cat) and fork() (fork_sequence with copy-on-write of shared blocks).
+Tensor::cat), fork() (fork_sequence with copy-on-write of shared blocks) and
+compact(keep) (tokens dropped from anywhere in the sequence).
 """
 from __future__ import annotations
 
 import ctypes
+
+import numpy as np
 
 from . import _lib
 from .pool import _dev, _stream_ptr, _torch
@@ -109,6 +112,19 @@ class PagedSessionCache:
 
     def truncate_to(self, pos):
         _lib.check(_lib.load().air_kv_session_truncate_to(self._h, pos), "truncate_to")
+
+    def compact(self, keep, stream=None):
+        """Keep the tokens at the ascending positions `keep`, in every layer, as
+        tokens 0, 1, ... and release the blocks past them (shared blocks that are
+        written are copied first)."""
+        keep = np.ascontiguousarray(keep, np.int64)
+        if keep.ndim != 1:
+            raise ValueError("keep must be one list of positions")
+        rc = _lib.load().air_kv_session_compact(self._h, _stream_ptr(stream), keep.ctypes.data_as(ctypes.c_void_p),
+                                                len(keep))
+        if rc == _lib.AIR_KV_E_OOM:
+            raise MemoryError(_lib.last_error())
+        _lib.check(rc, "compact")
 
     def fork(self):
         h = ctypes.c_void_p()

@@ -1,0 +1,560 @@
+// Differential decode attention over the paged cache (formulas: diff_common.hpp).
+//
+// The batch's cached tokens are cut into 16-token tiles and these into equal
+// contiguous slices per K/V pair, one wave each (decode_slices.hpp); a sequence
+// that several slices hold is joined by diff_decode_merge_kernel.
+//
+// A wave takes eight query pairs of its K/V pair as 16 rows: row n is map n / 8 of
+// query pair n % 8, so one accumulator tile holds both maps and the softmax works
+// on all 64 lanes.  Per tile:
+//   S  = K . Q^T  twice, with either key head; row n keeps the one of its map.
+//   P  = exp2(S * scale * log2 e - m)
+//   O^T += V^T . P^T over the 2 * head_dim columns of the pair's two value heads.
+// All products are v_mfma_f32_16x16x4_f32 on values widened (or dequantized) to
+// f32, so queries, keys, probabilities and values keep 24 bits, and no operand
+// needs a transpose: lane (n, q) holds S of tokens 4q .. 4q + 3, and step i of the
+// second product contracts over tokens {4q + i}, whose V rows lane (m, q) reads
+// straight from the page, CA consecutive columns from CA * m.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../pool.hpp"
+#include "decode_plan.hpp"
+#include "diff_common.hpp"
+
+namespace airkv {
+namespace {
+
+typedef diff_f32x4 f32x4;
+
+constexpr int kThreads = kSliceThreads;
+constexpr int kWaves = kThreads / 64;
+constexpr int kWavesPerSimd = 2;
+constexpr int kFullChunk = 4;              // tiles a slice holds at least once every SIMD has a wave
+
+struct DiffDecodeArgs : DecodeArgs {
+    DiffOut e;
+    int32_t pairs;                         // query pairs
+    int32_t kv_pairs, row_tiles;
+};
+
+__device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// x of lane l ^ 8 within each 16 lanes.
+__device__ __forceinline__ float dpp_ror8(float x) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xF, 0xF, false));
+}
+
+// BYTES (2, 4, 8, 16 or 32) bytes of a page at `off`.
+template <int BYTES>
+__device__ __forceinline__ void load_piece(const __amdgpu_buffer_rsrc_t &r, int off, uint32_t (&w)[(BYTES + 3) / 4]) {
+    if constexpr (BYTES == 2) {
+        w[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, 0, kDiffStream);
+    } else if constexpr (BYTES == 4) {
+        w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, kDiffStream);
+    } else if constexpr (BYTES == 8) {
+        const diff_u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, kDiffStream);
+        w[0] = x[0]; w[1] = x[1];
+    } else {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) {
+            const diff_u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * i, 0, kDiffStream);
+            w[4 * i] = x[0]; w[4 * i + 1] = x[1]; w[4 * i + 2] = x[2]; w[4 * i + 3] = x[3];
+        }
+    }
+}
+
+// N consecutive elements of a page row as f32.
+template <int DT, int N, int W>
+__device__ __forceinline__ void widen(const uint32_t (&w)[W], float s, float (&x)[N]) {
+    if constexpr (DT == AIR_KV_F32) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = __uint_as_float(w[i]);
+    } else if constexpr (DT == AIR_KV_BF16) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = __uint_as_float((i & 1) ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < (N + 3) / 4; ++i) {
+            const f32x4 v = code_values<DT>(w[i], s);
+#pragma unroll
+            for (int j = 0; j < 4 && 4 * i + j < N; ++j) x[4 * i + j] = v[j];
+        }
+    }
+}
+
+template <int D, int DT>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerSimd, kWavesPerSimd)))
+void diff_decode_kernel(DiffDecodeArgs a) {
+    static_assert(D % 32 == 0 && D <= 128, "steps of 32, two value heads of at most 256 columns");
+    constexpr bool QUANT = DT == AIR_KV_INT8 || DT == AIR_KV_FP8;
+    constexpr int EB = DT == AIR_KV_F32 ? 4 : DT == AIR_KV_BF16 ? 2 : 1;
+    constexpr int KS = D / 32;                         // steps of the first product
+    // columns of a value head in a lane: CA from CA * m, then CB from 16 * CA + CB * m
+    // (96 as 64 + 32: a run of 6 columns would straddle scale groups)
+    constexpr int CA = D == 96 ? 4 : D / 16, CB = D == 96 ? 2 : 0, C = CA + CB;
+    constexpr int KW = 8 * EB / 4, VA = (CA * EB + 3) / 4, VB = CB ? (CB * EB + 3) / 4 : 1;
+
+    __shared__ int32_t s_pre[kMaxBatch + 2];
+    __shared__ int32_t s_wsum[kWaves];
+
+    const int bs = a.block_size;
+    tile_prefix(a, bs, s_pre, s_wsum);
+    const int B = a.batch;
+    const int total = s_pre[B];
+    const int chunk = slice_chunk(total, a.slices, a.simd_slices, kFullChunk, s_pre[B + 1], a.max_splits);
+    if (blockIdx.x == 0) {                             // for the merge: prefix, then the chunk
+        for (int i = threadIdx.x; i <= B; i += kThreads) a.prefix[i] = s_pre[i];
+        if (threadIdx.x == 0) a.prefix[B + 1] = chunk;
+    }
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int q4 = lane >> 4, r16 = lane & 15;
+    // the row tiles of a K/V pair, then the pairs, are neighbours: their pages are the same, or lie in the same blocks
+    const int heads = a.kv_pairs * a.row_tiles;
+    const int gw = blockIdx.x * kWaves + wave;
+    const int hh = gw % heads, w = gw / heads;
+    if (w >= a.slices || (int64_t)w * chunk >= total) return;
+    const int kp = hh / a.row_tiles, rt = hh % a.row_tiles;
+    const int lo = w * chunk;
+    const int hi = total - lo < chunk ? total : lo + chunk;
+    const int64_t max_len = (int64_t)a.max_blocks * bs;
+    const int rows = a.group - 8 * rt < 8 ? a.group - 8 * rt : 8;       // query pairs of this wave
+    const int qp = r16 & 7;                                             // this lane's row: map r16 / 8 of pair qp
+    const bool map1 = r16 >= 8;
+    const bool live_row = qp < rows;
+
+    // Lane k describes tile c0 + k of a window of 64: block, tile within its sequence, valid tokens.
+    int32_t tbl = 0, seq_l = 0, j_l = 0, nv_l = 0;
+    uint64_t first_m = 0, last_m = 0;
+    auto load_window = [&](int c0) {
+        const int t = c0 + lane < hi ? c0 + lane : hi - 1;
+        const int bq = seq_of_tile(s_pre, B, t);
+        const int j = t - s_pre[bq];
+        const int64_t len = clamp_len(a.lens[bq], max_len);
+        tbl = a.tables[(int64_t)bq * a.max_blocks + (int64_t)16 * j / bs];
+        seq_l = bq;
+        j_l = j;
+        const int64_t rest = len - 16 * (int64_t)j;
+        nv_l = rest < 16 ? (int)rest : 16;
+        const bool valid = c0 + lane < hi;
+        first_m = __ballot(valid && (t == lo || j == 0));
+        last_m = __ballot(valid && (t + 1 == hi || t + 1 == s_pre[bq + 1]));
+    };
+
+    // Q^T as the B operand: lane (n, q) holds row n's elements 32 s + 8 q .. +8
+    float qf[KS][8];
+    auto load_q = [&](int bq) {
+        const int head = 2 * (kp * a.group + 8 * rt + qp) + (map1 ? 1 : 0);
+        const int64_t at = ((int64_t)bq * a.n_q_heads + (live_row ? head : 0)) * D + 8 * q4;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            if (a.q_dtype == AIR_KV_F32) {
+                const f32x4 *p = reinterpret_cast<const f32x4 *>((const float *)a.q + at + 32 * s);
+                const f32x4 x = p[0], y = p[1];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    qf[s][j] = x[j];
+                    qf[s][4 + j] = y[j];
+                }
+            } else {
+                const diff_u32x4 x = *reinterpret_cast<const diff_u32x4 *>((const uint16_t *)a.q + at + 32 * s);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    qf[s][j] = __uint_as_float((j & 1) ? x[j / 2] & 0xFFFF0000u : x[j / 2] << 16);
+            }
+        }
+    };
+
+    f32x4 acc[2][C];                                   // O^T: value head, column of the lane
+    float m_run = -INFINITY, l_run = 0.0f;
+
+    const int nsc = QUANT ? D / a.scale_group : 0;     // scales per row
+    // The column of acc[t][j][i] of this lane
+    auto col = [&](int t, int j, int i) {
+        const int m = 4 * q4 + i;
+        return t * D + (j < CA ? CA * m + j : 16 * CA + CB * m + j - CA);
+    };
+
+    // The piece of sequence bq that this wave holds ends.
+    auto emit = [&](int bq) {
+        const float l = sum_x32(sum_x16(l_run));
+        const int w0 = s_pre[bq] / chunk, w1 = (s_pre[bq + 1] - 1) / chunk;
+        if (w0 == w1) {                                // the whole sequence: its output rows
+            const int h = kp * a.group + 8 * rt + qp;
+            const float lam = live_row ? a.e.lam[bq * a.e.lam_stride + h] : 0.0f;
+            const float inv = (map1 ? -lam : 1.0f) / l;
+            float ss = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < C; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        // row n's and row n + 8's lanes (row_ror:8)
+                        const float x = acc[t][j][i] * inv;
+                        const float y = x + dpp_ror8(x);
+                        acc[t][j][i] = y;
+                        ss += y * y;
+                    }
+            const float f = diff_factor(a.e, a.e.norm ? sum_x32(sum_x16(ss)) : 0.0f, 2 * D);
+            if (live_row && !map1) {
+                const int64_t at = ((int64_t)bq * a.pairs + h) * (2 * D);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float x[C];
+#pragma unroll
+                        for (int j = 0; j < C; ++j)
+                            x[j] = acc[t][j][i] * ((a.e.norm && a.e.norm_w) ? f * a.e.norm_w[col(t, j, i)] : f);
+#pragma unroll
+                        for (int j = 0; j + 4 <= CA; j += 4)
+                            diff_store4(a.e, at + col(t, j, i), f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]});
+#pragma unroll
+                        for (int j = CA / 4 * 4; j < C; ++j) diff_store(a.e, at + col(t, j, i), x[j]);
+                    }
+            }
+        } else if (live_row) {
+            const int64_t row = ((int64_t)hh * a.slots + part_row(w, bq, w == w0)) * 16 + r16;
+            float *po = a.part_o + row * (2 * D);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                    for (int j = 0; j + 4 <= CA; j += 4)
+                        *reinterpret_cast<f32x4 *>(po + col(t, j, i)) =
+                            f32x4{acc[t][j][i], acc[t][j + 1][i], acc[t][j + 2][i], acc[t][j + 3][i]};
+#pragma unroll
+                    for (int j = CA / 4 * 4; j < C; ++j) po[col(t, j, i)] = acc[t][j][i];
+                }
+            if (q4 == 0) {
+                a.part_ml[row * 2] = m_run;
+                a.part_ml[row * 2 + 1] = l;
+            }
+        }
+    };
+
+    auto tile = [&](int k, int idx) {
+        int32_t blk = __builtin_amdgcn_readlane(tbl, idx);
+        const int jt = __builtin_amdgcn_readlane(j_l, idx);
+        const bool ok = blk >= 0 && blk < a.num_blocks;
+        blk = ok ? blk : 0;
+        // rows of the pair's first head; the second's are bs further
+        const int64_t row0 = ((int64_t)blk * a.n_kv_heads + 2 * kp) * bs + (int64_t)16 * jt % bs;
+        const int span = (bs + 16) * D * EB;           // to the end of the second head's tile
+        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+            (void *)((const char *)a.k_pages + row0 * D * EB), (short)0, span, kDiffBufferWord3);
+        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+            (void *)((const char *)a.v_pages + row0 * D * EB), (short)0, span, kDiffBufferWord3);
+        uint32_t kr[2][KS][KW], va[2][4][VA], vb[2][4][VB];
+        float ksc[2][KS], vsa[2][4], vsb[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+                load_piece<8 * EB>(rk, ((t * bs + r16) * D + 32 * s + 8 * q4) * EB, kr[t][s]);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = (t * bs + 4 * q4 + i) * D;
+                load_piece<CA * EB>(rv, (at + CA * r16) * EB, va[t][i]);
+                if constexpr (CB > 0) load_piece<CB * EB>(rv, (at + 16 * CA + CB * r16) * EB, vb[t][i]);
+            }
+        if constexpr (QUANT) {
+            const int sspan = (bs + 16) * nsc * 4;
+            const __amdgpu_buffer_rsrc_t rks = __builtin_amdgcn_make_buffer_rsrc(
+                (void *)(a.k_scales + row0 * nsc), (short)0, sspan, kDiffBufferWord3);
+            const __amdgpu_buffer_rsrc_t rvs = __builtin_amdgcn_make_buffer_rsrc(
+                (void *)(a.v_scales + row0 * nsc), (short)0, sspan, kDiffBufferWord3);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+                    ksc[t][s] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                        rks, ((t * bs + r16) * nsc + (32 * s + 8 * q4) / a.scale_group) * 4, 0, kDiffStream));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int at = (t * bs + 4 * q4 + i) * nsc;
+                    vsa[t][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                        rvs, (at + CA * r16 / a.scale_group) * 4, 0, kDiffStream));
+                    if constexpr (CB > 0)
+                        vsb[t][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                            rvs, (at + (16 * CA + CB * r16) / a.scale_group) * 4, 0, kDiffStream));
+                }
+            }
+        }
+
+        const int bq = __builtin_amdgcn_readlane(seq_l, idx);
+        if ((first_m >> idx) & 1) {                    // a sequence starts in this slice
+            if (k != lo) load_q(bq);
+            m_run = -INFINITY;
+            l_run = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < C; ++j) acc[t][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        // an entry outside the pool is counted once, by the first pair's wave, and its tile masked
+        if (!ok && lane == 0) atomicAdd(a.errors, 1ull);
+        const int nv = ok ? __builtin_amdgcn_readlane(nv_l, idx) : 0;
+        const bool full = nv == 16;
+
+        f32x4 s2[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            float x[2][8];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) widen<DT, 8>(kr[t][s], QUANT ? ksc[t][s] : 0.0f, x[t]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) s2[t] = mfma_f32(x[t][j], qf[s][j], s2[t]);
+        }
+        float sc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sc[i] = (map1 ? s2[1][i] : s2[0][i]) * a.scale_log2;
+            if (!full) sc[i] = 4 * q4 + i < nv ? sc[i] : -INFINITY;
+        }
+        float mt = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+        mt = max_x32(max_x16(mt));
+        // raised only past 2^8 times the present maximum (and on the first tile): most tiles skip the rescale
+        if (__ballot(mt > m_run + 8.0f) != 0ull) {
+            const float top = fmaxf(m_run, mt);
+            const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - top);
+            l_run *= alpha;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < C; ++j) acc[t][j] *= alpha;
+            m_run = top;
+        }
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = sc[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sc[i] - m_run);
+        l_run += (p[0] + p[1]) + (p[2] + p[3]);
+        // rows past the sequence hold what was there before, non-finite values too: they become zeros
+        if (!full) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool in = 4 * q4 + i < nv;
+#pragma unroll
+                    for (int j = 0; j < VA; ++j) va[t][i][j] = in ? va[t][i][j] : 0;
+#pragma unroll
+                    for (int j = 0; j < VB; ++j) vb[t][i][j] = in ? vb[t][i][j] : 0;
+                    if constexpr (QUANT) {
+                        vsa[t][i] = in ? vsa[t][i] : 0.0f;
+                        vsb[t][i] = in ? vsb[t][i] : 0.0f;
+                    }
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                float x[CA];
+                widen<DT, CA>(va[t][i], QUANT ? vsa[t][i] : 0.0f, x);
+#pragma unroll
+                for (int j = 0; j < CA; ++j) acc[t][j] = mfma_f32(x[j], p[i], acc[t][j]);
+                if constexpr (CB > 0) {
+                    float y[CB];
+                    widen<DT, CB>(vb[t][i], QUANT ? vsb[t][i] : 0.0f, y);
+#pragma unroll
+                    for (int j = 0; j < CB; ++j) acc[t][CA + j] = mfma_f32(y[j], p[i], acc[t][CA + j]);
+                }
+            }
+        if ((last_m >> idx) & 1) emit(bq);
+    };
+
+    for (int c0 = lo; c0 < hi; c0 += 64) {
+        load_window(c0);
+        if (c0 == lo) load_q(__builtin_amdgcn_readlane(seq_l, 0));
+        const int n = hi - c0 < 64 ? hi - c0 : 64;
+        for (int i = 0; i < n; ++i) tile(c0 + i, i);
+    }
+}
+
+// One query pair of one sequence: the pieces of its two rows folded by
+// log-sum-exp, WH waves sharing them, then the output row.  An empty sequence
+// gives zeros; lengths outside the table are counted.
+template <int D, int WH>
+__global__ __launch_bounds__(64 * WH) void diff_decode_merge_kernel(DiffDecodeArgs a) {
+    constexpr int V = D / 32, kBatch = 8;
+    __shared__ float s_ml[WH][4];
+    __shared__ float s_o[WH][2][64 * V];
+    const int b = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int p0 = a.prefix[b], p1 = a.prefix[b + 1], chunk = a.prefix[a.batch + 1];
+    const int len = a.lens[b];
+    const int64_t max_len = (int64_t)a.max_blocks * a.block_size;
+    if (threadIdx.x == 0 && h == 0 && (len < 0 || len > max_len)) atomicAdd(a.errors, 1ull);
+    if (p0 == p1) {
+        if (wave == 0)
+            for (int i = lane; i < 2 * D; i += 64) diff_store(a.e, ((int64_t)b * a.pairs + h) * (2 * D) + i, 0.0f);
+        return;
+    }
+    const int w0 = p0 / chunk, w1 = (p1 - 1) / chunk;
+    if (w0 == w1) return;                              // written by its slice
+    const int n = w1 - w0 + 1;
+    const int kp = h / a.group, j = h % a.group;
+    const int hh = kp * a.row_tiles + j / 8;
+    DiffFold<V> c;
+    c.clear();
+    for (int q0 = wave; q0 < n; q0 += WH * kBatch) {
+        float pm[kBatch][2], pl[kBatch][2], po[kBatch][2][V];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const bool in = q0 + WH * i < n;
+            const int p = in ? q0 + WH * i : q0;
+            const int64_t row = ((int64_t)hh * a.slots + part_row(w0 + p, b, p == 0)) * 16 + (j & 7);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                pm[i][k] = in ? a.part_ml[(row + 8 * k) * 2] : -INFINITY;
+                pl[i][k] = in ? a.part_ml[(row + 8 * k) * 2 + 1] : 0.0f;
+                diff_load<V>(a.part_o + (row + 8 * k) * (2 * D) + V * lane, po[i][k]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) c.fold(k, pm[i][k], pl[i][k], po[i][k]);
+    }
+    if constexpr (WH > 1) {
+        if (lane == 0) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                s_ml[wave][2 * k] = c.m[k];
+                s_ml[wave][2 * k + 1] = c.l[k];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) s_o[wave][k][V * lane + i] = c.o[k][i];
+        __syncthreads();
+        if (wave != 0) return;
+        for (int w = 1; w < WH; ++w)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float o[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[i] = s_o[w][k][V * lane + i];
+                c.fold(k, s_ml[w][2 * k], s_ml[w][2 * k + 1], o);
+            }
+    }
+    diff_finish<V>(a.e, b, h, a.pairs, c, lane);
+}
+
+template <int D, int DT>
+hipError_t launch_dt(const DiffDecodeArgs &a, hipStream_t s) {
+    const int64_t waves = (int64_t)a.kv_pairs * a.row_tiles * a.slices;
+    hipLaunchKernelGGL((diff_decode_kernel<D, DT>), dim3((unsigned)((waves + kWaves - 1) / kWaves)), dim3(kThreads), 0, s, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const dim3 grid((unsigned)a.batch, (unsigned)a.pairs);
+    // past a round trip's worth of pieces for an average sequence, four waves share them
+    if (a.slices > 8 * a.batch) hipLaunchKernelGGL((diff_decode_merge_kernel<D, 4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((diff_decode_merge_kernel<D, 1>), grid, dim3(64), 0, s, a);
+    return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_d(const DiffDecodeArgs &a, int dtype, hipStream_t s) {
+    return dtype == AIR_KV_F32    ? launch_dt<D, AIR_KV_F32>(a, s)
+           : dtype == AIR_KV_BF16 ? launch_dt<D, AIR_KV_BF16>(a, s)
+           : dtype == AIR_KV_INT8 ? launch_dt<D, AIR_KV_INT8>(a, s)
+                                  : launch_dt<D, AIR_KV_FP8>(a, s);
+}
+
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+}  // namespace
+
+// A slice for every wave slot, at most batch * max_splits.  The workspace holds
+// the tile prefix and the chunk, then a partial row of 16 rows for every cut
+// piece there can be.
+DiffDecodePlan plan_diff_decode(const air_kv_pool &p, int32_t n_q_heads, int32_t batch, int32_t max_blocks,
+                                int32_t max_splits) {
+    DiffDecodePlan pl;
+    const int kv_pairs = p.desc.n_kv_heads / 2;
+    pl.group = n_q_heads / p.desc.n_kv_heads;
+    pl.row_tiles = (pl.group + 7) / 8;
+    const int64_t tiles_per_seq =
+        std::max<int64_t>(1, std::min<int64_t>(((int64_t)max_blocks * p.desc.block_size + 15) / 16, ((int64_t)INT32_MAX + 15) / 16));
+    // tiles of a launch in 32 bits, with room for the window of 64 past the last
+    const int64_t nb = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(batch, kMaxBatch), (INT32_MAX - 65536) / tiles_per_seq));
+    const int64_t per_slice = (int64_t)kv_pairs * pl.row_tiles;
+    const int64_t waves = (int64_t)p.cus * 4 * kWavesPerSimd;
+    const int64_t sl = std::min<int64_t>((waves + per_slice - 1) / per_slice, nb * max_splits);
+    pl.batch_per_launch = (int32_t)nb;
+    pl.slices = (int32_t)sl;
+    pl.slots = (int32_t)part_rows(sl, nb);
+    const size_t rows = (size_t)per_slice * pl.slots * 16;
+    pl.ws_bytes = align256((size_t)(nb + 2) * 4) + align256(rows * 2 * 4) + rows * 2 * p.desc.head_dim * 4;
+    return pl;
+}
+
+hipError_t launch_diff_decode(const air_kv_pool &p, hipStream_t s, const DiffDecodePlan &plan, const void *q,
+                              int32_t q_dtype, int32_t n_q_heads, const int32_t *tables, const int32_t *lens,
+                              int32_t batch, int32_t max_blocks, float scale, int32_t max_splits, const DiffOut &out,
+                              void *workspace) {
+    const int d = p.desc.head_dim;
+    DiffDecodeArgs a{};
+    a.q_dtype = q_dtype;
+    a.n_q_heads = n_q_heads;
+    a.pairs = n_q_heads / 2;
+    a.kv_pairs = p.desc.n_kv_heads / 2;
+    a.row_tiles = plan.row_tiles;
+    a.group = plan.group;
+    a.max_blocks = max_blocks;
+    a.slices = plan.slices;
+    a.slots = plan.slots;
+    const int per_slice = a.kv_pairs * a.row_tiles;
+    a.simd_slices = (4 * p.cus + per_slice - 1) / per_slice;
+    a.max_splits = max_splits;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.n_kv_heads = p.desc.n_kv_heads;
+    a.block_size = p.desc.block_size;
+    a.scale_group = p.desc.scale_group;
+    a.head_dim = d;
+    a.num_blocks = p.desc.num_blocks;
+    a.k_pages = p.k_pages;
+    a.v_pages = p.v_pages;
+    a.k_scales = p.k_scales;
+    a.v_scales = p.v_scales;
+    a.errors = p.errors;
+    char *ws = (char *)workspace;
+    const size_t rows = (size_t)per_slice * plan.slots * 16;
+    a.prefix = (int32_t *)ws;
+    ws += align256((size_t)(plan.batch_per_launch + 2) * 4);
+    a.part_ml = (float *)ws;
+    ws += align256(rows * 2 * 4);
+    a.part_o = (float *)ws;
+    for (int32_t b0 = 0; b0 < batch; b0 += plan.batch_per_launch) {
+        a.batch = std::min(batch - b0, plan.batch_per_launch);
+        a.q = (const char *)q + (int64_t)b0 * n_q_heads * d * (q_dtype == AIR_KV_F32 ? 4 : 2);
+        a.tables = tables + (int64_t)b0 * max_blocks;
+        a.lens = lens + b0;
+        a.e = out;
+        a.e.lam = out.lam + (int64_t)b0 * out.lam_stride;
+        a.e.out = (char *)out.out + (int64_t)b0 * n_q_heads * d * (out.out_dtype == AIR_KV_F32 ? 4 : 2);
+        hipError_t e = d == 128 ? launch_d<128>(a, p.desc.dtype, s)
+                       : d == 96 ? launch_d<96>(a, p.desc.dtype, s)
+                       : d == 64 ? launch_d<64>(a, p.desc.dtype, s)
+                                 : launch_d<32>(a, p.desc.dtype, s);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+}  // namespace airkv

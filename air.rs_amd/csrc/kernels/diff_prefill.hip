@@ -1,0 +1,136 @@
+// Differential prefill: the launch plan, and the joining of blocks that several
+// slices computed (work division: diff_prefill_plan.hpp).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "../pool.hpp"
+#include "diff_prefill.hpp"
+
+namespace airkv {
+namespace {
+
+// One row of one cut block, one wave: its pieces folded by log-sum-exp, in order.
+template <int D>
+__global__ __launch_bounds__(256) void diff_prefill_merge_kernel(DiffPrefillArgs a) {
+    constexpr int V = D / 32, kBatch = 4;
+    const int w = blockIdx.x, kp = blockIdx.y, lane = threadIdx.x & 63;
+    const int row = blockIdx.z * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t at = (int64_t)kp * a.slices + w;
+    const int4 d = a.desc[at];
+    if (d.w == 0) return;
+    const int64_t k = (int64_t)((uint64_t)(uint32_t)d.y | (uint64_t)(uint32_t)d.z << 32);
+    DiffBlocks s;
+    diff_seq(a, d.x, s);
+    const int64_t f = k * a.rows + row;
+    if (f >= s.q * a.group) return;
+    DiffFold<V> c;
+    c.clear();
+    for (int p0 = 0; p0 < d.w; p0 += kBatch) {
+        float pm[kBatch][2], pl[kBatch][2], po[kBatch][2][V];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const bool in = p0 + i < d.w;
+            const int p = in ? p0 + i : p0;
+            const int64_t slot = 2 * (at + p) + (p == 0 ? 1 : 0);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                const int64_t r = (slot * a.rows + row) * 2 + m;
+                pm[i][m] = in ? a.part_ml[2 * r] : -INFINITY;
+                pl[i][m] = in ? a.part_ml[2 * r + 1] : 0.0f;
+                diff_load<V>(a.part_o + r * (2 * D) + V * lane, po[i][m]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) c.fold(m, pm[i][m], pl[i][m], po[i][m]);
+    }
+    diff_finish<V>(a.e, a.cu[d.x] + f / a.group, kp * a.group + (int)(f % a.group), a.pairs, c, lane);
+}
+
+}  // namespace
+
+hipError_t launch_diff_prefill_merge(const DiffPrefillArgs &a, int head_dim, hipStream_t s) {
+    if (a.slices < 2) return hipSuccess;               // nothing is cut
+    const dim3 grid((unsigned)a.slices, (unsigned)a.kv_pairs, (unsigned)(a.rows / 4));
+    if (head_dim == 128) hipLaunchKernelGGL((diff_prefill_merge_kernel<128>), grid, dim3(256), 0, s, a);
+    else if (head_dim == 96) hipLaunchKernelGGL((diff_prefill_merge_kernel<96>), grid, dim3(256), 0, s, a);
+    else if (head_dim == 64) hipLaunchKernelGGL((diff_prefill_merge_kernel<64>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((diff_prefill_merge_kernel<32>), grid, dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+namespace {
+
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// A slice for every workgroup that is resident at once, all K/V pairs together.
+struct Plan {
+    int32_t rows, slices, least;
+    size_t cells, halves;          // (pair, slice)s, rows' maps in the piece slots
+    size_t bytes(int d) const { return align256(cells * sizeof(int4)) + align256(halves * 2 * 4) + halves * 2 * d * 4; }
+};
+
+Plan plan_for(const air_kv_pool &p) {
+    Plan pl;
+    const int kv_pairs = p.desc.n_kv_heads / 2;
+    pl.rows = 64;
+    pl.slices = std::max(1, (2 * p.cus + kv_pairs - 1) / kv_pairs);
+    pl.least = 8;
+    pl.cells = (size_t)kv_pairs * pl.slices;
+    pl.halves = 2 * pl.cells * pl.rows * 2;
+    return pl;
+}
+
+}  // namespace
+
+size_t diff_prefill_workspace(const air_kv_pool &p) { return plan_for(p).bytes(p.desc.head_dim); }
+
+hipError_t launch_diff_prefill(const air_kv_pool &p, hipStream_t s, const void *q, int32_t q_dtype, int32_t n_q_heads,
+                               const int32_t *cu, int32_t total_q, const int32_t *tables, const int32_t *lens,
+                               int32_t batch, int32_t max_blocks, float scale, const DiffOut &out, void *workspace) {
+    const Plan plan = plan_for(p);
+    const int d = p.desc.head_dim;
+    DiffPrefillArgs a{};
+    a.q = q;
+    a.q_dtype = q_dtype;
+    a.pairs = n_q_heads / 2;
+    a.total_q = total_q;
+    a.max_blocks = max_blocks;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.kv_pairs = p.desc.n_kv_heads / 2;
+    a.group = n_q_heads / p.desc.n_kv_heads;
+    a.heads = p.desc.n_kv_heads;
+    a.bs = p.desc.block_size;
+    a.dtype = p.desc.dtype;
+    a.scale_group = p.desc.scale_group;
+    a.num_blocks = p.desc.num_blocks;
+    a.k_pages = p.k_pages;
+    a.v_pages = p.v_pages;
+    a.k_scales = p.k_scales;
+    a.v_scales = p.v_scales;
+    a.errors = p.errors;
+    a.e = out;
+    a.slices = plan.slices;
+    a.least = plan.least;
+    a.rows = plan.rows;
+    char *ws = (char *)workspace;
+    a.desc = (int4 *)ws;
+    ws += align256(plan.cells * sizeof(int4));
+    a.part_ml = (float *)ws;
+    ws += align256(plan.halves * 2 * 4);
+    a.part_o = (float *)ws;
+    for (int32_t b0 = 0; b0 < batch; b0 += kDiffPrefillBatch) {
+        a.batch = std::min(batch - b0, kDiffPrefillBatch);
+        a.cu = cu + b0;
+        a.tables = tables + (int64_t)b0 * max_blocks;
+        a.lens = lens + b0;
+        hipError_t e = launch_diff_prefill_f32(a, d, s);
+        if (e == hipSuccess) e = launch_diff_prefill_merge(a, d, s);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+}  // namespace airkv

@@ -62,6 +62,9 @@ hipError_t launch_decode(const air_kv_pool &pool, hipStream_t s, const DecodePla
                          const float *k_new = nullptr, const float *v_new = nullptr);
 hipError_t launch_copy_blocks(const air_kv_pool &pool, hipStream_t s, const int32_t *src,
                               const int32_t *dst, int32_t n);
+hipError_t launch_compact(const air_kv_pool &pool, hipStream_t s, const int32_t *tables, const int32_t *lens,
+                          int32_t batch, int32_t max_blocks, const int32_t *keep, const int32_t *cu_keep,
+                          int32_t total_keep);
 hipError_t launch_stage_blocks(const air_kv_pool &pool, hipStream_t s, const int32_t *ids, int32_t n,
                                void *staging, bool to_staging);
 size_t wire_block_bytes(const air_kv_pool &pool);

@@ -342,6 +342,104 @@ int air_kv_session_truncate_to(air_kv_session *s, int64_t pos) {
     return shrink_table(s);
 }
 
+static int session_compact(air_kv_session *s, void *stream, const int64_t *keep, int64_t n_keep) {
+    if (!s) return fail(AIR_KV_E_INVALID_ARG, "session is NULL");
+    if (n_keep < 0 || n_keep > INT32_MAX) return fail(AIR_KV_E_INVALID_ARG, "n_keep %lld out of range", (long long)n_keep);
+    if (n_keep > 0 && !keep) return fail(AIR_KV_E_INVALID_ARG, "keep is NULL");
+    const int64_t n = s->len[0];
+    for (int64_t l : s->len)
+        if (l != n) return fail(AIR_KV_E_STATE, "the layers hold %lld and %lld tokens", (long long)n, (long long)l);
+    if (n > INT32_MAX) return fail(AIR_KV_E_INVALID_ARG, "sequence too long");
+    for (int64_t i = 0; i < n_keep; ++i)
+        if (keep[i] < 0 || keep[i] >= n || (i > 0 && keep[i] <= keep[i - 1]))
+            return fail(AIR_KV_E_INVALID_ARG, "keep[%lld] = %lld: positions ascend, within the %lld tokens stored",
+                        (long long)i, (long long)keep[i], (long long)n);
+    int64_t stay = 0;                                  // the first tokens do not move
+    while (stay < n_keep && keep[stay] == stay) ++stay;
+    if (stay == n_keep) return air_kv_session_truncate_to(s, n_keep);
+    hipStream_t st = (hipStream_t)stream;
+    airkv::SequenceManager &m = manager(s);
+    const int32_t bs = m.block_size();
+    const airkv::BlockTable *t = m.table(s->seq);
+    if (!t) return fail(AIR_KV_E_NOT_FOUND, "sequence not found (%u)", s->seq);
+    const int64_t nb = (n + bs - 1) / bs;
+    if ((int64_t)t->physical_blocks.size() < nb)
+        return fail(AIR_KV_E_STATE, "sequence %u holds %lld blocks for %lld tokens (swapped out?)", s->seq,
+                    (long long)t->physical_blocks.size(), (long long)n);
+    // As in append: everything that can fail is checked, and the staging sized,
+    // before the table changes; blocks that are written and shared are copied.
+    const int64_t b0 = stay / bs, b1 = (n_keep - 1) / bs;
+    int64_t n_shared = 0;
+    for (int64_t i = b0; i <= b1; ++i)
+        if (m.allocator().ref_count(t->physical_blocks[(size_t)i]) > 1) ++n_shared;
+    if (!m.allocator().can_allocate(n_shared)) return fail(AIR_KV_E_OOM, "out of memory — no free blocks");
+    const size_t bytes = 4 * (size_t)(4 + n_keep + nb + 2 * n_shared);
+    if (int rc = reserve_stage(s, bytes)) return rc;
+    std::vector<int32_t> cow_src, cow_dst, host;
+    std::vector<int64_t> cow_idx;
+    cow_src.reserve((size_t)n_shared);
+    cow_dst.reserve((size_t)n_shared);
+    cow_idx.reserve((size_t)n_shared);
+    host.reserve(bytes / 4);
+    auto undo = [&]() {
+        for (size_t j = cow_idx.size(); j-- > 0;)
+            m.undo_cow(s->seq, (size_t)cow_idx[j], (uint32_t)cow_src[j], (uint32_t)cow_dst[j]);
+    };
+    for (int64_t i = b0; i <= b1; ++i) {
+        if (m.allocator().ref_count(m.table(s->seq)->physical_blocks[(size_t)i]) <= 1) continue;
+        uint32_t o, nbk;
+        if (int rc = m.cow_block(s->seq, i, &o, &nbk)) {
+            undo();
+            return rc;
+        }
+        cow_idx.push_back(i);
+        cow_src.push_back((int32_t)o);
+        cow_dst.push_back((int32_t)nbk);
+    }
+    t = m.table(s->seq);
+    // [cu_keep 2][length][pad][keep][table][copy sources][copy destinations]
+    for (int64_t x : {(int64_t)0, n_keep, n, (int64_t)0}) host.push_back((int32_t)x);
+    for (int64_t i = 0; i < n_keep; ++i) host.push_back((int32_t)keep[i]);
+    for (int64_t i = 0; i < nb; ++i) host.push_back((int32_t)t->physical_blocks[(size_t)i]);
+    host.insert(host.end(), cow_src.begin(), cow_src.end());
+    host.insert(host.end(), cow_dst.begin(), cow_dst.end());
+    void *dev;
+    if (int rc = stage(s, st, host.data(), 4 * host.size(), &dev)) {
+        undo();
+        return rc;
+    }
+    const int32_t *d = (const int32_t *)dev, *d_table = d + 4 + n_keep, *d_cow = d_table + nb;
+    const int32_t n_cow = (int32_t)cow_src.size();
+    int rc = AIR_KV_OK;
+    if (n_cow)
+        for (air_kv_pool *p : s->pools)
+            if ((rc = air_kv_copy_blocks(p, stream, d_cow, d_cow + n_cow, n_cow))) break;
+    // With shared blocks copied, an error before the first layer's launch leaves
+    // every page the table had as it was.
+    bool moved = false;
+    if (!rc)
+        for (air_kv_pool *p : s->pools) {
+            if ((rc = air_kv_compact(p, stream, d_table, d + 2, 1, (int32_t)nb, d + 4, d, (int32_t)n_keep))) break;
+            moved = true;
+        }
+    const int rc2 = mark_staged(s, st);
+    if (rc && !moved) {
+        undo();
+        return rc;
+    }
+    if (rc || rc2) return rc ? rc : rc2;
+    for (int64_t &l : s->len) l = n_keep;
+    return shrink_table(s);
+}
+
+int air_kv_session_compact(air_kv_session *s, void *stream, const int64_t *keep, int64_t n_keep) {
+    try {
+        return session_compact(s, stream, keep, n_keep);
+    } catch (const std::bad_alloc &) {
+        return fail(AIR_KV_E_OOM, "host allocation failed");
+    }
+}
+
 int air_kv_session_memory_usage(const air_kv_session *s, size_t *bytes) {
     if (!s || !bytes) return fail(AIR_KV_E_INVALID_ARG, "session or bytes is NULL");
     const airkv::BlockTable *t = s->mgr->impl->table(s->seq);

@@ -114,6 +114,10 @@ extern "C" {
     pub fn air_paged_decode_noalloc(pool: *mut air_kv_pool, stream: *mut c_void, q: *const c_void, q_dtype: i32, n_q_heads: i32, block_tables: *const i32, seq_lens: *const i32, batch: i32, max_blocks: i32, scale: f32, max_splits: i32, out: *mut c_void, out_dtype: i32) -> c_int;
     pub fn air_paged_prefill(pool: *mut air_kv_pool, stream: *mut c_void, q: *const c_void, q_dtype: i32, n_q_heads: i32, cu_q: *const i32, total_q: i32, max_q_len: i32, block_tables: *const i32, seq_lens: *const i32, batch: i32, max_blocks: i32, scale: f32, workspace: *mut c_void, ws_bytes: usize, out: *mut c_void, out_dtype: i32) -> c_int;
     pub fn air_paged_prefill_workspace_size(pool: *const air_kv_pool, n_q_heads: i32, batch: i32, max_q_len: i32, bytes: *mut usize) -> c_int;
+    pub fn air_paged_diff_decode_workspace_size(pool: *const air_kv_pool, n_q_heads: i32, batch: i32, max_blocks: i32, max_splits: i32, bytes: *mut usize) -> c_int;
+    pub fn air_paged_diff_decode(pool: *mut air_kv_pool, stream: *mut c_void, q: *const c_void, q_dtype: i32, n_q_heads: i32, lambda: *const f32, lambda_per_row: i32, block_tables: *const i32, seq_lens: *const i32, batch: i32, max_blocks: i32, scale: f32, max_splits: i32, norm_weight: *const f32, norm_eps: f32, out_scale: f32, workspace: *mut c_void, ws_bytes: usize, out: *mut c_void, out_dtype: i32) -> c_int;
+    pub fn air_paged_diff_prefill_workspace_size(pool: *const air_kv_pool, n_q_heads: i32, batch: i32, max_q_len: i32, bytes: *mut usize) -> c_int;
+    pub fn air_paged_diff_prefill(pool: *mut air_kv_pool, stream: *mut c_void, q: *const c_void, q_dtype: i32, n_q_heads: i32, lambda: *const f32, lambda_per_row: i32, cu_q: *const i32, total_q: i32, max_q_len: i32, block_tables: *const i32, seq_lens: *const i32, batch: i32, max_blocks: i32, scale: f32, norm_weight: *const f32, norm_eps: f32, out_scale: f32, workspace: *mut c_void, ws_bytes: usize, out: *mut c_void, out_dtype: i32) -> c_int;
     pub fn air_kv_session_create(mgr: *mut air_seq_manager, layer_pools: *const *mut air_kv_pool, n_layers: i32, out: *mut *mut air_kv_session) -> c_int;
     pub fn air_kv_session_destroy(s: *mut air_kv_session) -> c_int;
     pub fn air_kv_session_fork(parent: *mut air_kv_session, out: *mut *mut air_kv_session) -> c_int;
@@ -124,6 +128,7 @@ extern "C" {
     pub fn air_kv_session_load(s: *mut air_kv_session, stream: *mut c_void, layer: i32, out_k: *mut c_void, out_v: *mut c_void, out_dtype: i32) -> c_int;
     pub fn air_kv_session_clear(s: *mut air_kv_session) -> c_int;
     pub fn air_kv_session_truncate_to(s: *mut air_kv_session, pos: i64) -> c_int;
+    pub fn air_kv_session_compact(s: *mut air_kv_session, stream: *mut c_void, keep: *const i64, n_keep: i64) -> c_int;
     pub fn air_kv_session_memory_usage(s: *const air_kv_session, bytes: *mut usize) -> c_int;
     pub fn air_kv_block_wire_bytes(pool: *const air_kv_pool, bytes: *mut usize) -> c_int;
     pub fn air_kv_pack_blocks(pool: *mut air_kv_pool, stream: *mut c_void, ids: *const i32, n: i32, out: *mut c_void) -> c_int;
@@ -147,6 +152,7 @@ extern "C" {
     pub fn air_kv_compress_blocks(pool: *mut air_kv_pool, stream: *mut c_void, ids: *const i32, n: i32, key_bits: *mut u64, key_magnitude: *mut f32, key_mean: *mut f32, value_codes: *mut u8, value_scale: *mut f32, value_min: *mut f32) -> c_int;
     pub fn air_kv_qjl_compress_blocks(pool: *mut air_kv_pool, stream: *mut c_void, ids: *const i32, n: i32, proj: *const f32, proj_dim: i32, bits: *mut u64, magnitude: *mut f32) -> c_int;
     pub fn air_kv_copy_blocks(pool: *mut air_kv_pool, stream: *mut c_void, src_blocks: *const i32, dst_blocks: *const i32, n: i32) -> c_int;
+    pub fn air_kv_compact(pool: *mut air_kv_pool, stream: *mut c_void, block_tables: *const i32, seq_lens: *const i32, batch: i32, max_blocks: i32, keep: *const i32, cu_keep: *const i32, total_keep: i32) -> c_int;
     pub fn air_kv_read_blocks(pool: *mut air_kv_pool, stream: *mut c_void, ids: *const i32, n: i32, host_dst: *mut c_void) -> c_int;
     pub fn air_kv_write_blocks(pool: *mut air_kv_pool, stream: *mut c_void, ids: *const i32, n: i32, host_src: *const c_void) -> c_int;
     pub fn air_kv_pool_read_cb(ctx: *mut c_void, block: u32, dst: *mut u8, bytes: usize) -> c_int;

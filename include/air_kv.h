@@ -379,6 +379,60 @@ int air_paged_prefill_workspace_size(const air_kv_pool *pool, int32_t n_q_heads,
                                      int32_t max_q_len, size_t *bytes);
 
 /* ------------------------------------------------------------------------ */
+/* Differential attention over pages                                         */
+/* ------------------------------------------------------------------------ */
+
+/* No counterpart in the reference.  Attention by the difference of two softmax
+ * maps: K/V heads 2p and 2p + 1 of the pool are pair p (n_kv_heads even), query
+ * heads 2h and 2h + 1 are query pair h, which reads K/V pair h / group (group =
+ * n_q_heads / n_kv_heads) with both of its value heads side by side:
+ *   s_m = scale * q[2h + m] . K[2p + m]^T,  P_m = softmax(s_m)      m = 0, 1
+ *   x   = (P_0 - lambda P_1) . [V[2p] | V[2p + 1]]         (2 * head_dim values)
+ *   out[h] = out_scale * x                                 (norm_eps == 0)
+ *          = out_scale * x / sqrt(mean(x^2) + norm_eps) * norm_weight
+ * air_kv_append fills such a pool as any other: values of [n_kv_heads / 2]
+ * [2 * head_dim] per token lie in memory as [n_kv_heads][head_dim].
+ *
+ * lambda is f32 on the device: one per query pair ([n_q_heads / 2]) or, with
+ * lambda_per_row, one per row and query pair ([rows][n_q_heads / 2]).
+ * norm_weight is f32 [2 * head_dim] on the device, or NULL for ones; norm_eps is
+ * 0 (no norm, norm_weight NULL) or finite and > 0.  q is [rows][n_q_heads]
+ * [head_dim] as q_dtype, out [rows][n_q_heads / 2][2 * head_dim] as out_dtype
+ * (AIR_KV_F32 or AIR_KV_BF16), both 16-byte aligned.  head_dim is 32, 64, 96 or
+ * 128.  Scores, sums and the norm are held in 32 bits.
+ *
+ * Decode: one new token per sequence (already appended) over its seq_lens[b]
+ * cached tokens, with the work division, max_splits, workspace rules and error
+ * counting of air_paged_decode.  Queries, keys, probabilities and values keep
+ * f32 precision on every pool.  A sequence of length 0 produces zeros. */
+int air_paged_diff_decode_workspace_size(const air_kv_pool *pool, int32_t n_q_heads, int32_t batch,
+                                         int32_t max_blocks, int32_t max_splits, size_t *bytes);
+int air_paged_diff_decode(air_kv_pool *pool, void *stream, const void *q, int32_t q_dtype,
+                          int32_t n_q_heads, const float *lambda, int32_t lambda_per_row,
+                          const int32_t *block_tables, const int32_t *seq_lens, int32_t batch,
+                          int32_t max_blocks, float scale, int32_t max_splits,
+                          const float *norm_weight, float norm_eps, float out_scale, void *workspace,
+                          size_t ws_bytes, void *out, int32_t out_dtype);
+/* Prefill: sequence b's q_len = cu_q[b + 1] - cu_q[b] newest tokens (already
+ * appended), causal, with the arguments, refusals and error counting of
+ * air_paged_prefill: rows of a sequence that is refused are zero-filled,
+ * out-of-pool table entries are read as zero keys and values.  max_q_len is a
+ * hint (an upper bound of the q_len values).  Keys and values that are not finite
+ * reach only the rows that see them.  The workspace (16-byte aligned, of at least
+ * air_paged_diff_prefill_workspace_size bytes, no initialisation needed) holds
+ * the parts of blocks of rows that several workgroups share; calls that share
+ * one must be ordered (same stream). */
+int air_paged_diff_prefill_workspace_size(const air_kv_pool *pool, int32_t n_q_heads, int32_t batch,
+                                          int32_t max_q_len, size_t *bytes);
+int air_paged_diff_prefill(air_kv_pool *pool, void *stream, const void *q, int32_t q_dtype,
+                           int32_t n_q_heads, const float *lambda, int32_t lambda_per_row,
+                           const int32_t *cu_q, int32_t total_q, int32_t max_q_len,
+                           const int32_t *block_tables, const int32_t *seq_lens, int32_t batch,
+                           int32_t max_blocks, float scale, const float *norm_weight, float norm_eps,
+                           float out_scale, void *workspace, size_t ws_bytes, void *out,
+                           int32_t out_dtype);
+
+/* ------------------------------------------------------------------------ */
 /* SessionKvCache over pages                                                 */
 /* ------------------------------------------------------------------------ */
 
@@ -422,6 +476,13 @@ int air_kv_session_clear(air_kv_session *s);
 /* truncate_to(pos) (:445, src/kv_cache.rs:364-383): every layer keeps at most
  * pos tokens; blocks past them are released.  No device work. */
 int air_kv_session_truncate_to(air_kv_session *s, int64_t pos);
+/* No counterpart in the reference: keeps the tokens at positions keep[0 .. n_keep)
+ * (host memory, ascending, below the length, which every layer must share) in
+ * every layer, as tokens 0 .. n_keep - 1, by air_kv_compact; blocks that another
+ * sequence shares and that would be written are copied first, and the blocks past
+ * the kept tokens are released.  Keys keep the rotation they were appended with.
+ * An error before the first layer's rows move leaves the session as it was. */
+int air_kv_session_compact(air_kv_session *s, void *stream, const int64_t *keep, int64_t n_keep);
 /* Bytes of device memory the session's blocks occupy over all its layers
  * (the paged form of memory_usage, src/kv_cache.rs:388-414). */
 int air_kv_session_memory_usage(const air_kv_session *s, size_t *bytes);
@@ -551,6 +612,23 @@ int air_kv_qjl_compress_blocks(air_kv_pool *pool, void *stream, const int32_t *i
  * BlockAllocator::cow_write leaves to "a real impl" (src/paged_attention.rs:160). */
 int air_kv_copy_blocks(air_kv_pool *pool, void *stream, const int32_t *src_blocks,
                        const int32_t *dst_blocks, int32_t n);
+
+/* Compaction of sequences inside their own pages (no counterpart in the
+ * reference): sequence b keeps its tokens at positions keep[cu_keep[b] ..
+ * cu_keep[b + 1]) (int32, device, ascending), and they move, K, V and scales bit
+ * for bit, to its positions 0, 1, ...; rows behind them stay as they were.  The
+ * caller then shortens the sequence (air_seq_truncate frees the blocks past the
+ * kept tokens).  block_tables and seq_lens are air_paged_decode's; cu_keep is
+ * int32 [batch + 1] (device) over total_keep positions.  No other sequence may hold a
+ * block that is written (copy-on-write first), nor may one sequence be listed
+ * twice.  A position that does not lie above the one before it or not below the
+ * sequence's length, and one whose block, or whose destination's, is outside the
+ * pool, is skipped and counted (air_kv_pool_error_count); so are seq_lens outside
+ * [0, max_blocks * block_size] (clamped) and sequences whose range does not lie in
+ * [0, total_keep] (left alone). */
+int air_kv_compact(air_kv_pool *pool, void *stream, const int32_t *block_tables,
+                   const int32_t *seq_lens, int32_t batch, int32_t max_blocks, const int32_t *keep,
+                   const int32_t *cu_keep, int32_t total_keep);
 
 /* Page-granular device<->host copies for swap (the gpu_read / gpu_write
  * closures of src/kv_swap.rs:55-98).  ids are host int32; host buffers hold
