@@ -72,12 +72,13 @@ struct Plan {
     size_t bytes(int d) const { return align256(cells * sizeof(int4)) + align256(halves * 2 * 4) + halves * 2 * d * 4; }
 };
 
-Plan plan_for(const air_kv_pool &p) {
+// half: 16-bit products (diff_prefill_16.hip), else f32 ones
+Plan plan_for(const air_kv_pool &p, bool half) {
     Plan pl;
-    const int kv_pairs = p.desc.n_kv_heads / 2;
-    pl.rows = 64;
-    pl.slices = std::max(1, (2 * p.cus + kv_pairs - 1) / kv_pairs);
-    pl.least = 8;
+    const int kv_pairs = p.desc.n_kv_heads / 2, per_cu = half ? 1 : 2;
+    pl.rows = half ? 128 : 64;
+    pl.slices = std::max(1, (per_cu * p.cus + kv_pairs - 1) / kv_pairs);
+    pl.least = half ? 16 : 8;
     pl.cells = (size_t)kv_pairs * pl.slices;
     pl.halves = 2 * pl.cells * pl.rows * 2;
     return pl;
@@ -85,12 +86,15 @@ Plan plan_for(const air_kv_pool &p) {
 
 }  // namespace
 
-size_t diff_prefill_workspace(const air_kv_pool &p) { return plan_for(p).bytes(p.desc.head_dim); }
+size_t diff_prefill_workspace(const air_kv_pool &p) {
+    return std::max(plan_for(p, false).bytes(p.desc.head_dim), plan_for(p, true).bytes(p.desc.head_dim));
+}
 
 hipError_t launch_diff_prefill(const air_kv_pool &p, hipStream_t s, const void *q, int32_t q_dtype, int32_t n_q_heads,
                                const int32_t *cu, int32_t total_q, const int32_t *tables, const int32_t *lens,
                                int32_t batch, int32_t max_blocks, float scale, const DiffOut &out, void *workspace) {
-    const Plan plan = plan_for(p);
+    const bool half = p.desc.dtype != AIR_KV_F32 && q_dtype == AIR_KV_BF16 && out.out_dtype == AIR_KV_BF16;
+    const Plan plan = plan_for(p, half);
     const int d = p.desc.head_dim;
     DiffPrefillArgs a{};
     a.q = q;
@@ -126,7 +130,7 @@ hipError_t launch_diff_prefill(const air_kv_pool &p, hipStream_t s, const void *
         a.cu = cu + b0;
         a.tables = tables + (int64_t)b0 * max_blocks;
         a.lens = lens + b0;
-        hipError_t e = launch_diff_prefill_f32(a, d, s);
+        hipError_t e = half ? launch_diff_prefill_16(a, d, s) : launch_diff_prefill_f32(a, d, s);
         if (e == hipSuccess) e = launch_diff_prefill_merge(a, d, s);
         if (e != hipSuccess) return e;
     }

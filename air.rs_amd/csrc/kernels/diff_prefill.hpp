@@ -41,7 +41,7 @@ struct DiffItem {
 // The launch's units before each sequence (s_pre[B] in all) and each sequence's
 // share of errors, in LDS.  A sequence whose rows do not lie in [0, total_q], whose
 // length is outside its table or below its rows, has none; the workgroup of slice b
-// % slices of pair 0 counts it and zeroes its rows.  All 256 threads take part.
+// % slices of pair 0 counts it and zeroes its rows.
 __device__ __forceinline__ bool diff_seq(const DiffPrefillArgs &a, int b, DiffBlocks &s) {
     const int64_t r0 = a.cu[b], r1 = a.cu[b + 1], len = a.lens[b];
     s.g = a.group;
@@ -53,9 +53,11 @@ __device__ __forceinline__ bool diff_seq(const DiffPrefillArgs &a, int b, DiffBl
     return ok;
 }
 
-__device__ __forceinline__ void diff_units(const DiffPrefillArgs &a, int64_t *s_pre, int64_t *s_sum) {
+// All THREADS threads take part.
+template <int THREADS>
+__device__ __forceinline__ void diff_units(const DiffPrefillArgs &a, int64_t *s_pre, int64_t (&s_sum)[THREADS / 64]) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, B = a.batch;
-    const int per = (B + 255) / 256, lo = tid * per, hi = lo + per < B ? lo + per : B;
+    const int per = (B + THREADS - 1) / THREADS, lo = tid * per, hi = lo + per < B ? lo + per : B;
     int64_t mine = 0;
     for (int b = lo; b < hi; ++b) {
         DiffBlocks s;
@@ -133,6 +135,7 @@ hipError_t launch_diff_prefill(const air_kv_pool &p, hipStream_t s, const void *
                                const int32_t *cu, int32_t total_q, const int32_t *tables, const int32_t *lens,
                                int32_t batch, int32_t max_blocks, float scale, const DiffOut &out, void *workspace);
 hipError_t launch_diff_prefill_f32(const DiffPrefillArgs &a, int head_dim, hipStream_t s);
+hipError_t launch_diff_prefill_16(const DiffPrefillArgs &a, int head_dim, hipStream_t s);
 hipError_t launch_diff_prefill_merge(const DiffPrefillArgs &a, int head_dim, hipStream_t s);
 
 }  // namespace airkv

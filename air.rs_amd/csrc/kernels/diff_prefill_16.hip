@@ -1,0 +1,509 @@
+// Differential prefill with 16-bit products (formulas: diff_common.hpp; work
+// division: diff_prefill_plan.hpp): bf16 queries and outputs over bf16 or 1-byte pages.
+//
+// A workgroup's block is 128 rows; eight waves take 32 rows and one of the two maps
+// each (a wave with both maps' sums over the 2 * head_dim value columns would need 512
+// registers).  A wave walks its keys once, 32 at a time, with a running maximum and sum:
+//   S   = K . Q^T      v_mfma_f32_32x32x16, lane (n, h) holds 16 of the 32 keys of row n
+//   O^T += V^T . P^T   the same instruction; its contraction takes the keys in the order
+//                      in which the lanes hold P, so P never moves
+// and the two maps of a row meet when the block ends.  Keys and values are staged in LDS
+// as rows, in two buffers (a tile is loaded two tiles ahead and written one ahead, one
+// barrier a tile), with 16-byte chunks placed so that neither the rows' reads nor the
+// values' transposing reads meet in a bank.
+//
+// The second product takes f16 operands: values (exact when they come from bf16 pages
+// and lie in f16's range, else rounded to 11 bits) and probabilities rounded to 11 bits,
+// an error below the bf16 output's own rounding, where bf16 probabilities would add as
+// much again (measured against 64 bits: 1.7e-3 and 2.6e-3 of the result's norm).  The
+// first product takes bf16 operands as they are from bf16 pages, f16 ones (dequantized,
+// 11 bits) from 1-byte pages.  Powers of two keep f16's operands in its range whatever
+// the values: one per tile for keys, a running one for values (raised as the running
+// maximum is), one per row for queries.
+#include <hip/hip_runtime.h>
+
+#include "../pool.hpp"
+#include "diff_prefill.hpp"
+
+namespace airkv {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef diff_u32x4 u32x4;
+typedef diff_u32x2 u32x2;
+typedef diff_f32x4 f32x4;
+
+template <bool F16> __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Two values rounded to the products' type, x in the low half.
+template <bool F16> __device__ __forceinline__ uint32_t pack2(float x, float y) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), f16x2));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
+}
+
+// 2^(e - exponent of x) for a finite positive normal x, else 1.
+__device__ __forceinline__ float pow2_to(float x, int e) {
+    const int f = (int)((__float_as_uint(x) >> 23) & 0xFF);
+    const int k = 127 + e - (f - 127);
+    return f == 0 || f == 255 || k < 1 || k > 254 ? 1.0f : __uint_as_float((uint32_t)k << 23);
+}
+
+// The largest finite x >= 0 of the wave's lanes (its bits order as integers).
+__device__ __forceinline__ float wave_top(float x) {
+    int v = (int)__float_as_uint(x);
+    v = v >= 0x7F800000 || v < 0 ? 0 : v;
+    v = wave_scan(v, [](int a, int b) { return a > b ? a : b; });
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane(v, 63));
+}
+
+constexpr int kRows = 128;
+constexpr int kThreads16 = 512;
+
+// Where the 16-byte chunk c of row r of a staged head lies, in chunks.  Keys are read
+// 32 rows at a time, a chunk each: 16 rows' chunks c have to lie in 16 different
+// 16-byte columns of the 256 bytes that the banks span.  Values are read eight
+// rows at a time, 64 bytes each: four rows in a row, in different quarters.
+template <int D> __device__ __forceinline__ int key_chunk(int r, int c) {
+    if constexpr (D == 128) return c ^ (r & 15);
+    else if constexpr (D == 64) return c ^ ((r >> 1) & 7);
+    else if constexpr (D == 32) return c ^ ((r >> 2) & 3);
+    else return (c + ((r >> 2) & 3)) % 12;
+}
+template <int D> __device__ __forceinline__ int value_chunk(int r, int c) {
+    if constexpr (D == 128) return c ^ ((r & 3) << 2);
+    else if constexpr (D == 64) return c ^ (((r >> 1) & 1) << 2);
+    else return c;
+}
+
+template <int D, int DT>
+__global__ __launch_bounds__(kThreads16) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void diff_prefill_16_kernel(DiffPrefillArgs a) {
+    constexpr bool QUANT = DT != AIR_KV_BF16;
+    constexpr int EB = QUANT ? 1 : 2;
+    constexpr int RB = 2 * D;                          // bytes of a staged row
+    constexpr int HB = kDiffKeys * RB;                 // of a staged head; keys of both heads, then values
+    constexpr int KS = D / 16, CT = D / 16;            // steps of the first product, 32-column tiles of the second
+    // Staging: a wave's pass covers WR rows of one 16-key half of one head of keys or
+    // values, CP 8-element pieces a row (head_dim 96: 12 of 16 lanes), so its addresses
+    // differ between lanes by a constant only and its bounds are a buffer's.
+    constexpr int CP = D == 96 ? 16 : D / 8, WR = 64 / CP, NP = 4 * kDiffKeys / (8 * WR);
+    __shared__ int64_t s_pre[kDiffPrefillBatch + 1];
+    __shared__ int64_t s_sum[kThreads16 / 64];
+    __shared__ __align__(16) uint8_t s_t[2][4 * HB];
+    __shared__ float s_top[2][2][8];                   // largest key / value scale of a tile, per wave
+    // Values that are not finite, in tiles that not every row sees (a hidden key's
+    // probability of 0 times such a value would be NaN): staged as 0, and each column's
+    // first such key is kept here, from which on a row's column is NaN.
+    __shared__ int s_bad[2 * D];
+    __shared__ int s_any;
+    diff_refused(a, 2 * D);
+    diff_units<kThreads16>(a, s_pre, s_sum);
+    const int tid = threadIdx.x, lane = tid & 63, hf = lane >> 5, r32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rg = wave & 3, mp = wave >> 2;           // 32 rows, one map
+    const int w = blockIdx.x, kp = blockIdx.y, g = a.group;
+    const int64_t units = s_pre[a.batch];
+    const int64_t chunk = diff_prefill_chunk(units, a.slices, a.least);
+    const int64_t cell = (int64_t)kp * a.slices + w;
+    int4 begun = {0, 0, 0, 0};
+
+    // This lane's piece of every pass: row (of its 16-key half) and 16-byte chunk
+    const int nsc = QUANT ? D / a.scale_group : 0;
+    const int p_c = lane % CP, p_row0 = wave * WR;     // the wave's first row of pass 0, of the 128 staged
+    const int p_key = (p_row0 + lane / CP) % kDiffKeys;
+    const bool p_in = D != 96 || p_c < D / 8;
+    const int p_off = p_in ? ((p_key % 16) * D + 8 * p_c) * EB : 0x7FFFFFFF;
+    const int p_sc = p_in && QUANT ? ((p_key % 16) * nsc + 8 * p_c / a.scale_group) * 4 : 0x7FFFFFFF;
+    const int p_klds = p_key * RB + 16 * key_chunk<D>(p_key, p_c), p_vlds = p_key * RB + 16 * value_chunk<D>(p_key, p_c);
+    const int p_half = p_row0 % kDiffKeys / 16;        // of every pass: 8 WR rows are a multiple of 32
+
+    int64_t u = w * chunk;
+    const int64_t end = u + chunk < units ? u + chunk : units;
+    while (u < end) {
+        DiffItem it;
+        diff_find(a, s_pre, u, it);
+        DiffBlocks sq;
+        diff_seq(a, it.b, sq);
+        const int64_t nt = sq.tiles(it.k), len = sq.prefix + sq.q;
+        it.t1 = it.t0 + (end - u) < nt ? it.t0 + (end - u) : nt;
+        it.whole = it.t0 == 0 && it.t1 == nt;
+        const int64_t row0 = a.cu[it.b];
+        const int64_t rows = sq.q * g;
+        // this lane's row: token and query pair (of the last token, if there is none)
+        auto my_row = [&](int r, bool &live, int &tok, int &h) {
+            const int64_t f = it.k * kRows + 32 * rg + r;
+            live = f < rows;
+            tok = (int)(live ? f / g : sq.q - 1);
+            h = kp * g + (live ? (int)(f % g) : 0);
+        };
+        const int64_t f0 = it.k * kRows + 32 * rg, f1 = f0 + 31;
+        // the newest key, counted from the item's first tile: of this row, of the wave's first
+        // and last row, of the block's first, and the sequence's end (32-bit: at most 2^31 keys)
+        const int64_t key0 = it.t0 * kDiffKeys;
+        const int sees0 = (int)(sq.prefix + (f0 < rows ? f0 / g : sq.q - 1) - key0);
+        const int sees1 = (int)(sq.prefix + (f1 < rows ? f1 / g : sq.q - 1) - key0);
+        const int seesb = (int)(sq.prefix + it.k * kRows / g - key0);
+        const int rest = (int)(len - key0), tiles = (int)(it.t1 - it.t0);
+
+        // Q^T as the B operand: lane (n, h) holds elements 16 s + 8 h .. +8 of row n
+        u32x4 qf[KS];
+        float qs = a.scale_log2;
+        int sees;
+        {
+            bool live;
+            int tok, h;
+            my_row(r32, live, tok, h);
+            sees = (int)(sq.prefix + tok - key0);
+            const uint16_t *q = (const uint16_t *)a.q + ((row0 + tok) * 2 * a.pairs + 2 * h + mp) * D + 8 * hf;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4 *>(q + 16 * s);
+        }
+        if constexpr (QUANT) {
+            float top = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    top = fmaxf(top, fmaxf(__builtin_fabsf(__uint_as_float(qf[s][j] << 16)),
+                                           __builtin_fabsf(__uint_as_float(qf[s][j] & 0xFFFF0000u))));
+            const float fq = pow2_to(max_x32(top), 4);          // the row's largest element in [2^4, 2^5)
+            qs = a.scale_log2 / fq;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    qf[s][j] = pack2<true>(__uint_as_float(qf[s][j] << 16) * fq, __uint_as_float(qf[s][j] & 0xFFFF0000u) * fq);
+        }
+        f32x16 acc[CT];
+        float m_run = -INFINITY, l_run = 0.0f;
+        float fv = 0.0f;                               // the values' power of two (0: none yet)
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
+
+        const int32_t *table = a.tables + (int64_t)it.b * a.max_blocks + key0 / a.bs;
+        uint32_t raw[NP][2 * EB];                      // the tile on its way
+        float rsc[NP];
+        // the entry of the half-tile that this wave stages
+        auto entry = [&](int t) -> int32_t {
+            const int key = t * kDiffKeys + 16 * p_half;
+            return t < tiles && key < rest ? table[key / a.bs] : -1;
+        };
+        int32_t next = entry(0);
+        // tile t's loads (block `next`), then the entry of the next
+        auto load_tile = [&](int t) {
+            const bool ok = next >= 0 && next < a.num_blocks;
+            int left = rest - t * kDiffKeys - 16 * p_half;
+            // entries outside the pool, once per block of tokens
+            if (!ok && left > 0 && kp == 0 && p_row0 % 16 == 0 && p_row0 < kDiffKeys && (p_half == 0 || a.bs == 16) && lane == 0)
+                atomicAdd(a.errors, 1ull);
+            left = !ok || left < 0 ? 0 : left < 16 ? left : 16;
+            const int64_t row = ((int64_t)(ok ? next : 0) * a.heads + 2 * kp) * a.bs + (t * kDiffKeys + 16 * p_half) % a.bs;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int part = (p_row0 + 8 * WR * i) / kDiffKeys;          // keys of head 0, 1, values of head 0, 1
+                const int64_t at = row + (part & 1) * a.bs;
+                const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+                    (void *)((const uint8_t *)(part < 2 ? a.k_pages : a.v_pages) + at * (D * EB)), (short)0, left * D * EB, kDiffBufferWord3);
+                if constexpr (QUANT) {
+                    const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, p_off, 0, 0);
+                    raw[i][0] = x[0]; raw[i][1] = x[1];
+                    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+                        (void *)((part < 2 ? a.k_scales : a.v_scales) + at * nsc), (short)0, left * nsc * 4, kDiffBufferWord3);
+                    rsc[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, p_sc, 0, 0));
+                } else {
+                    const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, p_off, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) raw[i][j] = x[j];
+                }
+            }
+            next = entry(t + 1);
+        };
+        // the largest scales (keys', values') or values of the tile in registers, for all waves (before a barrier)
+        auto tops = [&](int t) {
+            float k = 0.0f, v = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const bool val = (p_row0 + 8 * WR * i) / kDiffKeys >= 2;
+                if constexpr (QUANT) {
+                    const float y = __builtin_fabsf(rsc[i]), x = y < INFINITY ? y : 0.0f;
+                    if (val) v = fmaxf(v, x);
+                    else k = fmaxf(k, x);
+                } else if (val) {
+                    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+                    u16x2 top = {0, 0};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, raw[i][j] & 0x7FFF7FFFu));
+                    uint32_t b = top[0] > top[1] ? top[0] : top[1];
+                    if (b >= 0x7F80u) {                // the largest finite one
+                        b = 0;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t x = raw[i][j / 2] >> (16 * (j & 1)) & 0x7FFFu;
+                            b = x < 0x7F80u && x > b ? x : b;
+                        }
+                    }
+                    v = fmaxf(v, __uint_as_float(b << 16));
+                }
+            }
+            if constexpr (QUANT) k = wave_top(k);
+            v = wave_top(v);
+            if (lane == 0) {
+                s_top[t & 1][0][wave] = k;
+                s_top[t & 1][1][wave] = v;
+            }
+        };
+        float fk = 1.0f, fk_next = 1.0f;               // the keys' power of two, of the present tile and the next
+        float fv_now = 0.0f;                           // the values', of the present tile
+        // the tile in registers into its buffer (after the barrier behind tops)
+        auto write_tile = [&](int t) {
+            float kt = 0.0f, vt = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                kt = fmaxf(kt, s_top[t & 1][0][i]);
+                vt = fmaxf(vt, s_top[t & 1][1][i]);
+            }
+            if constexpr (QUANT) {
+                fk_next = pow2_to(kt, 5);              // codes are below 2^9: products below 2^15
+                if (vt > 0.0f && (fv == 0.0f || vt * fv >= 64.0f)) fv = pow2_to(vt, 3);
+            } else if (vt > 0.0f && (fv == 0.0f || vt * fv >= 32768.0f)) {
+                fv = vt >= 0.125f && vt < 1024.0f ? 1.0f : pow2_to(vt, 8);
+            }
+            const float mulv = fv == 0.0f ? 1.0f : fv;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int part = (p_row0 + 8 * WR * i) / kDiffKeys;
+                const bool val = part >= 2;
+                u32x4 x;
+                if constexpr (QUANT) {
+                    const float s = rsc[i] * (val ? mulv : fk_next);
+                    const f32x4 lo = code_values<DT>(raw[i][0], s), hi = code_values<DT>(raw[i][1], s);
+                    x = u32x4{pack2<true>(lo[0], lo[1]), pack2<true>(lo[2], lo[3]), pack2<true>(hi[0], hi[1]), pack2<true>(hi[2], hi[3])};
+                } else {
+                    x = u32x4{raw[i][0], raw[i][1], raw[i][2], raw[i][3]};
+                    if (val) {
+                        if (mulv == 1.0f) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                x[j] = pack2<true>(__uint_as_float(x[j] << 16), __uint_as_float(x[j] & 0xFFFF0000u));
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                x[j] = pack2<true>(__uint_as_float(x[j] << 16) * mulv, __uint_as_float(x[j] & 0xFFFF0000u) * mulv);
+                        }
+                    }
+                }
+                if (val && t * kDiffKeys + kDiffKeys - 1 > seesb && p_in) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int sh = 16 * (j & 1);
+                        if ((x[j / 2] >> sh & 0x7C00u) != 0x7C00u) continue;
+                        x[j / 2] &= ~(0xFFFFu << sh);
+                        s_any = 1;
+                        atomicMin(&s_bad[(part & 1) * D + 8 * p_c + j], t * kDiffKeys + p_key);
+                    }
+                }
+                if (p_in) *reinterpret_cast<u32x4 *>(s_t[t & 1] + part * HB + (val ? p_vlds : p_klds)) = x;
+            }
+        };
+
+        // tile 0 in its buffer, tile 1 on its way
+        load_tile(0);
+        tops(0);
+        __syncthreads();                               // the buffers of the item before are free
+        if (tid < 2 * D) s_bad[tid] = INT32_MAX;
+        if (tid == 0) s_any = 0;
+        __syncthreads();
+        write_tile(0);
+        if (1 < tiles) load_tile(1);
+        for (int t = 0; t < tiles; ++t) {
+            if (t + 1 < tiles) tops(t + 1);
+            fk = fk_next;
+            if (fv_now != fv) {                        // the values' power of two was changed for this tile: the sums follow
+                if (fv_now != 0.0f) {
+                    const float k = fv / fv_now;
+#pragma unroll
+                    for (int c = 0; c < CT; ++c) acc[c] *= k;
+                }
+                fv_now = fv;
+            }
+            __syncthreads();                           // tile t is written, tile t - 1 used
+            if (t + 1 < tiles) write_tile(t + 1);
+            if (t + 2 < tiles) load_tile(t + 2);
+            if (t * kDiffKeys > sees1) continue;       // no row of this wave sees any of it
+            const float ft = qs / fk;
+            const uint8_t *sk = s_t[t & 1] + mp * HB + r32 * RB, *sv = s_t[t & 1] + 2 * HB;
+            f32x16 sc;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+                sc = mfma<QUANT>(*reinterpret_cast<const u32x4 *>(sk + 16 * key_chunk<D>(r32, 2 * s + hf)), qf[s], sc);
+            const bool cut = t * kDiffKeys + kDiffKeys - 1 > sees0;
+            if (cut) {
+                const int lim = sees - t * kDiffKeys;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sc[i] = 8 * (i / 4) + 4 * hf + i % 4 <= lim ? sc[i] : -INFINITY;
+            }
+            float top = sc[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
+            top = max_x32(top) * ft;
+            // raised only past 2^8 times the present maximum (and on the first tile)
+            if (__ballot(top > m_run + 8.0f) != 0ull) {
+                const float now = fmaxf(m_run, top);
+                const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - now);
+                l_run *= alpha;
+#pragma unroll
+                for (int c = 0; c < CT; ++c) acc[c] *= alpha;
+                m_run = now;
+            }
+            const float base = m_run == -INFINITY ? 0.0f : m_run;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], ft, -base));
+                l_run += sc[i];
+            }
+            u32x4 p[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p[s][j] = pack2<true>(sc[8 * s + 2 * j], sc[8 * s + 2 * j + 1]);
+            // V^T as the A operand: lane (m, h) takes keys 16 s + 8 b + 4 h .. +4 of column m, b = 0, 1.
+            // Within each 16-lane group, lane j of a transposing read receives element j % 4 of the 8
+            // bytes that lanes 4 k + j / 4 address, k = 0 .. 3: lane i points at key i / 4 of the four
+            // and columns 4 (i % 4) of the group's sixteen.
+            const int vr = 4 * hf + ((lane & 15) >> 2);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                const int hd = c / (D / 32), cl = c % (D / 32);
+                const int vc = 4 * cl + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+                const uint8_t *v = sv + hd * HB + vr * RB + 16 * value_chunk<D>(vr, vc) + 8 * (lane & 1);
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    typedef short s16x4 __attribute__((ext_vector_type(4)));
+                    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                        (__attribute__((address_space(3))) s16x4 *)(v + 16 * s * RB)));
+                    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                        (__attribute__((address_space(3))) s16x4 *)(v + (16 * s + 8) * RB)));
+                    acc[c] = mfma<true>(u32x4{x[0], x[1], y[0], y[1]}, p[s], acc[c]);
+                }
+            }
+        }
+
+        // lane (n, h): columns 32 c + 8 (i / 4) + 4 h + i % 4 of row n in acc[c][i]
+        const float l = sum_x32(l_run);
+        // the row again (its place in the output is not kept in registers through the tiles)
+        bool live;
+        int tok, h, r_end = r32;
+        asm volatile("" : "+v"(r_end));
+        my_row(r_end, live, tok, h);
+        __syncthreads();
+        if (s_any) {
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (s_bad[32 * c + 8 * (i / 4) + 4 * hf + i % 4] <= sees) acc[c][i] = __builtin_nanf("");
+        }
+        const float back = fv_now != 0.0f ? 1.0f / fv_now : 1.0f;
+        if (it.whole) {
+            // map 1's rows go to map 0's waves through the buffers, half of the columns at a time
+            const float lam = a.e.lam[(row0 + tok) * a.e.lam_stride + h];
+            const float inv = back * (mp ? -lam : 1.0f) / l;
+            constexpr int CR = CT / 2;
+            static_assert(4 * CR * 4 * 64 * sizeof(f32x4) <= sizeof(s_t), "the exchanged columns fit the buffers");
+            float ss = 0.0f;
+#pragma unroll
+            for (int c = 0; c < CT; ++c) acc[c] *= inv;
+#pragma unroll
+            for (int c0 = 0; c0 < CT; c0 += CR) {
+                f32x4 *x = reinterpret_cast<f32x4 *>(&s_t[0][0]) + rg * CR * 4 * 64 + lane;
+                __syncthreads();
+                if (mp) {
+#pragma unroll
+                    for (int c = c0; c < c0 + CR && c < CT; ++c)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            x[((c - c0) * 4 + i) * 64] = f32x4{acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]};
+                }
+                __syncthreads();
+                if (!mp) {
+#pragma unroll
+                    for (int c = c0; c < c0 + CR && c < CT; ++c)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const f32x4 y = x[((c - c0) * 4 + i) * 64];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                acc[c][4 * i + j] += y[j];
+                                ss += acc[c][4 * i + j] * acc[c][4 * i + j];
+                            }
+                        }
+                }
+            }
+            if (!mp && live) {
+                const float k = diff_factor(a.e, a.e.norm ? sum_x32(ss) : 0.0f, 2 * D);
+                const int64_t at = ((row0 + tok) * a.pairs + h) * (2 * D);
+#pragma unroll
+                for (int c = 0; c < CT; ++c)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const int col = 32 * c + 2 * i + 4 * hf;
+                        f32x4 x;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) x[j] = acc[c][i + j] * ((a.e.norm && a.e.norm_w) ? k * a.e.norm_w[col + j] : k);
+                        diff_store4(a.e, at + col, x);
+                    }
+            }
+        } else {
+            const int64_t slot = 2 * cell + (it.t0 == 0 ? 1 : 0);
+            const int64_t r = (slot * kRows + 32 * rg + r32) * 2 + mp;
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<f32x4 *>(a.part_o + r * (2 * D) + 32 * c + 2 * i + 4 * hf) =
+                        f32x4{acc[c][i] * back, acc[c][i + 1] * back, acc[c][i + 2] * back, acc[c][i + 3] * back};
+            if (hf == 0) {
+                a.part_ml[2 * r] = m_run;
+                a.part_ml[2 * r + 1] = l;
+            }
+            if (it.t0 == 0) {                          // begun here: its last unit's slice ends it
+                const int64_t last = u + nt - 1;
+                begun = int4{it.b, (int)(uint32_t)it.k, (int)(it.k >> 32), (int)(last / chunk - w + 1)};
+            }
+        }
+        u += it.t1 - it.t0;
+    }
+    if (tid == 0) a.desc[cell] = begun;
+}
+
+template <int D>
+hipError_t launch_d(const DiffPrefillArgs &a, hipStream_t s) {
+    const dim3 grid((unsigned)a.slices, (unsigned)a.kv_pairs);
+    if (a.dtype == AIR_KV_BF16) hipLaunchKernelGGL((diff_prefill_16_kernel<D, AIR_KV_BF16>), grid, dim3(kThreads16), 0, s, a);
+    else if (a.dtype == AIR_KV_INT8) hipLaunchKernelGGL((diff_prefill_16_kernel<D, AIR_KV_INT8>), grid, dim3(kThreads16), 0, s, a);
+    else hipLaunchKernelGGL((diff_prefill_16_kernel<D, AIR_KV_FP8>), grid, dim3(kThreads16), 0, s, a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_diff_prefill_16(const DiffPrefillArgs &a, int head_dim, hipStream_t s) {
+    return head_dim == 128 ? launch_d<128>(a, s) : head_dim == 96 ? launch_d<96>(a, s) : head_dim == 64 ? launch_d<64>(a, s) : launch_d<32>(a, s);
+}
+
+}  // namespace airkv

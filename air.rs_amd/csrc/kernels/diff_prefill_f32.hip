@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __shared__ int64_t s_bad;                          // the latest tile with a value that is not finite
     if (threadIdx.x == 0) s_bad = -1;
     diff_refused(a, 2 * D);
-    diff_units(a, s_pre, s_sum);
+    diff_units<256>(a, s_pre, s_sum);
     const int tid = threadIdx.x, lane = tid & 63, q4 = lane >> 4, r16 = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int w = blockIdx.x, kp = blockIdx.y, g = a.group;

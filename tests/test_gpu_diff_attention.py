@@ -139,8 +139,21 @@ def _prefill(c, qlens, group, q_f32, out_f32, norm, lam_rows, out_scale=0.75, ws
 
 # (cached, of them new) of each sequence
 CHUNKS = [(1, 1), (40, 33), (0, 0), (300, 17), (128, 128), (65, 64), (700, 1), (33, 32), (90, 0), (257, 250)]
-# probabilities enter the 16-bit products rounded to bf16
-P_STEP = 2.0 ** -8
+
+
+def _p_step(c):
+    """What the 16-bit products add to a probability's relative error: the probability
+    and the value (of 1-byte pages) are rounded to 11 bits, and so are the keys of
+    1-byte pages, whose scores err by 2^-11 sum |q k| scale (taken at 8 standard
+    deviations of normal rows: sum |q k| / sqrt(d) <= 2/pi sqrt(d) + 8), which moves a
+    probability by twice that (its own score, and the sum's).  Below f16's normal
+    numbers, 2^-14, a probability errs by 2^-25 of the largest."""
+    if c.pool.dtype == airkv.F32:
+        return 0.0
+    tiny = 2.0 ** -25 * c.lens.max(initial=1)
+    if c.pool.dtype == airkv.BF16:
+        return 2.0 ** -11 + tiny
+    return 2.0 ** -11 * (2 + 2 * (0.64 * c.d ** 0.5 + 8)) + tiny
 
 
 @pytest.mark.parametrize("d,kv,group,bs,scale_group", [(64, 8, 1, 16, 32), (128, 4, 4, 16, 32), (128, 2, 8, 32, 32), (32, 2, 3, 16, 8),
@@ -148,15 +161,17 @@ P_STEP = 2.0 ** -8
 @pytest.mark.parametrize("dtype", [airkv.F32, airkv.BF16, airkv.INT8, airkv.FP8])
 def test_diff_prefill(dtype, d, kv, group, bs, scale_group):
     for i, (q_f32, out_f32, norm, lam_rows) in enumerate([(True, True, True, False), (False, True, False, True),
-                                                          (True, False, True, False)]):
+                                                          (True, False, True, False), (False, False, True, True)]):
         c = Cache(dtype, d, kv, bs, [n for n, _ in CHUNKS], seed=d + group + i, scale_group=scale_group)
-        used = _prefill(c, [m for _, m in CHUNKS], group, q_f32, out_f32, norm, lam_rows)
+        used = _prefill(c, [m for _, m in CHUNKS], group, q_f32, out_f32, norm, lam_rows,
+                        p_step=0.0 if q_f32 or out_f32 else _p_step(c))
         log(f"diff prefill {NAMES[dtype]} d={d} group={group} q_f32={q_f32} out_f32={out_f32}: {used:.3f} of the bound")
 
 
 @pytest.mark.parametrize("chunks", [[(1, 1)], [(3000, 3000)], [(9000, 5)], [(2500, 700), (1, 1)], [(3, 3)] * 40, [(20, 2)] * 1030])
 def test_diff_prefill_shapes(chunks):
-    for dtype, d, group, f32 in ((airkv.BF16, 64, 2, True), (airkv.F32, 32, 1, True)):
+    for dtype, d, group, f32 in ((airkv.BF16, 64, 2, True), (airkv.F32, 32, 1, True), (airkv.BF16, 128, 3, False),
+                                 (airkv.INT8, 64, 1, False)):
         c = Cache(dtype, d, 2, 16, [n for n, _ in chunks], seed=len(chunks) + d)
-        used = _prefill(c, [m for _, m in chunks], group, f32, f32, True, True)
+        used = _prefill(c, [m for _, m in chunks], group, f32, f32, True, True, p_step=0.0 if f32 else _p_step(c))
         log(f"diff prefill {len(chunks)} x {chunks[0]} {NAMES[dtype]}: {used:.3f} of the bound")
