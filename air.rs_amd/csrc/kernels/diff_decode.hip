@@ -328,7 +328,7 @@ void diff_decode_kernel(DiffDecodeArgs a) {
         mt = max_x32(max_x16(mt));
         // raised only past 2^8 times the present maximum (and on the first tile): most tiles skip the rescale
         if (__ballot(mt > m_run + 8.0f) != 0ull) {
-            const float top = fmaxf(m_run, mt);
+            const float top = mt > m_run + 8.0f ? mt : m_run;
             const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - top);
             l_run *= alpha;
 #pragma unroll

@@ -34,8 +34,8 @@ struct DiffPrefillArgs {
 // What a row of the work list needs, for the workgroup's present block.
 struct DiffItem {
     int32_t b;
-    int64_t k, t0, t1;             // block, its tiles [t0, t1)
-    bool whole;
+    int64_t k;                     // block
+    int64_t from;                  // of its units, the first
 };
 
 // The launch's units before each sequence (s_pre[B] in all) and each sequence's
@@ -84,7 +84,7 @@ __device__ __forceinline__ void diff_units(const DiffPrefillArgs &a, int64_t *s_
     __syncthreads();
 }
 
-// The block and tile of unit u (below s_pre[B]); the wave's lanes probe 64 blocks
+// The block of unit u (below s_pre[B]) and its place there; the wave's lanes probe 64 blocks
 // at a time.  Every wave finds the same.
 __device__ __forceinline__ void diff_find(const DiffPrefillArgs &a, const int64_t *s_pre, int64_t u, DiffItem &it) {
     int lo = 0, hi = a.batch;
@@ -109,7 +109,16 @@ __device__ __forceinline__ void diff_find(const DiffPrefillArgs &a, const int64_
     }
     it.b = lo;
     it.k = k0;
-    it.t0 = at - s.before(k0);
+    it.from = at - s.before(k0);
+}
+
+// The block after: of the same sequence, or the first of the next that has one.
+__device__ __forceinline__ void diff_next(const DiffPrefillArgs &a, const int64_t *s_pre, const DiffBlocks &s, DiffItem &it) {
+    it.from = 0;
+    if (++it.k < s.blocks()) return;
+    it.k = 0;
+    do ++it.b;
+    while (it.b < a.batch && s_pre[it.b + 1] == s_pre[it.b]);
 }
 
 // Sequences that are refused: counted, and their rows (those there are) zeroed.

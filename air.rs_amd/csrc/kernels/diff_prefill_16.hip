@@ -42,6 +42,12 @@ template <bool F16> __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+__device__ __forceinline__ uint32_t bf16_pair(float x, float y) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
+}
+
 // Two values rounded to the products' type, x in the low half.
 template <bool F16> __device__ __forceinline__ uint32_t pack2(float x, float y) {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -56,14 +62,6 @@ __device__ __forceinline__ float pow2_to(float x, int e) {
     const int f = (int)((__float_as_uint(x) >> 23) & 0xFF);
     const int k = 127 + e - (f - 127);
     return f == 0 || f == 255 || k < 1 || k > 254 ? 1.0f : __uint_as_float((uint32_t)k << 23);
-}
-
-// The largest finite x >= 0 of the wave's lanes (its bits order as integers).
-__device__ __forceinline__ float wave_top(float x) {
-    int v = (int)__float_as_uint(x);
-    v = v >= 0x7F800000 || v < 0 ? 0 : v;
-    v = wave_scan(v, [](int a, int b) { return a > b ? a : b; });
-    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane(v, 63));
 }
 
 constexpr int kRows = 128;
@@ -99,13 +97,21 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
     constexpr int CP = D == 96 ? 16 : D / 8, WR = 64 / CP, NP = 4 * kDiffKeys / (8 * WR);
     __shared__ int64_t s_pre[kDiffPrefillBatch + 1];
     __shared__ int64_t s_sum[kThreads16 / 64];
-    __shared__ __align__(16) uint8_t s_t[2][4 * HB];
-    __shared__ float s_top[2][2][8];                   // largest key / value scale of a tile, per wave
+    // the two buffers; in them, at a block's end, CR column tiles of every wave's half
+    constexpr int CH = CT / 2, CR = D == 128 ? 2 : 1, XB = 8 * CR * 4 * 64 * 16;
+    __shared__ __align__(16) uint8_t s_mem[8 * HB > XB ? 8 * HB : XB];
+    auto s_t = [&](int t) { return s_mem + (t & 1) * 4 * HB; };
+    // Per tile (mod 3), keys' scale and values' (scale): the bits of the largest of those that
+    // leave f16's range under the present power of two (of all in a block's first tile)
+    __shared__ uint32_t s_top[3][2];
+    __shared__ __align__(16) float s_w[2 * D];         // the norm's weights
+    __shared__ float s_ss[2][4][32];                   // the halves' sums of squares
     // Values that are not finite, in tiles that not every row sees (a hidden key's
     // probability of 0 times such a value would be NaN): staged as 0, and each column's
     // first such key is kept here, from which on a row's column is NaN.
     __shared__ int s_bad[2 * D];
     __shared__ int s_any;
+    if (threadIdx.x < 2 * D) s_w[threadIdx.x] = a.e.norm && a.e.norm_w ? a.e.norm_w[threadIdx.x] : 1.0f;
     diff_refused(a, 2 * D);
     diff_units<kThreads16>(a, s_pre, s_sum);
     const int tid = threadIdx.x, lane = tid & 63, hf = lane >> 5, r32 = lane & 31;
@@ -127,16 +133,25 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
     const int p_klds = p_key * RB + 16 * key_chunk<D>(p_key, p_c), p_vlds = p_key * RB + 16 * value_chunk<D>(p_key, p_c);
     const int p_half = p_row0 % kDiffKeys / 16;        // of every pass: 8 WR rows are a multiple of 32
 
+    // The powers of two under which keys and values are staged, kept from block to block.
+    // The largest scale (a 2^9th of a value), or value, under it: below f16's largest; at
+    // least where values 2^-11 of it keep their bits; and where a new one puts it.
+    constexpr float kMost = QUANT ? 64.0f : 32768.0f, kLeast = QUANT ? 0.5f : 0.125f;
+    constexpr int kAim = QUANT ? 3 : 8;
+    float fk = 1.0f, fv = 1.0f;
     int64_t u = w * chunk;
     const int64_t end = u + chunk < units ? u + chunk : units;
-    while (u < end) {
-        DiffItem it;
-        diff_find(a, s_pre, u, it);
-        DiffBlocks sq;
+    DiffItem it;
+    DiffBlocks sq;
+    if (u < end) diff_find(a, s_pre, u, it);
+    for (; u < end; diff_next(a, s_pre, sq, it)) {
         diff_seq(a, it.b, sq);
         const int64_t nt = sq.tiles(it.k), len = sq.prefix + sq.q;
-        it.t1 = it.t0 + (end - u) < nt ? it.t0 + (end - u) : nt;
-        it.whole = it.t0 == 0 && it.t1 == nt;
+        const int64_t left = nt + kDiffBlockCost - it.from, mine = end - u < left ? end - u : left;
+        const int64_t t0 = diff_tile_of(it.from), t1 = diff_tile_of(it.from + mine);
+        u += mine;
+        if (t0 == t1) continue;                        // the slice ends before the block's first tile
+        const bool whole = t0 == 0 && t1 == nt;
         const int64_t row0 = a.cu[it.b];
         const int64_t rows = sq.q * g;
         // this lane's row: token and query pair (of the last token, if there is none)
@@ -149,11 +164,11 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
         const int64_t f0 = it.k * kRows + 32 * rg, f1 = f0 + 31;
         // the newest key, counted from the item's first tile: of this row, of the wave's first
         // and last row, of the block's first, and the sequence's end (32-bit: at most 2^31 keys)
-        const int64_t key0 = it.t0 * kDiffKeys;
+        const int64_t key0 = t0 * kDiffKeys;
         const int sees0 = (int)(sq.prefix + (f0 < rows ? f0 / g : sq.q - 1) - key0);
         const int sees1 = (int)(sq.prefix + (f1 < rows ? f1 / g : sq.q - 1) - key0);
         const int seesb = (int)(sq.prefix + it.k * kRows / g - key0);
-        const int rest = (int)(len - key0), tiles = (int)(it.t1 - it.t0);
+        const int rest = (int)(len - key0), tiles = (int)(t1 - t0);
 
         // Q^T as the B operand: lane (n, h) holds elements 16 s + 8 h .. +8 of row n
         u32x4 qf[KS];
@@ -186,7 +201,7 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
         }
         f32x16 acc[CT];
         float m_run = -INFINITY, l_run = 0.0f;
-        float fv = 0.0f;                               // the values' power of two (0: none yet)
+        float owed = 1.0f;                             // what the sums have to be multiplied by to be under fv
 #pragma unroll
         for (int c = 0; c < CT; ++c)
 #pragma unroll
@@ -230,16 +245,17 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
             }
             next = entry(t + 1);
         };
-        // the largest scales (keys', values') or values of the tile in registers, for all waves (before a barrier)
-        auto tops = [&](int t) {
-            float k = 0.0f, v = 0.0f;
+        // Scales and values of the tile in registers that leave f16's range are marked for all
+        // waves; behind the barrier the tile is staged again under another power of two.
+        auto mark = [&](int t) {
+            uint32_t k = 0, v = 0;                     // this lane's largest finite ones, as bits
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const bool val = (p_row0 + 8 * WR * i) / kDiffKeys >= 2;
                 if constexpr (QUANT) {
-                    const float y = __builtin_fabsf(rsc[i]), x = y < INFINITY ? y : 0.0f;
-                    if (val) v = fmaxf(v, x);
-                    else k = fmaxf(k, x);
+                    const uint32_t y = __float_as_uint(rsc[i]) & 0x7FFFFFFFu, x = y < 0x7F800000u ? y : 0;
+                    if (val) v = x > v ? x : v;
+                    else k = x > k ? x : k;
                 } else if (val) {
                     typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
                     u16x2 top = {0, 0};
@@ -247,7 +263,7 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                     for (int j = 0; j < 4; ++j)
                         top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, raw[i][j] & 0x7FFF7FFFu));
                     uint32_t b = top[0] > top[1] ? top[0] : top[1];
-                    if (b >= 0x7F80u) {                // the largest finite one
+                    if (b >= 0x7F80u) {
                         b = 0;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
@@ -255,53 +271,34 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                             b = x < 0x7F80u && x > b ? x : b;
                         }
                     }
-                    v = fmaxf(v, __uint_as_float(b << 16));
+                    v = b << 16 > v ? b << 16 : v;
                 }
             }
-            if constexpr (QUANT) k = wave_top(k);
-            v = wave_top(v);
-            if (lane == 0) {
-                s_top[t & 1][0][wave] = k;
-                s_top[t & 1][1][wave] = v;
-            }
+            if (QUANT && (t == 0 || __uint_as_float(k) * fk >= kMost)) atomicMax(&s_top[t % 3][0], k);
+            if (t == 0 || __uint_as_float(v) * fv >= kMost) atomicMax(&s_top[t % 3][1], v);
         };
-        float fk = 1.0f, fk_next = 1.0f;               // the keys' power of two, of the present tile and the next
-        float fv_now = 0.0f;                           // the values', of the present tile
-        // the tile in registers into its buffer (after the barrier behind tops)
+        // the tile in registers into its buffer
         auto write_tile = [&](int t) {
-            float kt = 0.0f, vt = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                kt = fmaxf(kt, s_top[t & 1][0][i]);
-                vt = fmaxf(vt, s_top[t & 1][1][i]);
-            }
-            if constexpr (QUANT) {
-                fk_next = pow2_to(kt, 5);              // codes are below 2^9: products below 2^15
-                if (vt > 0.0f && (fv == 0.0f || vt * fv >= 64.0f)) fv = pow2_to(vt, 3);
-            } else if (vt > 0.0f && (fv == 0.0f || vt * fv >= 32768.0f)) {
-                fv = vt >= 0.125f && vt < 1024.0f ? 1.0f : pow2_to(vt, 8);
-            }
-            const float mulv = fv == 0.0f ? 1.0f : fv;
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const int part = (p_row0 + 8 * WR * i) / kDiffKeys;
                 const bool val = part >= 2;
                 u32x4 x;
                 if constexpr (QUANT) {
-                    const float s = rsc[i] * (val ? mulv : fk_next);
+                    const float s = rsc[i] * (val ? fv : fk);
                     const f32x4 lo = code_values<DT>(raw[i][0], s), hi = code_values<DT>(raw[i][1], s);
                     x = u32x4{pack2<true>(lo[0], lo[1]), pack2<true>(lo[2], lo[3]), pack2<true>(hi[0], hi[1]), pack2<true>(hi[2], hi[3])};
                 } else {
                     x = u32x4{raw[i][0], raw[i][1], raw[i][2], raw[i][3]};
                     if (val) {
-                        if (mulv == 1.0f) {
+                        if (fv == 1.0f) {
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
                                 x[j] = pack2<true>(__uint_as_float(x[j] << 16), __uint_as_float(x[j] & 0xFFFF0000u));
                         } else {
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                x[j] = pack2<true>(__uint_as_float(x[j] << 16) * mulv, __uint_as_float(x[j] & 0xFFFF0000u) * mulv);
+                                x[j] = pack2<true>(__uint_as_float(x[j] << 16) * fv, __uint_as_float(x[j] & 0xFFFF0000u) * fv);
                         }
                     }
                 }
@@ -311,95 +308,113 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                         const int sh = 16 * (j & 1);
                         if ((x[j / 2] >> sh & 0x7C00u) != 0x7C00u) continue;
                         x[j / 2] &= ~(0xFFFFu << sh);
+                        // a finite value that left the range: the tile is staged again
+                        if constexpr (QUANT) {
+                            const float y = __builtin_fabsf(rsc[i]);
+                            if (y < INFINITY && y * fv >= kMost) continue;
+                        } else if ((raw[i][j / 2] >> sh & 0x7F80u) != 0x7F80u) {
+                            continue;
+                        }
                         s_any = 1;
                         atomicMin(&s_bad[(part & 1) * D + 8 * p_c + j], t * kDiffKeys + p_key);
                     }
                 }
-                if (p_in) *reinterpret_cast<u32x4 *>(s_t[t & 1] + part * HB + (val ? p_vlds : p_klds)) = x;
+                if (p_in) *reinterpret_cast<u32x4 *>(s_t(t) + part * HB + (val ? p_vlds : p_klds)) = x;
             }
         };
 
-        // tile 0 in its buffer, tile 1 on its way
         load_tile(0);
-        tops(0);
-        __syncthreads();                               // the buffers of the item before are free
+        __syncthreads();                               // the buffers of the block before are free
         if (tid < 2 * D) s_bad[tid] = INT32_MAX;
         if (tid == 0) s_any = 0;
+        if (tid < 6) s_top[tid / 2][tid % 2] = 0;
         __syncthreads();
+        mark(0);
         write_tile(0);
-        if (1 < tiles) load_tile(1);
         for (int t = 0; t < tiles; ++t) {
-            if (t + 1 < tiles) tops(t + 1);
-            fk = fk_next;
-            if (fv_now != fv) {                        // the values' power of two was changed for this tile: the sums follow
-                if (fv_now != 0.0f) {
-                    const float k = fv / fv_now;
-#pragma unroll
-                    for (int c = 0; c < CT; ++c) acc[c] *= k;
+            __syncthreads();                           // tile t is staged, tile t - 1 used
+            const uint32_t kt = __builtin_amdgcn_readfirstlane(s_top[t % 3][0]), vt = __builtin_amdgcn_readfirstlane(s_top[t % 3][1]);
+            if (tid < 2) s_top[(t + 2) % 3][tid] = 0;
+            if (kt | vt) {                             // the first tile, or one that left the range
+                const float kx = __uint_as_float(kt) * fk, vx = __uint_as_float(vt) * fv;
+                const bool newk = QUANT && kt && !(kx >= kLeast && kx < kMost), newv = vt && !(vx >= kLeast && vx < kMost);
+                if (newk || newv) {
+                    if (newk) fk = pow2_to(__uint_as_float(kt), kAim);
+                    if (newv) {                        // the sums follow when they are next rescaled
+                        const float now = pow2_to(__uint_as_float(vt), kAim);
+                        owed *= now / fv;
+                        fv = now;
+                    }
+                    write_tile(t);
+                    __syncthreads();
                 }
-                fv_now = fv;
             }
-            __syncthreads();                           // tile t is written, tile t - 1 used
-            if (t + 1 < tiles) write_tile(t + 1);
-            if (t + 2 < tiles) load_tile(t + 2);
-            if (t * kDiffKeys > sees1) continue;       // no row of this wave sees any of it
-            const float ft = qs / fk;
-            const uint8_t *sk = s_t[t & 1] + mp * HB + r32 * RB, *sv = s_t[t & 1] + 2 * HB;
-            f32x16 sc;
+            if (t + 1 < tiles) load_tile(t + 1);
+            if (t * kDiffKeys <= sees1) {              // some row of this wave sees some of it
+                const float ft = qs / fk;
+                const uint8_t *sk = s_t(t) + mp * HB + r32 * RB, *sv = s_t(t) + 2 * HB;
+                f32x16 sc;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
+                for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-                sc = mfma<QUANT>(*reinterpret_cast<const u32x4 *>(sk + 16 * key_chunk<D>(r32, 2 * s + hf)), qf[s], sc);
-            const bool cut = t * kDiffKeys + kDiffKeys - 1 > sees0;
-            if (cut) {
-                const int lim = sees - t * kDiffKeys;
+                for (int s = 0; s < KS; ++s)
+                    sc = mfma<QUANT>(*reinterpret_cast<const u32x4 *>(sk + 16 * key_chunk<D>(r32, 2 * s + hf)), qf[s], sc);
+                const bool cut = t * kDiffKeys + kDiffKeys - 1 > sees0;
+                if (cut) {
+                    const int lim = sees - t * kDiffKeys;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sc[i] = 8 * (i / 4) + 4 * hf + i % 4 <= lim ? sc[i] : -INFINITY;
-            }
-            float top = sc[0];
-#pragma unroll
-            for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
-            top = max_x32(top) * ft;
-            // raised only past 2^8 times the present maximum (and on the first tile)
-            if (__ballot(top > m_run + 8.0f) != 0ull) {
-                const float now = fmaxf(m_run, top);
-                const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - now);
-                l_run *= alpha;
-#pragma unroll
-                for (int c = 0; c < CT; ++c) acc[c] *= alpha;
-                m_run = now;
-            }
-            const float base = m_run == -INFINITY ? 0.0f : m_run;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], ft, -base));
-                l_run += sc[i];
-            }
-            u32x4 p[2];
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) p[s][j] = pack2<true>(sc[8 * s + 2 * j], sc[8 * s + 2 * j + 1]);
-            // V^T as the A operand: lane (m, h) takes keys 16 s + 8 b + 4 h .. +4 of column m, b = 0, 1.
-            // Within each 16-lane group, lane j of a transposing read receives element j % 4 of the 8
-            // bytes that lanes 4 k + j / 4 address, k = 0 .. 3: lane i points at key i / 4 of the four
-            // and columns 4 (i % 4) of the group's sixteen.
-            const int vr = 4 * hf + ((lane & 15) >> 2);
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                const int hd = c / (D / 32), cl = c % (D / 32);
-                const int vc = 4 * cl + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-                const uint8_t *v = sv + hd * HB + vr * RB + 16 * value_chunk<D>(vr, vc) + 8 * (lane & 1);
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    typedef short s16x4 __attribute__((ext_vector_type(4)));
-                    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                        (__attribute__((address_space(3))) s16x4 *)(v + 16 * s * RB)));
-                    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                        (__attribute__((address_space(3))) s16x4 *)(v + (16 * s + 8) * RB)));
-                    acc[c] = mfma<true>(u32x4{x[0], x[1], y[0], y[1]}, p[s], acc[c]);
+                    for (int i = 0; i < 16; ++i) sc[i] = 8 * (i / 4) + 4 * hf + i % 4 <= lim ? sc[i] : -INFINITY;
                 }
+                float top = sc[0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
+                top = max_x32(top) * ft;
+                // raised only past 2^8 times the present maximum (and on the first tile)
+                if (owed != 1.0f || __ballot(top > m_run + 8.0f) != 0ull) {
+                    const float now = top > m_run + 8.0f ? top : m_run;
+                    float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - now);
+                    l_run *= alpha;
+                    alpha *= owed;
+                    owed = 1.0f;
+#pragma unroll
+                    for (int c = 0; c < CT; ++c) acc[c] *= alpha;
+                    m_run = now;
+                }
+                const float base = m_run == -INFINITY ? 0.0f : m_run;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], ft, -base));
+                    l_run += sc[i];
+                }
+                u32x4 p[2];
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) p[s][j] = pack2<true>(sc[8 * s + 2 * j], sc[8 * s + 2 * j + 1]);
+                // V^T as the A operand: lane (m, h) takes keys 16 s + 8 b + 4 h .. +4 of column m, b = 0, 1.
+                // Within each 16-lane group, lane j of a transposing read receives element j % 4 of the 8
+                // bytes that lanes 4 k + j / 4 address, k = 0 .. 3: lane i points at key i / 4 of the four
+                // and columns 4 (i % 4) of the group's sixteen.
+                const int vr = 4 * hf + ((lane & 15) >> 2);
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    const int hd = c / (D / 32), cl = c % (D / 32);
+                    const int vc = 4 * cl + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+                    const uint8_t *v = sv + hd * HB + vr * RB + 16 * value_chunk<D>(vr, vc) + 8 * (lane & 1);
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        typedef short s16x4 __attribute__((ext_vector_type(4)));
+                        const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                            (__attribute__((address_space(3))) s16x4 *)(v + 16 * s * RB)));
+                        const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                            (__attribute__((address_space(3))) s16x4 *)(v + (16 * s + 8) * RB)));
+                        acc[c] = mfma<true>(u32x4{x[0], x[1], y[0], y[1]}, p[s], acc[c]);
+                    }
+                }
+            }
+            if (t + 1 < tiles) {
+                mark(t + 1);
+                write_tile(t + 1);
             }
         }
 
@@ -418,58 +433,61 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                 for (int i = 0; i < 16; ++i)
                     if (s_bad[32 * c + 8 * (i / 4) + 4 * hf + i % 4] <= sees) acc[c][i] = __builtin_nanf("");
         }
-        const float back = fv_now != 0.0f ? 1.0f / fv_now : 1.0f;
-        if (it.whole) {
-            // map 1's rows go to map 0's waves through the buffers, half of the columns at a time
+        const float back = owed / fv;
+        if (whole) {
+            // the row's other map comes through the buffers: map 0's waves end the first half
+            // of the columns, map 1's the second, CR tiles of those at a time
             const float lam = a.e.lam[(row0 + tok) * a.e.lam_stride + h];
             const float inv = back * (mp ? -lam : 1.0f) / l;
-            constexpr int CR = CT / 2;
-            static_assert(4 * CR * 4 * 64 * sizeof(f32x4) <= sizeof(s_t), "the exchanged columns fit the buffers");
             float ss = 0.0f;
+            f32x4 *x = reinterpret_cast<f32x4 *>(s_mem) + lane;
 #pragma unroll
-            for (int c = 0; c < CT; ++c) acc[c] *= inv;
-#pragma unroll
-            for (int c0 = 0; c0 < CT; c0 += CR) {
-                f32x4 *x = reinterpret_cast<f32x4 *>(&s_t[0][0]) + rg * CR * 4 * 64 + lane;
+            for (int c0 = 0; c0 < CH; c0 += CR) {
                 __syncthreads();
-                if (mp) {
 #pragma unroll
-                    for (int c = c0; c < c0 + CR && c < CT; ++c)
+                for (int c = c0; c < c0 + CR && c < CH; ++c)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            x[((c - c0) * 4 + i) * 64] = f32x4{acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]};
-                }
+                    for (int i = 0; i < 4; ++i) {
+                        f32x4 o;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o[j] = (mp ? acc[c][4 * i + j] : acc[CH + c][4 * i + j]) * inv;
+                        x[(((4 * mp + rg) * CR + c - c0) * 4 + i) * 64] = o;
+                    }
                 __syncthreads();
-                if (!mp) {
 #pragma unroll
-                    for (int c = c0; c < c0 + CR && c < CT; ++c)
+                for (int c = c0; c < c0 + CR && c < CH; ++c)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const f32x4 y = x[((c - c0) * 4 + i) * 64];
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x4 y = x[(((4 * (1 - mp) + rg) * CR + c - c0) * 4 + i) * 64];
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                acc[c][4 * i + j] += y[j];
-                                ss += acc[c][4 * i + j] * acc[c][4 * i + j];
-                            }
+                        for (int j = 0; j < 4; ++j) {
+                            const float z = (mp ? acc[CH + c][4 * i + j] : acc[c][4 * i + j]) * inv + y[j];
+                            acc[c][4 * i + j] = z;
+                            ss += z * z;
                         }
-                }
+                    }
             }
-            if (!mp && live) {
-                const float k = diff_factor(a.e, a.e.norm ? sum_x32(ss) : 0.0f, 2 * D);
-                const int64_t at = ((row0 + tok) * a.pairs + h) * (2 * D);
+            float k = a.e.scale;
+            if (a.e.norm) {
+                ss = sum_x32(ss);
+                if (hf == 0) s_ss[mp][rg][r32] = ss;
+                __syncthreads();
+                k = diff_factor(a.e, ss + s_ss[1 - mp][rg][r32], 2 * D);
+            }
+            if (live) {
+                uint16_t *o = (uint16_t *)a.e.out + ((row0 + tok) * a.pairs + h) * (2 * D) + mp * D + 4 * hf;
 #pragma unroll
-                for (int c = 0; c < CT; ++c)
+                for (int c = 0; c < CH; ++c)
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const int col = 32 * c + 2 * i + 4 * hf;
-                        f32x4 x;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) x[j] = acc[c][i + j] * ((a.e.norm && a.e.norm_w) ? k * a.e.norm_w[col + j] : k);
-                        diff_store4(a.e, at + col, x);
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x4 n = *reinterpret_cast<const f32x4 *>(s_w + mp * D + 32 * c + 8 * i + 4 * hf) * k;
+                        *reinterpret_cast<u32x2 *>(o + 32 * c + 8 * i) =
+                            u32x2{bf16_pair(acc[c][4 * i] * n[0], acc[c][4 * i + 1] * n[1]),
+                                  bf16_pair(acc[c][4 * i + 2] * n[2], acc[c][4 * i + 3] * n[3])};
                     }
             }
         } else {
-            const int64_t slot = 2 * cell + (it.t0 == 0 ? 1 : 0);
+            const int64_t slot = 2 * cell + (t0 == 0 ? 1 : 0);
             const int64_t r = (slot * kRows + 32 * rg + r32) * 2 + mp;
 #pragma unroll
             for (int c = 0; c < CT; ++c)
@@ -481,12 +499,11 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                 a.part_ml[2 * r] = m_run;
                 a.part_ml[2 * r + 1] = l;
             }
-            if (it.t0 == 0) {                          // begun here: its last unit's slice ends it
-                const int64_t last = u + nt - 1;
+            if (t0 == 0) {                          // begun here: its last unit's slice ends it
+                const int64_t last = u - t1 + nt - 1;      // of the launch's units
                 begun = int4{it.b, (int)(uint32_t)it.k, (int)(it.k >> 32), (int)(last / chunk - w + 1)};
             }
         }
-        u += it.t1 - it.t0;
     }
     if (tid == 0) a.desc[cell] = begun;
 }

@@ -39,8 +39,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __shared__ int64_t s_sum[4];
     __shared__ __align__(16) float s_k[2 * kDiffKeys * KP];
     __shared__ __align__(16) float s_v[kDiffKeys * VP];
-    __shared__ int64_t s_bad;                          // the latest tile with a value that is not finite
-    if (threadIdx.x == 0) s_bad = -1;
+    // Values that are not finite, in tiles that not every row sees (a hidden key's
+    // probability of 0 times such a value would be NaN): staged as 0, and each column's
+    // first such key is kept here, from which on a row's column is NaN.
+    __shared__ int s_bad[2 * D];
+    __shared__ int s_any;
+    __shared__ __align__(16) float s_w[2 * D];         // the norm's weights
+    if (threadIdx.x < 2 * D) s_w[threadIdx.x] = a.e.norm && a.e.norm_w ? a.e.norm_w[threadIdx.x] : 1.0f;
     diff_refused(a, 2 * D);
     diff_units<256>(a, s_pre, s_sum);
     const int tid = threadIdx.x, lane = tid & 63, q4 = lane >> 4, r16 = lane & 15;
@@ -52,14 +57,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     int4 begun = {0, 0, 0, 0};
     int64_t u = w * chunk;
     const int64_t end = u + chunk < units ? u + chunk : units;
-    while (u < end) {
-        DiffItem it;
-        diff_find(a, s_pre, u, it);
-        DiffBlocks sq;
+    DiffItem it;
+    DiffBlocks sq;
+    if (u < end) diff_find(a, s_pre, u, it);
+    for (; u < end; diff_next(a, s_pre, sq, it)) {
         diff_seq(a, it.b, sq);
         const int64_t nt = sq.tiles(it.k), len = sq.prefix + sq.q;
-        it.t1 = it.t0 + (end - u) < nt ? it.t0 + (end - u) : nt;
-        it.whole = it.t0 == 0 && it.t1 == nt;
+        const int64_t left = nt + kDiffBlockCost - it.from, mine = end - u < left ? end - u : left;
+        const int64_t t0 = diff_tile_of(it.from), t1 = diff_tile_of(it.from + mine);
+        u += mine;
+        if (t0 == t1) continue;                        // the slice ends before the block's first tile
+        const bool whole = t0 == 0 && t1 == nt;
         const int64_t row0 = a.cu[it.b];
         // this lane's row, and the newest key it sees
         const int64_t f = it.k * R + 16 * wave + r16, rows = sq.q * g;
@@ -70,6 +78,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const int64_t f0 = it.k * R + 16 * wave, f1 = f0 + 15;
         const int64_t sees0 = sq.prefix + (f0 < rows ? f0 / g : sq.q - 1);       // every row of the wave
         const int64_t sees1 = sq.prefix + (f1 < rows ? f1 / g : sq.q - 1);       // some row of it
+        const int64_t seesb = sq.prefix + it.k * R / g;                          // the block's first row
+        __syncthreads();
+        if (tid < 2 * D) s_bad[tid] = INT32_MAX;
+        if (tid == 0) s_any = 0;
         float qf[2][KS][4];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
@@ -97,7 +109,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 for (int j = 0; j < 4; ++j) acc[m][c][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
         const int32_t *table = a.tables + (int64_t)it.b * a.max_blocks;
-        for (int64_t t = it.t0; t < it.t1; ++t) {
+        for (int64_t t = t0; t < t1; ++t) {
             __syncthreads();                           // the tile before has been used
             // keys and values of both heads, 8 elements a thread and pass; what lies past the sequence is zero
             for (int i = tid; i < 2 * kDiffKeys * (D / 8); i += 256) {
@@ -116,14 +128,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                     }
                 }
                 float *k = s_k + (m * kDiffKeys + key) * KP + 8 * c, *v = s_v + key * VP + m * D + 8 * c;
+                if (t * kDiffKeys + kDiffKeys - 1 > seesb) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        if (__builtin_fabsf(y[j]) < INFINITY) continue;
+                        y[j] = 0.0f;
+                        s_any = 1;
+                        atomicMin(&s_bad[m * D + 8 * c + j], (int)at);
+                    }
+                }
                 *reinterpret_cast<f32x4 *>(k) = f32x4{x[0], x[1], x[2], x[3]};
                 *reinterpret_cast<f32x4 *>(k + 4) = f32x4{x[4], x[5], x[6], x[7]};
                 *reinterpret_cast<f32x4 *>(v) = f32x4{y[0], y[1], y[2], y[3]};
                 *reinterpret_cast<f32x4 *>(v + 4) = f32x4{y[4], y[5], y[6], y[7]};
-                bool bad = false;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) bad |= !(__builtin_fabsf(y[j]) < INFINITY);
-                if (bad) s_bad = t;
             }
             __syncthreads();
             if (t * kDiffKeys > sees1) continue;       // no row of this wave sees any of it
@@ -163,7 +180,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 top = max_x32(max_x16(top));
                 // raised only past 2^8 times the present maximum (and on the first tile)
                 if (__ballot(top > m_run[m] + 8.0f) != 0ull) {
-                    const float now = fmaxf(m_run[m], top);
+                    const float now = top > m_run[m] + 8.0f ? top : m_run[m];
                     const float alpha = m_run[m] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[m] - now);
                     l_run[m] *= alpha;
 #pragma unroll
@@ -182,32 +199,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                         l_run[m] += p;
                     }
             }
-            if (cut && s_bad == t) {
-                // values that are not finite, and rows that do not see all of them: 0 times
-                // such a value is NaN, so each row adds only what it sees, key by key
-                for (int kq = 0; kq < 4; ++kq)
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int key = 16 * b + 4 * kq + i;
-                            float p[2];
-#pragma unroll
-                            for (int m = 0; m < 2; ++m) p[m] = __shfl(sc[m][b][i], 16 * kq + r16);
-                            if (t * kDiffKeys + key > sees) continue;
-#pragma unroll
-                            for (int c = 0; c < G; ++c)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                                    for (int j = 0; j < 4; ++j) {
-                                        const float v = s_v[key * VP + 64 * c + 16 * q4 + 4 * e + j];
-#pragma unroll
-                                        for (int m = 0; m < 2; ++m) acc[m][c][j][e] += p[m] * v;
-                                    }
-                        }
-                continue;
-            }
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -223,10 +214,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
 
         // lane (n, q): columns 64 c + 16 q + 4 i + j of row n in acc[m][c][j][i]
+        __syncthreads();
+        if (s_any) {
+#pragma unroll
+            for (int c = 0; c < G; ++c)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (s_bad[64 * c + 16 * q4 + 4 * i + j] <= sees) acc[0][c][j][i] = acc[1][c][j][i] = __builtin_nanf("");
+        }
         float l[2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) l[m] = sum_x32(sum_x16(l_run[m]));
-        if (it.whole) {
+        if (whole) {
             const float lam = a.e.lam[(row0 + tok) * a.e.lam_stride + h];
             const float i0 = 1.0f / l[0], i1 = lam / l[1];
             float ss = 0.0f;
@@ -248,14 +249,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int col = 64 * c + 16 * q4 + 4 * i;
-                        f32x4 x;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) x[j] = acc[0][c][j][i] * ((a.e.norm && a.e.norm_w) ? k * a.e.norm_w[col + j] : k);
-                        diff_store4(a.e, at + col, x);
+                        const f32x4 n = *reinterpret_cast<const f32x4 *>(s_w + col) * k;
+                        diff_store4(a.e, at + col, f32x4{acc[0][c][0][i] * n[0], acc[0][c][1][i] * n[1], acc[0][c][2][i] * n[2],
+                                                         acc[0][c][3][i] * n[3]});
                     }
             }
         } else {
-            const int64_t slot = 2 * cell + (it.t0 == 0 ? 1 : 0);
+            const int64_t slot = 2 * cell + (t0 == 0 ? 1 : 0);
             const int64_t r = (slot * R + 16 * wave + r16) * 2;
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
@@ -270,12 +270,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                     a.part_ml[2 * (r + m) + 1] = l[m];
                 }
             }
-            if (it.t0 == 0) {                          // begun here: its last unit's slice ends it
-                const int64_t last = u + nt - 1;
+            if (t0 == 0) {                          // begun here: its last unit's slice ends it
+                const int64_t last = u - t1 + nt - 1;      // of the launch's units
                 begun = int4{it.b, (int)(uint32_t)it.k, (int)(it.k >> 32), (int)(last / chunk - w + 1)};
             }
         }
-        u += it.t1 - it.t0;
     }
     if (tid == 0) a.desc[cell] = begun;
 }

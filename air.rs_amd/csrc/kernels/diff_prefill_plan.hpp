@@ -4,8 +4,10 @@
 // A sequence's rows are its (new token, query pair of the K/V pair) combinations,
 // token after token: row f is token f / g, pair f % g.  A block is `rows`
 // consecutive ones; it needs the keys its last token sees, in tiles of kDiffKeys.
-// One block's tile is a unit of work; a K/V pair's units, sequence after sequence,
-// block after block, tile after tile, are cut into equal slices, one workgroup each.
+// A block counts as kDiffBlockCost units (what beginning and ending it costs, in
+// tiles' time) and one for each of its tiles; a K/V pair's units, sequence after
+// sequence, block after block, are cut into equal slices, one workgroup each.  The
+// slice that holds a block's first tile begins it.
 #pragma once
 
 #include <stdint.h>
@@ -19,6 +21,7 @@
 namespace airkv {
 
 constexpr int kDiffKeys = 32;
+constexpr int kDiffBlockCost = 4;
 
 // sum of floor((a * i + b) / m) over i = 0 .. n - 1, by the Euclidean descent on
 // (m, a): lattice points under a line, exchanging the axes at each step.
@@ -55,16 +58,20 @@ struct DiffBlocks {
         return prefix + last + 1;
     }
     AIRKV_DP_HD int64_t tiles(int64_t k) const { return (keys(k) + kDiffKeys - 1) / kDiffKeys; }
-    // tiles of the blocks before k (k < blocks(): all of them full)
+    // units of block k, and of the blocks before it (k < blocks(): all of them full)
+    AIRKV_DP_HD int64_t cost(int64_t k) const { return kDiffBlockCost + tiles(k); }
     AIRKV_DP_HD int64_t before(int64_t k) const {
-        return (int64_t)floor_sum((uint64_t)k, (uint64_t)kDiffKeys * g, (uint64_t)rows,
+        return kDiffBlockCost * k + (int64_t)floor_sum((uint64_t)k, (uint64_t)kDiffKeys * g, (uint64_t)rows,
                                   (uint64_t)(prefix + kDiffKeys) * g + rows - 1);
     }
     AIRKV_DP_HD int64_t units() const {
         const int64_t n = blocks();
-        return n ? before(n - 1) + tiles(n - 1) : 0;
+        return n ? before(n - 1) + cost(n - 1) : 0;
     }
 };
+
+// The tiles [t0, t1) of a block that its units [from, to) hold.
+AIRKV_DP_HD inline int64_t diff_tile_of(int64_t unit) { return unit > kDiffBlockCost ? unit - kDiffBlockCost : 0; }
 
 // Units per slice: an equal share, but at least `least`, so that small launches
 // are not cut into pieces whose joining costs more than their work.

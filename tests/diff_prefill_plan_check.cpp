@@ -21,11 +21,11 @@ static void sums(DiffBlocks s) {
     const int64_t n = s.blocks();
     int64_t at = 0;
     for (int64_t k = 0; k < n; ++k) {
-        check(s.before(k) == at, "tiles before a block", s.q, s.prefix, k);
+        check(s.before(k) == at, "units before a block", s.q, s.prefix, k);
         // the keys its last row sees, counted row by row
         const int64_t last = std::min((k + 1) * s.rows, s.q * s.g) - 1;
         check(s.keys(k) == s.prefix + last / s.g + 1, "keys of a block", s.q, s.prefix, k);
-        at += (s.keys(k) + kDiffKeys - 1) / kDiffKeys;
+        at += kDiffBlockCost + (s.keys(k) + kDiffKeys - 1) / kDiffKeys;
     }
     check(s.units() == at, "units of a sequence", s.q, s.prefix, s.g);
 }
@@ -48,19 +48,22 @@ static void walk(const std::vector<DiffBlocks> &seqs, int64_t slices, int64_t le
             const DiffBlocks &s = seqs[b];
             int64_t k = 0;
             while (k + 1 < s.blocks() && s.before(k + 1) <= u - pre[b]) ++k;
-            const int64_t t0 = u - pre[b] - s.before(k), nt = s.tiles(k), t1 = std::min(t0 + end - u, nt);
-            check(t0 >= 0 && t0 < nt && done[{b, k}] == t0, "a block's tiles in order", b, k, t0);
+            const int64_t from = u - pre[b] - s.before(k), nt = s.tiles(k), mine = std::min(end - u, kDiffBlockCost + nt - from);
+            check(from >= 0 && mine > 0, "a block's units", b, k, from);
+            const int64_t t0 = diff_tile_of(from), t1 = diff_tile_of(from + mine);
+            check(t0 <= t1 && t1 <= nt && (done[{b, k}]) == t0, "a block's tiles in order", b, k, t0);
             done[{b, k}] = t1;
+            u += mine;
+            if (t0 == t1) continue;
             if (!(t0 == 0 && t1 == nt)) {
                 const int64_t slot = 2 * w + (t0 == 0 ? 1 : 0);
                 check(used.insert(slot).second && slot < 2 * slices, "a piece slot of its own", slot, w, t0);
                 pieces[{b, k}].push_back(slot);
                 if (t0 == 0) {
-                    const int64_t n = (u + nt - 1) / chunk - w + 1;
+                    const int64_t n = (u - t1 + nt - 1) / chunk - w + 1;
                     for (int64_t i = 0; i < n; ++i) joined[{b, k}].push_back(2 * (w + i) + (i == 0 ? 1 : 0));
                 }
             }
-            u += t1 - t0;
         }
     }
     for (size_t b = 0; b < seqs.size(); ++b)

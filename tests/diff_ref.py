@@ -94,7 +94,7 @@ def attend(q, k, v, lam, scale, sees, norm_weight=None, norm_eps=None, out_scale
 
 def check(got, out, bound, out_dtype, what, p_step=0.0):
     """got within the bound of out, and of its own rounding."""
-    bound = bound * (1 + EPS[out_dtype]) + EPS[out_dtype] * np.abs(out) + 1e-30
+    bound = bound * (1 + EPS[out_dtype]) + EPS[out_dtype] * np.abs(out) + 2.0 ** -149
     bad = ~(np.abs(got - out) <= bound)
     assert not bad.any(), (f"{what}: {bad.sum()} of {bad.size} beyond the bound, at {np.argwhere(bad)[:3].tolist()}: "
                            f"{got[bad][:3]} against {out[bad][:3]}, allowed {bound[bad][:3]}")

@@ -114,7 +114,7 @@ def test_diff_decode_batches(batch, lens):
     log(f"diff decode batch {batch}: {_decode(c, 2, False, True, True, True, splits=(64, 3)):.3f} of the bound")
 
 
-def _prefill(c, qlens, group, q_f32, out_f32, norm, lam_rows, out_scale=0.75, ws=None, p_step=0.0):
+def _prefill(c, qlens, group, q_f32, out_f32, norm, lam_rows, out_scale=0.75, ws=None, p_step=0.0, floor=0.0):
     torch = torch_mod()
     cu = np.concatenate([[0], np.cumsum(qlens)]).astype(np.int32)
     total = int(cu[-1])
@@ -127,6 +127,7 @@ def _prefill(c, qlens, group, q_f32, out_f32, norm, lam_rows, out_scale=0.75, ws
         k, v = (sequence(x, c.tables[i], int(m), c.bs) for x in (kv, vv))
         s = slice(cu[i], cu[i + 1])
         want[s], bound[s] = attend(q64[s], k, v, lam64[s], scale, m - ql + np.arange(ql), p_step=p_step, **more)
+        bound[s] += floor * out_scale * (1 + np.abs(lam64[s]).max(initial=0)) * np.abs(v).max(initial=0)
     tables, lens = c.device()
     out = torch.full((total, lam64.shape[1], 2 * c.d), float("nan"), device="cuda",
                      dtype=torch.float32 if out_f32 else torch.bfloat16)
@@ -175,3 +176,74 @@ def test_diff_prefill_shapes(chunks):
         c = Cache(dtype, d, 2, 16, [n for n, _ in chunks], seed=len(chunks) + d)
         used = _prefill(c, [m for _, m in chunks], group, f32, f32, True, True, p_step=0.0 if f32 else _p_step(c))
         log(f"diff prefill {len(chunks)} x {chunks[0]} {NAMES[dtype]}: {used:.3f} of the bound")
+
+
+def _refill(c, k_mul, v_mul):
+    """The cache's rows again, times a factor per token."""
+    torch = torch_mod()
+    slots = np.concatenate([c.tables[i, np.arange(n) // c.bs].astype(np.int64) * c.bs + np.arange(n) % c.bs
+                            for i, n in enumerate(c.lens)])
+    f = [np.concatenate([m(np.arange(n)) * np.ones(n) for n in c.lens]).astype(np.float32)[:, None, None] for m in (k_mul, v_mul)]
+    c.pool.append(*(torch.from_numpy((x * y).astype(np.float32)).cuda() for x, y in zip((c.k, c.v), f)), torch.from_numpy(slots).cuda())
+
+
+@pytest.mark.parametrize("dtype", [airkv.F32, airkv.BF16, airkv.INT8, airkv.FP8])
+@pytest.mark.parametrize("case", ["tiny", "huge", "growing", "falling", "far_apart", "keys_tiny", "keys_growing"])
+def test_diff_value_ranges(dtype, case):
+    """Values and keys far from 1, and ones whose size changes along the sequence, in
+    decode and prefill at f32 and at 16-bit products.  (Outputs are not normalised, so
+    each row's error is held to its own values' size.)"""
+    one = lambda t: 1.0
+    k_mul, v_mul = {
+        "tiny": (one, lambda t: 1e-30), "huge": (one, lambda t: 1e30), "growing": (one, lambda t: 2.0 ** (t / 12 - 20)),
+        "falling": (one, lambda t: 2.0 ** (20 - t / 12)), "far_apart": (one, lambda t: np.where(t % 70 < 35, 1e12, 1e-3)),
+        "keys_tiny": (lambda t: 1e-6, one), "keys_growing": (lambda t: 2.0 ** (t / 40 - 12), one)}[case]
+    for f32 in (True, False):
+        c = Cache(dtype, 64, 2, 16, [500, 130, 33], seed=3)
+        _refill(c, k_mul, v_mul)
+        # a value far below the block's largest keeps f16's absolute resolution: 2^-25 of it
+        wide = dtype != airkv.F32 and not f32
+        used = _prefill(c, [400, 5, 33], 2, f32, f32, False, True, p_step=_p_step(c) if wide else 0.0, floor=2.0 ** -24 if wide else 0.0)
+        more = _decode(c, 2, f32, f32, False, True, splits=(64, 1))
+        log(f"diff {case} {NAMES[dtype]} f32={f32}: prefill {used:.3f}, decode {more:.3f} of the bound")
+
+
+@pytest.mark.parametrize("dtype", [airkv.F32, airkv.BF16, airkv.INT8, airkv.FP8])
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_diff_prefill_hidden_values_that_are_not_finite(dtype, f32, bad):
+    """Keys and values that are not finite at tokens a row does not see do not reach
+    it; rows that see them are not finite in those columns."""
+    torch = torch_mod()
+    n, first, at = 200, 100, [130, 131, 171, 199]
+    c = Cache(dtype, 64, 4, 16, [n, n], seed=9)
+    row = c.tables[0]
+    clean = None
+    q, lam, _, _, _, _ = c.rows(2 * (n - first), 3, f32, False, False)
+    cu = torch.tensor([0, n - first, 2 * (n - first)], dtype=torch.int32, device="cuda")
+    tables, lens = c.device()
+    out = torch.empty(q.shape[0], 6, 128, device="cuda", dtype=torch.float32 if f32 else torch.bfloat16)
+    for step in range(2):
+        c.pool.paged_diff_prefill(q, lam, cu, tables, lens, out.fill_(7.0))
+        got = out.float().cpu().numpy()
+        if clean is None:
+            clean = got
+            assert np.isfinite(clean).all()
+            # one column of head 1 and the whole of head 3's group of 32, of four tokens of sequence 0
+            x = torch.from_numpy(c.v[:n][at].copy()).cuda()
+            x[:, 1, 5] = bad
+            x[:, 3, 32:64] = bad
+            k = torch.from_numpy(c.k[:n][at].copy()).cuda()
+            k[2, 0, 7] = bad                                # token 171
+            slots = torch.from_numpy(np.array([int(row[t // 16]) * 16 + t % 16 for t in at], np.int64)).cuda()
+            c.pool.append(k, x, slots)
+    r = n - first
+    assert np.array_equal(got[r:], clean[r:])               # the other sequence
+    assert np.array_equal(got[:at[0] - first], clean[:at[0] - first])
+    after = got[at[0] - first:r]
+    if dtype in (airkv.INT8, airkv.FP8):
+        return                                              # what a pool stores for such a group is its own rule
+    assert not np.isfinite(after[:, :3, 64 + 5]).any() and not np.isfinite(after[:, 3:, 64 + 32:]).any()
+    same = after[:at[2] - at[0]]                            # rows that see no bad key: other columns as they were
+    ref = clean[at[0] - first:at[2] - first]
+    assert np.array_equal(same[:, :3, :64], ref[:, :3, :64]) and np.array_equal(same[:, 3:, :64], ref[:, 3:, :64])
