@@ -31,6 +31,12 @@ struct DiffPrefillArgs {
     float *part_ml, *part_o;
 };
 
+// x, the same in every lane of the wave, in scalar registers.
+__device__ __forceinline__ int64_t diff_uniform(int64_t x) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 // What a row of the work list needs, for the workgroup's present block.
 struct DiffItem {
     int32_t b;
@@ -96,7 +102,7 @@ __device__ __forceinline__ void diff_find(const DiffPrefillArgs &a, const int64_
     lo = __builtin_amdgcn_readfirstlane(lo);
     DiffBlocks s;
     diff_seq(a, lo, s);
-    const int64_t at = u - s_pre[lo];
+    const int64_t at = u - diff_uniform(s_pre[lo]);
     int64_t k0 = 0, k1 = s.blocks();               // before(k0) <= at, and the block is in [k0, k1)
     const int lane = threadIdx.x & 63;
     while (k1 - k0 > 1) {
@@ -108,8 +114,8 @@ __device__ __forceinline__ void diff_find(const DiffPrefillArgs &a, const int64_
         k1 = k0 + step < k1 ? k0 + step : k1;
     }
     it.b = lo;
-    it.k = k0;
-    it.from = at - s.before(k0);
+    it.k = diff_uniform(k0);
+    it.from = diff_uniform(at - s.before(it.k));
 }
 
 // The block after: of the same sequence, or the first of the next that has one.
@@ -118,7 +124,7 @@ __device__ __forceinline__ void diff_next(const DiffPrefillArgs &a, const int64_
     if (++it.k < s.blocks()) return;
     it.k = 0;
     do ++it.b;
-    while (it.b < a.batch && s_pre[it.b + 1] == s_pre[it.b]);
+    while (it.b < a.batch && diff_uniform(s_pre[it.b + 1]) == diff_uniform(s_pre[it.b]));
 }
 
 // Sequences that are refused: counted, and their rows (those there are) zeroed.

@@ -64,6 +64,19 @@ __device__ __forceinline__ float pow2_to(float x, int e) {
     return f == 0 || f == 255 || k < 1 || k > 254 ? 1.0f : __uint_as_float((uint32_t)k << 23);
 }
 
+// The schedule of N matrix products that take READS LDS reads each: the reads of the
+// first AHEAD, then a product and the reads of the next in turn.
+template <int N, int AHEAD, int READS> __device__ __forceinline__ void read_ahead() {
+    constexpr int kMfma = 0x008, kLdsRead = 0x100;
+    __builtin_amdgcn_sched_group_barrier(kLdsRead, READS * AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < N - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kLdsRead, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(kMfma, AHEAD, 0);
+}
+
 constexpr int kRows = 128;
 constexpr int kThreads16 = 512;
 
@@ -118,7 +131,7 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rg = wave & 3, mp = wave >> 2;           // 32 rows, one map
     const int w = blockIdx.x, kp = blockIdx.y, g = a.group;
-    const int64_t units = s_pre[a.batch];
+    const int64_t units = diff_uniform(s_pre[a.batch]);
     const int64_t chunk = diff_prefill_chunk(units, a.slices, a.least);
     const int64_t cell = (int64_t)kp * a.slices + w;
     int4 begun = {0, 0, 0, 0};
@@ -210,21 +223,23 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
         const int32_t *table = a.tables + (int64_t)it.b * a.max_blocks + key0 / a.bs;
         uint32_t raw[NP][2 * EB];                      // the tile on its way
         float rsc[NP];
-        // the entry of the half-tile that this wave stages
-        auto entry = [&](int t) -> int32_t {
-            const int key = t * kDiffKeys + 16 * p_half;
-            return t < tiles && key < rest ? table[key / a.bs] : -1;
+        // Lane k: the entry of the half that this wave stages of tile t + k, for a window of
+        // 64 tiles (an entry a tile would be waited for behind that tile's loads).
+        int32_t window = 0;
+        auto look_up = [&](int t) {
+            const int key = (t + lane < tiles ? t + lane : tiles - 1) * kDiffKeys + 16 * p_half;
+            window = key < rest ? table[key / a.bs] : -1;
         };
-        int32_t next = entry(0);
-        // tile t's loads (block `next`), then the entry of the next
         auto load_tile = [&](int t) {
-            const bool ok = next >= 0 && next < a.num_blocks;
+            if (t % 64 == 0) look_up(t);
+            const int32_t blk = __builtin_amdgcn_readlane(window, t % 64);
+            const bool ok = blk >= 0 && blk < a.num_blocks;
             int left = rest - t * kDiffKeys - 16 * p_half;
             // entries outside the pool, once per block of tokens
             if (!ok && left > 0 && kp == 0 && p_row0 % 16 == 0 && p_row0 < kDiffKeys && (p_half == 0 || a.bs == 16) && lane == 0)
                 atomicAdd(a.errors, 1ull);
             left = !ok || left < 0 ? 0 : left < 16 ? left : 16;
-            const int64_t row = ((int64_t)(ok ? next : 0) * a.heads + 2 * kp) * a.bs + (t * kDiffKeys + 16 * p_half) % a.bs;
+            const int64_t row = ((int64_t)(ok ? blk : 0) * a.heads + 2 * kp) * a.bs + (t * kDiffKeys + 16 * p_half) % a.bs;
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const int part = (p_row0 + 8 * WR * i) / kDiffKeys;          // keys of head 0, 1, values of head 0, 1
@@ -243,7 +258,6 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                     for (int j = 0; j < 4; ++j) raw[i][j] = x[j];
                 }
             }
-            next = entry(t + 1);
         };
         // Scales and values of the tile in registers that leave f16's range are marked for all
         // waves; behind the barrier the tile is staged again under another power of two.
@@ -352,13 +366,23 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
             if (t + 1 < tiles) load_tile(t + 1);
             if (t * kDiffKeys <= sees1) {              // some row of this wave sees some of it
                 const float ft = qs / fk;
-                const uint8_t *sk = s_t(t) + mp * HB + r32 * RB, *sv = s_t(t) + 2 * HB;
+                const uint8_t *sk = s_t(t) + mp * HB, *sv = s_t(t) + 2 * HB;
                 f32x16 sc;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
+                {
+                    // a fragment is read while the products of those before it run
+                    constexpr int AHEAD = KS < 3 ? KS : 3;
+                    int at = r32;                      // (the chunks' places are not kept in registers from tile to tile)
+                    asm volatile("" : "+v"(at));
+                    u32x4 kf[KS];
 #pragma unroll
-                for (int s = 0; s < KS; ++s)
-                    sc = mfma<QUANT>(*reinterpret_cast<const u32x4 *>(sk + 16 * key_chunk<D>(r32, 2 * s + hf)), qf[s], sc);
+                    for (int s = 0; s < KS; ++s)
+                        kf[s] = *reinterpret_cast<const u32x4 *>(sk + at * RB + 16 * key_chunk<D>(at, 2 * s + hf));
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) sc = mfma<QUANT>(kf[s], qf[s], sc);
+                    read_ahead<KS, AHEAD, 1>();
+                }
                 const bool cut = t * kDiffKeys + kDiffKeys - 1 > sees0;
                 if (cut) {
                     const int lim = sees - t * kDiffKeys;
@@ -395,12 +419,15 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                 // Within each 16-lane group, lane j of a transposing read receives element j % 4 of the 8
                 // bytes that lanes 4 k + j / 4 address, k = 0 .. 3: lane i points at key i / 4 of the four
                 // and columns 4 (i % 4) of the group's sixteen.
-                const int vr = 4 * hf + ((lane & 15) >> 2);
+                int ln = lane;
+                asm volatile("" : "+v"(ln));
+                const int vr = 4 * (ln >> 5) + ((ln & 15) >> 2);
+                u32x4 vf[CT][2];
 #pragma unroll
                 for (int c = 0; c < CT; ++c) {
                     const int hd = c / (D / 32), cl = c % (D / 32);
-                    const int vc = 4 * cl + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-                    const uint8_t *v = sv + hd * HB + vr * RB + 16 * value_chunk<D>(vr, vc) + 8 * (lane & 1);
+                    const int vc = 4 * cl + 2 * ((ln >> 4) & 1) + ((ln & 3) >> 1);
+                    const uint8_t *v = sv + hd * HB + vr * RB + 16 * value_chunk<D>(vr, vc) + 8 * (ln & 1);
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
                         typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -408,9 +435,14 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                                             (__attribute__((address_space(3))) s16x4 *)(v + 16 * s * RB)));
                         const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                             (__attribute__((address_space(3))) s16x4 *)(v + (16 * s + 8) * RB)));
-                        acc[c] = mfma<true>(u32x4{x[0], x[1], y[0], y[1]}, p[s], acc[c]);
+                        vf[c][s] = u32x4{x[0], x[1], y[0], y[1]};
                     }
                 }
+#pragma unroll
+                for (int c = 0; c < CT; ++c)
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) acc[c] = mfma<true>(vf[c][s], p[s], acc[c]);
+                read_ahead<2 * CT, 3, 2>();
             }
             if (t + 1 < tiles) {
                 mark(t + 1);

@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int tid = threadIdx.x, lane = tid & 63, q4 = lane >> 4, r16 = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int w = blockIdx.x, kp = blockIdx.y, g = a.group;
-    const int64_t units = s_pre[a.batch];
+    const int64_t units = diff_uniform(s_pre[a.batch]);
     const int64_t chunk = diff_prefill_chunk(units, a.slices, a.least);
     const int64_t cell = (int64_t)kp * a.slices + w;
     int4 begun = {0, 0, 0, 0};
