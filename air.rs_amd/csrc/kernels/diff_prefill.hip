@@ -67,7 +67,7 @@ size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // A slice for every workgroup that is resident at once, all K/V pairs together.
 struct Plan {
-    int32_t rows, slices, least;
+    int32_t rows, extra, slices, least;
     size_t cells, halves;          // (pair, slice)s, rows' maps in the piece slots
     size_t bytes(int d) const { return align256(cells * sizeof(int4)) + align256(halves * 2 * 4) + halves * 2 * d * 4; }
 };
@@ -77,6 +77,7 @@ Plan plan_for(const air_kv_pool &p, bool half) {
     Plan pl;
     const int kv_pairs = p.desc.n_kv_heads / 2, per_cu = half ? 1 : 2;
     pl.rows = half ? 128 : 64;
+    pl.extra = half ? 7 : 1;       // 16 us and 2.1 us a tile; 20 us and 10 to 25 us
     pl.slices = std::max(1, (per_cu * p.cus + kv_pairs - 1) / kv_pairs);
     pl.least = half ? 16 : 8;
     pl.cells = (size_t)kv_pairs * pl.slices;
@@ -119,6 +120,7 @@ hipError_t launch_diff_prefill(const air_kv_pool &p, hipStream_t s, const void *
     a.slices = plan.slices;
     a.least = plan.least;
     a.rows = plan.rows;
+    a.extra = plan.extra;
     char *ws = (char *)workspace;
     a.desc = (int4 *)ws;
     ws += align256(plan.cells * sizeof(int4));

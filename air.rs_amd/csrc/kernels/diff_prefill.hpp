@@ -22,7 +22,7 @@ struct DiffPrefillArgs {
     DiffOut e;
     int32_t slices;                // per K/V pair
     int32_t least;                 // units a slice holds at least
-    int32_t rows;                  // of a block
+    int32_t rows, extra;           // of a block; the units it counts beside its tiles
     // cut blocks: per (pair, slice) the block it began and did not end, {sequence,
     // block (low, high), pieces}; two piece slots per (pair, slice), 2w for a block
     // begun before, 2w + 1 for one that goes on: [slot][row][map] of (max, sum), and
@@ -52,6 +52,7 @@ __device__ __forceinline__ bool diff_seq(const DiffPrefillArgs &a, int b, DiffBl
     const int64_t r0 = a.cu[b], r1 = a.cu[b + 1], len = a.lens[b];
     s.g = a.group;
     s.rows = a.rows;
+    s.extra = a.extra;
     s.q = r1 - r0;
     s.prefix = len - s.q;
     const bool ok = r0 >= 0 && r1 >= r0 && r1 <= a.total_q && len >= 0 && len <= (int64_t)a.max_blocks * a.bs && s.q <= len;

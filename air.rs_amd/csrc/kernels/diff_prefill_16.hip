@@ -8,8 +8,7 @@
 //   O^T += V^T . P^T   the same instruction; its contraction takes the keys in the order
 //                      in which the lanes hold P, so P never moves
 // and the two maps of a row meet when the block ends.  Keys and values are staged in LDS
-// as rows, in two buffers (a tile is loaded two tiles ahead and written one ahead, one
-// barrier a tile), with 16-byte chunks placed so that neither the rows' reads nor the
+// as rows, in three buffers (two tiles ahead, loaded three ahead, one barrier a tile), with 16-byte chunks placed so that neither the rows' reads nor the
 // values' transposing reads meet in a bank.
 //
 // The second product takes f16 operands: values (exact when they come from bf16 pages
@@ -110,10 +109,10 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
     constexpr int CP = D == 96 ? 16 : D / 8, WR = 64 / CP, NP = 4 * kDiffKeys / (8 * WR);
     __shared__ int64_t s_pre[kDiffPrefillBatch + 1];
     __shared__ int64_t s_sum[kThreads16 / 64];
-    // the two buffers; in them, at a block's end, CR column tiles of every wave's half
+    // the three buffers; in them, at a block's end, CR column tiles of every wave's half
     constexpr int CH = CT / 2, CR = D == 128 ? 2 : 1, XB = 8 * CR * 4 * 64 * 16;
-    __shared__ __align__(16) uint8_t s_mem[8 * HB > XB ? 8 * HB : XB];
-    auto s_t = [&](int t) { return s_mem + (t & 1) * 4 * HB; };
+    __shared__ __align__(16) uint8_t s_mem[12 * HB > XB ? 12 * HB : XB];
+    auto s_t = [&](int t) __attribute__((always_inline)) { return s_mem + t % 3 * (4 * HB); };
     // Per tile (mod 3), keys' scale and values' (scale): the bits of the largest of those that
     // leave f16's range under the present power of two (of all in a block's first tile)
     __shared__ uint32_t s_top[3][2];
@@ -141,8 +140,8 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
     const int p_c = lane % CP, p_row0 = wave * WR;     // the wave's first row of pass 0, of the 128 staged
     const int p_key = (p_row0 + lane / CP) % kDiffKeys;
     const bool p_in = D != 96 || p_c < D / 8;
-    const int p_off = p_in ? ((p_key % 16) * D + 8 * p_c) * EB : 0x7FFFFFFF;
-    const int p_sc = p_in && QUANT ? ((p_key % 16) * nsc + 8 * p_c / a.scale_group) * 4 : 0x7FFFFFFF;
+    const int p_off = p_in ? ((p_key % 16) * D + 8 * p_c) * EB : 0x40000000;
+    const int p_sc = p_in && QUANT ? ((p_key % 16) * nsc + 8 * p_c / a.scale_group) * 4 : 0x40000000;
     const int p_klds = p_key * RB + 16 * key_chunk<D>(p_key, p_c), p_vlds = p_key * RB + 16 * value_chunk<D>(p_key, p_c);
     const int p_half = p_row0 % kDiffKeys / 16;        // of every pass: 8 WR rows are a multiple of 32
 
@@ -160,15 +159,15 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
     for (; u < end; diff_next(a, s_pre, sq, it)) {
         diff_seq(a, it.b, sq);
         const int64_t nt = sq.tiles(it.k), len = sq.prefix + sq.q;
-        const int64_t left = nt + kDiffBlockCost - it.from, mine = end - u < left ? end - u : left;
-        const int64_t t0 = diff_tile_of(it.from), t1 = diff_tile_of(it.from + mine);
+        const int64_t left = nt + a.extra - it.from, mine = end - u < left ? end - u : left;
+        const int64_t t0 = diff_tile_of(it.from, a.extra), t1 = diff_tile_of(it.from + mine, a.extra);
         u += mine;
         if (t0 == t1) continue;                        // the slice ends before the block's first tile
         const bool whole = t0 == 0 && t1 == nt;
         const int64_t row0 = a.cu[it.b];
         const int64_t rows = sq.q * g;
         // this lane's row: token and query pair (of the last token, if there is none)
-        auto my_row = [&](int r, bool &live, int &tok, int &h) {
+        auto my_row = [&](int r, bool &live, int &tok, int &h) __attribute__((always_inline)) {
             const int64_t f = it.k * kRows + 32 * rg + r;
             live = f < rows;
             tok = (int)(live ? f / g : sq.q - 1);
@@ -214,60 +213,85 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
         }
         f32x16 acc[CT];
         float m_run = -INFINITY, l_run = 0.0f;
-        float owed = 1.0f;                             // what the sums have to be multiplied by to be under fv
+        // what the sums have to be multiplied by to be under the present tile's power of two,
+        // and for the next tile's
+        float owed = 1.0f, owed_next = 1.0f;
 #pragma unroll
         for (int c = 0; c < CT; ++c)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
 
         const int32_t *table = a.tables + (int64_t)it.b * a.max_blocks + key0 / a.bs;
-        uint32_t raw[NP][2 * EB];                      // the tile on its way
-        float rsc[NP];
-        // Lane k: the entry of the half that this wave stages of tile t + k, for a window of
-        // 64 tiles (an entry a tile would be waited for behind that tile's loads).
-        int32_t window = 0;
-        auto look_up = [&](int t) {
-            const int key = (t + lane < tiles ? t + lane : tiles - 1) * kDiffKeys + 16 * p_half;
-            window = key < rest ? table[key / a.bs] : -1;
+        struct Raw {                                   // a tile on its way
+            uint32_t w[NP][2 * EB];
+            float s[NP];
         };
-        auto load_tile = [&](int t) {
+        // Lane k: the entry of the half that this wave stages of tile t + k, for a window of
+        // 64 tiles (an entry a tile would be waited for behind that tile's loads); entries
+        // outside the pool are counted once per block of tokens, and read nothing.
+        const int shift = a.bs == 32 ? 5 : 4;
+        int32_t window = 0;
+        auto look_up = [&](int t) __attribute__((always_inline)) {
+            const int key = (t + lane < tiles ? t + lane : tiles - 1) * kDiffKeys + 16 * p_half;
+            window = key < rest ? table[key >> shift] : 0;
+            const bool out = t + lane < tiles && (window < 0 || window >= a.num_blocks);
+            window = out || key >= rest ? -1 : window;
+            if (kp == 0 && p_row0 % 16 == 0 && p_row0 < kDiffKeys && (p_half == 0 || a.bs == 16)) {
+                const int n = __popcll(__ballot(out));
+                if (n && lane == 0) atomicAdd(a.errors, (unsigned long long)n);
+            }
+        };
+        // A head's rows of a block lie bs rows behind the head's before: one buffer holds both
+        // heads', and a lane whose key is not there reads outside of it: zeros.
+        const int head_step = a.bs * D * EB, head_sc = a.bs * nsc * 4;
+        auto load_tile = [&](int t, Raw &r) __attribute__((always_inline)) {
             if (t % 64 == 0) look_up(t);
             const int32_t blk = __builtin_amdgcn_readlane(window, t % 64);
-            const bool ok = blk >= 0 && blk < a.num_blocks;
-            int left = rest - t * kDiffKeys - 16 * p_half;
-            // entries outside the pool, once per block of tokens
-            if (!ok && left > 0 && kp == 0 && p_row0 % 16 == 0 && p_row0 < kDiffKeys && (p_half == 0 || a.bs == 16) && lane == 0)
-                atomicAdd(a.errors, 1ull);
-            left = !ok || left < 0 ? 0 : left < 16 ? left : 16;
-            const int64_t row = ((int64_t)(ok ? blk : 0) * a.heads + 2 * kp) * a.bs + (t * kDiffKeys + 16 * p_half) % a.bs;
+            const int left = blk < 0 ? 0 : rest - t * kDiffKeys - 16 * p_half;
+            const int off = (p_key & 15) < left ? p_off : 0x40000000;
+            const int64_t row = (((int64_t)(blk < 0 ? 0 : blk) * a.heads + 2 * kp) << shift) + (16 * p_half & (a.bs - 1));
+            const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+                (void *)((const uint8_t *)a.k_pages + row * (D * EB)), (short)0, head_step + 16 * D * EB, kDiffBufferWord3);
+            const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+                (void *)((const uint8_t *)a.v_pages + row * (D * EB)), (short)0, head_step + 16 * D * EB, kDiffBufferWord3);
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const int part = (p_row0 + 8 * WR * i) / kDiffKeys;          // keys of head 0, 1, values of head 0, 1
-                const int64_t at = row + (part & 1) * a.bs;
-                const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-                    (void *)((const uint8_t *)(part < 2 ? a.k_pages : a.v_pages) + at * (D * EB)), (short)0, left * D * EB, kDiffBufferWord3);
+                const int step = (part & 1) * head_step;
                 if constexpr (QUANT) {
-                    const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, p_off, 0, 0);
-                    raw[i][0] = x[0]; raw[i][1] = x[1];
-                    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-                        (void *)((part < 2 ? a.k_scales : a.v_scales) + at * nsc), (short)0, left * nsc * 4, kDiffBufferWord3);
-                    rsc[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, p_sc, 0, 0));
+                    const u32x2 x = part < 2 ? __builtin_amdgcn_raw_buffer_load_b64(rk, off, step, 0)
+                                             : __builtin_amdgcn_raw_buffer_load_b64(rv, off, step, 0);
+                    r.w[i][0] = x[0]; r.w[i][1] = x[1];
                 } else {
-                    const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, p_off, 0, 0);
+                    const u32x4 x = part < 2 ? __builtin_amdgcn_raw_buffer_load_b128(rk, off, step, 0)
+                                             : __builtin_amdgcn_raw_buffer_load_b128(rv, off, step, 0);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) raw[i][j] = x[j];
+                    for (int j = 0; j < 4; ++j) r.w[i][j] = x[j];
+                }
+            }
+            if constexpr (QUANT) {
+                const int osc = (p_key & 15) < left ? p_sc : 0x40000000;
+                const __amdgpu_buffer_rsrc_t sk = __builtin_amdgcn_make_buffer_rsrc((void *)(a.k_scales + row * nsc), (short)0,
+                                                                                    head_sc + 16 * nsc * 4, kDiffBufferWord3);
+                const __amdgpu_buffer_rsrc_t sv = __builtin_amdgcn_make_buffer_rsrc((void *)(a.v_scales + row * nsc), (short)0,
+                                                                                    head_sc + 16 * nsc * 4, kDiffBufferWord3);
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    const int part = (p_row0 + 8 * WR * i) / kDiffKeys, step = (part & 1) * head_sc;
+                    r.s[i] = __uint_as_float(part < 2 ? __builtin_amdgcn_raw_buffer_load_b32(sk, osc, step, 0)
+                                                      : __builtin_amdgcn_raw_buffer_load_b32(sv, osc, step, 0));
                 }
             }
         };
         // Scales and values of the tile in registers that leave f16's range are marked for all
         // waves; behind the barrier the tile is staged again under another power of two.
-        auto mark = [&](int t) {
+        auto mark = [&](int t, const Raw &r) __attribute__((always_inline)) {
             uint32_t k = 0, v = 0;                     // this lane's largest finite ones, as bits
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const bool val = (p_row0 + 8 * WR * i) / kDiffKeys >= 2;
                 if constexpr (QUANT) {
-                    const uint32_t y = __float_as_uint(rsc[i]) & 0x7FFFFFFFu, x = y < 0x7F800000u ? y : 0;
+                    const uint32_t y = __float_as_uint(r.s[i]) & 0x7FFFFFFFu, x = y < 0x7F800000u ? y : 0;
                     if (val) v = x > v ? x : v;
                     else k = x > k ? x : k;
                 } else if (val) {
@@ -275,35 +299,45 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                     u16x2 top = {0, 0};
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, raw[i][j] & 0x7FFF7FFFu));
+                        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, r.w[i][j] & 0x7FFF7FFFu));
                     uint32_t b = top[0] > top[1] ? top[0] : top[1];
                     if (b >= 0x7F80u) {
                         b = 0;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            const uint32_t x = raw[i][j / 2] >> (16 * (j & 1)) & 0x7FFFu;
+                            const uint32_t x = r.w[i][j / 2] >> (16 * (j & 1)) & 0x7FFFu;
                             b = x < 0x7F80u && x > b ? x : b;
                         }
                     }
                     v = b << 16 > v ? b << 16 : v;
                 }
             }
-            if (QUANT && (t == 0 || __uint_as_float(k) * fk >= kMost)) atomicMax(&s_top[t % 3][0], k);
-            if (t == 0 || __uint_as_float(v) * fv >= kMost) atomicMax(&s_top[t % 3][1], v);
+            if (t == 0) {                              // of all lanes: one atomic a wave
+                auto most = [](int x, int y) { return x > y ? x : y; };
+                if (QUANT) k = __builtin_amdgcn_readlane(wave_scan((int)k, most), 63);
+                v = __builtin_amdgcn_readlane(wave_scan((int)v, most), 63);
+                if (lane == 0) {
+                    if (QUANT) atomicMax(&s_top[0][0], k);
+                    atomicMax(&s_top[0][1], v);
+                }
+            } else {
+                if (QUANT && __uint_as_float(k) * fk >= kMost) atomicMax(&s_top[t % 3][0], k);
+                if (__uint_as_float(v) * fv >= kMost) atomicMax(&s_top[t % 3][1], v);
+            }
         };
         // the tile in registers into its buffer
-        auto write_tile = [&](int t) {
+        auto write_tile = [&](int t, const Raw &r) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const int part = (p_row0 + 8 * WR * i) / kDiffKeys;
                 const bool val = part >= 2;
                 u32x4 x;
                 if constexpr (QUANT) {
-                    const float s = rsc[i] * (val ? fv : fk);
-                    const f32x4 lo = code_values<DT>(raw[i][0], s), hi = code_values<DT>(raw[i][1], s);
+                    const float s = r.s[i] * (val ? fv : fk);
+                    const f32x4 lo = code_values<DT>(r.w[i][0], s), hi = code_values<DT>(r.w[i][1], s);
                     x = u32x4{pack2<true>(lo[0], lo[1]), pack2<true>(lo[2], lo[3]), pack2<true>(hi[0], hi[1]), pack2<true>(hi[2], hi[3])};
                 } else {
-                    x = u32x4{raw[i][0], raw[i][1], raw[i][2], raw[i][3]};
+                    x = u32x4{r.w[i][0], r.w[i][1], r.w[i][2], r.w[i][3]};
                     if (val) {
                         if (fv == 1.0f) {
 #pragma unroll
@@ -324,9 +358,9 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                         x[j / 2] &= ~(0xFFFFu << sh);
                         // a finite value that left the range: the tile is staged again
                         if constexpr (QUANT) {
-                            const float y = __builtin_fabsf(rsc[i]);
+                            const float y = __builtin_fabsf(r.s[i]);
                             if (y < INFINITY && y * fv >= kMost) continue;
-                        } else if ((raw[i][j / 2] >> sh & 0x7F80u) != 0x7F80u) {
+                        } else if ((r.w[i][j / 2] >> sh & 0x7F80u) != 0x7F80u) {
                             continue;
                         }
                         s_any = 1;
@@ -337,37 +371,53 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
             }
         };
 
-        load_tile(0);
-        __syncthreads();                               // the buffers of the block before are free
-        if (tid < 2 * D) s_bad[tid] = INT32_MAX;
-        if (tid == 0) s_any = 0;
-        if (tid < 6) s_top[tid / 2][tid % 2] = 0;
-        __syncthreads();
-        mark(0);
-        write_tile(0);
-        for (int t = 0; t < tiles; ++t) {
-            __syncthreads();                           // tile t is staged, tile t - 1 used
-            const uint32_t kt = __builtin_amdgcn_readfirstlane(s_top[t % 3][0]), vt = __builtin_amdgcn_readfirstlane(s_top[t % 3][1]);
-            if (tid < 2) s_top[(t + 2) % 3][tid] = 0;
-            if (kt | vt) {                             // the first tile, or one that left the range
-                const float kx = __uint_as_float(kt) * fk, vx = __uint_as_float(vt) * fv;
-                const bool newk = QUANT && kt && !(kx >= kLeast && kx < kMost), newv = vt && !(vx >= kLeast && vx < kMost);
-                if (newk || newv) {
-                    if (newk) fk = pow2_to(__uint_as_float(kt), kAim);
-                    if (newv) {                        // the sums follow when they are next rescaled
-                        const float now = pow2_to(__uint_as_float(vt), kAim);
-                        owed *= now / fv;
-                        fv = now;
-                    }
-                    write_tile(t);
-                    __syncthreads();
-                }
+        float fk_now = fk;                             // the keys' power of two of the present tile
+        // Behind the barrier after tile j was staged: whether its marks (largest key scale kt,
+        // value vt) ask for another power of two; then it has to be staged again.
+        auto settle = [&](uint32_t kt, uint32_t vt) __attribute__((always_inline)) -> bool {
+            const float kx = __uint_as_float(kt) * fk, vx = __uint_as_float(vt) * fv;
+            const bool newk = QUANT && kt && !(kx >= kLeast && kx < kMost), newv = vt && !(vx >= kLeast && vx < kMost);
+            if (newk) fk = pow2_to(__uint_as_float(kt), kAim);
+            if (newv) {
+                const float now = pow2_to(__uint_as_float(vt), kAim);
+                owed_next *= now / fv;
+                fv = now;
             }
-            if (t + 1 < tiles) load_tile(t + 1);
-            if (t * kDiffKeys <= sees1) {              // some row of this wave sees some of it
-                const float ft = qs / fk;
-                const uint8_t *sk = s_t(t) + mp * HB, *sv = s_t(t) + 2 * HB;
-                f32x16 sc;
+            return newk || newv;
+        };
+        Raw raw;
+        {
+            Raw r0;
+            load_tile(0, r0);
+            if (1 < tiles) load_tile(1, raw);
+            __syncthreads();                           // the buffers of the block before are free
+            if (tid < 2 * D) s_bad[tid] = INT32_MAX;
+            if (tid == 0) s_any = 0;
+            if (tid < 6) s_top[tid / 2][tid % 2] = 0;
+            __syncthreads();
+            mark(0, r0);
+            write_tile(0, r0);
+            __syncthreads();
+            if (settle(__builtin_amdgcn_readfirstlane(s_top[0][0]), __builtin_amdgcn_readfirstlane(s_top[0][1]))) {
+                write_tile(0, r0);
+                __syncthreads();
+            }
+            if (1 < tiles) {
+                mark(1, raw);
+                write_tile(1, raw);
+                if (2 < tiles) load_tile(2, raw);
+            }
+        }
+        fk_now = fk;
+        owed_next = 1.0f;                              // the sums are empty
+        f32x16 sc;
+        // A tile is staged two ahead, with one barrier a tile.  Map 0's waves pass it before
+        // a tile's first product, map 1's between that product and the softmax, so that on
+        // each SIMD one wave's products meet the other's arithmetic.
+        for (int t = 0; t < tiles; ++t) {
+            const bool some = t * kDiffKeys <= sees1;  // some row of this wave sees some of it
+            auto scores = [&]() __attribute__((always_inline)) {
+                const uint8_t *sk = s_t(t) + mp * HB;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
                 {
@@ -383,6 +433,23 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                     for (int s = 0; s < KS; ++s) sc = mfma<QUANT>(kf[s], qf[s], sc);
                     read_ahead<KS, AHEAD, 1>();
                 }
+            };
+            if (mp && some) scores();
+            __syncthreads();                           // tile t + 1 is staged, tile t - 1 used
+            const uint32_t kt = s_top[(t + 1) % 3][0], vt = s_top[(t + 1) % 3][1];
+            if (tid < 2) s_top[t % 3][tid] = 0;
+            if (!mp && some) scores();
+            if (__builtin_amdgcn_readfirstlane(kt | vt)) {
+                if (settle(__builtin_amdgcn_readfirstlane(kt), __builtin_amdgcn_readfirstlane(vt))) {       // rare
+                    load_tile(t + 1, raw);
+                    write_tile(t + 1, raw);
+                    __syncthreads();
+                    if (t + 2 < tiles) load_tile(t + 2, raw);
+                }
+            }
+            if (some) {
+                const float ft = qs / fk_now;
+                const uint8_t *sv = s_t(t) + 2 * HB;
                 const bool cut = t * kDiffKeys + kDiffKeys - 1 > sees0;
                 if (cut) {
                     const int lim = sees - t * kDiffKeys;
@@ -444,10 +511,14 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                     for (int s = 0; s < 2; ++s) acc[c] = mfma<true>(vf[c][s], p[s], acc[c]);
                 read_ahead<2 * CT, 3, 2>();
             }
-            if (t + 1 < tiles) {
-                mark(t + 1);
-                write_tile(t + 1);
+            if (t + 2 < tiles) {
+                mark(t + 2, raw);
+                write_tile(t + 2, raw);
+                if (t + 3 < tiles) load_tile(t + 3, raw);
             }
+            fk_now = fk;
+            owed *= owed_next;
+            owed_next = 1.0f;
         }
 
         // lane (n, h): columns 32 c + 8 (i / 4) + 4 h + i % 4 of row n in acc[c][i]

@@ -63,8 +63,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     for (; u < end; diff_next(a, s_pre, sq, it)) {
         diff_seq(a, it.b, sq);
         const int64_t nt = sq.tiles(it.k), len = sq.prefix + sq.q;
-        const int64_t left = nt + kDiffBlockCost - it.from, mine = end - u < left ? end - u : left;
-        const int64_t t0 = diff_tile_of(it.from), t1 = diff_tile_of(it.from + mine);
+        const int64_t left = nt + a.extra - it.from, mine = end - u < left ? end - u : left;
+        const int64_t t0 = diff_tile_of(it.from, a.extra), t1 = diff_tile_of(it.from + mine, a.extra);
         u += mine;
         if (t0 == t1) continue;                        // the slice ends before the block's first tile
         const bool whole = t0 == 0 && t1 == nt;

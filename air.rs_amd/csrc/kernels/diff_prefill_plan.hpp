@@ -4,8 +4,8 @@
 // A sequence's rows are its (new token, query pair of the K/V pair) combinations,
 // token after token: row f is token f / g, pair f % g.  A block is `rows`
 // consecutive ones; it needs the keys its last token sees, in tiles of kDiffKeys.
-// A block counts as kDiffBlockCost units (what beginning and ending it costs, in
-// tiles' time) and one for each of its tiles; a K/V pair's units, sequence after
+// A block counts as `extra` units (what beginning and ending it costs, in tiles'
+// time) and one for each of its tiles; a K/V pair's units, sequence after
 // sequence, block after block, are cut into equal slices, one workgroup each.  The
 // slice that holds a block's first tile begins it.
 #pragma once
@@ -21,7 +21,6 @@
 namespace airkv {
 
 constexpr int kDiffKeys = 32;
-constexpr int kDiffBlockCost = 4;
 
 // sum of floor((a * i + b) / m) over i = 0 .. n - 1, by the Euclidean descent on
 // (m, a): lattice points under a line, exchanging the axes at each step.
@@ -50,7 +49,7 @@ AIRKV_DP_HD inline uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64
 // One sequence: q new tokens behind `prefix` cached ones, g query pairs.
 struct DiffBlocks {
     int64_t q, prefix;
-    int g, rows;
+    int g, rows, extra;
     AIRKV_DP_HD int64_t blocks() const { return (q * g + rows - 1) / rows; }
     // keys and key tiles of block k: up to the last token it holds
     AIRKV_DP_HD int64_t keys(int64_t k) const {
@@ -59,9 +58,9 @@ struct DiffBlocks {
     }
     AIRKV_DP_HD int64_t tiles(int64_t k) const { return (keys(k) + kDiffKeys - 1) / kDiffKeys; }
     // units of block k, and of the blocks before it (k < blocks(): all of them full)
-    AIRKV_DP_HD int64_t cost(int64_t k) const { return kDiffBlockCost + tiles(k); }
+    AIRKV_DP_HD int64_t cost(int64_t k) const { return extra + tiles(k); }
     AIRKV_DP_HD int64_t before(int64_t k) const {
-        return kDiffBlockCost * k + (int64_t)floor_sum((uint64_t)k, (uint64_t)kDiffKeys * g, (uint64_t)rows,
+        return extra * k + (int64_t)floor_sum((uint64_t)k, (uint64_t)kDiffKeys * g, (uint64_t)rows,
                                   (uint64_t)(prefix + kDiffKeys) * g + rows - 1);
     }
     AIRKV_DP_HD int64_t units() const {
@@ -71,7 +70,7 @@ struct DiffBlocks {
 };
 
 // The tiles [t0, t1) of a block that its units [from, to) hold.
-AIRKV_DP_HD inline int64_t diff_tile_of(int64_t unit) { return unit > kDiffBlockCost ? unit - kDiffBlockCost : 0; }
+AIRKV_DP_HD inline int64_t diff_tile_of(int64_t unit, int extra) { return unit > extra ? unit - extra : 0; }
 
 // Units per slice: an equal share, but at least `least`, so that small launches
 // are not cut into pieces whose joining costs more than their work.

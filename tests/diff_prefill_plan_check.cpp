@@ -25,7 +25,7 @@ static void sums(DiffBlocks s) {
         // the keys its last row sees, counted row by row
         const int64_t last = std::min((k + 1) * s.rows, s.q * s.g) - 1;
         check(s.keys(k) == s.prefix + last / s.g + 1, "keys of a block", s.q, s.prefix, k);
-        at += kDiffBlockCost + (s.keys(k) + kDiffKeys - 1) / kDiffKeys;
+        at += s.extra + (s.keys(k) + kDiffKeys - 1) / kDiffKeys;
     }
     check(s.units() == at, "units of a sequence", s.q, s.prefix, s.g);
 }
@@ -48,9 +48,9 @@ static void walk(const std::vector<DiffBlocks> &seqs, int64_t slices, int64_t le
             const DiffBlocks &s = seqs[b];
             int64_t k = 0;
             while (k + 1 < s.blocks() && s.before(k + 1) <= u - pre[b]) ++k;
-            const int64_t from = u - pre[b] - s.before(k), nt = s.tiles(k), mine = std::min(end - u, kDiffBlockCost + nt - from);
+            const int64_t from = u - pre[b] - s.before(k), nt = s.tiles(k), mine = std::min(end - u, s.extra + nt - from);
             check(from >= 0 && mine > 0, "a block's units", b, k, from);
-            const int64_t t0 = diff_tile_of(from), t1 = diff_tile_of(from + mine);
+            const int64_t t0 = diff_tile_of(from, s.extra), t1 = diff_tile_of(from + mine, s.extra);
             check(t0 <= t1 && t1 <= nt && (done[{b, k}]) == t0, "a block's tiles in order", b, k, t0);
             done[{b, k}] = t1;
             u += mine;
@@ -83,12 +83,12 @@ int main() {
         ++cases;
     }
     for (int i = 0; i < 1500; ++i)
-        sums({pick(0, 900), i % 3 ? pick(0, 5000) : 0, pick(1, i % 5 ? 16 : 300), i % 2 ? 64 : 128});
-    sums({131072, 1 << 20, 8, 64});                    // sums of long sequences stay exact
+        sums({pick(0, 900), i % 3 ? pick(0, 5000) : 0, pick(1, i % 5 ? 16 : 300), i % 2 ? 64 : 128, i % 8});
+    sums({131072, 1 << 20, 8, 64, 7});                   // sums of long sequences stay exact
     for (int i = 0; i < 600; ++i) {
         std::vector<DiffBlocks> seqs;
-        const int g = pick(1, 20), rows = i % 2 ? 64 : 128;
-        for (int n = pick(1, 12); n > 0; --n) seqs.push_back({pick(0, 3) ? pick(1, 200) : 0, pick(0, 2) ? pick(0, 2000) : 0, g, rows});
+        const int g = pick(1, 20), rows = i % 2 ? 64 : 128, extra = pick(0, 9);
+        for (int n = pick(1, 12); n > 0; --n) seqs.push_back({pick(0, 3) ? pick(1, 200) : 0, pick(0, 2) ? pick(0, 2000) : 0, g, rows, extra});
         for (auto &s : seqs)
             if (!s.q) s.prefix = 0;
         walk(seqs, pick(1, 140), pick(1, 32));
