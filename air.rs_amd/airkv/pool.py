@@ -304,14 +304,14 @@ class KvPool:
 
     # -- differential attention ---------------------------------------------------
 
-    def diff_decode_workspace_size(self, n_q_heads, batch, max_blocks, max_splits=64):
+    def diff_decode_workspace_size(self, n_q_heads, batch, max_blocks, max_splits=256):
         out = ctypes.c_size_t()
         _lib.check(_lib.load().air_paged_diff_decode_workspace_size(self.handle, n_q_heads, batch, max_blocks,
                                                                     max_splits, ctypes.byref(out)),
                    "air_paged_diff_decode_workspace_size")
         return out.value
 
-    def new_diff_workspace(self, n_q_heads, batch, max_blocks, max_splits=64):
+    def new_diff_workspace(self, n_q_heads, batch, max_blocks, max_splits=256):
         torch = _torch()
         n = self.diff_decode_workspace_size(n_q_heads, batch, max_blocks, max_splits)
         return torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
@@ -368,7 +368,7 @@ class KvPool:
             ws_at, workspace.nbytes) + tail, workspace
 
     def paged_diff_decode(self, q, lam, block_tables, seq_lens, out, norm_weight=None, norm_eps=None, out_scale=1.0,
-                          scale=None, max_splits=64, workspace=None, stream=None):
+                          scale=None, max_splits=256, workspace=None, stream=None):
         """Differential attention of one token per sequence (air_paged_diff_decode):
         K/V heads 2p and 2p + 1 are a pair, as are query heads 2h and 2h + 1, and
         out[b, h] = out_scale * norm((P_0 - lam P_1) [V_2p | V_2p+1]).  q [batch,
@@ -380,7 +380,7 @@ class KvPool:
         return out
 
     def bind_diff_decode(self, q, lam, block_tables, seq_lens, out, norm_weight=None, norm_eps=None, out_scale=1.0,
-                         scale=None, max_splits=64, workspace=None, stream=None):
+                         scale=None, max_splits=256, workspace=None, stream=None):
         """Validate once, return a zero-argument launcher."""
         args, ws = self._diff_decode_args(q, lam, block_tables, seq_lens, out, norm_weight, norm_eps, out_scale,
                                           scale, max_splits, workspace, stream)

@@ -36,20 +36,11 @@ typedef uint32_t diff_u32x2 __attribute__((ext_vector_type(2)));
 constexpr int kDiffBufferWord3 = 0x00020000;       // raw buffer access
 constexpr int kDiffStream = 2;                     // non-temporal: pages are read once
 
-// Codes whose exponent field is zero decode to zero (the pools' E4M3 has no
-// subnormal numbers, the hardware's has): the bytes of w that hold one, cleared.
-// A field of 8 or more (it is kept in place) carries into bit 7 when 0x78 is
-// added, so h marks the bytes to keep, and 255 times its marks is their mask.
-__device__ __forceinline__ uint32_t fp8_no_subnormals(uint32_t w) {
-    const uint32_t h = ((w & 0x78787878u) + 0x78787878u) & 0x80808080u;
-    return w & ((h << 1) - (h >> 7));
-}
-
 // The values of the four 1-byte codes in w times their scale, each rounded once:
 // int8 as (code + 128) * s - 128 s in one fused step, fp8 by the hardware's
-// conversion (exact) and a product.  0xFF, -480 in the pools' E4M3 and NaN in
-// the hardware's, is a code the append never writes; it reads as NaN here, as in
-// the matrix-core kernels of paged_decode and paged_prefill.
+// conversion (exact) and a product.  The pools' E4M3 and the hardware's differ
+// in codes that the append never writes only (zero exponents are +-0, no 0xFF);
+// they read as the hardware's here, as in the other matrix-core kernels.
 template <int DT>
 __device__ __forceinline__ diff_f32x4 code_values(uint32_t w, float s) {
     if constexpr (DT == AIR_KV_INT8) {
@@ -59,7 +50,6 @@ __device__ __forceinline__ diff_f32x4 code_values(uint32_t w, float s) {
                           __builtin_fmaf((float)((u >> 16) & 0xFFu), s, off), __builtin_fmaf((float)(u >> 24), s, off)};
     } else {
         typedef float f32x2 __attribute__((ext_vector_type(2)));
-        w = fp8_no_subnormals(w);
         const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
         return diff_f32x4{lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
     }
@@ -74,6 +64,11 @@ __device__ __forceinline__ void diff_store4(const DiffOut &e, int64_t idx, diff_
             diff_u32x2{(uint32_t)bf16_rne(v[0]) | ((uint32_t)bf16_rne(v[1]) << 16),
                        (uint32_t)bf16_rne(v[2]) | ((uint32_t)bf16_rne(v[3]) << 16)};
     }
+}
+// Two (idx even).
+__device__ __forceinline__ void diff_store2(const DiffOut &e, int64_t idx, float x, float y) {
+    if (e.out_dtype == AIR_KV_F32) *reinterpret_cast<float2 *>((float *)e.out + idx) = make_float2(x, y);
+    else *reinterpret_cast<uint32_t *>((uint16_t *)e.out + idx) = (uint32_t)bf16_rne(x) | ((uint32_t)bf16_rne(y) << 16);
 }
 __device__ __forceinline__ void diff_store(const DiffOut &e, int64_t idx, float v) {
     if (e.out_dtype == AIR_KV_F32) ((float *)e.out)[idx] = v;

@@ -28,6 +28,8 @@ namespace airkv {
 namespace {
 
 typedef diff_f32x4 f32x4;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = kSliceThreads;
 constexpr int kWaves = kThreads / 64;
@@ -44,63 +46,103 @@ __device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
+__device__ __forceinline__ f32x4 mfma_bf16(diff_u32x4 a, diff_u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma_bf16(diff_u32x2 a, diff_u32x2 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+}
+
+// The upper (HI) or lower halves of two words, a's in the low half.
+template <bool HI> __device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b) {
+    return __builtin_amdgcn_perm(b, a, HI ? 0x07060302u : 0x05040100u);
+}
+
+// x, y = the sum of three bf16 pairs, each holding the next eight bits: exact,
+// and every part has its value's sign.
+__device__ __forceinline__ void split3(float x, float y, uint32_t &p0, uint32_t &p1, uint32_t &p2) {
+    p0 = halves<true>(__float_as_uint(x), __float_as_uint(y));
+    x -= __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+    y -= __uint_as_float(__float_as_uint(y) & 0xFFFF0000u);
+    p1 = halves<true>(__float_as_uint(x), __float_as_uint(y));
+    x -= __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+    y -= __uint_as_float(__float_as_uint(y) & 0xFFFF0000u);
+    p2 = halves<true>(__float_as_uint(x), __float_as_uint(y));
+}
+
+// Eight 1-byte codes as bf16, exactly.
+template <int DT> __device__ __forceinline__ diff_u32x4 codes_bf16(const uint32_t (&w)[2]) {
+    diff_u32x4 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t c = w[i / 2];
+        if constexpr (DT == AIR_KV_INT8) {
+            const float lo = (float)(int8_t)(c >> (16 * (i & 1))), hi = (float)(int8_t)(c >> (16 * (i & 1) + 8));
+            x[i] = halves<true>(__float_as_uint(lo), __float_as_uint(hi));
+        } else {
+            x[i] = (i & 1) ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c, 1.0f, true))
+                           : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c, 1.0f, false));
+        }
+    }
+    return x;
+}
+
 // x of lane l ^ 8 within each 16 lanes.
 __device__ __forceinline__ float dpp_ror8(float x) {
     return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xF, 0xF, false));
 }
 
-// BYTES (2, 4, 8, 16 or 32) bytes of a page at `off`.
+// BYTES (2, 4, 8, 12, 16 or 32) bytes of a page at base + off.
 template <int BYTES>
-__device__ __forceinline__ void load_piece(const __amdgpu_buffer_rsrc_t &r, int off, uint32_t (&w)[(BYTES + 3) / 4]) {
+__device__ __forceinline__ void load_piece(const __amdgpu_buffer_rsrc_t &r, int off, int base,
+                                           uint32_t (&w)[(BYTES + 3) / 4]) {
     if constexpr (BYTES == 2) {
-        w[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, 0, kDiffStream);
+        w[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, base, kDiffStream);
     } else if constexpr (BYTES == 4) {
-        w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, kDiffStream);
+        w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, base, kDiffStream);
     } else if constexpr (BYTES == 8) {
-        const diff_u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, kDiffStream);
+        const diff_u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off, base, kDiffStream);
         w[0] = x[0]; w[1] = x[1];
+    } else if constexpr (BYTES == 12) {
+        const auto x = __builtin_amdgcn_raw_buffer_load_b96(r, off, base, kDiffStream);
+        w[0] = x[0]; w[1] = x[1]; w[2] = x[2];
     } else {
 #pragma unroll
         for (int i = 0; i < BYTES / 16; ++i) {
-            const diff_u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * i, 0, kDiffStream);
+            const diff_u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * i, base, kDiffStream);
             w[4 * i] = x[0]; w[4 * i + 1] = x[1]; w[4 * i + 2] = x[2]; w[4 * i + 3] = x[3];
         }
     }
 }
 
-// N consecutive elements of a page row as f32.
-template <int DT, int N, int W>
-__device__ __forceinline__ void widen(const uint32_t (&w)[W], float s, float (&x)[N]) {
-    if constexpr (DT == AIR_KV_F32) {
+// N 1-byte codes times their scale.
+template <int DT, int N> __device__ __forceinline__ void widen(const uint32_t *w, float s, float *x) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = __uint_as_float(w[i]);
-    } else if constexpr (DT == AIR_KV_BF16) {
+    for (int i = 0; i < N; i += 4) {
+        const f32x4 v = code_values<DT>(w[i / 4], s);
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = __uint_as_float((i & 1) ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
-    } else {
-#pragma unroll
-        for (int i = 0; i < (N + 3) / 4; ++i) {
-            const f32x4 v = code_values<DT>(w[i], s);
-#pragma unroll
-            for (int j = 0; j < 4 && 4 * i + j < N; ++j) x[4 * i + j] = v[j];
-        }
+        for (int j = i; j < i + 4 && j < N; ++j) x[j] = v[j - i];
     }
 }
 
-template <int D, int DT>
+template <int D, int DT, bool WIDE, bool FINE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerSimd, kWavesPerSimd)))
 void diff_decode_kernel(DiffDecodeArgs a) {
     static_assert(D % 32 == 0 && D <= 128, "steps of 32, two value heads of at most 256 columns");
-    constexpr bool QUANT = DT == AIR_KV_INT8 || DT == AIR_KV_FP8;
+    constexpr bool F32 = DT == AIR_KV_F32, QUANT = DT == AIR_KV_INT8 || DT == AIR_KV_FP8;
     constexpr int EB = DT == AIR_KV_F32 ? 4 : DT == AIR_KV_BF16 ? 2 : 1;
     constexpr int KS = D / 32;                         // steps of the first product
+    constexpr int NS = FINE ? D / 8 : KS, SL = (16 * NS + 63) / 64;  // scales of a row at most, a lane's loads of them
+    constexpr int QP = WIDE ? 3 : 1;                   // bf16 parts of a query
     // columns of a value head in a lane: CA from CA * m, then CB from 16 * CA + CB * m
-    // (96 as 64 + 32: a run of 6 columns would straddle scale groups)
+    // (96 as 64 + 32: every run a power of two). 
     constexpr int CA = D == 96 ? 4 : D / 16, CB = D == 96 ? 2 : 0, C = CA + CB;
+    constexpr int PW = D % 64 == 0 ? 4 : 2, PC = C / PW, NP = 4 * PC;      // pieces of consecutive columns of a lane
     constexpr int KW = 8 * EB / 4, VA = (CA * EB + 3) / 4, VB = CB ? (CB * EB + 3) / 4 : 1;
 
     __shared__ int32_t s_pre[kMaxBatch + 2];
     __shared__ int32_t s_wsum[kWaves];
+    __shared__ f32x4 s_scale[QUANT ? kWaves : 1][2][2][NS][4];       // K and V; [head][group] of 16 tokens
 
     const int bs = a.block_size;
     tile_prefix(a, bs, s_pre, s_wsum);
@@ -128,8 +170,9 @@ void diff_decode_kernel(DiffDecodeArgs a) {
     const int qp = r16 & 7;                                             // this lane's row: map r16 / 8 of pair qp
     const bool map1 = r16 >= 8;
     const bool live_row = qp < rows;
+    const bool wide_q = WIDE && a.q_dtype == AIR_KV_F32, wide_out = WIDE && a.e.out_dtype == AIR_KV_F32;
 
-    // Lane k describes tile c0 + k of a window of 64: block, tile within its sequence, valid tokens.
+    // Lane k describes tile c0 + k of a window of 64: block, its first row there, sequence, valid tokens.
     int32_t tbl = 0, seq_l = 0, j_l = 0, nv_l = 0;
     uint64_t first_m = 0, last_m = 0;
     auto load_window = [&](int c0) {
@@ -137,9 +180,10 @@ void diff_decode_kernel(DiffDecodeArgs a) {
         const int bq = seq_of_tile(s_pre, B, t);
         const int j = t - s_pre[bq];
         const int64_t len = clamp_len(a.lens[bq], max_len);
-        tbl = a.tables[(int64_t)bq * a.max_blocks + (int64_t)16 * j / bs];
+        const int per = bs / 16, in_row = j / per;     // tiles of a block; the tile's block
+        tbl = a.tables[(int64_t)bq * a.max_blocks + in_row];
         seq_l = bq;
-        j_l = j;
+        j_l = 16 * (j - in_row * per);
         const int64_t rest = len - 16 * (int64_t)j;
         nv_l = rest < 16 ? (int)rest : 16;
         const bool valid = c0 + lane < hi;
@@ -147,26 +191,55 @@ void diff_decode_kernel(DiffDecodeArgs a) {
         last_m = __ballot(valid && (t + 1 == hi || t + 1 == s_pre[bq + 1]));
     };
 
-    // Q^T as the B operand: lane (n, q) holds row n's elements 32 s + 8 q .. +8
-    float qf[KS][8];
+    // Q^T as the B operand: lane (n, q) holds eight of row n's elements from 32 s + q_at
+    // (order_k leaves the keys' elements in this order)
+    const int q_at = QUANT ? 16 * (q4 & 1) + 8 * (q4 >> 1) : 8 * q4;
+    // (f32 pages), or the same as bf16 parts: bf16 queries one, f32 queries three
+    float qf[F32 ? KS : 1][8];
+    diff_u32x4 qb[F32 || !WIDE ? 1 : 3][KS];
     auto load_q = [&](int bq) {
         const int head = 2 * (kp * a.group + 8 * rt + qp) + (map1 ? 1 : 0);
-        const int64_t at = ((int64_t)bq * a.n_q_heads + (live_row ? head : 0)) * D + 8 * q4;
+        const int64_t at = ((int64_t)bq * a.n_q_heads + (live_row ? head : 0)) * D + q_at;
+        if (wide_q) {
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            if (a.q_dtype == AIR_KV_F32) {
+            for (int s = 0; s < KS; ++s) {
                 const f32x4 *p = reinterpret_cast<const f32x4 *>((const float *)a.q + at + 32 * s);
                 const f32x4 x = p[0], y = p[1];
+                if constexpr (F32) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    qf[s][j] = x[j];
-                    qf[s][4 + j] = y[j];
+                    for (int j = 0; j < 8; ++j) qf[s][j] = j < 4 ? x[j] : y[j - 4];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t w[3];
+                        const f32x4 z = j < 2 ? x : y;
+                        split3(z[2 * (j & 1)], z[2 * (j & 1) + 1], w[0], w[1], w[2]);
+#pragma unroll
+                        for (int k = 0; k < (WIDE ? 3 : 1); ++k) qb[k][s][j] = w[k];
+                    }
                 }
-            } else {
-                const diff_u32x4 x = *reinterpret_cast<const diff_u32x4 *>((const uint16_t *)a.q + at + 32 * s);
+            }
+        } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    qf[s][j] = __uint_as_float((j & 1) ? x[j / 2] & 0xFFFF0000u : x[j / 2] << 16);
+            for (int s = 0; s < KS; ++s) {
+                const diff_u32x4 x = *reinterpret_cast<const diff_u32x4 *>((const uint16_t *)a.q + at + 32 * s);
+                if constexpr (F32) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        qf[s][j] = __uint_as_float((j & 1) ? x[j / 2] & 0xFFFF0000u : x[j / 2] << 16);
+                } else {
+                    qb[0][s] = x;
+                }
+            }
+        }
+        // waited for here: where no sequence starts, the loads of tiles stay in flight
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            if constexpr (F32) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(qf[s][j]));
+            } else {
+                asm volatile("" : "+v"(qb[0][s]));
             }
         }
     };
@@ -174,10 +247,13 @@ void diff_decode_kernel(DiffDecodeArgs a) {
     f32x4 acc[2][C];                                   // O^T: value head, column of the lane
     float m_run = -INFINITY, l_run = 0.0f;
 
-    const int nsc = QUANT ? D / a.scale_group : 0;     // scales per row
-    // The column of acc[t][j][i] of this lane
-    auto col = [&](int t, int j, int i) {
-        const int m = 4 * q4 + i;
+    const int sg = QUANT ? FINE ? __builtin_ctz(a.scale_group) : 5 : 0, nsc = D >> sg;      // scales per row
+    // Piece i of a value head: its values and the first's column
+    auto piece = [&](int t, int i, float (&x)[PW]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < PW; ++e)
+            x[e] = acc[t][PW * (i % PC) + e][i / PC];
+        const int m = 4 * q4 + i / PC, j = PW * (i % PC);
         return t * D + (j < CA ? CA * m + j : 16 * CA + CB * m + j - CA);
     };
 
@@ -205,19 +281,22 @@ void diff_decode_kernel(DiffDecodeArgs a) {
             const float f = diff_factor(a.e, a.e.norm ? sum_x32(sum_x16(ss)) : 0.0f, 2 * D);
             if (live_row && !map1) {
                 const int64_t at = ((int64_t)bq * a.pairs + h) * (2 * D);
+                // no weights: an empty view, which reads as zeros
+                const bool weights = a.e.norm && a.e.norm_w;
+                const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
+                    (void *)a.e.norm_w, (short)0, weights ? 2 * D * 4 : 0, kDiffBufferWord3);
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float x[C];
+                    for (int i = 0; i < NP; ++i) {
+                        float x[PW];
+                        const int c = piece(t, i, x);
+                        uint32_t wt[PW];
+                        load_piece<4 * PW>(rw, 4 * c, 0, wt);
 #pragma unroll
-                        for (int j = 0; j < C; ++j)
-                            x[j] = acc[t][j][i] * ((a.e.norm && a.e.norm_w) ? f * a.e.norm_w[col(t, j, i)] : f);
-#pragma unroll
-                        for (int j = 0; j + 4 <= CA; j += 4)
-                            diff_store4(a.e, at + col(t, j, i), f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]});
-#pragma unroll
-                        for (int j = CA / 4 * 4; j < C; ++j) diff_store(a.e, at + col(t, j, i), x[j]);
+                        for (int e = 0; e < PW; ++e) x[e] *= weights ? f * __uint_as_float(wt[e]) : f;
+                        if constexpr (PW == 4) diff_store4(a.e, at + c, f32x4{x[0], x[1], x[2], x[3]});
+                        else diff_store2(a.e, at + c, x[0], x[1]);
                     }
             }
         } else if (live_row) {
@@ -226,13 +305,11 @@ void diff_decode_kernel(DiffDecodeArgs a) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                    for (int j = 0; j + 4 <= CA; j += 4)
-                        *reinterpret_cast<f32x4 *>(po + col(t, j, i)) =
-                            f32x4{acc[t][j][i], acc[t][j + 1][i], acc[t][j + 2][i], acc[t][j + 3][i]};
-#pragma unroll
-                    for (int j = CA / 4 * 4; j < C; ++j) po[col(t, j, i)] = acc[t][j][i];
+                for (int i = 0; i < NP; ++i) {
+                    float x[PW];
+                    const int c = piece(t, i, x);
+                    if constexpr (PW == 4) *reinterpret_cast<f32x4 *>(po + c) = f32x4{x[0], x[1], x[2], x[3]};
+                    else *reinterpret_cast<float2 *>(po + c) = make_float2(x[0], x[1]);
                 }
             if (q4 == 0) {
                 a.part_ml[row * 2] = m_run;
@@ -241,60 +318,116 @@ void diff_decode_kernel(DiffDecodeArgs a) {
         }
     };
 
-    auto tile = [&](int k, int idx) {
-        int32_t blk = __builtin_amdgcn_readlane(tbl, idx);
-        const int jt = __builtin_amdgcn_readlane(j_l, idx);
+    // The next tile: its first row (of the pair's first head; the second's are bs further), its tokens and flags
+    int64_t row0 = 0;
+    int nv = 0, bq = 0;
+    bool first = false, last = false;
+    auto look = [&](int k) __attribute__((always_inline)) {
+        const int idx = (k - lo) & 63;
+        if (idx == 0) load_window(k);
+        const int blk = __builtin_amdgcn_readlane(tbl, idx), jt = __builtin_amdgcn_readlane(j_l, idx);
         const bool ok = blk >= 0 && blk < a.num_blocks;
-        blk = ok ? blk : 0;
-        // rows of the pair's first head; the second's are bs further
-        const int64_t row0 = ((int64_t)blk * a.n_kv_heads + 2 * kp) * bs + (int64_t)16 * jt % bs;
-        const int span = (bs + 16) * D * EB;           // to the end of the second head's tile
-        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
-            (void *)((const char *)a.k_pages + row0 * D * EB), (short)0, span, kDiffBufferWord3);
-        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
-            (void *)((const char *)a.v_pages + row0 * D * EB), (short)0, span, kDiffBufferWord3);
-        uint32_t kr[2][KS][KW], va[2][4][VA], vb[2][4][VB];
-        float ksc[2][KS], vsa[2][4], vsb[2][4];
+        row0 = ((int64_t)(ok ? blk : 0) * a.n_kv_heads + 2 * kp) * bs + jt;
+        nv = ok ? __builtin_amdgcn_readlane(nv_l, idx) : 0;
+        bq = __builtin_amdgcn_readlane(seq_l, idx);
+        first = (first_m >> idx) & 1;
+        last = (last_m >> idx) & 1;
+        // an entry outside the pool is counted once, by the first pair's wave, and its tile masked
+        if (!ok && lane == 0 && hh == 0) atomicAdd(a.errors, 1ull);
+    };
+    // The tile at `row`, `width` bytes a row, to the end of the second head's (nothing, unless `in`)
+    auto view = [&](const void *p, int64_t row, int width, bool in) __attribute__((always_inline)) {
+        return __builtin_amdgcn_make_buffer_rsrc((void *)((const char *)p + row * width), (short)0,
+                                                 in ? (bs + 16) * width : 0, kDiffBufferWord3);
+    };
+    constexpr int VW = VA + (CB ? VB : 0);
+    uint32_t kr[2][KS][KW], vr[2][4][VW];
+    uint32_t ksc[2][SL], vsc[2][SL];                   // a tile's scales in order, either head's
+    const int head1 = bs * D * EB;                     // the second head's rows, in bytes
+    auto load_scales = [&](const float *p, bool in, uint32_t (&x)[2][SL]) __attribute__((always_inline)) {
+        const __amdgpu_buffer_rsrc_t rs = view(p, row0, 4 * nsc, in);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < SL; ++i)
+                x[t][i] = __builtin_amdgcn_raw_buffer_load_b32(rs, lane + 64 * i < 16 * nsc ? 4 * lane + 256 * i : 0x40000000,
+                                                               t ? 4 * bs * nsc : 0, kDiffStream);
+    };
+    auto load_k = [&](bool in) __attribute__((always_inline)) {
+        const __amdgpu_buffer_rsrc_t rk = view(a.k_pages, row0, D * EB, in);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int s = 0; s < KS; ++s)
-                load_piece<8 * EB>(rk, ((t * bs + r16) * D + 32 * s + 8 * q4) * EB, kr[t][s]);
+                if (QUANT && (s | 1) < KS) {           // 64 bytes of a row at once; order_k makes steps of them
+                    if (s & 1) continue;
+                    uint32_t w[4];
+                    load_piece<16>(rk, r16 * D + 32 * s + 16 * q4, t ? head1 : 0, w);
+                    kr[t][s][0] = w[0]; kr[t][s][1] = w[1];
+                    kr[t][s + 1][0] = w[2]; kr[t][s + 1][1] = w[3];
+                } else {
+                    load_piece<8 * EB>(rk, (r16 * D + 32 * s + q_at) * EB, t ? head1 : 0, kr[t][s]);
+                }
+        if constexpr (QUANT) {
+            load_scales(a.k_scales, in, ksc);
+        }
+    };
+    auto load_v = [&](bool in) __attribute__((always_inline)) {
+        const __amdgpu_buffer_rsrc_t rv = view(a.v_pages, row0, D * EB, in);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int at = (t * bs + 4 * q4 + i) * D;
-                load_piece<CA * EB>(rv, (at + CA * r16) * EB, va[t][i]);
-                if constexpr (CB > 0) load_piece<CB * EB>(rv, (at + 16 * CA + CB * r16) * EB, vb[t][i]);
-            }
-        if constexpr (QUANT) {
-            const int sspan = (bs + 16) * nsc * 4;
-            const __amdgpu_buffer_rsrc_t rks = __builtin_amdgcn_make_buffer_rsrc(
-                (void *)(a.k_scales + row0 * nsc), (short)0, sspan, kDiffBufferWord3);
-            const __amdgpu_buffer_rsrc_t rvs = __builtin_amdgcn_make_buffer_rsrc(
-                (void *)(a.v_scales + row0 * nsc), (short)0, sspan, kDiffBufferWord3);
+                const int at = (4 * q4 + i) * D;
+                {
+                    uint32_t w[VA], z[VB];
+                    load_piece<CA * EB>(rv, (at + CA * r16) * EB, t ? head1 : 0, w);
+                    if constexpr (CB > 0) load_piece<CB * EB>(rv, (at + 16 * CA + CB * r16) * EB, t ? head1 : 0, z);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                for (int s = 0; s < KS; ++s)
-                    ksc[t][s] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                        rks, ((t * bs + r16) * nsc + (32 * s + 8 * q4) / a.scale_group) * 4, 0, kDiffStream));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int at = (t * bs + 4 * q4 + i) * nsc;
-                    vsa[t][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                        rvs, (at + CA * r16 / a.scale_group) * 4, 0, kDiffStream));
-                    if constexpr (CB > 0)
-                        vsb[t][i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                            rvs, (at + (16 * CA + CB * r16) / a.scale_group) * 4, 0, kDiffStream));
+                    for (int j = 0; j < VW; ++j) vr[t][i][j] = j < VA ? w[j] : z[j - VA];
                 }
             }
+        if constexpr (QUANT) {
+            load_scales(a.v_scales, in, vsc);
         }
+    };
 
-        const int bq = __builtin_amdgcn_readlane(seq_l, idx);
-        if ((first_m >> idx) & 1) {                    // a sequence starts in this slice
-            if (k != lo) load_q(bq);
+    // A tile's scales by token, [head][group][token], those of tokens from n on as zeros
+    auto put_scales = [&](int kv, const uint32_t (&x)[2][SL], int n) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < SL; ++i) {
+            const int at = lane + 64 * i, tok = FINE ? at / nsc : at / KS, g = at - tok * nsc;
+            if (tok < 16)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) ((uint32_t *)&s_scale[wave][kv][t][g])[tok] = tok < n ? x[t][i] : 0;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+
+    // Steps s and s + 1 are loaded 16 bytes a lane: the lower two words of lanes q = 2, 3
+    // (step s + 1) change places with the upper two of lanes 0, 1 (step s).
+    auto order_k = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int s = 0; s + 1 < KS; s += 2)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const auto r = __builtin_amdgcn_permlane32_swap(kr[t][s][i], kr[t][s + 1][i], false, false);
+                    kr[t][s][i] = r[0];
+                    kr[t][s + 1][i] = r[1];
+                }
+    };
+
+    // The keys of the next tile are loaded once this one's scores are there, its
+    // values after this one's product: either is in flight while the other is used.
+    look(lo);
+    load_k(true);
+    load_v(true);
+    for (int k = lo; k < hi; ++k) {
+        if (first) {                                   // a sequence starts in this slice
+            load_q(bq);
             m_run = -INFINITY;
             l_run = 0.0f;
 #pragma unroll
@@ -302,27 +435,72 @@ void diff_decode_kernel(DiffDecodeArgs a) {
 #pragma unroll
                 for (int j = 0; j < C; ++j) acc[t][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        // an entry outside the pool is counted once, by the first pair's wave, and its tile masked
-        if (!ok && lane == 0) atomicAdd(a.errors, 1ull);
-        const int nv = ok ? __builtin_amdgcn_readlane(nv_l, idx) : 0;
-        const bool full = nv == 16;
+        const int n = nv, seq = bq;
+        const bool full = n == 16, end = last, more = k + 1 < hi;
 
-        f32x4 s2[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+        // S of the lane's row and tokens 4 q + i
+        f32x4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (F32) {
+            f32x4 s2[2] = {sc, sc};
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            float x[2][8];
+            for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) widen<DT, 8>(kr[t][s], QUANT ? ksc[t][s] : 0.0f, x[t]);
+                for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+                    for (int t = 0; t < 2; ++t) s2[t] = mfma_f32(__uint_as_float(kr[t][s][j]), qf[s][j], s2[t]);
+            sc = map1 ? s2[1] : s2[0];
+        } else if constexpr (!QUANT) {
+            f32x4 s2[2] = {sc, sc};
 #pragma unroll
-                for (int t = 0; t < 2; ++t) s2[t] = mfma_f32(x[t][j], qf[s][j], s2[t]);
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const diff_u32x4 x = {kr[t][s][0], kr[t][s][1], kr[t][s][2], kr[t][s][3]};
+                    s2[t] = mfma_bf16(x, qb[0][s], s2[t]);
+                }
+            if constexpr (WIDE)
+                if (wide_q)
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const diff_u32x4 x = {kr[t][s][0], kr[t][s][1], kr[t][s][2], kr[t][s][3]};
+                        s2[t] = mfma_bf16(x, qb[2][s], mfma_bf16(x, qb[1][s], s2[t]));
+                    }
+            sc = map1 ? s2[1] : s2[0];
+        } else {
+            // the codes' products, a scale group at a time, then the scales (f32)
+            const f32x4 zero = sc;
+            put_scales(0, ksc, 16);
+            order_k();
+            // groups of 8 or 16: those of a step's 32 elements one by one, the other lanes' elements as zeros
+            auto pass = [&](bool rest) __attribute__((always_inline)) {
+                for (int g = 0; g < (FINE ? 32 : 1); g += FINE ? 1 << sg : 1) {
+                    const uint32_t mine = !FINE || (q_at >= g && q_at < g + (1 << sg)) ? ~0u : 0u;
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        f32x4 s2[2];
+                        const f32x4 ks = s_scale[wave][0][map1 ? 1 : 0][FINE ? (32 * s + g) >> sg : s][q4];
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            const uint32_t w[2] = {kr[t][s][0] & mine, kr[t][s][1] & mine};
+                            const diff_u32x4 x = codes_bf16<DT>(w);
+                            s2[t] = rest ? mfma_bf16(x, qb[QP - 1][s], mfma_bf16(x, qb[QP / 2][s], zero)) : mfma_bf16(x, qb[0][s], zero);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sc[i] += (map1 ? s2[1][i] : s2[0][i]) * ks[i];
+                    }
+                }
+            };
+            pass(false);
+            if (wide_q) pass(true);
         }
-        float sc[4];
+        if (more) look(k + 1);
+        load_k(more);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            sc[i] = (map1 ? s2[1][i] : s2[0][i]) * a.scale_log2;
-            if (!full) sc[i] = 4 * q4 + i < nv ? sc[i] : -INFINITY;
+            sc[i] *= a.scale_log2;
+            if (!full) sc[i] = 4 * q4 + i < n ? sc[i] : -INFINITY;
         }
         float mt = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
         mt = max_x32(max_x16(mt));
@@ -347,40 +525,66 @@ void diff_decode_kernel(DiffDecodeArgs a) {
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const bool in = 4 * q4 + i < nv;
+                    const bool in = 4 * q4 + i < n;
 #pragma unroll
-                    for (int j = 0; j < VA; ++j) va[t][i][j] = in ? va[t][i][j] : 0;
-#pragma unroll
-                    for (int j = 0; j < VB; ++j) vb[t][i][j] = in ? vb[t][i][j] : 0;
-                    if constexpr (QUANT) {
-                        vsa[t][i] = in ? vsa[t][i] : 0.0f;
-                        vsb[t][i] = in ? vsb[t][i] : 0.0f;
-                    }
+                    for (int j = 0; j < VW; ++j) vr[t][i][j] = in ? vr[t][i][j] : 0;
                 }
         }
+        if constexpr (DT != AIR_KV_BF16) {
+            f32x4 vs[2], vt[2];                            // the scales of the lane's columns, by token
+            if constexpr (QUANT) {
+                put_scales(1, vsc, n);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                float x[CA];
-                widen<DT, CA>(va[t][i], QUANT ? vsa[t][i] : 0.0f, x);
-#pragma unroll
-                for (int j = 0; j < CA; ++j) acc[t][j] = mfma_f32(x[j], p[i], acc[t][j]);
-                if constexpr (CB > 0) {
-                    float y[CB];
-                    widen<DT, CB>(vb[t][i], QUANT ? vsb[t][i] : 0.0f, y);
-#pragma unroll
-                    for (int j = 0; j < CB; ++j) acc[t][CA + j] = mfma_f32(y[j], p[i], acc[t][CA + j]);
+                for (int t = 0; t < 2; ++t) {
+                    vs[t] = s_scale[wave][1][t][CA * r16 >> sg][q4];
+                    if constexpr (CB > 0) vt[t] = s_scale[wave][1][t][(16 * CA + CB * r16) >> sg][q4];
                 }
             }
-        if ((last_m >> idx) & 1) emit(bq);
-    };
-
-    for (int c0 = lo; c0 < hi; c0 += 64) {
-        load_window(c0);
-        if (c0 == lo) load_q(__builtin_amdgcn_readlane(seq_l, 0));
-        const int n = hi - c0 < 64 ? hi - c0 : 64;
-        for (int i = 0; i < n; ++i) tile(c0 + i, i);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    float x[C];
+                    if constexpr (QUANT) {
+                        widen<DT, CA>(&vr[t][i][0], vs[t][i], &x[0]);
+                        if constexpr (CB > 0) widen<DT, CB>(&vr[t][i][VA], vt[t][i], &x[CA]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < C; ++j) x[j] = __uint_as_float(vr[t][i][j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < C; ++j) acc[t][j] = mfma_f32(x[j], p[i], acc[t][j]);
+                }
+        } else {
+            // rest: the third parts, for f32 outputs (two leave 2^-16 of a probability, bf16 outputs 2^-8)
+            diff_u32x2 pb[3];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint32_t w[3];
+                split3(p[2 * i], p[2 * i + 1], w[0], w[1], w[2]);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) pb[k][i] = w[k];
+            }
+            auto pass = [&](bool rest) __attribute__((always_inline)) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int g = 0; g < VW; ++g) {
+                        const uint32_t w[4] = {vr[t][0][g], vr[t][1][g], vr[t][2][g], vr[t][3][g]};
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const diff_u32x2 x = e ? diff_u32x2{halves<true>(w[0], w[1]), halves<true>(w[2], w[3])}
+                                                   : diff_u32x2{halves<false>(w[0], w[1]), halves<false>(w[2], w[3])};
+                            f32x4 &c = acc[t][2 * g + e];
+                            c = rest ? mfma_bf16(x, pb[2], c) : mfma_bf16(x, pb[1], mfma_bf16(x, pb[0], c));
+                        }
+                    }
+            };
+            pass(false);
+            if (wide_out) pass(true);
+        }
+        load_v(more);
+        if (end) emit(seq);
     }
 }
 
@@ -457,8 +661,13 @@ __global__ __launch_bounds__(64 * WH) void diff_decode_merge_kernel(DiffDecodeAr
 
 template <int D, int DT>
 hipError_t launch_dt(const DiffDecodeArgs &a, hipStream_t s) {
+    constexpr bool QUANT = DT == AIR_KV_INT8 || DT == AIR_KV_FP8, F32 = DT == AIR_KV_F32;
     const int64_t waves = (int64_t)a.kv_pairs * a.row_tiles * a.slices;
-    hipLaunchKernelGGL((diff_decode_kernel<D, DT>), dim3((unsigned)((waves + kWaves - 1) / kWaves)), dim3(kThreads), 0, s, a);
+    const dim3 blocks((unsigned)((waves + kWaves - 1) / kWaves));
+    const bool wide = a.q_dtype == AIR_KV_F32 || a.e.out_dtype == AIR_KV_F32, fine = QUANT && a.scale_group != 32;
+    if (fine) hipLaunchKernelGGL((diff_decode_kernel<D, DT, true, QUANT>), blocks, dim3(kThreads), 0, s, a);
+    else if (F32 || wide) hipLaunchKernelGGL((diff_decode_kernel<D, DT, true, false>), blocks, dim3(kThreads), 0, s, a);
+    else hipLaunchKernelGGL((diff_decode_kernel<D, DT, F32, false>), blocks, dim3(kThreads), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const dim3 grid((unsigned)a.batch, (unsigned)a.pairs);
