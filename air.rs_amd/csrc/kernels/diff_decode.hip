@@ -115,13 +115,22 @@ __device__ __forceinline__ void load_piece(const __amdgpu_buffer_rsrc_t &r, int 
     }
 }
 
-// N 1-byte codes times their scale.
-template <int DT, int N> __device__ __forceinline__ void widen(const uint32_t *w, float s, float *x) {
+// Two 1-byte codes (the lower halves of w, or the upper) of four rows as bf16,
+// exactly: x[e] holds code e of rows 0 .. 3.
+template <int DT, bool HI> __device__ __forceinline__ void codes_by_row(const uint32_t (&w)[4], diff_u32x2 (&x)[2]) {
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-        const f32x4 v = code_values<DT>(w[i / 4], s);
+    for (int i = 0; i < 2; ++i) {
+        // code 0 of rows 2 i and 2 i + 1, then code 1
+        const uint32_t c = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], HI ? 0x07030602u : 0x05010400u);
+        if constexpr (DT == AIR_KV_INT8) {
 #pragma unroll
-        for (int j = i; j < i + 4 && j < N; ++j) x[j] = v[j - i];
+            for (int e = 0; e < 2; ++e)
+                x[e][i] = halves<true>(__float_as_uint((float)(int8_t)(c >> (16 * e))),
+                                       __float_as_uint((float)(int8_t)(c >> (16 * e + 8))));
+        } else {
+            x[0][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c, 1.0f, false));
+            x[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c, 1.0f, true));
+        }
     }
 }
 
@@ -137,7 +146,7 @@ void diff_decode_kernel(DiffDecodeArgs a) {
     // columns of a value head in a lane: CA from CA * m, then CB from 16 * CA + CB * m
     // (96 as 64 + 32: every run a power of two). 
     constexpr int CA = D == 96 ? 4 : D / 16, CB = D == 96 ? 2 : 0, C = CA + CB;
-    constexpr int PW = D % 64 == 0 ? 4 : 2, PC = C / PW, NP = 4 * PC;      // pieces of consecutive columns of a lane
+    constexpr int PW = !QUANT && D % 64 == 0 ? 4 : 2, PC = C / PW, NP = 4 * PC;      // pieces of consecutive columns of a lane
     constexpr int KW = 8 * EB / 4, VA = (CA * EB + 3) / 4, VB = CB ? (CB * EB + 3) / 4 : 1;
 
     __shared__ int32_t s_pre[kMaxBatch + 2];
@@ -254,6 +263,8 @@ void diff_decode_kernel(DiffDecodeArgs a) {
         for (int e = 0; e < PW; ++e)
             x[e] = acc[t][PW * (i % PC) + e][i / PC];
         const int m = 4 * q4 + i / PC, j = PW * (i % PC);
+        if constexpr (QUANT)
+            return t * D + 32 * (j / 2) + (j / 2 < KS / 2 * 2 ? 16 * (q4 & 1) + 4 * (i / PC) + 2 * (q4 >> 1) : 2 * m);
         return t * D + (j < CA ? CA * m + j : 16 * CA + CB * m + j - CA);
     };
 
@@ -340,7 +351,8 @@ void diff_decode_kernel(DiffDecodeArgs a) {
         return __builtin_amdgcn_make_buffer_rsrc((void *)((const char *)p + row * width), (short)0,
                                                  in ? (bs + 16) * width : 0, kDiffBufferWord3);
     };
-    constexpr int VW = VA + (CB ? VB : 0);
+    // 1-byte pages: words of two groups (order_v), the last of an odd number alone
+    constexpr int VW = QUANT ? (KS + 1) / 2 : VA + (CB ? VB : 0);
     uint32_t kr[2][KS][KW], vr[2][4][VW];
     uint32_t ksc[2][SL], vsc[2][SL];                   // a tile's scales in order, either head's
     const int head1 = bs * D * EB;                     // the second head's rows, in bytes
@@ -379,7 +391,15 @@ void diff_decode_kernel(DiffDecodeArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int at = (4 * q4 + i) * D;
-                {
+                if constexpr (QUANT) {
+#pragma unroll
+                    for (int h = 0; h < VW; ++h) {
+                        uint32_t w[1];
+                        if (2 * h + 1 < KS) load_piece<4>(rv, at + 64 * h + 4 * r16, t ? head1 : 0, w);
+                        else load_piece<2>(rv, at + 64 * h + 2 * r16, t ? head1 : 0, w);
+                        vr[t][i][h] = w[0];
+                    }
+                } else {
                     uint32_t w[VA], z[VB];
                     load_piece<CA * EB>(rv, (at + CA * r16) * EB, t ? head1 : 0, w);
                     if constexpr (CB > 0) load_piece<CB * EB>(rv, (at + 16 * CA + CB * r16) * EB, t ? head1 : 0, z);
@@ -417,6 +437,21 @@ void diff_decode_kernel(DiffDecodeArgs a) {
                     const auto r = __builtin_amdgcn_permlane32_swap(kr[t][s][i], kr[t][s + 1][i], false, false);
                     kr[t][s][i] = r[0];
                     kr[t][s + 1][i] = r[1];
+                }
+    };
+
+    // 64 columns of a row, four to a lane: lanes m and m ^ 8 exchange halves, so that each
+    // has two columns of either scale group and a product's 16 columns share a row's scale.
+    auto order_v = [&]() __attribute__((always_inline)) {
+        const uint32_t pick = r16 < 8 ? 0x05040100u : 0x03020706u;     // own low, other's low; other's high, own high
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int h = 0; 2 * h + 1 < KS; ++h) {
+                    const uint32_t o = (uint32_t)__builtin_amdgcn_mov_dpp((int)vr[t][i][h], 0x128, 0xF, 0xF, false);
+                    vr[t][i][h] = __builtin_amdgcn_perm(o, vr[t][i][h], pick);
                 }
     };
 
@@ -530,55 +565,60 @@ void diff_decode_kernel(DiffDecodeArgs a) {
                     for (int j = 0; j < VW; ++j) vr[t][i][j] = in ? vr[t][i][j] : 0;
                 }
         }
-        if constexpr (DT != AIR_KV_BF16) {
-            f32x4 vs[2], vt[2];                            // the scales of the lane's columns, by token
-            if constexpr (QUANT) {
-                put_scales(1, vsc, n);
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    vs[t] = s_scale[wave][1][t][CA * r16 >> sg][q4];
-                    if constexpr (CB > 0) vt[t] = s_scale[wave][1][t][(16 * CA + CB * r16) >> sg][q4];
-                }
-            }
+        if constexpr (F32) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    float x[C];
-                    if constexpr (QUANT) {
-                        widen<DT, CA>(&vr[t][i][0], vs[t][i], &x[0]);
-                        if constexpr (CB > 0) widen<DT, CB>(&vr[t][i][VA], vt[t][i], &x[CA]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < C; ++j) x[j] = __uint_as_float(vr[t][i][j]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < C; ++j) acc[t][j] = mfma_f32(x[j], p[i], acc[t][j]);
-                }
-        } else {
-            // rest: the third parts, for f32 outputs (two leave 2^-16 of a probability, bf16 outputs 2^-8)
-            diff_u32x2 pb[3];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                uint32_t w[3];
-                split3(p[2 * i], p[2 * i + 1], w[0], w[1], w[2]);
-#pragma unroll
-                for (int k = 0; k < 3; ++k) pb[k][i] = w[k];
-            }
-            auto pass = [&](bool rest) __attribute__((always_inline)) {
-#pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int g = 0; g < VW; ++g) {
-                        const uint32_t w[4] = {vr[t][0][g], vr[t][1][g], vr[t][2][g], vr[t][3][g]};
+                    for (int j = 0; j < C; ++j) acc[t][j] = mfma_f32(__uint_as_float(vr[t][i][j]), p[i], acc[t][j]);
+        } else {
+            auto parts = [&](float y0, float y1, float y2, float y3, diff_u32x2 (&pb)[3]) __attribute__((always_inline)) {
+                uint32_t w[2][3];
+                split3(y0, y1, w[0][0], w[0][1], w[0][2]);
+                split3(y2, y3, w[1][0], w[1][1], w[1][2]);
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const diff_u32x2 x = e ? diff_u32x2{halves<true>(w[0], w[1]), halves<true>(w[2], w[3])}
-                                                   : diff_u32x2{halves<false>(w[0], w[1]), halves<false>(w[2], w[3])};
-                            f32x4 &c = acc[t][2 * g + e];
-                            c = rest ? mfma_bf16(x, pb[2], c) : mfma_bf16(x, pb[1], mfma_bf16(x, pb[0], c));
+                for (int k = 0; k < 3; ++k) pb[k] = diff_u32x2{w[0][k], w[1][k]};
+            };
+            // rest: the third parts, for f32 outputs (two leave 2^-16 of a probability, bf16 outputs 2^-8)
+            auto add = [&](bool rest, diff_u32x2 x, const diff_u32x2 (&pb)[3], f32x4 &c) __attribute__((always_inline)) {
+                c = rest ? mfma_bf16(x, pb[2], c) : mfma_bf16(x, pb[1], mfma_bf16(x, pb[0], c));
+            };
+            diff_u32x2 pb[3];
+            if constexpr (QUANT) {
+                put_scales(1, vsc, n);
+                order_v();
+            } else {
+                parts(p[0], p[1], p[2], p[3], pb);
+            }
+            auto pass = [&](bool rest) __attribute__((always_inline)) {
+                for (int h = 0; h < (FINE ? 32 : 1); h += FINE ? 1 << sg : 1) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int g = 0; g < VW; ++g) {
+                            const uint32_t w[4] = {vr[t][0][g], vr[t][1][g], vr[t][2][g], vr[t][3][g]};
+                            if constexpr (QUANT) {
+#pragma unroll
+                                for (int b = 0; b < 2 && 2 * g + b < KS; ++b) {
+                                    // the scales, folded into the probabilities; groups of 8 or 16 as in the scores
+                                    const int col = 2 * g + 1 < KS || b ? 4 * (r16 & 7) + 2 * (r16 >> 3) : 2 * r16;
+                                    const uint32_t mine = !FINE || (col >= h && col < h + (1 << sg)) ? ~0u : 0u;
+                                    const uint32_t wm[4] = {w[0] & mine, w[1] & mine, w[2] & mine, w[3] & mine};
+                                    const f32x4 vs = s_scale[wave][1][t][FINE ? (32 * (2 * g + b) + h) >> sg : 2 * g + b][q4];
+                                    diff_u32x2 x[2];
+                                    if (b) codes_by_row<DT, true>(wm, x);
+                                    else codes_by_row<DT, false>(wm, x);
+                                    parts(p[0] * vs[0], p[1] * vs[1], p[2] * vs[2], p[3] * vs[3], pb);
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e) add(rest, x[e], pb, acc[t][2 * (2 * g + b) + e]);
+                                }
+                            } else {
+                                add(rest, diff_u32x2{halves<false>(w[0], w[1]), halves<false>(w[2], w[3])}, pb, acc[t][2 * g]);
+                                add(rest, diff_u32x2{halves<true>(w[0], w[1]), halves<true>(w[2], w[3])}, pb, acc[t][2 * g + 1]);
+                            }
                         }
-                    }
+                }
             };
             pass(false);
             if (wide_out) pass(true);
