@@ -126,11 +126,23 @@ __device__ __forceinline__ float diff_wave_sum(float x) {
     return sum_x32(sum_x16(x));
 }
 
-// The output row of a folded (row, query pair): lane l holds columns V l .. +V of 64 V.
+// What the output row of (row, query pair) needs beside its sums: lane l holds
+// the weights of columns V l .. +V of 64 V.
+template <int V> struct DiffTail {
+    float lam, w[V];
+    __device__ __forceinline__ DiffTail(const DiffOut &e, int64_t row, int h, int lane) {
+        lam = e.lam[row * e.lam_stride + h];
+        const bool weights = e.norm && e.norm_w;
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[i] = 1.0f;
+        if (weights) diff_load<V>(e.norm_w + V * lane, w);
+    }
+};
+
 template <int V>
-__device__ __forceinline__ void diff_finish(const DiffOut &e, int64_t row, int h, int pairs, const DiffFold<V> &c, int lane) {
-    const float lam = e.lam[row * e.lam_stride + h];
-    const float i0 = 1.0f / c.l[0], i1 = lam / c.l[1];
+__device__ __forceinline__ void diff_finish(const DiffOut &e, int64_t row, int h, int pairs, const DiffFold<V> &c,
+                                            const DiffTail<V> &tail, int lane) {
+    const float i0 = 1.0f / c.l[0], i1 = tail.lam / c.l[1];
     float x[V], ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -140,7 +152,7 @@ __device__ __forceinline__ void diff_finish(const DiffOut &e, int64_t row, int h
     const float f = diff_factor(e, e.norm ? diff_wave_sum(ss) : 0.0f, 64 * V);
     const int64_t at = (row * pairs + h) * (64 * V) + V * lane;
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] *= (e.norm && e.norm_w) ? f * e.norm_w[V * lane + i] : f;
+    for (int i = 0; i < V; ++i) x[i] *= f * tail.w[i];
     if constexpr (V == 4) {
         diff_store4(e, at, diff_f32x4{x[0], x[1], x[2], x[3]});
     } else {

@@ -634,8 +634,8 @@ void diff_decode_kernel(DiffDecodeArgs a) {
 template <int D, int WH>
 __global__ __launch_bounds__(64 * WH) void diff_decode_merge_kernel(DiffDecodeArgs a) {
     constexpr int V = D / 32, kBatch = 8;
-    __shared__ float s_ml[WH][4];
-    __shared__ float s_o[WH][2][64 * V];
+    __shared__ float s_ml[WH][2][2];
+    __shared__ float s_o[WH][2][V][64];
     const int b = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int p0 = a.prefix[b], p1 = a.prefix[b + 1], chunk = a.prefix[a.batch + 1];
@@ -650,6 +650,7 @@ __global__ __launch_bounds__(64 * WH) void diff_decode_merge_kernel(DiffDecodeAr
     const int w0 = p0 / chunk, w1 = (p1 - 1) / chunk;
     if (w0 == w1) return;                              // written by its slice
     const int n = w1 - w0 + 1;
+    const DiffTail<V> tail(a.e, b, h, lane);           // loaded along with the pieces
     const int kp = h / a.group, j = h % a.group;
     const int hh = kp * a.row_tiles + j / 8;
     DiffFold<V> c;
@@ -674,29 +675,36 @@ __global__ __launch_bounds__(64 * WH) void diff_decode_merge_kernel(DiffDecodeAr
             for (int k = 0; k < 2; ++k) c.fold(k, pm[i][k], pl[i][k], po[i][k]);
     }
     if constexpr (WH > 1) {
-        if (lane == 0) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                s_ml[wave][2 * k] = c.m[k];
-                s_ml[wave][2 * k + 1] = c.l[k];
+        for (int k = 0; k < 2; ++k) {
+            if (lane == 0) {
+                s_ml[wave][k][0] = c.m[k];
+                s_ml[wave][k][1] = c.l[k];
             }
+#pragma unroll
+            for (int i = 0; i < V; ++i) s_o[wave][k][i][lane] = c.o[k][i];
         }
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int i = 0; i < V; ++i) s_o[wave][k][V * lane + i] = c.o[k][i];
         __syncthreads();
         if (wave != 0) return;
-        for (int w = 1; w < WH; ++w)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                float o[V];
+        for (int k = 0; k < 2; ++k) {
+            float top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < V; ++i) o[i] = s_o[w][k][V * lane + i];
-                c.fold(k, s_ml[w][2 * k], s_ml[w][2 * k + 1], o);
+            for (int w = 0; w < WH; ++w) top = fmaxf(top, s_ml[w][k][0]);
+            c.m[k] = top;
+            c.l[k] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) c.o[k][i] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WH; ++w) {
+                const float m = s_ml[w][k][0], f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+                c.l[k] += m == -INFINITY ? s_ml[w][k][1] : s_ml[w][k][1] * f;      // a NaN of it stays
+#pragma unroll
+                for (int i = 0; i < V; ++i) c.o[k][i] += s_o[w][k][i][lane] * f;
             }
+        }
     }
-    diff_finish<V>(a.e, b, h, a.pairs, c, lane);
+    diff_finish<V>(a.e, b, h, a.pairs, c, tail, lane);
 }
 
 template <int D, int DT>
@@ -711,8 +719,10 @@ hipError_t launch_dt(const DiffDecodeArgs &a, hipStream_t s) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const dim3 grid((unsigned)a.batch, (unsigned)a.pairs);
-    // past a round trip's worth of pieces for an average sequence, four waves share them
-    if (a.slices > 8 * a.batch) hipLaunchKernelGGL((diff_decode_merge_kernel<D, 4>), grid, dim3(256), 0, s, a);
+    // waves enough that an average sequence's pieces take each one round trip
+    const int64_t tiles = ((int64_t)a.max_blocks * a.block_size + 15) / 16, pieces = std::min<int64_t>(a.slices / a.batch, tiles);
+    if (pieces > 32) hipLaunchKernelGGL((diff_decode_merge_kernel<D, 16>), grid, dim3(1024), 0, s, a);
+    else if (pieces > 8) hipLaunchKernelGGL((diff_decode_merge_kernel<D, 4>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((diff_decode_merge_kernel<D, 1>), grid, dim3(64), 0, s, a);
     return hipGetLastError();
 }

@@ -24,6 +24,9 @@ __global__ __launch_bounds__(256) void diff_prefill_merge_kernel(DiffPrefillArgs
     diff_seq(a, d.x, s);
     const int64_t f = k * a.rows + row;
     if (f >= s.q * a.group) return;
+    const int64_t out_row = a.cu[d.x] + f / a.group;
+    const int h = kp * a.group + (int)(f % a.group);
+    const DiffTail<V> tail(a.e, out_row, h, lane);
     DiffFold<V> c;
     c.clear();
     for (int p0 = 0; p0 < d.w; p0 += kBatch) {
@@ -46,7 +49,7 @@ __global__ __launch_bounds__(256) void diff_prefill_merge_kernel(DiffPrefillArgs
 #pragma unroll
             for (int m = 0; m < 2; ++m) c.fold(m, pm[i][m], pl[i][m], po[i][m]);
     }
-    diff_finish<V>(a.e, a.cu[d.x] + f / a.group, kp * a.group + (int)(f % a.group), a.pairs, c, lane);
+    diff_finish<V>(a.e, out_row, h, a.pairs, c, tail, lane);
 }
 
 }  // namespace
