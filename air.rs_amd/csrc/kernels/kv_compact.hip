@@ -12,7 +12,7 @@
 // two chains: they touch different bytes.
 //
 // Bound by memory: each moved row is read once and written once.  64 sequences of
-// 512 to 4096 tokens, half kept: 666 MB in 126 us, 5.3 TB/s; 4 of 32K to 64K moved
+// 512 to 4096 tokens, half kept: 666 MB in 141 us, 4.7 TB/s; 4 of 32K to 64K moved
 // behind their first tokens, 128 chains: 1.37 GB in 326 us, 4.2 TB/s, what half of
 // the CUs carry (a chain's steps are in order; more chains would split lines).
 #include <hip/hip_runtime.h>
@@ -27,13 +27,12 @@ namespace {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWindow = 1024;              // kept tokens whose rows are resolved at a time
-constexpr int kUnroll = 8;                 // pieces of a step per thread (4: 128 and 331 us)
+constexpr int kUnroll = 8;                 // pieces of a step per thread (4: 143 and 332 us)
 
-// Few chains take a CU each and stream their stores past the L2 (4 sequences of 32K to
-// 64K tokens of 8 heads: 326 us, 342 with stores that stay in it); many share the CUs
-// and keep them (64 of 512 to 4096: 126 us, 150 past it).  Loads are past it in both
-// (as cached ones 151 and 353 us).
-constexpr int kWide = 1024, kNarrow = 256; // threads of a chain
+// Threads of a chain: the wide ones where sequences fill half a step of theirs (64 that
+// keep 256 to 2048 of 8 heads' bf16 rows: 141 against 151 us), the narrow ones where
+// they do not (100 that keep 10 to 100: 20 against 40 us).
+constexpr int kWide = 1024, kNarrow = 256;
 
 struct CompactArgs {
     const int32_t *tables, *lens, *keep, *cu;
@@ -90,11 +89,8 @@ __device__ __forceinline__ void walk(const CompactArgs &a, uint8_t *base, int64_
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
                 const int i = at + u * per + my;
-                if (my < per && i < wn && (*s_src)[i] >= 0) {
-                    T *to = reinterpret_cast<T *>(base + ((*s_dst)[i] + head_row) * row_bytes) + piece;
-                    if constexpr (THREADS == kWide) __builtin_nontemporal_store(x[u], to);
-                    else *to = x[u];
-                }
+                if (my < per && i < wn && (*s_src)[i] >= 0)
+                    __builtin_nontemporal_store(x[u], reinterpret_cast<T *>(base + ((*s_dst)[i] + head_row) * row_bytes) + piece);
             }
         };
         // the rows are in registers (not on their way) when the barrier is passed
@@ -164,7 +160,8 @@ hipError_t launch_compact(const air_kv_pool &p, hipStream_t s, const int32_t *ta
     a.scale_row_bytes = quant ? p.desc.head_dim / p.desc.scale_group * 4 : 0;
     a.errors = p.errors;
     // few chains: rows of two lines or more are walked in column parts of a line
-    // (half lines: 553 us where lines take 331)
+    // (half lines: 553 us where lines take 331); loads and stores go past the L2 (345 us
+    // with stores, 353 with loads that stay in it)
     const int64_t stripes = (int64_t)batch * 2 * a.heads;
     a.part_pieces = a.row_bytes / 16;
     a.parts = 1;
@@ -173,7 +170,8 @@ hipError_t launch_compact(const air_kv_pool &p, hipStream_t s, const int32_t *ta
         a.parts = (a.row_bytes / 16 + 7) / 8;
     }
     const dim3 grid((unsigned)batch, (unsigned)(2 * a.heads * a.parts + (quant ? 2 * a.heads : 0)));
-    if (stripes * a.parts < 4 * p.cus) hipLaunchKernelGGL((kv_compact_kernel<kWide>), grid, dim3(kWide), 0, s, a);
+    const int64_t half_step = (int64_t)kUnroll * (kWide / 2) / a.part_pieces;      // rows
+    if (total_keep >= half_step * batch || stripes * a.parts < 4 * p.cus) hipLaunchKernelGGL((kv_compact_kernel<kWide>), grid, dim3(kWide), 0, s, a);
     else hipLaunchKernelGGL((kv_compact_kernel<kNarrow>), grid, dim3(kNarrow), 0, s, a);
     return hipGetLastError();
 }
