@@ -78,11 +78,11 @@ struct Plan {
 // half: 16-bit products (diff_prefill_16.hip), else f32 ones
 Plan plan_for(const air_kv_pool &p, bool half) {
     Plan pl;
-    const int kv_pairs = p.desc.n_kv_heads / 2, per_cu = half ? 1 : 2;
+    const int kv_pairs = p.desc.n_kv_heads / 2;
     pl.rows = half ? 128 : 64;
-    pl.extra = half ? 7 : 1;       // 16 us and 2.1 us a tile; 20 us and 10 to 25 us
-    pl.slices = std::max(1, (per_cu * p.cus + kv_pairs - 1) / kv_pairs);
-    pl.least = half ? 16 : 8;
+    pl.extra = half ? 7 : 1;       // a block begins and ends in 16 us beside 2.1 us a tile; at f32 precision in 3 beside 3 to 5
+    pl.slices = std::max(1, (p.cus + kv_pairs - 1) / kv_pairs);
+    pl.least = half ? 16 : 3;
     pl.cells = (size_t)kv_pairs * pl.slices;
     pl.halves = 2 * pl.cells * pl.rows * 2;
     return pl;
