@@ -402,9 +402,13 @@ int air_paged_prefill_workspace_size(const air_kv_pool *pool, int32_t n_q_heads,
  * 128.  Scores, sums and the norm are held in 32 bits.
  *
  * Decode: one new token per sequence (already appended) over its seq_lens[b]
- * cached tokens, with the work division, max_splits, workspace rules and error
- * counting of air_paged_decode.  Queries, keys, probabilities and values keep
- * f32 precision on every pool.  A sequence of length 0 produces zeros. */
+ * cached tokens, with the workspace rules of air_paged_decode and its refusals:
+ * out-of-pool table entries are skipped and counted, seq_lens outside [0,
+ * max_blocks * block_size] are clamped and counted, a sequence of length 0
+ * produces zeros.  max_splits (1 to 256) bounds the slices that share a sequence;
+ * with 1, its result does not depend on the others'.  Queries, keys and values
+ * keep f32 precision on every pool; so do probabilities under f32 outputs, while
+ * bf16 outputs take 16 bits of them. */
 int air_paged_diff_decode_workspace_size(const air_kv_pool *pool, int32_t n_q_heads, int32_t batch,
                                          int32_t max_blocks, int32_t max_splits, size_t *bytes);
 int air_paged_diff_decode(air_kv_pool *pool, void *stream, const void *q, int32_t q_dtype,
@@ -418,7 +422,9 @@ int air_paged_diff_decode(air_kv_pool *pool, void *stream, const void *q, int32_
  * air_paged_prefill: rows of a sequence that is refused are zero-filled,
  * out-of-pool table entries are read as zero keys and values.  max_q_len is a
  * hint (an upper bound of the q_len values).  Keys and values that are not finite
- * reach only the rows that see them.  The workspace (16-byte aligned, of at least
+ * reach only the rows that see them.  bf16 queries with bf16 outputs on BF16, INT8
+ * and FP8 pools take 16-bit products (probabilities, and what 1-byte pages hold,
+ * rounded to 11 bits); everything else keeps f32 precision.  The workspace (16-byte aligned, of at least
  * air_paged_diff_prefill_workspace_size bytes, no initialisation needed) holds
  * the parts of blocks of rows that several workgroups share; calls that share
  * one must be ordered (same stream). */
