@@ -134,6 +134,9 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
     const int64_t chunk = diff_prefill_chunk(units, a.slices, a.least);
     const int64_t cell = (int64_t)kp * a.slices + w;
     int4 begun = {0, 0, 0, 0};
+    // A SIMD has one wave of either map: map 1's goes first, so that the two stay out of phase
+    // and one's products run beside the other's arithmetic (8192 tokens 1.08 -> 1.04 ms).
+    if (mp) __builtin_amdgcn_s_setprio(1);
 
     // This lane's piece of every pass: row (of its 16-key half) and 16-byte chunk
     const int nsc = QUANT ? D / a.scale_group : 0;
