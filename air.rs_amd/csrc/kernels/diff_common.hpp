@@ -55,6 +55,23 @@ __device__ __forceinline__ diff_f32x4 code_values(uint32_t w, float s) {
     }
 }
 
+// The upper (HI) or lower halves of two words, a's in the low half.
+template <bool HI> __device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b) {
+    return __builtin_amdgcn_perm(b, a, HI ? 0x07060302u : 0x05040100u);
+}
+
+// x, y = the sum of three bf16 pairs, each holding the next eight bits: exact,
+// and every part has its value's sign.
+__device__ __forceinline__ void split3(float x, float y, uint32_t &p0, uint32_t &p1, uint32_t &p2) {
+    p0 = halves<true>(__float_as_uint(x), __float_as_uint(y));
+    x -= __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+    y -= __uint_as_float(__float_as_uint(y) & 0xFFFF0000u);
+    p1 = halves<true>(__float_as_uint(x), __float_as_uint(y));
+    x -= __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+    y -= __uint_as_float(__float_as_uint(y) & 0xFFFF0000u);
+    p2 = halves<true>(__float_as_uint(x), __float_as_uint(y));
+}
+
 // Four consecutive outputs (idx a multiple of 4).
 __device__ __forceinline__ void diff_store4(const DiffOut &e, int64_t idx, diff_f32x4 v) {
     if (e.out_dtype == AIR_KV_F32) {

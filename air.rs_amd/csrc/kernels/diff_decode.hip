@@ -53,23 +53,6 @@ __device__ __forceinline__ f32x4 mfma_bf16(diff_u32x2 a, diff_u32x2 b, f32x4 c) 
     return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
 }
 
-// The upper (HI) or lower halves of two words, a's in the low half.
-template <bool HI> __device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b) {
-    return __builtin_amdgcn_perm(b, a, HI ? 0x07060302u : 0x05040100u);
-}
-
-// x, y = the sum of three bf16 pairs, each holding the next eight bits: exact,
-// and every part has its value's sign.
-__device__ __forceinline__ void split3(float x, float y, uint32_t &p0, uint32_t &p1, uint32_t &p2) {
-    p0 = halves<true>(__float_as_uint(x), __float_as_uint(y));
-    x -= __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
-    y -= __uint_as_float(__float_as_uint(y) & 0xFFFF0000u);
-    p1 = halves<true>(__float_as_uint(x), __float_as_uint(y));
-    x -= __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
-    y -= __uint_as_float(__float_as_uint(y) & 0xFFFF0000u);
-    p2 = halves<true>(__float_as_uint(x), __float_as_uint(y));
-}
-
 // Eight 1-byte codes as bf16, exactly.
 template <int DT> __device__ __forceinline__ diff_u32x4 codes_bf16(const uint32_t (&w)[2]) {
     diff_u32x4 x;

@@ -44,6 +44,16 @@ struct DiffItem {
     int64_t from;                  // of its units, the first
 };
 
+// Where the 16-byte chunk c of row r of a staged head of 16-bit keys lies, in chunks: 16
+// rows' chunks c are read at once, and have to lie in 16 different 16-byte columns of the
+// 256 bytes that the banks span.
+template <int D> __device__ __forceinline__ int key_chunk(int r, int c) {
+    if constexpr (D == 128) return c ^ (r & 15);
+    else if constexpr (D == 64) return c ^ ((r >> 1) & 7);
+    else if constexpr (D == 32) return c ^ ((r >> 2) & 3);
+    else return (c + ((r >> 2) & 3)) % 12;
+}
+
 // The launch's units before each sequence (s_pre[B] in all) and each sequence's
 // share of errors, in LDS.  A sequence whose rows do not lie in [0, total_q], whose
 // length is outside its table or below its rows, has none; the workgroup of slice b

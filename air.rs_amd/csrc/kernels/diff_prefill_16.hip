@@ -79,16 +79,8 @@ template <int N, int AHEAD, int READS> __device__ __forceinline__ void read_ahea
 constexpr int kRows = 128;
 constexpr int kThreads16 = 512;
 
-// Where the 16-byte chunk c of row r of a staged head lies, in chunks.  Keys are read
-// 32 rows at a time, a chunk each: 16 rows' chunks c have to lie in 16 different
-// 16-byte columns of the 256 bytes that the banks span.  Values are read eight
-// rows at a time, 64 bytes each: four rows in a row, in different quarters.
-template <int D> __device__ __forceinline__ int key_chunk(int r, int c) {
-    if constexpr (D == 128) return c ^ (r & 15);
-    else if constexpr (D == 64) return c ^ ((r >> 1) & 7);
-    else if constexpr (D == 32) return c ^ ((r >> 2) & 3);
-    else return (c + ((r >> 2) & 3)) % 12;
-}
+// Where the 16-byte chunk c of row r of a staged head of values lies, in chunks: they
+// are read eight rows at a time, 64 bytes each: four rows in a row, in different quarters.
 template <int D> __device__ __forceinline__ int value_chunk(int r, int c) {
     if constexpr (D == 128) return c ^ ((r & 3) << 2);
     else if constexpr (D == 64) return c ^ (((r >> 1) & 1) << 2);

@@ -3,16 +3,18 @@
 //
 // A workgroup's block is 64 rows.  A wave takes one map of 16 of them: its sums over
 // the 2 * head_dim value columns stay in registers, and it walks the block's keys
-// once, 32 at a time, with a running maximum and sum.  Keys and values are staged in
-// LDS as f32 (dequantized as gather does), in two buffers: while a tile is used, the
-// next one's elements are on their way in registers and the one after's table
-// entries too.  Both products are v_mfma_f32_16x16x4_f32:
-//   S   = K . Q^T      lane (n, q) holds S of keys 4q .. 4q + 3 of a 16-key half
-//   O^T += V^T . P^T   step i contracts over keys {4q + i}: P stays where it is
-// Bound by the f32 matrix rate, a sixteenth of the bf16 one: 2048 tokens of 16 query
-// pairs of 128 on f32 pages in 535 us, 64 TFLOP/s, 338 us of them the products
-// themselves; four chunks of 500 to 1000 behind up to 4000 bf16 tokens 1.95 ms, 72.
-// (Four waves of both maps, without tiles ahead: 31 TFLOP/s.)
+// once, 32 at a time, with a running maximum and sum.
+//
+// Both products are v_mfma_f32_16x16x32_bf16 on parts: a value is the sum of three bf16
+// numbers of 8 bits each, and of two values' nine products the six down to 2^-16 of the
+// whole are added (the others are below 2^-23 of it); elements of bf16 pages are one
+// part, exactly.  That is 6 (3) products in the time of 16 on f32 operands.
+//   S   = K . Q^T      lane (n, q) holds S of keys 4q .. 4q + 3 of both 16-key halves
+//   O^T += V^T . P^T   contracts over those eight: P stays where it is
+// Keys and values are staged as parts in LDS (1-byte codes times their scale), in two
+// buffers where they fit; while a tile is used, the next one's elements are on their
+// way in registers and the one after's table entries too.
+// FIGS
 #include <hip/hip_runtime.h>
 
 #include "../pool.hpp"
@@ -23,8 +25,39 @@ namespace {
 
 typedef diff_f32x4 f32x4;
 
-__device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f32x4 mfma_bf16(diff_u32x4 a, diff_u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// The products of parts a[i] b[j], i + j < 3, the smallest first.
+template <int N>
+__device__ __forceinline__ f32x4 mfma_parts(const diff_u32x4 (&a)[N], const diff_u32x4 (&b)[3], f32x4 c) {
+#pragma unroll
+    for (int k = 2; k >= 0; --k)
+#pragma unroll
+        for (int i = N - 1 < k ? N - 1 : k; i >= 0; --i) c = mfma_bf16(a[i], b[k - i], c);
+    return c;
+}
+
+// Eight values as parts.
+__device__ __forceinline__ void parts8(const float (&x)[8], diff_u32x4 (&p)[3]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t w[3];
+        split3(x[2 * j], x[2 * j + 1], w[0], w[1], w[2]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) p[k][j] = w[k];
+    }
+}
+
+// Where the chunk c of row r of a staged head of values lies: they are read eight rows at
+// a time, two chunks each.
+template <int D> __device__ __forceinline__ int value_chunk8(int r, int c) {
+    if constexpr (D == 128) return c ^ ((r & 7) << 1);
+    else if constexpr (D == 64) return c ^ (((r >> 1) & 3) << 1);
+    else return c ^ (((r >> 2) & 1) << 1);
 }
 
 // 8 elements of a page row as loaded, and as f32.
@@ -66,14 +99,17 @@ template <int DT> __device__ __forceinline__ void wide8(const Raw8<DT> &r, float
 
 template <int D, int DT>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void diff_prefill_f32_kernel(DiffPrefillArgs a) {
-    constexpr int R = 64, KP = D + 4, VP = 2 * D + 4, KS = D / 16, G = 2 * D / 64, T = 512;
+    constexpr int R = 64, VP = 2 * D + 4, KS = D / 32, CT = 2 * D / 16, T = 512;
     constexpr bool QUANT = DT == AIR_KV_INT8 || DT == AIR_KV_FP8;
     constexpr int C8 = 2 * kDiffKeys * (D / 8), NC = (C8 + T - 1) / T;       // pieces of 8 elements of a tile; a thread's
-    constexpr int BUF = 2 * kDiffKeys * KP + kDiffKeys * VP, EX = R * VP;
+    constexpr int NP = DT == AIR_KV_BF16 ? 1 : 3;      // parts of a cached element
+    constexpr int RB = 2 * D, HB = kDiffKeys * RB;     // bytes of a staged row, of a head's part
+    constexpr int BUF = NP * 4 * HB, NB = BUF > 65536 ? 1 : 2, EX = R * VP * 4;
     __shared__ int64_t s_pre[kDiffPrefillBatch + 1];
     __shared__ int64_t s_sum[8];
-    // [buffer][K: (head, key) rows of KP | V: key rows of VP]; at a block's end map 1's rows of VP
-    __shared__ __align__(16) float s_buf[2 * BUF > EX ? 2 * BUF : EX];
+    // [buffer][part][keys of both heads, then values][key]; at a block's end map 1's rows of VP floats
+    __shared__ __align__(16) uint8_t s_buf[NB * BUF > EX ? NB * BUF : EX];
+    auto s_t = [&](int64_t t) __attribute__((always_inline)) { return s_buf + (NB == 2 && (t & 1) ? BUF : 0); };
     // Values that are not finite, in tiles that not every row sees (a hidden key's
     // probability of 0 times such a value would be NaN): staged as 0, and each column's
     // first such key is kept here, from which on a row's column is NaN.
@@ -118,32 +154,31 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         __syncthreads();
         if (tid < 2 * D) s_bad[tid] = INT32_MAX;
         if (tid == 0) s_any = 0;
-        float qf[KS][4];
+        // Q^T as the B operand: lane (n, q) holds elements 32 s + 8 q .. +8 of row n, in parts
+        diff_u32x4 qf[KS][3];
         {
-            const int64_t at = ((row0 + tok) * 2 * a.pairs + 2 * h + mp) * D + 4 * q4;
+            const int64_t at = ((row0 + tok) * 2 * a.pairs + 2 * h + mp) * D + 8 * q4;
             if (a.q_dtype == AIR_KV_F32) {
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
-                    const f32x4 x = *reinterpret_cast<const f32x4 *>((const float *)a.q + at + 16 * s);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) qf[s][j] = x[j];
+                    const f32x4 *p = reinterpret_cast<const f32x4 *>((const float *)a.q + at + 32 * s);
+                    const f32x4 lo = p[0], hi = p[1];
+                    const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                    parts8(x, qf[s]);
                 }
             } else {
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
-                    const diff_u32x2 x = *reinterpret_cast<const diff_u32x2 *>((const uint16_t *)a.q + at + 16 * s);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) qf[s][j] = __uint_as_float((j & 1) ? x[j / 2] & 0xFFFF0000u : x[j / 2] << 16);
+                    qf[s][0] = *reinterpret_cast<const diff_u32x4 *>((const uint16_t *)a.q + at + 32 * s);
+                    qf[s][1] = qf[s][2] = diff_u32x4{0, 0, 0, 0};
                 }
             }
         }
         const float lam = whole ? a.e.lam[(row0 + tok) * a.e.lam_stride + h] : 0.0f;
-        f32x4 acc[G][4];
+        f32x4 acc[CT];
         float m_run = -INFINITY, l_run = 0.0f;
 #pragma unroll
-        for (int c = 0; c < G; ++c)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[c][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = 0; c < CT; ++c) acc[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
         const int32_t *table = a.tables + (int64_t)it.b * a.max_blocks;
         int32_t blk[NC];
@@ -189,7 +224,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         };
         auto write = [&](int64_t t) __attribute__((always_inline)) {
             if (t >= t1) return;
-            float *s_k = s_buf + ((t - t0) & 1 ? BUF : 0), *s_v = s_k + 2 * kDiffKeys * KP;
+            uint8_t *to = s_t(t - t0);
             const bool some = t * kDiffKeys + kDiffKeys - 1 > seesb;         // hidden from some row
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
@@ -198,7 +233,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 float x[8], y[8];
                 wide8<DT>(rk[n], x);
                 wide8<DT>(rv[n], y);
-                float *k = s_k + (m * kDiffKeys + key) * KP + 8 * c, *v = s_v + key * VP + m * D + 8 * c;
                 if (some) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
@@ -208,10 +242,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                         atomicMin(&s_bad[m * D + 8 * c + j], (int)(t * kDiffKeys + key));
                     }
                 }
-                *reinterpret_cast<f32x4 *>(k) = f32x4{x[0], x[1], x[2], x[3]};
-                *reinterpret_cast<f32x4 *>(k + 4) = f32x4{x[4], x[5], x[6], x[7]};
-                *reinterpret_cast<f32x4 *>(v) = f32x4{y[0], y[1], y[2], y[3]};
-                *reinterpret_cast<f32x4 *>(v + 4) = f32x4{y[4], y[5], y[6], y[7]};
+                diff_u32x4 xp[3], yp[3];
+                parts8(x, xp);
+                parts8(y, yp);
+                uint8_t *k = to + m * HB + key * RB + 16 * key_chunk<D>(key, c);
+                uint8_t *v = to + (2 + m) * HB + key * RB + 16 * value_chunk8<D>(key, c);
+#pragma unroll
+                for (int p = 0; p < NP; ++p) {
+                    *reinterpret_cast<diff_u32x4 *>(k + p * 4 * HB) = xp[p];
+                    *reinterpret_cast<diff_u32x4 *>(v + p * 4 * HB) = yp[p];
+                }
             }
         };
         look(t0);
@@ -223,19 +263,20 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         look(t0 + 2);
         __syncthreads();
         for (int64_t t = t0; t < t1; ++t) {
-            const float *s_k = s_buf + ((t - t0) & 1 ? BUF : 0) + mp * kDiffKeys * KP, *s_v = s_buf + ((t - t0) & 1 ? BUF : 0) + 2 * kDiffKeys * KP;
+            const uint8_t *from = s_t(t - t0);
             if (t * kDiffKeys <= sees1) {              // else no row of this wave sees any of it
                 f32x4 sc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    f32x4 x[2];
+                for (int s = 0; s < KS; ++s)
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) x[b] = *reinterpret_cast<const f32x4 *>(s_k + (16 * b + r16) * KP + 16 * s + 4 * q4);
+                    for (int b = 0; b < 2; ++b) {
+                        const int key = 16 * b + r16;
+                        const uint8_t *k = from + mp * HB + key * RB + 16 * key_chunk<D>(key, 4 * s + q4);
+                        diff_u32x4 x[NP];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int b = 0; b < 2; ++b) sc[b] = mfma_f32(x[b][j], qf[s][j], sc[b]);
-                }
+                        for (int p = 0; p < NP; ++p) x[p] = *reinterpret_cast<const diff_u32x4 *>(k + p * 4 * HB);
+                        sc[b] = mfma_parts<NP>(x, qf[s], sc[b]);
+                    }
                 const bool cut = t * kDiffKeys + kDiffKeys - 1 > sees0;
                 float top = -INFINITY;
 #pragma unroll
@@ -254,9 +295,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                     const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - now);
                     l_run *= alpha;
 #pragma unroll
-                    for (int c = 0; c < G; ++c)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[c][j] *= alpha;
+                    for (int c = 0; c < CT; ++c) acc[c] *= alpha;
                     m_run = now;
                 }
 #pragma unroll
@@ -268,82 +307,79 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                         sc[b][i] = p;
                         l_run += p;
                     }
+                const float y[8] = {sc[0][0], sc[0][1], sc[0][2], sc[0][3], sc[1][0], sc[1][1], sc[1][2], sc[1][3]};
+                diff_u32x4 pp[3];
+                parts8(y, pp);
+                // V^T as the A operand: lane (m, q) takes keys 4 q .. +4 of both halves of column m.
+                // Within each 16-lane group, lane j of a transposing read receives element j % 4 of the
+                // 8 bytes that lanes 4 k + j / 4 address, k = 0 .. 3: lane i points at key i / 4 of the
+                // four and columns 4 (i % 4) of the sixteen.
+                const int vr = 4 * q4 + (r16 >> 2);
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                for (int c = 0; c < CT; ++c) {
+                    const int hd = c / (D / 16), vc = 2 * (c % (D / 16)) + ((r16 & 3) >> 1);
+                    const uint8_t *v = from + (2 + hd) * HB + 8 * (r16 & 1);
+                    diff_u32x4 x[NP];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int p = 0; p < NP; ++p)
 #pragma unroll
-                        for (int c = 0; c < G; ++c) {
-                            const f32x4 v = *reinterpret_cast<const f32x4 *>(s_v + (16 * b + 4 * q4 + i) * VP + 64 * c + 4 * r16);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) acc[c][j] = mfma_f32(v[j], sc[b][i], acc[c][j]);
+                        for (int b = 0; b < 2; ++b) {
+                            typedef short s16x4 __attribute__((ext_vector_type(4)));
+                            const int key = 16 * b + vr;
+                            const diff_u32x2 w = __builtin_bit_cast(diff_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (__attribute__((address_space(3))) s16x4 *)(v + p * 4 * HB + key * RB + 16 * value_chunk8<D>(key, vc))));
+                            x[p][2 * b] = w[0];
+                            x[p][2 * b + 1] = w[1];
                         }
+                    acc[c] = mfma_parts<NP>(x, pp, acc[c]);
+                }
             }
+            if (NB == 1) __syncthreads();              // one buffer: the tile has been used
             write(t + 1);
             load(t + 2);
             look(t + 3);
             __syncthreads();
         }
 
-        // lane (n, q): columns 64 c + 16 q + 4 i + j of row n in acc[c][j][i]
+        // lane (n, q): columns 16 c + 4 q + i of row n in acc[c][i]
         if (s_any) {
 #pragma unroll
-            for (int c = 0; c < G; ++c)
+            for (int c = 0; c < CT; ++c)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (s_bad[64 * c + 16 * q4 + 4 * i + j] <= sees) acc[c][j][i] = __builtin_nanf("");
+                for (int i = 0; i < 4; ++i)
+                    if (s_bad[16 * c + 4 * q4 + i] <= sees) acc[c][i] = __builtin_nanf("");
         }
         const float l = sum_x32(sum_x16(l_run));
         if (whole) {
             const float inv = (mp ? lam : 1.0f) / l;
-            float *s_x = s_buf + (16 * rg + r16) * VP;
+            float *s_x = (float *)s_buf + (16 * rg + r16) * VP + 4 * q4;
             if (mp)
 #pragma unroll
-                for (int c = 0; c < G; ++c)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        *reinterpret_cast<f32x4 *>(s_x + 64 * c + 16 * q4 + 4 * i) =
-                            f32x4{acc[c][0][i], acc[c][1][i], acc[c][2][i], acc[c][3][i]} * inv;
+                for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4 *>(s_x + 16 * c) = acc[c] * inv;
             __syncthreads();
             if (!mp) {
                 float ss = 0.0f;
 #pragma unroll
-                for (int c = 0; c < G; ++c)
+                for (int c = 0; c < CT; ++c) {
+                    acc[c] = acc[c] * inv - *reinterpret_cast<const f32x4 *>(s_x + 16 * c);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const f32x4 y = *reinterpret_cast<const f32x4 *>(s_x + 64 * c + 16 * q4 + 4 * i);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float x = acc[c][j][i] * inv - y[j];
-                            acc[c][j][i] = x;
-                            ss += x * x;
-                        }
-                    }
+                    for (int i = 0; i < 4; ++i) ss += acc[c][i] * acc[c][i];
+                }
                 const float k = diff_factor(a.e, a.e.norm ? sum_x32(sum_x16(ss)) : 0.0f, 2 * D);
                 if (live) {
                     const int64_t at = ((row0 + tok) * a.pairs + h) * (2 * D);
 #pragma unroll
-                    for (int c = 0; c < G; ++c)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int col = 64 * c + 16 * q4 + 4 * i;
-                            const f32x4 n = *reinterpret_cast<const f32x4 *>(s_w + col) * k;
-                            diff_store4(a.e, at + col, f32x4{acc[c][0][i] * n[0], acc[c][1][i] * n[1], acc[c][2][i] * n[2],
-                                                             acc[c][3][i] * n[3]});
-                        }
+                    for (int c = 0; c < CT; ++c) {
+                        const int col = 16 * c + 4 * q4;
+                        diff_store4(a.e, at + col, acc[c] * (*reinterpret_cast<const f32x4 *>(s_w + col) * k));
+                    }
                 }
             }
         } else {
             const int64_t slot = 2 * cell + (t0 == 0 ? 1 : 0);
             const int64_t r = (slot * R + 16 * rg + r16) * 2 + mp;
 #pragma unroll
-            for (int c = 0; c < G; ++c)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<f32x4 *>(a.part_o + r * (2 * D) + 64 * c + 16 * q4 + 4 * i) =
-                        f32x4{acc[c][0][i], acc[c][1][i], acc[c][2][i], acc[c][3][i]};
+            for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4 *>(a.part_o + r * (2 * D) + 16 * c + 4 * q4) = acc[c];
             if (q4 == 0) {
                 a.part_ml[2 * r] = m_run;
                 a.part_ml[2 * r + 1] = l;
