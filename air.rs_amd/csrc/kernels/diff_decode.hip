@@ -10,11 +10,26 @@
 //   S  = K . Q^T  twice, with either key head; row n keeps the one of its map.
 //   P  = exp2(S * scale * log2 e - m)
 //   O^T += V^T . P^T over the 2 * head_dim columns of the pair's two value heads.
-// All products are v_mfma_f32_16x16x4_f32 on values widened (or dequantized) to
-// f32, so queries, keys, probabilities and values keep 24 bits, and no operand
-// needs a transpose: lane (n, q) holds S of tokens 4q .. 4q + 3, and step i of the
-// second product contracts over tokens {4q + i}, whose V rows lane (m, q) reads
-// straight from the page, CA consecutive columns from CA * m.
+// No operand needs a transpose: lane (n, q) holds S of tokens 4q .. 4q + 3, and the
+// second product contracts over just these, whose V rows the lane reads from the page.
+//
+// Products, by page type:
+//   f32     v_mfma_f32_16x16x4_f32, 24 bits.
+//   bf16    bf16 products of the pages as they are with queries and probabilities split
+//           into parts of 8 bits, three of each (exact); bf16 queries are one part, and
+//           bf16 outputs take two parts of a probability: the third is below 2^-16 of it,
+//           the output's own rounding 2^-9.
+//   1-byte  the same on the codes, which bf16 holds exactly; a key's scales multiply the
+//           scores in f32, a value's the probabilities before they are split (so a product
+//           of 16 columns has to lie in one scale group: order_v).  f32 products of
+//           dequantized values took 160 and 350 us where these take 125 and 296.
+//
+// Bound by the reads of the pages: 64 sequences of 512 to 4096 tokens (bf16, 8 heads of
+// 128) 569 MB in 102 us, 5.6 TB/s, 32 of 8192 (int8) 605 MB in 118 us, 5.1, 8 of 32K to
+// 128K (fp8) 1.56 GB in 287 us, 5.4; the joining takes 7 to 10 us more.  A lone short
+// sequence takes two dependent kernels of a few memory round trips, 15 us.  What carried
+// it there: 16 bytes a lane of a row (64 bytes of it at once; 8 a lane left 431 us of the
+// 350 above), and the next tile's keys in flight while this one's values are used.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -80,7 +80,10 @@ Plan plan_for(const air_kv_pool &p, bool half) {
     Plan pl;
     const int kv_pairs = p.desc.n_kv_heads / 2;
     pl.rows = half ? 128 : 64;
-    pl.extra = half ? 7 : 1;       // a block begins and ends in 16 us beside 2.1 us a tile; at f32 precision in 3 beside 3 to 5
+    // what a block's beginning and end cost beside a tile (4 and 1: 399 us for eight chunks and
+    // 382 us for 2048 tokens at f32 precision, 362 and 364 so), and the smallest piece of one
+    // that is worth its joining (at f32 precision 6, 4, 3, 2: 44, 38, 35, 37 us for four prompts)
+    pl.extra = half ? 7 : 2;
     pl.slices = std::max(1, (p.cus + kv_pairs - 1) / kv_pairs);
     pl.least = half ? 16 : 3;
     pl.cells = (size_t)kv_pairs * pl.slices;

@@ -15,9 +15,9 @@
 // buffers where they fit; while a tile is used, the next one's elements are on their
 // way in registers and the one after's table entries too.
 // Bound by the chain of a tile (one workgroup to a CU at head_dim 128): 2048 tokens of 16
-// query pairs of 128 on f32 pages in 372 us, 92 TFLOP/s; four chunks of 500 to 1000 behind
-// up to 4000 bf16 tokens 0.82 ms, 171.  On f32 operands 535 us and 1.96 ms; four waves
-// of both maps, without tiles ahead, half as fast again.
+// query pairs of 128 on f32 pages in 364 us, 94 TFLOP/s; four chunks of 500 to 1000 behind
+// up to 4000 bf16 tokens 0.77 ms, 182.  (On f32 operands 535 us and 1.96 ms; four waves of
+// both maps, without tiles ahead, twice that.)
 #include <hip/hip_runtime.h>
 
 #include "../pool.hpp"
