@@ -143,22 +143,24 @@ __device__ __forceinline__ float diff_wave_sum(float x) {
     return sum_x32(sum_x16(x));
 }
 
-// What the output row of (row, query pair) needs beside its sums: lane l holds
+// What the output row of (row, query pair h) needs beside its sums: lane l holds
 // the weights of columns V l .. +V of 64 V.
 template <int V> struct DiffTail {
+    int64_t row;
+    int h;
     float lam, w[V];
-    __device__ __forceinline__ DiffTail(const DiffOut &e, int64_t row, int h, int lane) {
+    __device__ __forceinline__ void load(const DiffOut &e, int64_t row_, int h_, int lane) {
+        row = row_;
+        h = h_;
         lam = e.lam[row * e.lam_stride + h];
-        const bool weights = e.norm && e.norm_w;
 #pragma unroll
         for (int i = 0; i < V; ++i) w[i] = 1.0f;
-        if (weights) diff_load<V>(e.norm_w + V * lane, w);
+        if (e.norm && e.norm_w) diff_load<V>(e.norm_w + V * lane, w);
     }
 };
 
 template <int V>
-__device__ __forceinline__ void diff_finish(const DiffOut &e, int64_t row, int h, int pairs, const DiffFold<V> &c,
-                                            const DiffTail<V> &tail, int lane) {
+__device__ __forceinline__ void diff_finish(const DiffOut &e, int pairs, const DiffFold<V> &c, const DiffTail<V> &tail, int lane) {
     const float i0 = 1.0f / c.l[0], i1 = tail.lam / c.l[1];
     float x[V], ss = 0.0f;
 #pragma unroll
@@ -167,7 +169,7 @@ __device__ __forceinline__ void diff_finish(const DiffOut &e, int64_t row, int h
         ss += x[i] * x[i];
     }
     const float f = diff_factor(e, e.norm ? diff_wave_sum(ss) : 0.0f, 64 * V);
-    const int64_t at = (row * pairs + h) * (64 * V) + V * lane;
+    const int64_t at = (tail.row * pairs + tail.h) * (64 * V) + V * lane;
 #pragma unroll
     for (int i = 0; i < V; ++i) x[i] *= f * tail.w[i];
     if constexpr (V == 4) {

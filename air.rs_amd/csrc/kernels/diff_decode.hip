@@ -648,7 +648,8 @@ __global__ __launch_bounds__(64 * WH) void diff_decode_merge_kernel(DiffDecodeAr
     const int w0 = p0 / chunk, w1 = (p1 - 1) / chunk;
     if (w0 == w1) return;                              // written by its slice
     const int n = w1 - w0 + 1;
-    const DiffTail<V> tail(a.e, b, h, lane);           // loaded along with the pieces
+    DiffTail<V> tail;
+    tail.load(a.e, b, h, lane);                        // along with the pieces
     const int kp = h / a.group, j = h % a.group;
     const int hh = kp * a.row_tiles + j / 8;
     DiffFold<V> c;
@@ -702,7 +703,7 @@ __global__ __launch_bounds__(64 * WH) void diff_decode_merge_kernel(DiffDecodeAr
             }
         }
     }
-    diff_finish<V>(a.e, b, h, a.pairs, c, tail, lane);
+    diff_finish<V>(a.e, a.pairs, c, tail, lane);
 }
 
 template <int D, int DT>

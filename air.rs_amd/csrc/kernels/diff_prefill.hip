@@ -10,61 +10,105 @@
 namespace airkv {
 namespace {
 
-// One row of one cut block, one wave: its pieces folded by log-sum-exp, in order.
-template <int D>
+typedef diff_f32x4 f32x4;
+
+// A lane's V columns of a piece's row.
+template <int V, bool HALF> __device__ __forceinline__ void load_piece(const void *p, int64_t at, float (&x)[V]) {
+    if constexpr (!HALF) {
+        diff_load<V>((const float *)p + at, x);
+    } else {
+        typedef _Float16 f16xV __attribute__((ext_vector_type(V == 4 ? 4 : V == 2 ? 2 : 1)));
+        const _Float16 *h = (const _Float16 *)p + at;
+        if constexpr (V == 4 || V == 2) {
+            const f16xV w = *reinterpret_cast<const f16xV *>(h);
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[i] = (float)w[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[i] = (float)h[i];
+        }
+    }
+}
+
+// Rows of one cut block, one wave: their pieces folded by log-sum-exp, in order.  HALF:
+// pieces of the 16-bit products, four rows at once (mostly of two pieces); the smaller
+// launches at f32 precision take one (four prompts: 30.4 us in all, 31.8 with four).
+constexpr int merge_rows(bool half) { return half ? 4 : 1; }
+template <int D, bool HALF>
 __global__ __launch_bounds__(256) void diff_prefill_merge_kernel(DiffPrefillArgs a) {
-    constexpr int V = D / 32, kBatch = 4;
-    const int w = blockIdx.x, kp = blockIdx.y, lane = threadIdx.x & 63;
-    const int row = blockIdx.z * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int V = D / 32, N = merge_rows(HALF), kBatch = HALF ? 2 : 4;
+    const int w = blockIdx.y, kp = blockIdx.z, lane = threadIdx.x & 63;
+    const int row = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * N;
     const int64_t at = (int64_t)kp * a.slices + w;
     const int4 d = a.desc[at];
     if (d.w == 0) return;
-    const int64_t k = (int64_t)((uint64_t)(uint32_t)d.y | (uint64_t)(uint32_t)d.z << 32);
-    DiffBlocks s;
-    diff_seq(a, d.x, s);
-    const int64_t f = k * a.rows + row;
-    if (f >= s.q * a.group) return;
-    const int64_t out_row = a.cu[d.x] + f / a.group;
-    const int h = kp * a.group + (int)(f % a.group);
-    const DiffTail<V> tail(a.e, out_row, h, lane);
-    DiffFold<V> c;
-    c.clear();
-    for (int p0 = 0; p0 < d.w; p0 += kBatch) {
-        float pm[kBatch][2], pl[kBatch][2], po[kBatch][2][V];
+    // rows past the sequence's last are read as they are (slots are whole) and not written
+    f32x4 ml[N][kBatch][2];
+    float po[N][kBatch][2][V];
+    auto load = [&](int p0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const bool in = p0 + i < d.w;
-            const int p = in ? p0 + i : p0;
-            const int64_t slot = 2 * (at + p) + (p == 0 ? 1 : 0);
+        for (int j = 0; j < N; ++j)
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                const int64_t r = (slot * a.rows + row) * 2 + m;
-                pm[i][m] = in ? a.part_ml[2 * r] : -INFINITY;
-                pl[i][m] = in ? a.part_ml[2 * r + 1] : 0.0f;
-                diff_load<V>(a.part_o + r * (2 * D) + V * lane, po[i][m]);
+            for (int i = 0; i < kBatch; ++i) {
+                const int p = p0 + i < d.w ? p0 + i : p0;
+                const int64_t slot = 2 * (at + p) + (p == 0 ? 1 : 0);
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    const int64_t r = (slot * a.rows + row + j) * 2 + m;
+                    ml[j][i][m] = *reinterpret_cast<const f32x4 *>(a.part_ml + kDiffMl * r);
+                    load_piece<V, HALF>(a.part_o, r * (2 * D) + V * lane, po[j][i][m]);
+                }
             }
-        }
+    };
+    load(0);                                           // before what the rows' places wait for
+    const int64_t k = (int64_t)((uint64_t)(uint32_t)d.y | (uint64_t)(uint32_t)d.z << 32);
+    const int64_t r0 = a.cu[d.x], f = k * a.rows + row, rows = (a.cu[d.x + 1] - r0) * a.group;
+    if (f >= rows) return;
+    const int n = rows - f < N ? (int)(rows - f) : N;
+    const bool narrow = f >> 32 == 0;                  // (a fifth of the instructions)
+    const int64_t tok = narrow ? (int64_t)((uint32_t)f / (uint32_t)a.group) : f / a.group;
+    const int pair = (int)(f - tok * a.group);
+    DiffTail<V> tail[N];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-#pragma unroll
-            for (int m = 0; m < 2; ++m) c.fold(m, pm[i][m], pl[i][m], po[i][m]);
+    for (int j = 0; j < N; ++j) {
+        const int x = pair + j, more = x / a.group;
+        tail[j].load(a.e, j < n ? r0 + tok + more : r0 + tok, kp * a.group + (j < n ? x - more * a.group : pair), lane);
     }
-    diff_finish<V>(a.e, out_row, h, a.pairs, c, tail, lane);
+    DiffFold<V> c[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) c[j].clear();
+    for (int p0 = 0; p0 < d.w; p0 += kBatch) {
+        if (p0) load(p0);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    if (p0 + i >= d.w) continue;
+                    const float l = ml[j][i][m][1];
+                    if constexpr (HALF) {
+#pragma unroll
+                        for (int e = 0; e < V; ++e) po[j][i][m][e] *= ml[j][i][m][2] * l;
+                    }
+                    c[j].fold(m, ml[j][i][m][0], l, po[j][i][m]);
+                }
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        if (j < n) diff_finish<V>(a.e, a.pairs, c[j], tail[j], lane);
 }
 
-}  // namespace
-
-hipError_t launch_diff_prefill_merge(const DiffPrefillArgs &a, int head_dim, hipStream_t s) {
+template <bool HALF> hipError_t launch_merge(const DiffPrefillArgs &a, int head_dim, hipStream_t s) {
     if (a.slices < 2) return hipSuccess;               // nothing is cut
-    const dim3 grid((unsigned)a.slices, (unsigned)a.kv_pairs, (unsigned)(a.rows / 4));
-    if (head_dim == 128) hipLaunchKernelGGL((diff_prefill_merge_kernel<128>), grid, dim3(256), 0, s, a);
-    else if (head_dim == 96) hipLaunchKernelGGL((diff_prefill_merge_kernel<96>), grid, dim3(256), 0, s, a);
-    else if (head_dim == 64) hipLaunchKernelGGL((diff_prefill_merge_kernel<64>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((diff_prefill_merge_kernel<32>), grid, dim3(256), 0, s, a);
+    // the rows of a block run together: its slots, powers of two apart, share their memory channels
+    const dim3 grid((unsigned)(a.rows / (4 * merge_rows(HALF))), (unsigned)a.slices, (unsigned)a.kv_pairs);
+    if (head_dim == 128) hipLaunchKernelGGL((diff_prefill_merge_kernel<128, HALF>), grid, dim3(256), 0, s, a);
+    else if (head_dim == 96) hipLaunchKernelGGL((diff_prefill_merge_kernel<96, HALF>), grid, dim3(256), 0, s, a);
+    else if (head_dim == 64) hipLaunchKernelGGL((diff_prefill_merge_kernel<64, HALF>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((diff_prefill_merge_kernel<32, HALF>), grid, dim3(256), 0, s, a);
     return hipGetLastError();
 }
-
-namespace {
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
@@ -72,7 +116,7 @@ size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 struct Plan {
     int32_t rows, extra, slices, least;
     size_t cells, halves;          // (pair, slice)s, rows' maps in the piece slots
-    size_t bytes(int d) const { return align256(cells * sizeof(int4)) + align256(halves * 2 * 4) + halves * 2 * d * 4; }
+    size_t bytes(int d) const { return align256(cells * sizeof(int4)) + align256(halves * kDiffMl * 4) + halves * 2 * d * 4; }
 };
 
 // half: 16-bit products (diff_prefill_16.hip), else f32 ones
@@ -131,7 +175,7 @@ hipError_t launch_diff_prefill(const air_kv_pool &p, hipStream_t s, const void *
     a.desc = (int4 *)ws;
     ws += align256(plan.cells * sizeof(int4));
     a.part_ml = (float *)ws;
-    ws += align256(plan.halves * 2 * 4);
+    ws += align256(plan.halves * kDiffMl * 4);
     a.part_o = (float *)ws;
     for (int32_t b0 = 0; b0 < batch; b0 += kDiffPrefillBatch) {
         a.batch = std::min(batch - b0, kDiffPrefillBatch);
@@ -139,7 +183,7 @@ hipError_t launch_diff_prefill(const air_kv_pool &p, hipStream_t s, const void *
         a.tables = tables + (int64_t)b0 * max_blocks;
         a.lens = lens + b0;
         hipError_t e = half ? launch_diff_prefill_16(a, d, s) : launch_diff_prefill_f32(a, d, s);
-        if (e == hipSuccess) e = launch_diff_prefill_merge(a, d, s);
+        if (e == hipSuccess) e = half ? launch_merge<true>(a, d, s) : launch_merge<false>(a, d, s);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;

@@ -594,15 +594,21 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
         } else {
             const int64_t slot = 2 * cell + (t0 == 0 ? 1 : 0);
             const int64_t r = (slot * kRows + 32 * rg + r32) * 2 + mp;
+            // the piece's means, under the values' power of two as the values are: they are
+            // rounded to 11 bits as these, and half as long to write and read as f32 sums
+            // (eight chunks 358 -> 350 us)
+            const float inv = l > 0.0f ? owed / l : owed;
+            uint16_t *o = (uint16_t *)a.part_o + r * (2 * D) + 4 * hf;
 #pragma unroll
             for (int c = 0; c < CT; ++c)
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
-                    *reinterpret_cast<f32x4 *>(a.part_o + r * (2 * D) + 32 * c + 2 * i + 4 * hf) =
-                        f32x4{acc[c][i] * back, acc[c][i + 1] * back, acc[c][i + 2] * back, acc[c][i + 3] * back};
+                    *reinterpret_cast<u32x2 *>(o + 32 * c + 2 * i) =
+                        u32x2{pack2<true>(acc[c][i] * inv, acc[c][i + 1] * inv), pack2<true>(acc[c][i + 2] * inv, acc[c][i + 3] * inv)};
             if (hf == 0) {
-                a.part_ml[2 * r] = m_run;
-                a.part_ml[2 * r + 1] = l;
+                a.part_ml[kDiffMl * r] = m_run;
+                a.part_ml[kDiffMl * r + 1] = l;
+                a.part_ml[kDiffMl * r + 2] = 1.0f / fv;
             }
             if (t0 == 0) {                          // begun here: its last unit's slice ends it
                 const int64_t last = u - t1 + nt - 1;      // of the launch's units

@@ -148,13 +148,15 @@ def _p_step(c):
     1-byte pages, whose scores err by 2^-11 sum |q k| scale (taken at 8 standard
     deviations of normal rows: sum |q k| / sqrt(d) <= 2/pi sqrt(d) + 8), which moves a
     probability by twice that (its own score, and the sum's).  Below f16's normal
-    numbers, 2^-14, a probability errs by 2^-25 of the largest."""
+    numbers, 2^-14, a probability errs by 2^-25 of the largest.  Where a block of rows is
+    cut, each piece's means, at most its sum of p |v| in size, are rounded to 11 bits too:
+    another 2^-11 of the whole."""
     if c.pool.dtype == airkv.F32:
         return 0.0
     tiny = 2.0 ** -25 * c.lens.max(initial=1)
     if c.pool.dtype == airkv.BF16:
-        return 2.0 ** -11 + tiny
-    return 2.0 ** -11 * (2 + 2 * (0.64 * c.d ** 0.5 + 8)) + tiny
+        return 2.0 ** -11 * 2 + tiny
+    return 2.0 ** -11 * (3 + 2 * (0.64 * c.d ** 0.5 + 8)) + tiny
 
 
 @pytest.mark.parametrize("d,kv,group,bs,scale_group", [(64, 8, 1, 16, 32), (128, 4, 4, 16, 32), (128, 2, 8, 32, 32), (32, 2, 3, 16, 8),
