@@ -28,8 +28,8 @@
 // 128) 569 MB in 102 us, 5.6 TB/s, 32 of 8192 (int8) 605 MB in 118 us, 5.1, 8 of 32K to
 // 128K (fp8) 1.56 GB in 287 us, 5.4; the joining takes 7 to 10 us more.  A lone short
 // sequence takes two dependent kernels of a few memory round trips, 15 us.  What carried
-// it there: 16 bytes a lane of a row (64 bytes of it at once; 8 a lane left 431 us of the
-// 350 above), and the next tile's keys in flight while this one's values are used.
+// it there: 16 bytes a lane of a key row (64 bytes of it at once; with 8 the fp8 case took 431 us
+// where it then took 350), and the next tile's keys in flight while this one's values are used.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
