@@ -161,7 +161,8 @@ template <int V> struct DiffTail {
 
 template <int V>
 __device__ __forceinline__ void diff_finish(const DiffOut &e, int pairs, const DiffFold<V> &c, const DiffTail<V> &tail, int lane) {
-    const float i0 = 1.0f / c.l[0], i1 = tail.lam / c.l[1];
+    // no key at all (every block of the sequence outside the pool): zeros
+    const float i0 = c.l[0] == 0.0f ? 0.0f : 1.0f / c.l[0], i1 = c.l[1] == 0.0f ? 0.0f : tail.lam / c.l[1];
     float x[V], ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {

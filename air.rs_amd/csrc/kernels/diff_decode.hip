@@ -273,7 +273,7 @@ void diff_decode_kernel(DiffDecodeArgs a) {
         if (w0 == w1) {                                // the whole sequence: its output rows
             const int h = kp * a.group + 8 * rt + qp;
             const float lam = live_row ? a.e.lam[bq * a.e.lam_stride + h] : 0.0f;
-            const float inv = (map1 ? -lam : 1.0f) / l;
+            const float inv = l == 0.0f ? 0.0f : (map1 ? -lam : 1.0f) / l;      // no block of it is in the pool: zeros
             float ss = 0.0f;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -360,7 +360,7 @@ void diff_decode_kernel(DiffDecodeArgs a) {
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < SL; ++i)
-                x[t][i] = __builtin_amdgcn_raw_buffer_load_b32(rs, lane + 64 * i < 16 * nsc ? 4 * lane + 256 * i : 0x40000000,
+                x[t][i] = __builtin_amdgcn_raw_buffer_load_b32(rs, lane + 64 * i < 16 * nsc ? 4 * lane + 256 * i : 0,
                                                                t ? 4 * bs * nsc : 0, kDiffStream);
     };
     auto load_k = [&](bool in) __attribute__((always_inline)) {

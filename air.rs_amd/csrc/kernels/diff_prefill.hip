@@ -114,9 +114,9 @@ size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // A slice for every workgroup that is resident at once, all K/V pairs together.
 struct Plan {
-    int32_t rows, extra, slices, least;
+    int32_t rows, extra, slices, least, elem;      // elem: bytes of a piece's sum
     size_t cells, halves;          // (pair, slice)s, rows' maps in the piece slots
-    size_t bytes(int d) const { return align256(cells * sizeof(int4)) + align256(halves * kDiffMl * 4) + halves * 2 * d * 4; }
+    size_t bytes(int d) const { return align256(cells * sizeof(int4)) + align256(halves * kDiffMl * 4) + halves * 2 * d * elem; }
 };
 
 // half: 16-bit products (diff_prefill_16.hip), else f32 ones
@@ -130,6 +130,7 @@ Plan plan_for(const air_kv_pool &p, bool half) {
     pl.extra = half ? 7 : 2;
     pl.slices = std::max(1, (p.cus + kv_pairs - 1) / kv_pairs);
     pl.least = half ? 16 : 3;
+    pl.elem = half ? 2 : 4;
     pl.cells = (size_t)kv_pairs * pl.slices;
     pl.halves = 2 * pl.cells * pl.rows * 2;
     return pl;

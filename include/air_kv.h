@@ -404,8 +404,8 @@ int air_paged_prefill_workspace_size(const air_kv_pool *pool, int32_t n_q_heads,
  * Decode: one new token per sequence (already appended) over its seq_lens[b]
  * cached tokens, with the workspace rules of air_paged_decode and its refusals:
  * out-of-pool table entries are skipped and counted, seq_lens outside [0,
- * max_blocks * block_size] are clamped and counted, a sequence of length 0
- * produces zeros.  max_splits (1 to 256) bounds the slices that share a sequence;
+ * max_blocks * block_size] are clamped and counted, a sequence of length 0 (or
+ * with no block in the pool) produces zeros.  max_splits (1 to 256) bounds the slices that share a sequence;
  * with 1, its result does not depend on the others'.  Queries, keys and values
  * keep f32 precision on every pool; so do probabilities under f32 outputs, while
  * bf16 outputs take 16 bits of them. */

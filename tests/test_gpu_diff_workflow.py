@@ -127,6 +127,12 @@ def test_decode_tables_and_lengths_outside(dtype, bs, splits):
     want, bound = _decode_ref(c, q64, lam64, w64, 1.0, [cols * bs, 80, 16, 80, 0, 33], c.tables)
     check(out.cpu().numpy(), want, bound, airkv.F32, "clamped")
     assert c.pool.error_count(reset=True) == 1
+    # no block of a sequence in the pool: zeros
+    tables = c.tables.copy()
+    tables[[0, 2]] = -1
+    c.pool.paged_diff_decode(q, _dev(lam.cpu().numpy()), _dev(tables), _dev(c.lens), out, norm_weight=w, norm_eps=1e-5, max_splits=splits)
+    assert (out[0] == 0).all() and (out[2] == 0).all() and torch.isfinite(out).all()
+    assert c.pool.error_count(reset=True) == -(-300 // 16) + 1
 
 
 @pytest.mark.parametrize("dtype,f32", [(airkv.F32, True), (airkv.BF16, False), (airkv.INT8, False), (airkv.FP8, True)])
