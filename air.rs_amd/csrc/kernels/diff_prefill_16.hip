@@ -63,6 +63,13 @@ template <bool F16> __device__ __forceinline__ uint32_t pack2(float x, float y) 
     else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
 }
 
+// Lanes (n, 0) and (n, 1) hold columns 0 .. 3 and 4 .. 7 of a row's eight in x, and of the
+// next eight in y: the eight of x to lane (n, 0), those of y to (n, 1).
+__device__ __forceinline__ u32x4 eight(u32x2 x, u32x2 y) {
+    const auto a = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false), b = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
+    return u32x4{a[0], b[0], a[1], b[1]};
+}
+
 // 2^(e - exponent of x) for a finite positive normal x, else 1.
 __device__ __forceinline__ float pow2_to(float x, int e) {
     const int f = (int)((__float_as_uint(x) >> 23) & 0xFF);
@@ -580,15 +587,19 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                 k = diff_factor(a.e, ss + s_ss[1 - mp][rg][r32], 2 * D);
             }
             if (live) {
-                uint16_t *o = (uint16_t *)a.e.out + ((row0 + tok) * a.pairs + h) * (2 * D) + mp * D + 4 * hf;
+                uint16_t *o = (uint16_t *)a.e.out + ((row0 + tok) * a.pairs + h) * (2 * D) + mp * D + 8 * hf;
 #pragma unroll
                 for (int c = 0; c < CH; ++c)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const f32x4 n = *reinterpret_cast<const f32x4 *>(s_w + mp * D + 32 * c + 8 * i + 4 * hf) * k;
-                        *reinterpret_cast<u32x2 *>(o + 32 * c + 8 * i) =
-                            u32x2{bf16_pair(acc[c][4 * i] * n[0], acc[c][4 * i + 1] * n[1]),
-                                  bf16_pair(acc[c][4 * i + 2] * n[2], acc[c][4 * i + 3] * n[3])};
+                    for (int i = 0; i < 4; i += 2) {
+                        u32x2 x[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const f32x4 n = *reinterpret_cast<const f32x4 *>(s_w + mp * D + 32 * c + 8 * (i + e) + 4 * hf) * k;
+                            x[e] = u32x2{bf16_pair(acc[c][4 * (i + e)] * n[0], acc[c][4 * (i + e) + 1] * n[1]),
+                                         bf16_pair(acc[c][4 * (i + e) + 2] * n[2], acc[c][4 * (i + e) + 3] * n[3])};
+                        }
+                        *reinterpret_cast<u32x4 *>(o + 32 * c + 8 * i) = eight(x[0], x[1]);
                     }
             }
         } else {
@@ -598,13 +609,18 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
             // rounded to 11 bits as these, and half as long to write and read as f32 sums
             // (eight chunks 358 -> 350 us)
             const float inv = l > 0.0f ? owed / l : owed;
-            uint16_t *o = (uint16_t *)a.part_o + r * (2 * D) + 4 * hf;
+            uint16_t *o = (uint16_t *)a.part_o + r * (2 * D) + 8 * hf;
 #pragma unroll
             for (int c = 0; c < CT; ++c)
 #pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                    *reinterpret_cast<u32x2 *>(o + 32 * c + 2 * i) =
-                        u32x2{pack2<true>(acc[c][i] * inv, acc[c][i + 1] * inv), pack2<true>(acc[c][i + 2] * inv, acc[c][i + 3] * inv)};
+                for (int i = 0; i < 16; i += 8) {
+                    u32x2 x[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        x[e] = u32x2{pack2<true>(acc[c][i + 4 * e] * inv, acc[c][i + 4 * e + 1] * inv),
+                                     pack2<true>(acc[c][i + 4 * e + 2] * inv, acc[c][i + 4 * e + 3] * inv)};
+                    *reinterpret_cast<u32x4 *>(o + 32 * c + 2 * i) = eight(x[0], x[1]);
+                }
             if (hf == 0) {
                 a.part_ml[kDiffMl * r] = m_run;
                 a.part_ml[kDiffMl * r + 1] = l;
