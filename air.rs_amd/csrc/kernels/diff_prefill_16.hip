@@ -23,9 +23,10 @@
 //
 // Bound by vector issue and the tile's chain: per tile and SIMD 1540 of 4300 clocks are
 // products, 2000 arithmetic (exponentials, the values' rounding, staging), which overlap
-// in part.  8192 tokens of 16 query pairs of 128 in 1.05 ms: 520 TFLOP/s of 8 d a (query
-// pair, key), 780 of the 12 d that two running maps take; eight chunks of 200 to 512
-// behind up to 6000 tokens 351 us, 450 TFLOP/s; int8 pages, 32 query pairs, 622 us, 437.
+// in part.  8192 tokens of 16 query pairs of 128 in 1.02 ms: 540 TFLOP/s of 8 d a (query
+// pair, key), 810 of the 12 d that two running maps take; eight chunks of 200 to 512
+// behind up to 6000 tokens 335 us, 470 TFLOP/s; int8 pages, 32 query pairs, 599 us, 454
+// (a tenth more on cards whose clock drops further).
 #include <hip/hip_runtime.h>
 
 #include "../pool.hpp"
