@@ -90,7 +90,7 @@ __device__ __forceinline__ float dpp_ror8(float x) {
     return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xF, 0xF, false));
 }
 
-// BYTES (2, 4, 8, 12, 16 or 32) bytes of a page at base + off.
+// BYTES (2, 4, 8, 16 or 32) bytes of a page at base + off.
 template <int BYTES>
 __device__ __forceinline__ void load_piece(const __amdgpu_buffer_rsrc_t &r, int off, int base,
                                            uint32_t (&w)[(BYTES + 3) / 4]) {
@@ -101,9 +101,6 @@ __device__ __forceinline__ void load_piece(const __amdgpu_buffer_rsrc_t &r, int 
     } else if constexpr (BYTES == 8) {
         const diff_u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off, base, kDiffStream);
         w[0] = x[0]; w[1] = x[1];
-    } else if constexpr (BYTES == 12) {
-        const auto x = __builtin_amdgcn_raw_buffer_load_b96(r, off, base, kDiffStream);
-        w[0] = x[0]; w[1] = x[1]; w[2] = x[2];
     } else {
 #pragma unroll
         for (int i = 0; i < BYTES / 16; ++i) {

@@ -433,3 +433,42 @@ def test_many_pieces():
                 c.pool.paged_diff_decode(q, lam, tables, lens, out, norm_weight=w, norm_eps=1e-5, max_splits=splits)
                 used = check(out.float().cpu().numpy(), want, bound, airkv.F32 if f32 else airkv.BF16, f"splits {splits}")
                 log(f"many pieces dtype={dtype} f32={f32} splits={splits}: {used:.3f} of the bound")
+
+
+@pytest.mark.parametrize("dtype,d,scale_group", [(airkv.F32, 128, 32), (airkv.BF16, 96, 32), (airkv.INT8, 128, 128), (airkv.FP8, 64, 64),
+                                                 (airkv.INT8, 96, 8), (airkv.FP8, 128, 32), (airkv.INT8, 32, 16)])
+@pytest.mark.parametrize("q_f32,out_f32", [(True, False), (False, True)])
+def test_mixed_types_and_scale_groups(dtype, d, scale_group, q_f32, out_f32):
+    """f32 queries with bf16 outputs and the other way round, scale groups from 8 to the whole row."""
+    torch = torch_mod()
+    c = Cache(dtype, d, 4, 16, [1, 77, 1040, 16, 300], seed=d + scale_group, scale_group=scale_group)
+    q, lam, w, q64, lam64, w64 = c.rows(5, 9, q_f32, True, True)
+    tables, lens = c.device()
+    odt = airkv.F32 if out_f32 else airkv.BF16
+    out = torch.full((5, 18, 2 * d), float("nan"), device="cuda", dtype=torch.float32 if out_f32 else torch.bfloat16)
+    want, bound = _decode_ref(c, q64, lam64, w64, 1.0, c.lens, c.tables)
+    for splits in (256, 1):
+        c.pool.paged_diff_decode(q, lam, tables, lens, out, norm_weight=w, norm_eps=1e-5, max_splits=splits)
+        used = check(out.float().cpu().numpy(), want, bound, odt, f"splits {splits}")
+    cu = _dev(np.arange(6, dtype=np.int32))                     # the same rows as prompts' last tokens
+    c.pool.paged_diff_prefill(q, lam, cu, tables, lens, out.fill_(float("nan")), max_q_len=1, norm_weight=w, norm_eps=1e-5)
+    more = check(out.float().cpu().numpy(), want, bound, odt, "prefill")
+    log(f"mixed types dtype={dtype} d={d} scale_group={scale_group}: decode {used:.3f}, prefill {more:.3f} of the bound")
+    assert c.pool.error_count() == 0
+
+
+def test_a_block_in_several_tables():
+    """Sequences that share a prefix's blocks, one of them twice in one table."""
+    torch = torch_mod()
+    c = Cache(airkv.BF16, 64, 2, 16, [64, 40, 50], seed=21)
+    tables = c.tables.copy()
+    tables[1, :2] = tables[0, :2]
+    tables[2, 3] = tables[2, 0]
+    q, lam, w, q64, lam64, w64 = c.rows(3, 2, True, False, True)
+    out = torch.empty(3, 2, 128, device="cuda")
+    want, bound = _decode_ref(c, q64, lam64, w64, 1.0, c.lens, tables)
+    c.pool.paged_diff_decode(q, lam, _dev(tables), _dev(c.lens), out, norm_weight=w, norm_eps=1e-5)
+    check(out.cpu().numpy(), want, bound, airkv.F32, "decode")
+    c.pool.paged_diff_prefill(q, lam, _dev(np.arange(4, dtype=np.int32)), _dev(tables), _dev(c.lens), out.fill_(3.0), max_q_len=1,
+                              norm_weight=w, norm_eps=1e-5)
+    check(out.cpu().numpy(), want, bound, airkv.F32, "prefill")
