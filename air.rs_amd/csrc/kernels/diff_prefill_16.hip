@@ -254,9 +254,7 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
         // A head's rows of a block lie bs rows behind the head's before: one buffer holds both
         // heads', and a lane whose key is not there reads outside of it: zeros.
         const int head_step = a.bs * D * EB, head_sc = a.bs * nsc * 4;
-        auto load_tile = [&](int t, Raw &r) __attribute__((always_inline)) {
-            if (t % 64 == 0) look_up(t);
-            const int32_t blk = __builtin_amdgcn_readlane(window, t % 64);
+        auto load_rows = [&](int t, int32_t blk, Raw &r) __attribute__((always_inline)) {
             const int left = blk < 0 ? 0 : rest - t * kDiffKeys - 16 * p_half;
             const int off = (p_key & 15) < left ? p_off : 0x40000000;
             const int64_t row = (((int64_t)(blk < 0 ? 0 : blk) * a.heads + 2 * kp) << shift) + (16 * p_half & (a.bs - 1));
@@ -292,6 +290,15 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                                                       : __builtin_amdgcn_raw_buffer_load_b32(sv, osc, step, 0));
                 }
             }
+        };
+        // The next tile, and the blocks of the last two: a tile that is staged again is loaded
+        // from its block here, not from the window, which may have gone on past it.
+        int32_t blk_at = -1, blk_before = -1;
+        auto load_tile = [&](int t, Raw &r) __attribute__((always_inline)) {
+            if (t % 64 == 0) look_up(t);
+            blk_before = blk_at;
+            blk_at = __builtin_amdgcn_readlane(window, t % 64);
+            load_rows(t, blk_at, r);
         };
         // Scales and values of the tile in registers that leave f16's range are marked for all
         // waves; behind the barrier the tile is staged again under another power of two.
@@ -451,10 +458,11 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
             if (!mp && some) scores();
             if (__builtin_amdgcn_readfirstlane(kt | vt)) {
                 if (settle(__builtin_amdgcn_readfirstlane(kt), __builtin_amdgcn_readfirstlane(vt))) {       // rare
-                    load_tile(t + 1, raw);
+                    const bool ahead = t + 2 < tiles;  // (it is in the registers)
+                    load_rows(t + 1, ahead ? blk_before : blk_at, raw);
                     write_tile(t + 1, raw);
                     __syncthreads();
-                    if (t + 2 < tiles) load_tile(t + 2, raw);
+                    if (ahead) load_rows(t + 2, blk_at, raw);
                 }
             }
             if (some) {
