@@ -78,6 +78,9 @@ __device__ __forceinline__ float pow2_to(float x, int e) {
     return f == 0 || f == 255 || k < 1 || k > 254 ? 1.0f : __uint_as_float((uint32_t)k << 23);
 }
 
+// The exponent of a power of two (a normal number).
+__device__ __forceinline__ int exponent(float x) { return (int)(__float_as_uint(x) >> 23) - 127; }
+
 // The schedule of N matrix products that take READS LDS reads each: the reads of the
 // first AHEAD, then a product and the reads of the next in turn.
 template <int N, int AHEAD, int READS> __device__ __forceinline__ void read_ahead() {
@@ -194,7 +197,7 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
 
         // Q^T as the B operand: lane (n, h) holds elements 16 s + 8 h .. +8 of row n
         u32x4 qf[KS];
-        float qs = a.scale_log2;
+        int qe = 0;                                    // (the power of two they are under)
         int sees;
         {
             bool live;
@@ -214,7 +217,7 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                     top = fmaxf(top, fmaxf(__builtin_fabsf(__uint_as_float(qf[s][j] << 16)),
                                            __builtin_fabsf(__uint_as_float(qf[s][j] & 0xFFFF0000u))));
             const float fq = pow2_to(max_x32(top), 4);          // the row's largest element in [2^4, 2^5)
-            qs = a.scale_log2 / fq;
+            qe = exponent(fq);
 #pragma unroll
             for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -466,7 +469,12 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                 }
             }
             if (some) {
-                const float ft = qs / fk_now;
+                // what the products have to be multiplied by.  Neither 0 nor infinite: a masked
+                // score, -inf, times 0 would be NaN, and so would 0 times infinity.  (Products are
+                // below 2^32: under the least factor here their scores are 0 all the same.)
+                float ft = a.scale_log2;
+                if constexpr (QUANT) ft = __builtin_amdgcn_ldexpf(ft, -(qe + exponent(fk_now)));
+                ft = fminf(fmaxf(ft, 0x1p-126f), 0x1.fffffep127f);
                 const uint8_t *sv = s_t(t) + 2 * HB;
                 const bool cut = t * kDiffKeys + kDiffKeys - 1 > sees0;
                 if (cut) {
