@@ -71,11 +71,11 @@ __device__ __forceinline__ u32x4 eight(u32x2 x, u32x2 y) {
     return u32x4{a[0], b[0], a[1], b[1]};
 }
 
-// 2^(e - exponent of x) for a finite positive normal x, else 1.
+// 2^(e - exponent of x) for a finite x >= 0, from 2^-126 to 2^112 (subnormal x, and normal
+// ones below 2^(e - 112), get the largest), else 1.
 __device__ __forceinline__ float pow2_to(float x, int e) {
-    const int f = (int)((__float_as_uint(x) >> 23) & 0xFF);
-    const int k = 127 + e - (f - 127);
-    return f == 0 || f == 255 || k < 1 || k > 254 ? 1.0f : __uint_as_float((uint32_t)k << 23);
+    const int f = (int)((__float_as_uint(x) >> 23) & 0xFF), k = 127 + e - (f - 127);
+    return f == 255 ? 1.0f : __uint_as_float((uint32_t)(k < 1 ? 1 : k > 239 ? 239 : k) << 23);
 }
 
 // The exponent of a power of two (a normal number).

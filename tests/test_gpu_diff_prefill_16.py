@@ -60,3 +60,28 @@ def test_a_factor_past_the_largest_float(dtype):
     q[:, :, 0] = 0
     _, used = _prefill(c, [50, 3, 7], q, lam, _p_step(c))
     log(f"a factor past the largest float dtype={dtype}: {used:.3f} of the bound")
+
+
+@pytest.mark.parametrize("dtype,v_mul,k_mul", [(airkv.BF16, 2.0 ** -122, 1.0), (airkv.INT8, 2.0 ** -118, 1.0),
+                                               (airkv.INT8, 1.0, 2.0 ** -118)])
+def test_values_and_keys_near_the_smallest_normal_float(dtype, v_mul, k_mul):
+    """Nothing is lost of values, keys or queries that the largest power of two brings into
+    f16's range."""
+    torch = torch_mod()
+    c = Cache(dtype, 64, 2, 16, [100, 33, 7], seed=55)
+    _refill(c, lambda t: k_mul, lambda t: v_mul)
+    q, lam, _, _, _, _ = c.rows(60, 2, False, False, False)
+    q = (q.float() / k_mul).to(torch.bfloat16)
+    # outputs of this size are scaled up before they are rounded
+    _, used = _prefill(c, [50, 3, 7], q, lam, _p_step(c), out_scale=1 / v_mul)
+    log(f"near the smallest normal float dtype={dtype} v_mul={v_mul:.2g} k_mul={k_mul:.2g}: {used:.3f} of the bound")
+
+
+def test_small_queries_and_large_keys():
+    torch = torch_mod()
+    c = Cache(airkv.INT8, 64, 2, 16, [100, 33, 7], seed=56)
+    _refill(c, lambda t: 2.0 ** 118, lambda t: 1.0)
+    q, lam, _, _, _, _ = c.rows(60, 2, False, False, False)
+    q = (q.float() * 2.0 ** -118).to(torch.bfloat16)
+    _, used = _prefill(c, [50, 3, 7], q, lam, _p_step(c))
+    log(f"small queries, large keys: {used:.3f} of the bound")
