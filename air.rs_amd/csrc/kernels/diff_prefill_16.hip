@@ -124,7 +124,7 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
     __shared__ __align__(16) uint8_t s_mem[12 * HB > XB ? 12 * HB : XB];
     auto s_t = [&](int t) __attribute__((always_inline)) { return s_mem + t % 3 * (4 * HB); };
     // Per tile (mod 3), keys' scale and values' (scale): the bits of the largest of those that
-    // leave f16's range under the present power of two (of all in a block's first tile)
+    // leave f16's range under the present power of two (of all, as long as a block had zeros only)
     __shared__ uint32_t s_top[3][2];
     __shared__ __align__(16) float s_w[2 * D];         // the norm's weights
     __shared__ float s_ss[2][4][32];                   // the halves' sums of squares
@@ -304,14 +304,19 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
             load_rows(t, blk_at, r);
         };
         // Scales and values of the tile in registers that leave f16's range are marked for all
-        // waves; behind the barrier the tile is staged again under another power of two.
+        // waves; behind the barrier the tile is staged again under another power of two.  Until a
+        // tile has something that is not zero the power of two is another block's, and too small
+        // ones count too.  (The scale 1 that the append gives a group of zeros does not count.)
+        uint32_t lim_k = 1, lim_v = 1;                 // the bits from which on one is marked
         auto mark = [&](int t, const Raw &r) __attribute__((always_inline)) {
             uint32_t k = 0, v = 0;                     // this lane's largest finite ones, as bits
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const bool val = (p_row0 + 8 * WR * i) / kDiffKeys >= 2;
                 if constexpr (QUANT) {
-                    const uint32_t y = __float_as_uint(r.s[i]) & 0x7FFFFFFFu, x = y < 0x7F800000u ? y : 0;
+                    const uint32_t y = __float_as_uint(r.s[i]) & 0x7FFFFFFFu;
+                    const bool zeros = ((r.w[i][0] | r.w[i][1]) & (DT == AIR_KV_FP8 ? 0x7F7F7F7Fu : ~0u)) == 0 && y <= 0x3F800000u;
+                    const uint32_t x = y < 0x7F800000u && !zeros ? y : 0;
                     if (val) v = x > v ? x : v;
                     else k = x > k ? x : k;
                 } else if (val) {
@@ -341,8 +346,8 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                     atomicMax(&s_top[0][1], v);
                 }
             } else {
-                if (QUANT && __uint_as_float(k) * fk >= kMost) atomicMax(&s_top[t % 3][0], k);
-                if (__uint_as_float(v) * fv >= kMost) atomicMax(&s_top[t % 3][1], v);
+                if (QUANT && k >= lim_k) atomicMax(&s_top[t % 3][0], k);
+                if (v >= lim_v) atomicMax(&s_top[t % 3][1], v);
             }
         };
         // the tile in registers into its buffer
@@ -400,9 +405,16 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
             if (newk) fk = pow2_to(__uint_as_float(kt), kAim);
             if (newv) {
                 const float now = pow2_to(__uint_as_float(vt), kAim);
-                owed_next *= now / fv;
+                if (lim_v != 1) owed_next *= now / fv; // (else the sums are zeros)
                 fv = now;
             }
+            // where kMost lies without the power of two (past the largest float: nothing is marked)
+            auto limit = [&](float f) __attribute__((always_inline)) {
+                const int e = exponent(kMost) - exponent(f);
+                return e > 127 ? 0x7F800000u : (uint32_t)(e + 127) << 23;
+            };
+            if (kt) lim_k = limit(fk);
+            if (vt) lim_v = limit(fv);
             return newk || newv;
         };
         Raw raw;
@@ -429,7 +441,6 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
             }
         }
         fk_now = fk;
-        owed_next = 1.0f;                              // the sums are empty
         f32x16 sc;
         // A tile is staged two ahead, with one barrier a tile.  Map 0's waves pass it before
         // a tile's first product, map 1's between that product and the softmax, so that on

@@ -85,3 +85,54 @@ def test_small_queries_and_large_keys():
     q = (q.float() * 2.0 ** -118).to(torch.bfloat16)
     _, used = _prefill(c, [50, 3, 7], q, lam, _p_step(c))
     log(f"small queries, large keys: {used:.3f} of the bound")
+
+
+def _two(dtype, v_mul, k_mul=lambda t: 1.0, q_mul=1.0, out=False, seed=52):
+    """A short sequence and a long one behind it, which share a workgroup (128 pairs, two
+    workgroups a pair: the first has the short one and the long one's first nine tiles).
+    v_mul, k_mul: factors of the long one's tokens; the short one's values are 1e20 times
+    those of normal rows.  out: the long one's first 64 tokens lie outside the pool."""
+    torch = torch_mod()
+    c = Cache(dtype, 32, 256, 16, [20, 1000], seed=seed)
+    t = np.arange(1000)
+    f = np.concatenate([np.full(20, 1e20), v_mul(t) * np.ones(1000)]).astype(np.float32)[:, None, None]
+    g = np.concatenate([np.ones(20), k_mul(t) * np.ones(1000)]).astype(np.float32)[:, None, None]
+    slots = np.concatenate([c.tables[i, np.arange(n) // 16].astype(np.int64) * 16 + np.arange(n) % 16 for i, n in enumerate(c.lens)])
+    c.pool.append(torch.from_numpy(c.k * g).cuda(), torch.from_numpy(c.v * f).cuda(), torch.from_numpy(slots).cuda())
+    tables = c.tables.copy()
+    if out:
+        tables[1, :4] = -1
+    q, lam, _, _, _, _ = c.rows(5, 1, False, False, False)
+    q[1:] = (q[1:].float() * q_mul).to(torch.bfloat16)
+    return _prefill(c, [1, 4], q, lam, _p_step(c), tables=tables)[1]
+
+
+@pytest.mark.parametrize("dtype", [airkv.BF16, airkv.INT8, airkv.FP8])
+def test_a_sequence_that_begins_with_zeros_behind_a_large_one(dtype):
+    """What a sequence's values are rounded to does not come from the one before it: zeros
+    (or, on 1-byte pages, tokens outside the pool, which are zeros with a scale of 0) say
+    nothing about the power of two."""
+    used = _two(dtype, lambda t: np.where(t < 64, 0.0, 1.0))
+    more = _two(dtype, lambda t: 1.0, out=True)
+    log(f"zeros first dtype={dtype}: {used:.3f}, outside the pool {more:.3f} of the bound")
+
+
+@pytest.mark.parametrize("dtype,size", [(airkv.BF16, 1e-30), (airkv.INT8, 1e-30), (airkv.FP8, 1e-7)])
+def test_zeros_first_then_small_values(dtype, size):
+    used = _two(dtype, lambda t: np.where(t < 64, 0.0, size), seed=53)
+    log(f"zeros, then {size} dtype={dtype}: {used:.3f} of the bound")
+
+
+@pytest.mark.parametrize("dtype,size", [(airkv.INT8, 1e-30), (airkv.FP8, 1e-7)])
+def test_zero_keys_first_then_small_ones(dtype, size):
+    """Queries as large as the keys are small: scores of normal rows."""
+    used = _two(dtype, lambda t: 1.0, lambda t: np.where(t < 64, 0.0, size), 1 / size, seed=54)
+    log(f"zero keys, then {size} dtype={dtype}: {used:.3f} of the bound")
+
+
+@pytest.mark.parametrize("dtype", [airkv.INT8, airkv.FP8])
+def test_zeros_among_small_values(dtype):
+    """Groups of zeros (their scale is 1) between values that are all small."""
+    size = 1e-34 if dtype == airkv.INT8 else 1e-7
+    used = _two(dtype, lambda t: np.where(t % 3 == 1, 0.0, size), seed=57)
+    log(f"zeros among {size} dtype={dtype}: {used:.3f} of the bound")
