@@ -94,6 +94,12 @@ template <int N, int AHEAD, int READS> __device__ __forceinline__ void read_ahea
     __builtin_amdgcn_sched_group_barrier(kMfma, AHEAD, 0);
 }
 
+// Probabilities are held 2^kUp times their size, so that f16 has 11 bits of those down to
+// 2^-25 of the running maximum's, and an absolute step of 2^-35 of it below: of a key among a
+// million that none of them stands out from, too.  kSlack: how far the running maximum may lag
+// (f16 ends at 2^16).
+constexpr float kUp = 11.0f, kSlack = 4.0f;
+
 constexpr int kRows = 128;
 constexpr int kThreads16 = 512;
 
@@ -497,9 +503,9 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
 #pragma unroll
                 for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
                 top = max_x32(top) * ft;
-                // raised only past 2^8 times the present maximum (and on the first tile)
-                if (owed != 1.0f || __ballot(top > m_run + 8.0f) != 0ull) {
-                    const float now = top > m_run + 8.0f ? top : m_run;
+                // raised only past 2^kSlack times the present maximum (and on the first tile)
+                if (owed != 1.0f || __ballot(top > m_run + kSlack) != 0ull) {
+                    const float now = top > m_run + kSlack ? top : m_run;
                     float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - now);
                     l_run *= alpha;
                     alpha *= owed;
@@ -508,7 +514,7 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                     for (int c = 0; c < CT; ++c) acc[c] *= alpha;
                     m_run = now;
                 }
-                const float base = m_run == -INFINITY ? 0.0f : m_run;
+                const float base = m_run == -INFINITY ? 0.0f : m_run - kUp;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], ft, -base));
@@ -651,7 +657,7 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                 }
             if (hf == 0) {
                 a.part_ml[kDiffMl * r] = m_run;
-                a.part_ml[kDiffMl * r + 1] = l;
+                a.part_ml[kDiffMl * r + 1] = l * __builtin_amdgcn_exp2f(-kUp);
                 a.part_ml[kDiffMl * r + 2] = 1.0f / fv;
             }
             if (t0 == 0) {                          // begun here: its last unit's slice ends it

@@ -136,3 +136,33 @@ def test_zeros_among_small_values(dtype):
     size = 1e-34 if dtype == airkv.INT8 else 1e-7
     used = _two(dtype, lambda t: np.where(t % 3 == 1, 0.0, size), seed=57)
     log(f"zeros among {size} dtype={dtype}: {used:.3f} of the bound")
+
+
+@pytest.mark.parametrize("dtype", [airkv.BF16, airkv.INT8, airkv.FP8])
+@pytest.mark.parametrize("bits,n", [(12.0, 5000), (20.0, 131072), (22.7, 131072), (25.5, 131072)])
+def test_many_small_probabilities(dtype, bits, n):
+    """One key that takes nearly all of a row's attention and whose values are 0, and many
+    behind it, each 2^-bits as probable: the result is what those sum to.  A probability
+    is off by 2^-11 of itself or, below f16's normal numbers, 2^-36 of the largest.  256
+    sequences over the same blocks: a workgroup each, which walks all of its keys."""
+    torch = torch_mod()
+    c = Cache(dtype, 32, 2, 16, [n], seed=58)
+    c.k[:] = 0
+    c.k[0] = bits * np.log(2.0) / np.sqrt(32.0)         # against queries of ones
+    c.v[:] = 1 + 0.1 * c.v
+    c.v[0] = 0
+    _refill(c, lambda t: 1.0, lambda t: 1.0)
+    k, v = (sequence(x, c.tables[0], n, 16) for x in pool_values(c.pool))
+    # values (of 1-byte pages) and pieces round to 11 bits; the scores of 1-byte keys err by
+    # 2^-11 of themselves, `bits` at most, and move a probability by twice that
+    p_step = 2.0 ** -11 * (2 if dtype == airkv.BF16 else 3 + 2 * bits)
+    want, bound = attend(np.ones((1, 2, 32)), k, v, np.full((1, 1), 0.25), 32 ** -0.5, [n - 1], p_step=p_step)
+    bound += 2.0 ** -36 * n * 1.25 * np.abs(v).max()
+    many = 256
+    q = torch.ones(many, 2, 32, device="cuda", dtype=torch.bfloat16)
+    tables, lens = (torch.from_numpy(np.repeat(x, many, 0)).cuda() for x in (c.tables, c.lens))
+    out = torch.full((many, 1, 64), float("nan"), device="cuda", dtype=torch.bfloat16)
+    c.pool.paged_diff_prefill(q, torch.full((1,), 0.25, device="cuda"), torch.arange(many + 1, dtype=torch.int32, device="cuda"),
+                              tables, lens, out, max_q_len=1)
+    used = check(out.float().cpu().numpy(), np.repeat(want, many, 0), np.repeat(bound, many, 0), airkv.BF16, "small", p_step)
+    log(f"small probabilities dtype={dtype} 2^-{bits}: {used:.3f} of the bound")
