@@ -10,28 +10,8 @@
 namespace airkv {
 namespace {
 
-typedef diff_f32x4 f32x4;
-
-// A lane's V columns of a piece's row.
-template <int V, bool HALF> __device__ __forceinline__ void load_piece(const void *p, int64_t at, float (&x)[V]) {
-    if constexpr (!HALF) {
-        diff_load<V>((const float *)p + at, x);
-    } else {
-        typedef _Float16 f16xV __attribute__((ext_vector_type(V == 4 ? 4 : V == 2 ? 2 : 1)));
-        const _Float16 *h = (const _Float16 *)p + at;
-        if constexpr (V == 4 || V == 2) {
-            const f16xV w = *reinterpret_cast<const f16xV *>(h);
-#pragma unroll
-            for (int i = 0; i < V; ++i) x[i] = (float)w[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) x[i] = (float)h[i];
-        }
-    }
-}
-
 // Rows of one cut block, one wave: their pieces folded by log-sum-exp, in order.  HALF:
-// pieces of the 16-bit products, four rows at once (mostly of two pieces); the smaller
+// the 16-bit products' blocks, four rows at once (mostly of two pieces); the smaller
 // launches at f32 precision take one (four prompts: 30.4 us in all, 31.8 with four).
 constexpr int merge_rows(bool half) { return half ? 4 : 1; }
 template <int D, bool HALF>
@@ -43,7 +23,7 @@ __global__ __launch_bounds__(256) void diff_prefill_merge_kernel(DiffPrefillArgs
     const int4 d = a.desc[at];
     if (d.w == 0) return;
     // rows past the sequence's last are read as they are (slots are whole) and not written
-    f32x4 ml[N][kBatch][2];
+    float2 ml[N][kBatch][2];
     float po[N][kBatch][2][V];
     auto load = [&](int p0) __attribute__((always_inline)) {
 #pragma unroll
@@ -55,8 +35,8 @@ __global__ __launch_bounds__(256) void diff_prefill_merge_kernel(DiffPrefillArgs
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
                     const int64_t r = (slot * a.rows + row + j) * 2 + m;
-                    ml[j][i][m] = *reinterpret_cast<const f32x4 *>(a.part_ml + kDiffMl * r);
-                    load_piece<V, HALF>(a.part_o, r * (2 * D) + V * lane, po[j][i][m]);
+                    ml[j][i][m] = *reinterpret_cast<const float2 *>(a.part_ml + 2 * r);
+                    diff_load<V>(a.part_o + r * (2 * D) + V * lane, po[j][i][m]);
                 }
             }
     };
@@ -85,13 +65,7 @@ __global__ __launch_bounds__(256) void diff_prefill_merge_kernel(DiffPrefillArgs
             for (int i = 0; i < kBatch; ++i)
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
-                    if (p0 + i >= d.w) continue;
-                    const float l = ml[j][i][m][1];
-                    if constexpr (HALF) {
-#pragma unroll
-                        for (int e = 0; e < V; ++e) po[j][i][m][e] *= ml[j][i][m][2] * l;
-                    }
-                    c[j].fold(m, ml[j][i][m][0], l, po[j][i][m]);
+                    if (p0 + i < d.w) c[j].fold(m, ml[j][i][m].x, ml[j][i][m].y, po[j][i][m]);
                 }
     }
 #pragma unroll
@@ -114,9 +88,9 @@ size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 // A slice for every workgroup that is resident at once, all K/V pairs together.
 struct Plan {
-    int32_t rows, extra, slices, least, elem;      // elem: bytes of a piece's sum
+    int32_t rows, extra, slices, least;
     size_t cells, halves;          // (pair, slice)s, rows' maps in the piece slots
-    size_t bytes(int d) const { return align256(cells * sizeof(int4)) + align256(halves * kDiffMl * 4) + halves * 2 * d * elem; }
+    size_t bytes(int d) const { return align256(cells * sizeof(int4)) + align256(halves * 2 * 4) + halves * 2 * d * 4; }
 };
 
 // half: 16-bit products (diff_prefill_16.hip), else f32 ones
@@ -130,7 +104,6 @@ Plan plan_for(const air_kv_pool &p, bool half) {
     pl.extra = half ? 7 : 2;
     pl.slices = std::max(1, (p.cus + kv_pairs - 1) / kv_pairs);
     pl.least = half ? 16 : 3;
-    pl.elem = half ? 2 : 4;
     pl.cells = (size_t)kv_pairs * pl.slices;
     pl.halves = 2 * pl.cells * pl.rows * 2;
     return pl;
@@ -176,7 +149,7 @@ hipError_t launch_diff_prefill(const air_kv_pool &p, hipStream_t s, const void *
     a.desc = (int4 *)ws;
     ws += align256(plan.cells * sizeof(int4));
     a.part_ml = (float *)ws;
-    ws += align256(plan.halves * kDiffMl * 4);
+    ws += align256(plan.halves * 2 * 4);
     a.part_o = (float *)ws;
     for (int32_t b0 = 0; b0 < batch; b0 += kDiffPrefillBatch) {
         a.batch = std::min(batch - b0, kDiffPrefillBatch);

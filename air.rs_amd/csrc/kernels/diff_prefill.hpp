@@ -8,8 +8,6 @@ namespace airkv {
 
 constexpr int kDiffPrefillBatch = 1024;    // sequences per launch (the host splits larger batches)
 
-constexpr int kDiffMl = 4;                 // floats of a piece's row and map beside its sums
-
 struct DiffPrefillArgs {
     const void *q;                 // [total_q][query heads][head_dim]
     int32_t q_dtype, pairs;        // query pairs
@@ -27,11 +25,10 @@ struct DiffPrefillArgs {
     int32_t rows, extra;           // of a block; the units it counts beside its tiles
     // cut blocks: per (pair, slice) the block it began and did not end, {sequence,
     // block (low, high), pieces}; two piece slots per (pair, slice), 2w for a block
-    // begun before, 2w + 1 for one that goes on: [slot][row][map] of (max, sum, unit),
-    // and of 2 * head_dim sums -- 16-bit products: f16 means, in units of `unit`
+    // begun before, 2w + 1 for one that goes on: [slot][row][map] of (max, sum), and
+    // of 2 * head_dim sums
     int4 *desc;
-    float *part_ml;                // kDiffMl a row and map
-    void *part_o;
+    float *part_ml, *part_o;
 };
 
 // x, the same in every lane of the wave, in scalar registers.

@@ -639,26 +639,19 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
         } else {
             const int64_t slot = 2 * cell + (t0 == 0 ? 1 : 0);
             const int64_t r = (slot * kRows + 32 * rg + r32) * 2 + mp;
-            // the piece's means, under the values' power of two as the values are: they are
-            // rounded to 11 bits as these, and half as long to write and read as f32 sums
-            // (eight chunks 358 -> 350 us)
-            const float inv = l > 0.0f ? owed / l : owed;
-            uint16_t *o = (uint16_t *)a.part_o + r * (2 * D) + 8 * hf;
+            // the piece's sums, without the probabilities' and the values' powers of two (f16 means
+            // in their place would err by 2^-12 of a map, which the difference of two alike does not keep)
+            const float down = __builtin_amdgcn_exp2f(-kUp), unit = back * down;
+            float *o = a.part_o + r * (2 * D) + 4 * hf;
 #pragma unroll
             for (int c = 0; c < CT; ++c)
 #pragma unroll
-                for (int i = 0; i < 16; i += 8) {
-                    u32x2 x[2];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        x[e] = u32x2{pack2<true>(acc[c][i + 4 * e] * inv, acc[c][i + 4 * e + 1] * inv),
-                                     pack2<true>(acc[c][i + 4 * e + 2] * inv, acc[c][i + 4 * e + 3] * inv)};
-                    *reinterpret_cast<u32x4 *>(o + 32 * c + 2 * i) = eight(x[0], x[1]);
-                }
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<f32x4 *>(o + 32 * c + 2 * i) =
+                        f32x4{acc[c][i] * unit, acc[c][i + 1] * unit, acc[c][i + 2] * unit, acc[c][i + 3] * unit};
             if (hf == 0) {
-                a.part_ml[kDiffMl * r] = m_run;
-                a.part_ml[kDiffMl * r + 1] = l * __builtin_amdgcn_exp2f(-kUp);
-                a.part_ml[kDiffMl * r + 2] = 1.0f / fv;
+                a.part_ml[2 * r] = m_run;
+                a.part_ml[2 * r + 1] = l * down;
             }
             if (t0 == 0) {                          // begun here: its last unit's slice ends it
                 const int64_t last = u - t1 + nt - 1;      // of the launch's units

@@ -390,10 +390,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             const int64_t slot = 2 * cell + (t0 == 0 ? 1 : 0);
             const int64_t r = (slot * R + 16 * rg + r16) * 2 + mp;
 #pragma unroll
-            for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4 *>((float *)a.part_o + r * (2 * D) + 16 * c + 4 * q4) = acc[c];
+            for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4 *>(a.part_o + r * (2 * D) + 16 * c + 4 * q4) = acc[c];
             if (q4 == 0) {
-                a.part_ml[kDiffMl * r] = m_run;
-                a.part_ml[kDiffMl * r + 1] = l;
+                a.part_ml[2 * r] = m_run;
+                a.part_ml[2 * r + 1] = l;
             }
             if (t0 == 0) {                          // begun here: its last unit's slice ends it
                 const int64_t last = u - t1 + nt - 1;      // of the launch's units

@@ -166,3 +166,62 @@ def test_many_small_probabilities(dtype, bits, n):
                               tables, lens, out, max_q_len=1)
     used = check(out.float().cpu().numpy(), np.repeat(want, many, 0), np.repeat(bound, many, 0), airkv.BF16, "small", p_step)
     log(f"small probabilities dtype={dtype} 2^-{bits}: {used:.3f} of the bound")
+
+
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+def test_two_maps_that_nearly_cancel(d):
+    """Two maps whose means differ by 2^-12 of themselves, over a block that several
+    workgroups share.  Map 0 sees every key alike, map 1 every second one; values are
+    1 + j 2^-7 and lambda 1: probabilities are 0 or 1, every sum of them and of their
+    products is a number of 24 bits, and what is left to round is the two quotients and
+    their difference, 8 half steps of 2^-24 of values below 2 together, and the output."""
+    torch = torch_mod()
+    n, new, scale = 2000, 8, float(np.float32(1.0) / np.sqrt(np.float32(d)))
+    c = Cache(airkv.BF16, d, 4, 16, [n], seed=59)
+    c.k[:] = 0
+    c.k[1::2, 1::2] = -1000.0                           # map 1's keys at odd tokens
+    c.v[:] = 1 + c.r.integers(0, 4, c.v.shape) * 2.0 ** -7
+    _refill(c, lambda t: 1.0, lambda t: 1.0)
+    q = torch.zeros(new, 8, d, device="cuda", dtype=torch.bfloat16)
+    q[:, 1::2] = 1.0
+    assert 1000.0 * d * scale > 200                     # 2^-200 and less: 0 beside 1
+    out = torch.full((new, 4, 2 * d), float("nan"), device="cuda", dtype=torch.bfloat16)
+    tables, lens = c.device()
+    c.pool.paged_diff_prefill(q, torch.ones(4, device="cuda"), torch.tensor([0, new], dtype=torch.int32, device="cuda"), tables, lens,
+                              out, max_q_len=new)
+    got = out.float().cpu().numpy()
+    v = c.v.astype(np.float64)                          # exact in bf16
+    for r in range(new):
+        m = n - new + r + 1
+        for h in range(4):
+            x = np.concatenate([v[:m, 2 * (h // 2)], v[:m, 2 * (h // 2) + 1]], -1)
+            want = x.mean(0) - x[::2].mean(0)
+            bad = np.abs(got[r, h] - want) > 8 * 2.0 ** -24 * 2 + 2.0 ** -8 * np.abs(want)
+            assert not bad.any(), (r, h, int(bad.sum()), got[r, h][bad][:4], want[bad][:4])
+
+
+@pytest.mark.parametrize("d,group,scale_group", [(128, 4, 32), (64, 1, 32), (96, 3, 32), (32, 8, 8)])
+@pytest.mark.parametrize("dtype", [airkv.BF16, airkv.INT8, airkv.FP8])
+def test_the_error_of_normal_rows(dtype, d, group, scale_group):
+    """The whole result's error: roundings of random sign add up by squares.  The output's
+    is 2^-9 of a value at most; probability, value and key (of 1-byte pages) err by 2^-12
+    of themselves at most, independently from key to key, as the result's own terms are."""
+    torch = torch_mod()
+    n, new = [1500, 700, 40], [300, 700, 40]
+    c = Cache(dtype, d, 4, 16, n, seed=60, scale_group=scale_group)
+    q, lam, _, q64, lam64, _ = c.rows(sum(new), group, False, True, False)
+    cu = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    tables, lens = c.device()
+    out = torch.empty(sum(new), lam64.shape[1], 2 * d, device="cuda", dtype=torch.bfloat16)
+    c.pool.paged_diff_prefill(q, lam, torch.from_numpy(cu).cuda(), tables, lens, out, max_q_len=max(new))
+    got = out.float().cpu().numpy()
+    kv, vv = pool_values(c.pool)
+    scale = float(np.float32(1.0) / np.sqrt(np.float32(d)))
+    limit = ((2.0 ** -9) ** 2 + 3 * (2.0 ** -12) ** 2) ** 0.5
+    for i in range(3):
+        k, v = (sequence(x, c.tables[i], n[i], 16) for x in (kv, vv))
+        s = slice(cu[i], cu[i + 1])
+        want, _ = attend(q64[s], k, v, lam64[s], scale, n[i] - new[i] + np.arange(new[i]))
+        rel = np.linalg.norm(got[s] - want) / np.linalg.norm(want)
+        log(f"normal rows dtype={dtype} d={d} sequence {i}: {rel:.3g} of {limit:.3g}")
+        assert rel <= limit
