@@ -59,6 +59,19 @@ def _dev(t, dtype, what, shape=None):
     return t.data_ptr()
 
 
+def _workspace(nbytes, stream):
+    """Device memory for calls on `stream` (None: the current one), of that stream's own: what
+    it is given out for next there runs after those calls, whenever the tensor is dropped.
+    (The current stream's could be in use again while another stream's kernels still write it.)"""
+    torch = _torch()
+    if stream is None:
+        return torch.empty(max(nbytes, 16), dtype=torch.uint8, device="cuda")
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(stream.cuda_stream)
+    with torch.cuda.stream(stream):
+        return torch.empty(max(nbytes, 16), dtype=torch.uint8, device="cuda")
+
+
 def _launcher(fn, args, name, keep):
     """A zero-argument launcher of fn(*args).  args holds raw device
     addresses, so the launcher also holds `keep`, every tensor (and stream)
@@ -160,10 +173,9 @@ class KvPool:
                                                                ctypes.byref(out)))
         return out.value
 
-    def new_workspace(self, n_q_heads, batch, max_blocks, max_splits=64):
-        torch = _torch()
-        n = self.decode_workspace_size(n_q_heads, batch, max_blocks, max_splits)
-        return torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
+    def new_workspace(self, n_q_heads, batch, max_blocks, max_splits=64, stream=None):
+        """A workspace to keep, for calls on `stream` (None: the current one)."""
+        return _workspace(self.decode_workspace_size(n_q_heads, batch, max_blocks, max_splits), stream)
 
     def _decode_args(self, q, block_tables, seq_lens, out, scale, max_splits, workspace, stream):
         torch = _torch()
@@ -180,7 +192,7 @@ class KvPool:
             raise ValueError("block_tables rows differ from batch")
         lens_at = _dev(seq_lens, torch.int32, "seq_lens", (batch,))
         if workspace is None:
-            workspace = self.new_workspace(n_q, batch, max_blocks, max_splits)
+            workspace = self.new_workspace(n_q, batch, max_blocks, max_splits, stream)
         ws_at = _dev(workspace, workspace.dtype, "workspace")
         head = (self.handle, _stream_ptr(stream), q_at, qdt, n_q)
         tail = (tables_at, lens_at, batch, max_blocks, self._scale if scale is None else scale, max_splits, ws_at,
@@ -222,7 +234,7 @@ class KvPool:
         """Validate once, return a zero-argument launcher (for timing loops:
         no per-call Python checks between launches)."""
         if workspace is None:
-            workspace = self.new_workspace(q.shape[1], q.shape[0], block_tables.shape[1], max_splits)
+            workspace = self.new_workspace(q.shape[1], q.shape[0], block_tables.shape[1], max_splits, stream)
         self.paged_decode(q, block_tables, seq_lens, out, scale, max_splits, workspace, stream)
         head, tail = self._decode_args(q, block_tables, seq_lens, out, scale, max_splits, workspace, stream)
         return _launcher(_lib.load().air_paged_decode, head + tail, "air_paged_decode",
@@ -233,7 +245,7 @@ class KvPool:
         """bind_decode for paged_decode_append.  The launcher appends on every
         call: a timing loop rewrites the same rows with the same values."""
         if workspace is None:
-            workspace = self.new_workspace(q.shape[1], q.shape[0], block_tables.shape[1], max_splits)
+            workspace = self.new_workspace(q.shape[1], q.shape[0], block_tables.shape[1], max_splits, stream)
         self.paged_decode_append(q, k_new, v_new, block_tables, seq_lens, out, scale, max_splits,
                                  workspace, stream)
         head, tail = self._decode_args(q, block_tables, seq_lens, out, scale, max_splits, workspace, stream)
@@ -270,7 +282,7 @@ class KvPool:
         if split and workspace is None and batch:
             n = self.prefill_workspace_size(n_q, batch, max_q_len)
             if n:
-                workspace = torch.empty(n, dtype=torch.uint8, device="cuda")
+                workspace = _workspace(n, stream)
         if not split:
             workspace = None
         ws_at, ws_bytes = (workspace.data_ptr(), workspace.nbytes) if workspace is not None else (None, 0)
@@ -311,10 +323,9 @@ class KvPool:
                    "air_paged_diff_decode_workspace_size")
         return out.value
 
-    def new_diff_workspace(self, n_q_heads, batch, max_blocks, max_splits=256):
-        torch = _torch()
-        n = self.diff_decode_workspace_size(n_q_heads, batch, max_blocks, max_splits)
-        return torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
+    def new_diff_workspace(self, n_q_heads, batch, max_blocks, max_splits=256, stream=None):
+        """A workspace to keep, for calls on `stream` (None: the current one)."""
+        return _workspace(self.diff_decode_workspace_size(n_q_heads, batch, max_blocks, max_splits), stream)
 
     def diff_prefill_workspace_size(self, n_q_heads, batch, max_q_len):
         out = ctypes.c_size_t()
@@ -323,10 +334,9 @@ class KvPool:
                    "air_paged_diff_prefill_workspace_size")
         return out.value
 
-    def new_diff_prefill_workspace(self, n_q_heads, batch, max_q_len):
-        torch = _torch()
-        n = self.diff_prefill_workspace_size(n_q_heads, batch, max_q_len)
-        return torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
+    def new_diff_prefill_workspace(self, n_q_heads, batch, max_q_len, stream=None):
+        """A workspace to keep, for calls on `stream` (None: the current one)."""
+        return _workspace(self.diff_prefill_workspace_size(n_q_heads, batch, max_q_len), stream)
 
     def _diff_args(self, q, lam, out, norm_weight, norm_eps, out_scale):
         """(q and lambda arguments, norm arguments, output arguments) of a differential call."""
@@ -361,7 +371,7 @@ class KvPool:
             raise ValueError("block_tables rows differ from batch")
         lens_at = _dev(seq_lens, torch.int32, "seq_lens", (batch,))
         if workspace is None:
-            workspace = self.new_diff_workspace(n_q, batch, max_blocks, max_splits)
+            workspace = self.new_diff_workspace(n_q, batch, max_blocks, max_splits, stream)
         ws_at = _dev(workspace, workspace.dtype, "workspace")
         return (self.handle, _stream_ptr(stream)) + head + (
             tables_at, lens_at, batch, max_blocks, self._scale if scale is None else scale, max_splits) + norm + (
@@ -401,7 +411,7 @@ class KvPool:
         if max_q_len is None:
             max_q_len = int((cu_q[1:] - cu_q[:-1]).max().item()) if batch else 0
         if workspace is None:
-            workspace = self.new_diff_prefill_workspace(n_q, batch, max_q_len)
+            workspace = self.new_diff_prefill_workspace(n_q, batch, max_q_len, stream)
         ws_at = _dev(workspace, workspace.dtype, "workspace")
         return (self.handle, _stream_ptr(stream)) + head + (
             cu_at, total_q, max_q_len, tables_at, lens_at, batch, max_blocks,
