@@ -354,8 +354,8 @@ class KvPool:
             if norm_weight is not None:
                 raise ValueError("norm_weight needs norm_eps")
             norm = (None, 0.0)
-        elif not norm_eps > 0:
-            raise ValueError("norm_eps must be positive (None: no norm)")
+        elif not ctypes.c_float(norm_eps).value > 0:
+            raise ValueError("norm_eps must be positive in float32 (None: no norm)")
         else:
             norm = (None if norm_weight is None else _dev(norm_weight, torch.float32, "norm_weight", (2 * d,)), norm_eps)
         return (q_at, qdt, n_q, lam_at, per_row), norm + (out_scale,), (out_at, odt)

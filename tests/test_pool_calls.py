@@ -79,3 +79,14 @@ def test_a_calls_own_workspace_is_its_streams(call, name):
     assert call.allocated == [77] and call.launched
     call.calls[name](None)
     assert call.allocated == [77, None]
+
+
+@pytest.mark.parametrize("name", ["paged_diff_decode", "bind_diff_decode", "paged_diff_prefill", "bind_diff_prefill"])
+def test_a_norm_eps_that_is_no_float32_is_refused(call, name):
+    """What float32 holds as 0 would be a call without the norm."""
+    for eps in (1e-50, 0.0, -1e-5, float("nan")):
+        with pytest.raises(ValueError, match="norm_eps"):
+            call.calls[name](None, norm_eps=eps)
+    assert not call.launched
+    call.calls[name](None, norm_eps=1e-40)              # a subnormal float32
+    assert call.launched
