@@ -409,7 +409,7 @@ class KvPool:
         lens_at = _dev(seq_lens, torch.int32, "seq_lens", (batch,))
         cu_at = _dev(cu_q, torch.int32, "cu_q", (batch + 1,))
         if max_q_len is None:
-            max_q_len = int((cu_q[1:] - cu_q[:-1]).max().item()) if batch else 0
+            max_q_len = total_q
         if workspace is None:
             workspace = self.new_diff_prefill_workspace(n_q, batch, max_q_len, stream)
         ws_at = _dev(workspace, workspace.dtype, "workspace")
@@ -422,8 +422,8 @@ class KvPool:
         """Differential attention, causal, of each sequence's newest cu_q[b+1] -
         cu_q[b] tokens over its pages (air_paged_diff_prefill); q [total_q, n_q, d],
         out [total_q, n_q / 2, 2 d], lam float32 [n_q / 2] or [total_q, n_q / 2].
-        max_q_len defaults to the largest q_len (read back from cu_q, which
-        synchronises)."""
+        max_q_len is an upper bound of the q_len values (None: total_q); nothing is
+        read back."""
         args, _ws = self._diff_prefill_args(q, lam, cu_q, block_tables, seq_lens, out, max_q_len, norm_weight,
                                             norm_eps, out_scale, scale, workspace, stream)
         _lib.check(_lib.load().air_paged_diff_prefill(*args), "air_paged_diff_prefill")

@@ -40,3 +40,28 @@ def test_a_call_on_a_busy_stream_keeps_its_workspace():
         same = torch.equal(out, want), torch.equal(plain, want_plain)
         assert all(same) and len(held) == 4
     assert c.pool.error_count() == 0
+
+
+def test_a_captured_prefill_without_max_q_len():
+    """Captured with nothing but the tensors it needs, replayed with other queries."""
+    torch = torch_mod()
+    c = Cache(airkv.BF16, 64, 4, 16, [300, 90], seed=71)
+    q, lam, _, _, _, _ = c.rows(40, 2, False, False, False)
+    tables, lens = c.device()
+    cu = torch.tensor([0, 30, 40], dtype=torch.int32, device="cuda")
+    ws = c.pool.new_diff_prefill_workspace(8, 2, 30)
+    out = torch.zeros(40, 4, 128, device="cuda", dtype=torch.bfloat16)
+    want = torch.zeros_like(out)
+    c.pool.paged_diff_prefill(q, lam, cu, tables, lens, out, workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.pool.paged_diff_prefill(q, lam, cu, tables, lens, out, workspace=ws)
+    for i in range(3):
+        q.copy_(torch.from_numpy(np.random.default_rng(i).standard_normal(tuple(q.shape)).astype(np.float32)))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        c.pool.paged_diff_prefill(q, lam, cu, tables, lens, want, max_q_len=30)
+        torch.cuda.synchronize()
+        assert bool((out == want).all()), i

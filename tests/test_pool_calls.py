@@ -90,3 +90,14 @@ def test_a_norm_eps_that_is_no_float32_is_refused(call, name):
     assert not call.launched
     call.calls[name](None, norm_eps=1e-40)              # a subnormal float32
     assert call.launched
+
+
+@pytest.mark.parametrize("name", ["paged_diff_prefill", "bind_diff_prefill"])
+def test_differential_prefill_reads_nothing_back(call, name, monkeypatch):
+    """Without max_q_len too: no wait for the device, so the call can be captured."""
+    def waits(*a, **k):
+        raise AssertionError("read back")
+    for f in ("item", "cpu", "tolist", "__int__", "__bool__"):
+        monkeypatch.setattr(torch.Tensor, f, waits)
+    call.calls[name](None)
+    assert call.launched and call.launched[-1][1][9] == 3                # the rows there are
