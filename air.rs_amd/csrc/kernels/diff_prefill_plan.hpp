@@ -22,28 +22,38 @@ namespace airkv {
 
 constexpr int kDiffKeys = 32;
 
-// sum of floor((a * i + b) / m) over i = 0 .. n - 1, by the Euclidean descent on
-// (m, a): lattice points under a line, exchanging the axes at each step.
+// The sum of floor((a i + b) / m) over i = 0 .. n - 1, for small a.  What a has of whole m's
+// leaves the floor (nothing else is left of it where the pairs divide rows / 32).  The rest, by
+// Hermite's identity floor(a x) = sum of floor(x + s / a) over s = 0 .. a - 1 with
+// x = (a i + b) / (a m):
+//   floor((a i + b) / m) = sum over s of floor((i + c_s) / m),  c_s = floor((b + s m) / a),
+// and over i each s runs through the numerators from c_s to c_s + n.  The sum of
+// floor(y / m) over y < N, w = floor(N / m), is w N - m w (w + 1) / 2; the c_s lie within m
+// of the first, so that its w serves all of them, plus what N has past m (w + 1).
 AIRKV_DP_HD inline uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
+    if (n == 0) return 0;
+    auto half = [](uint64_t w) { return w & 1 ? (w + 1) / 2 * w : w / 2 * (w + 1); };      // w (w + 1) / 2
     uint64_t sum = 0;
-    while (n) {
-        if (a >= m) {
-            sum += n * (n - 1) / 2 * (a / m);
-            a %= m;
-        }
-        if (b >= m) {
-            sum += n * (b / m);
-            b %= m;
-        }
-        const uint64_t top = a * n + b;
-        if (top < m) break;
-        n = top / m;
-        b = top % m;
-        const uint64_t t = m;
-        m = a;
-        a = t;
+    if (a >= m) {
+        sum = a / m * half(n - 1);
+        a %= m;
     }
-    return sum;
+    if (a == 0) return sum + n * (b / m);
+    const uint64_t step = m / a, step_rest = m - step * a;
+    uint64_t c = b / a, c_rest = b - c * a;
+    const uint64_t w0 = c / m, w1 = (c + n) / m, top0 = w0 * m + m, top1 = w1 * m + m;
+    uint64_t all = 0, past = 0;                        // of the c_s; past the tops
+    for (uint64_t s = 0; s < a; ++s) {
+        all += c;
+        past += (c + n > top1 ? c + n - top1 : 0) - (c > top0 ? c - top0 : 0);
+        c += step;
+        c_rest += step_rest;
+        if (c_rest >= a) {
+            c_rest -= a;
+            ++c;
+        }
+    }
+    return sum + w1 * (all + a * n) - w0 * all - a * m * (half(w1) - half(w0)) + past;
 }
 
 // One sequence: q new tokens behind `prefix` cached ones, g query pairs.
@@ -59,9 +69,11 @@ struct DiffBlocks {
     AIRKV_DP_HD int64_t tiles(int64_t k) const { return (keys(k) + kDiffKeys - 1) / kDiffKeys; }
     // units of block k, and of the blocks before it (k < blocks(): all of them full)
     AIRKV_DP_HD int64_t cost(int64_t k) const { return extra + tiles(k); }
+    // (rows and kDiffKeys are multiples of 32: the tiles of a full block are
+    // floor((rows k + c) / (kDiffKeys g)), and 32 goes out of both)
     AIRKV_DP_HD int64_t before(int64_t k) const {
-        return extra * k + (int64_t)floor_sum((uint64_t)k, (uint64_t)kDiffKeys * g, (uint64_t)rows,
-                                  (uint64_t)(prefix + kDiffKeys) * g + rows - 1);
+        const uint64_t c = (uint64_t)(prefix + kDiffKeys) * g + rows - 1;
+        return extra * k + (int64_t)floor_sum((uint64_t)k, (uint64_t)(kDiffKeys / 32) * g, (uint64_t)rows / 32, c / 32);
     }
     AIRKV_DP_HD int64_t units() const {
         const int64_t n = blocks();
