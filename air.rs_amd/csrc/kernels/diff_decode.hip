@@ -534,9 +534,10 @@ void diff_decode_kernel(DiffDecodeArgs a) {
         }
         float mt = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
         mt = max_x32(max_x16(mt));
-        // raised only past 2^8 times the present maximum (and on the first tile): most tiles skip the rescale
-        if (__ballot(mt > m_run + 8.0f) != 0ull) {
-            const float top = mt > m_run + 8.0f ? mt : m_run;
+        // most tiles have no new maximum and skip the rescale (no slack: probabilities above 1
+        // would overflow on values near the largest f32)
+        if (__ballot(mt > m_run) != 0ull) {
+            const float top = mt > m_run ? mt : m_run;
             const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - top);
             l_run *= alpha;
 #pragma unroll

@@ -641,14 +641,15 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
             const int64_t r = (slot * kRows + 32 * rg + r32) * 2 + mp;
             // the piece's sums, without the probabilities' and the values' powers of two (f16 means
             // in their place would err by 2^-12 of a map, which the difference of two alike does not keep)
-            const float down = __builtin_amdgcn_exp2f(-kUp), unit = back * down;
+            // and under 2^-24, so that sums over a million keys of values near the largest f32 are finite
+            const float down = __builtin_amdgcn_exp2f(-kUp - 24.0f);
             float *o = a.part_o + r * (2 * D) + 4 * hf;
 #pragma unroll
             for (int c = 0; c < CT; ++c)
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
                     *reinterpret_cast<f32x4 *>(o + 32 * c + 2 * i) =
-                        f32x4{acc[c][i] * unit, acc[c][i + 1] * unit, acc[c][i + 2] * unit, acc[c][i + 3] * unit};
+                        f32x4{acc[c][i] * down * back, acc[c][i + 1] * down * back, acc[c][i + 2] * down * back, acc[c][i + 3] * down * back};
             if (hf == 0) {
                 a.part_ml[2 * r] = m_run;
                 a.part_ml[2 * r + 1] = l * down;

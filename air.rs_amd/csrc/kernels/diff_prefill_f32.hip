@@ -297,9 +297,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                         top = fmaxf(top, v);
                     }
                 top = max_x32(max_x16(top));
-                // raised only past 2^8 times the present maximum (and on the first tile)
-                if (__ballot(top > m_run + 8.0f) != 0ull) {
-                    const float now = top > m_run + 8.0f ? top : m_run;
+                // (no slack: probabilities above 1 would overflow on values near the largest f32)
+                if (__ballot(top > m_run) != 0ull) {
+                    const float now = top > m_run ? top : m_run;
                     const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - now);
                     l_run *= alpha;
 #pragma unroll
