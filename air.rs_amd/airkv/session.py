@@ -117,9 +117,12 @@ class PagedSessionCache:
         """Keep the tokens at the ascending positions `keep`, in every layer, as
         tokens 0, 1, ... and release the blocks past them (shared blocks that are
         written are copied first)."""
-        keep = np.ascontiguousarray(keep, np.int64)
+        keep = np.asarray(keep)
         if keep.ndim != 1:
             raise ValueError("keep must be one list of positions")
+        if keep.size and keep.dtype.kind not in "iu":   # a mask, or numbers that would be cut off
+            raise TypeError(f"keep must hold integers, got {keep.dtype}")
+        keep = np.ascontiguousarray(keep, np.int64)
         rc = _lib.load().air_kv_session_compact(self._h, _stream_ptr(stream), keep.ctypes.data_as(ctypes.c_void_p),
                                                 len(keep))
         if rc == _lib.AIR_KV_E_OOM:

@@ -101,3 +101,30 @@ def test_differential_prefill_reads_nothing_back(call, name, monkeypatch):
         monkeypatch.setattr(torch.Tensor, f, waits)
     call.calls[name](None)
     assert call.launched and call.launched[-1][1][9] == 3                # the rows there are
+
+
+def test_a_sessions_compaction_takes_positions_only(monkeypatch):
+    """A mask is no list of positions, and a fraction none of them."""
+    import numpy as np
+    from airkv import session as session_module
+    got = []
+
+    class Lib:
+        @staticmethod
+        def air_kv_session_compact(h, stream, keep, n):
+            got.append(n)
+            return 0
+
+    monkeypatch.setattr(session_module._lib, "load", lambda: Lib)
+    monkeypatch.setattr(session_module, "_stream_ptr", lambda s: 0)
+    s = airkv.PagedSessionCache.__new__(airkv.PagedSessionCache)
+    s._h = None
+    for bad in (np.array([False, True]), [True, False, True], [0.0, 1.5], np.array([0.0])):
+        with pytest.raises(TypeError, match="integers"):
+            s.compact(bad)
+    with pytest.raises(ValueError):
+        s.compact([[0, 1]])
+    assert not got
+    for good in ([], [0, 2], np.arange(3, dtype=np.int32), np.arange(4, dtype=np.uint8), (1, 2)):
+        s.compact(good)
+    assert got == [0, 2, 3, 4, 2]
