@@ -55,13 +55,11 @@ __device__ __forceinline__ uint32_t bf16_pair(float x, float y) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
 }
 
-// Two values rounded to the products' type, x in the low half.
-template <bool F16> __device__ __forceinline__ uint32_t pack2(float x, float y) {
+// Two values rounded to f16, x in the low half.
+__device__ __forceinline__ uint32_t f16_pair(float x, float y) {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
-    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-    if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), f16x2));
-    else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), f16x2));
 }
 
 // Lanes (n, 0) and (n, 1) hold columns 0 .. 3 and 4 .. 7 of a row's eight in x, and of the
@@ -228,7 +226,7 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
             for (int s = 0; s < KS; ++s)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    qf[s][j] = pack2<true>(__uint_as_float(qf[s][j] << 16) * fq, __uint_as_float(qf[s][j] & 0xFFFF0000u) * fq);
+                    qf[s][j] = f16_pair(__uint_as_float(qf[s][j] << 16) * fq, __uint_as_float(qf[s][j] & 0xFFFF0000u) * fq);
         }
         f32x16 acc[CT];
         float m_run = -INFINITY, l_run = 0.0f;
@@ -366,18 +364,18 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                 if constexpr (QUANT) {
                     const float s = r.s[i] * (val ? fv : fk);
                     const f32x4 lo = code_values<DT>(r.w[i][0], s), hi = code_values<DT>(r.w[i][1], s);
-                    x = u32x4{pack2<true>(lo[0], lo[1]), pack2<true>(lo[2], lo[3]), pack2<true>(hi[0], hi[1]), pack2<true>(hi[2], hi[3])};
+                    x = u32x4{f16_pair(lo[0], lo[1]), f16_pair(lo[2], lo[3]), f16_pair(hi[0], hi[1]), f16_pair(hi[2], hi[3])};
                 } else {
                     x = u32x4{r.w[i][0], r.w[i][1], r.w[i][2], r.w[i][3]};
                     if (val) {
                         if (fv == 1.0f) {
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                x[j] = pack2<true>(__uint_as_float(x[j] << 16), __uint_as_float(x[j] & 0xFFFF0000u));
+                                x[j] = f16_pair(__uint_as_float(x[j] << 16), __uint_as_float(x[j] & 0xFFFF0000u));
                         } else {
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                x[j] = pack2<true>(__uint_as_float(x[j] << 16) * fv, __uint_as_float(x[j] & 0xFFFF0000u) * fv);
+                                x[j] = f16_pair(__uint_as_float(x[j] << 16) * fv, __uint_as_float(x[j] & 0xFFFF0000u) * fv);
                         }
                     }
                 }
@@ -524,7 +522,7 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) p[s][j] = pack2<true>(sc[8 * s + 2 * j], sc[8 * s + 2 * j + 1]);
+                    for (int j = 0; j < 4; ++j) p[s][j] = f16_pair(sc[8 * s + 2 * j], sc[8 * s + 2 * j + 1]);
                 // V^T as the A operand: lane (m, h) takes keys 16 s + 8 b + 4 h .. +4 of column m, b = 0, 1.
                 // Within each 16-lane group, lane j of a transposing read receives element j % 4 of the 8
                 // bytes that lanes 4 k + j / 4 address, k = 0 .. 3: lane i points at key i / 4 of the four
