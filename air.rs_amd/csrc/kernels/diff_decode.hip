@@ -25,7 +25,7 @@
 //           dequantized values took 160 and 350 us where these take 125 and 296.
 //
 // Bound by the reads of the pages: 64 sequences of 512 to 4096 tokens (bf16, 8 heads of
-// 128) 569 MB in 102 us, 5.6 TB/s, 32 of 8192 (int8) 605 MB in 118 us, 5.1, 8 of 32K to
+// 128) 569 MB in 102 us, 5.6 TB/s, 32 of 8192 (int8) 605 MB in 120 us, 5.0, 8 of 32K to
 // 128K (fp8) 1.56 GB in 287 us, 5.4; the joining takes 7 to 10 us more.  A lone short
 // sequence takes two dependent kernels of a few memory round trips, 15 us.  What carried
 // it there: 16 bytes a lane of a key row (64 bytes of it at once; with 8 the fp8 case took 431 us

@@ -13,20 +13,21 @@
 // meet in a bank.
 //
 // The second product takes f16 operands: values (exact when they come from bf16 pages
-// and lie in f16's range, else rounded to 11 bits) and probabilities rounded to 11 bits,
-// an error below the bf16 output's own rounding, where bf16 probabilities would add as
+// and lie in f16's normal range, else rounded to 11 bits) and probabilities rounded to 11
+// bits, an error below the bf16 output's own rounding, where bf16 probabilities would add as
 // much again (measured against 64 bits: 1.7e-3 and 2.6e-3 of the result's norm).  The
 // first product takes bf16 operands as they are from bf16 pages, f16 ones (dequantized,
-// 11 bits) from 1-byte pages.  Powers of two keep f16's operands in its range whatever
-// the values: one per tile for keys, a running one for values (raised as the running
-// maximum is), one per row for queries.
+// 11 bits) from 1-byte pages.  Powers of two bring f16's operands into its range: a running
+// one for keys and one for values, by the largest so far, one per row for queries, a constant
+// for probabilities.  What lies far below the largest keeps f16's absolute step, 2^-21 of it
+// (kLeast) at the coarsest.
 //
 // Bound by vector issue and the tile's chain: per tile and SIMD 1540 of 4300 clocks are
 // products, 2000 arithmetic (exponentials, the values' rounding, staging), which overlap
-// in part.  8192 tokens of 16 query pairs of 128 in 1.02 ms: 540 TFLOP/s of 8 d a (query
-// pair, key), 810 of the 12 d that two running maps take; eight chunks of 200 to 512
-// behind up to 6000 tokens 335 us, 470 TFLOP/s; int8 pages, 32 query pairs, 599 us, 454
-// (a tenth more on cards whose clock drops further).
+// in part.  8192 tokens of 16 query pairs of 128 in 1.06 ms: 519 TFLOP/s of 8 d a (query
+// pair, key), 778 of the 12 d that two running maps take; eight chunks of 200 to 512
+// behind up to 6000 tokens 347 us, 454 TFLOP/s; int8 pages, 32 query pairs, 611 us, 445
+// (up to 7% more on cards whose clock drops further).
 #include <hip/hip_runtime.h>
 
 #include "../pool.hpp"

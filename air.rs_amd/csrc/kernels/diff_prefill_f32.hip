@@ -15,9 +15,10 @@
 // buffers where they fit; while a tile is used, the next one's elements are on their
 // way in registers and the one after's table entries too.
 // Bound by the chain of a tile (one workgroup to a CU at head_dim 128): 2048 tokens of 16
-// query pairs of 128 on f32 pages in 364 us, 94 TFLOP/s; four chunks of 500 to 1000 behind
-// up to 4000 bf16 tokens 0.77 ms, 182.  (On f32 operands 535 us and 1.96 ms; four waves of
-// both maps, without tiles ahead, twice that.)
+// query pairs of 128 on f32 pages in 415 us, 83 TFLOP/s (364 on the fastest card met); four
+// chunks of 500 to 1000 behind up to 4000 bf16 tokens 0.69 ms, 176.  (On f32 operands half as
+// long again for the first, more than twice as long for the second; four waves of both maps,
+// without tiles ahead, twice that.)
 #include <hip/hip_runtime.h>
 
 #include "../pool.hpp"

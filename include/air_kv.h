@@ -399,7 +399,9 @@ int air_paged_prefill_workspace_size(const air_kv_pool *pool, int32_t n_q_heads,
  * 0 (no norm, norm_weight NULL) or finite and > 0.  q is [rows][n_q_heads]
  * [head_dim] as q_dtype, out [rows][n_q_heads / 2][2 * head_dim] as out_dtype
  * (AIR_KV_F32 or AIR_KV_BF16), both 16-byte aligned.  head_dim is 32, 64, 96 or
- * 128.  Scores, sums and the norm are held in 32 bits.
+ * 128.  Scores, sums and the norm are held in 32 bits.  Products at f32 precision
+ * are of bf16 parts: what lies below 2^-133 of an f32 page's value (prefill), or
+ * of a 1-byte page's scale times a probability (decode), is cut off.
  *
  * Decode: one new token per sequence (already appended) over its seq_lens[b]
  * cached tokens, with the workspace rules of air_paged_decode and its refusals:
@@ -423,8 +425,12 @@ int air_paged_diff_decode(air_kv_pool *pool, void *stream, const void *q, int32_
  * out-of-pool table entries are read as zero keys and values.  max_q_len is a
  * hint (an upper bound of the q_len values).  Keys and values that are not finite
  * reach only the rows that see them.  bf16 queries with bf16 outputs on BF16, INT8
- * and FP8 pools take 16-bit products (probabilities, and what 1-byte pages hold,
- * rounded to 11 bits); everything else keeps f32 precision.  The workspace (16-byte aligned, of at least
+ * and FP8 pools take 16-bit products: probabilities, values and the keys of 1-byte
+ * pages are rounded to 11 bits (BF16 pages' are exact), and no finer than 2^-36 of
+ * a row's largest probability, 2^-22 of the largest value or key so far among
+ * those its block of rows reads.  Each map errs by that much, also where the two
+ * nearly cancel.  Everything else (f32 queries or f32 outputs on any pool) keeps
+ * f32 precision.  The workspace (16-byte aligned, of at least
  * air_paged_diff_prefill_workspace_size bytes, no initialisation needed) holds
  * the parts of blocks of rows that several workgroups share; calls that share
  * one must be ordered (same stream). */
