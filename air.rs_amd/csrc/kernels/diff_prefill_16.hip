@@ -96,7 +96,7 @@ template <int N, int AHEAD, int READS> __device__ __forceinline__ void read_ahea
 // Probabilities are held 2^kUp times their size, so that f16 has 11 bits of those down to
 // 2^-25 of the running maximum's, and an absolute step of 2^-35 of it below: of a key among a
 // million that none of them stands out from, too.  kSlack: how far the running maximum may lag
-// (f16 ends at 2^16).
+// (f16 ends at 2^16; a score's rounding is a factor of at most 2^(1/2) where it is below 2^22).
 constexpr float kUp = 11.0f, kSlack = 4.0f;
 
 constexpr int kRows = 128;
@@ -230,7 +230,8 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                     qf[s][j] = f16_pair(__uint_as_float(qf[s][j] << 16) * fq, __uint_as_float(qf[s][j] & 0xFFFF0000u) * fq);
         }
         f32x16 acc[CT];
-        float m_run = -INFINITY, l_run = 0.0f;
+        // probabilities are 2^(score - base); a row's scores past `lim` ask for another base
+        float base = -INFINITY, lim = -INFINITY, l_run = 0.0f;
         // what the sums have to be multiplied by to be under the present tile's power of two,
         // and for the next tile's
         float owed = 1.0f, owed_next = 1.0f;
@@ -502,21 +503,30 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
 #pragma unroll
                 for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
                 top = max_x32(top) * ft;
-                // raised only past 2^kSlack times the present maximum (and on the first tile)
-                if (owed != 1.0f || __ballot(top > m_run + kSlack) != 0ull) {
-                    const float now = top > m_run + kSlack ? top : m_run;
-                    float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - now);
+                // another base where a probability would pass 2^(kUp + kSlack), and on the first tile.
+                // Scores past 2^22 are whole numbers or nearly: kUp would be lost in their rounding, and
+                // each is rounded as the largest was, so that its distance from the base is exact.
+                if (__ballot(top > lim) != 0ull) {
+                    const float now = top - base > kUp + kSlack ? top - (__builtin_fabsf(top) < 0x1p22f ? kUp : 0.0f) : base;
+                    float alpha = base == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(base - now);
                     l_run *= alpha;
                     alpha *= owed;
                     owed = 1.0f;
 #pragma unroll
                     for (int c = 0; c < CT; ++c) acc[c] *= alpha;
-                    m_run = now;
+                    base = now;
+                    const bool far = !(__builtin_fabsf(base) < 0x1p22f);
+                    lim = far ? -INFINITY : base + (kUp + kSlack);
+                    if (__ballot(far) != 0ull) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sc[i] *= ft;
+                        ft = 1.0f;
+                    }
                 }
-                const float base = m_run == -INFINITY ? 0.0f : m_run - kUp;
+                const float from = base == -INFINITY ? 0.0f : base;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], ft, -base));
+                    sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], ft, -from));
                     l_run += sc[i];
                 }
                 u32x4 p[2];
@@ -559,8 +569,11 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                 if (t + 3 < tiles) load_tile(t + 3, raw);
             }
             fk_now = fk;
-            owed *= owed_next;
-            owed_next = 1.0f;
+            if (owed_next != 1.0f) {                   // rare; paid with the next change of base, at once
+                owed *= owed_next;
+                owed_next = 1.0f;
+                lim = -INFINITY;
+            }
         }
 
         // lane (n, h): columns 32 c + 8 (i / 4) + 4 h + i % 4 of row n in acc[c][i]
@@ -650,7 +663,7 @@ void diff_prefill_16_kernel(DiffPrefillArgs a) {
                     *reinterpret_cast<f32x4 *>(o + 32 * c + 2 * i) =
                         f32x4{acc[c][i] * down * back, acc[c][i + 1] * down * back, acc[c][i + 2] * down * back, acc[c][i + 3] * down * back};
             if (hf == 0) {
-                a.part_ml[2 * r] = m_run;
+                a.part_ml[2 * r] = base;
                 a.part_ml[2 * r + 1] = l * down;
             }
             if (t0 == 0) {                          // begun here: its last unit's slice ends it

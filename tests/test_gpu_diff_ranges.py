@@ -83,3 +83,57 @@ def test_sums_of_a_long_block_near_the_largest_float(dtype):
     c.pool.paged_diff_prefill(q, lam, torch.tensor([0, 4], dtype=torch.int32, device="cuda"), tables, lens, out, max_q_len=4)
     used = check(out.float().cpu().numpy(), want, bound, airkv.BF16, "prefill", p_step)
     log(f"long sums dtype={dtype}: {used:.3f} of the bound")
+
+
+@pytest.mark.parametrize("dtype", [airkv.F32, airkv.BF16, airkv.INT8, airkv.FP8])
+@pytest.mark.parametrize("f32", [True, False])
+def test_scores_that_f32_rounds_by_whole_numbers(dtype, f32):
+    """Scores of 2^20 to 2^36, whose roundings are a probability's factor of up to 2^12.  The
+    largest of a row lies so far above the others that the row is its values."""
+    torch = torch_mod()
+    d, n, new = 64, [500, 90, 33], [100, 90, 33]
+    odt = airkv.F32 if f32 else airkv.BF16
+    for e in range(10, 20, 2):
+        c = Cache(dtype, d, 2, 16, n, seed=82 + e)
+        _refill(c, lambda t: 2.0 ** e, lambda t: 1.0)
+        kv, vv = pool_values(c.pool)
+        cu = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        q, lam, _, _, lam64, _ = c.rows(int(cu[-1]), 2, f32, True, False)
+        q = (q.float() * 2.0 ** e).to(q.dtype)
+        q64 = q.float().cpu().numpy().astype(np.float64)
+        tables, lens = c.device()
+        out = torch.full((int(cu[-1]), 2, 2 * d), float("nan"), device="cuda", dtype=q.dtype)
+        c.pool.paged_diff_prefill(q, lam, torch.from_numpy(cu).cuda(), tables, lens, out, max_q_len=max(new))
+        got = out.float().cpu().numpy()
+        assert np.isfinite(got).all(), e
+        last = torch.from_numpy(cu[1:].astype(np.int64) - 1).cuda()
+        dec = torch.full((3, 2, 2 * d), float("nan"), device="cuda", dtype=q.dtype)
+        c.pool.paged_diff_decode(q[last].contiguous(), lam[last].contiguous(), tables, lens, dec)
+        dec = dec.float().cpu().numpy()
+        assert np.isfinite(dec).all(), e
+        seen = 0
+        for i in range(3):
+            k, v = (sequence(x, c.tables[i], n[i], 16) for x in (kv, vv))
+            for r in range(new[i]):
+                row, m = cu[i] + r, n[i] - new[i] + r + 1
+                for h in range(2):
+                    want, sure = 0.0, True
+                    for a in range(2):
+                        s = k[a, :m] @ q64[row, 2 * h + a]
+                        top = np.sort(s)[::-1]
+                        # scores in 32 bits, from keys of 1-byte pages in 11: apart by more than they can err
+                        size = (np.abs(k[a, :m]) @ np.abs(q64[row, 2 * h + a])).max()
+                        sure &= m == 1 or (top[0] - top[1]) > size * (2.0 ** -9 if dtype in (airkv.INT8, airkv.FP8) else 2.0 ** -16) + 800
+                        best = int(s.argmax())
+                        want = want + (1.0 if a == 0 else -lam64[row, h]) * np.concatenate([v[0, best], v[1, best]])
+                    if not sure:
+                        continue
+                    seen += 1
+                    # values in 11 bits under the 16-bit products, two maps' errors and the output's
+                    tol = (2.0 ** -10 if not f32 else 2.0 ** -20) * (1 + abs(lam64[row, h])) * np.abs(v).max() + \
+                        (2.0 ** -8 if not f32 else 0.0) * np.abs(want)
+                    assert (np.abs(got[row, h] - want) <= tol).all(), (e, i, r, h)
+                    if r == new[i] - 1:
+                        assert (np.abs(dec[i, h] - want) <= tol).all(), (e, i, h, "decode")
+        assert seen > 200, seen
+    assert c.pool.error_count() == 0
