@@ -24,10 +24,10 @@
 //
 // Bound by vector issue and the tile's chain: per tile and SIMD 1540 of 4300 clocks are
 // products, 2000 arithmetic (exponentials, the values' rounding, staging), which overlap
-// in part.  8192 tokens of 16 query pairs of 128 in 1.06 ms: 519 TFLOP/s of 8 d a (query
-// pair, key), 778 of the 12 d that two running maps take; eight chunks of 200 to 512
-// behind up to 6000 tokens 347 us, 454 TFLOP/s; int8 pages, 32 query pairs, 611 us, 445
-// (up to 7% more on cards whose clock drops further).
+// in part.  8192 tokens of 16 query pairs of 128 in 1.08 ms: 510 TFLOP/s of 8 d a (query
+// pair, key), 765 of the 12 d that two running maps take; eight chunks of 200 to 512
+// behind up to 6000 tokens 361 us, 437 TFLOP/s; int8 pages, 32 query pairs, 621 us, 438
+// (2 to 3% less or more from card to card).
 #include <hip/hip_runtime.h>
 
 #include "../pool.hpp"
