@@ -105,10 +105,10 @@ template <int DT> __device__ __forceinline__ void wide8(const Raw8<DT> &r, float
     }
 }
 
-// How far the running maximum may lag.  Probabilities are held 2^-kSlack times their size:
-// above 1 they would overflow on values near the largest f32 (without a lag
-// 2048 tokens take 423 us and four chunks 718 where these take 415 and 691).
-constexpr float kSlack = 4.0f;
+// A tile's largest score puts the base of the probabilities 2^kLead above itself, so that they
+// stay below 1 (values near the largest f32 do not overflow) and most tiles keep the base
+// (with none 2048 tokens take 423 us and four chunks 718 where these take 415 and 691).
+constexpr float kLead = 4.0f;
 
 template <int D, int DT>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void diff_prefill_f32_kernel(DiffPrefillArgs a) {
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
         const float lam = whole ? a.e.lam[(row0 + tok) * a.e.lam_stride + h] : 0.0f;
         f32x4 acc[CT];
-        float m_run = -INFINITY, l_run = 0.0f;
+        float base = -INFINITY, l_run = 0.0f;          // probabilities are 2^(score - base)
 #pragma unroll
         for (int c = 0; c < CT; ++c) acc[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
@@ -303,21 +303,20 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                         top = fmaxf(top, v);
                     }
                 top = max_x32(max_x16(top));
-                // raised only past 2^kSlack times the present maximum (and on the first tile)
-                if (__ballot(top > m_run + kSlack) != 0ull) {
-                    const float now = top > m_run + kSlack ? top : m_run;
-                    const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - now);
+                if (__ballot(top > base) != 0ull) {
+                    const float now = top > base ? top + kLead : base;
+                    const float alpha = base == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(base - now);
                     l_run *= alpha;
 #pragma unroll
                     for (int c = 0; c < CT; ++c) acc[c] *= alpha;
-                    m_run = now;
+                    base = now;
                 }
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float v = sc[b][i];
-                        const float p = v == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v - (m_run + kSlack));
+                        const float p = v == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v - base);
                         sc[b][i] = p;
                         l_run += p;
                     }
@@ -398,7 +397,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
             for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4 *>(a.part_o + r * (2 * D) + 16 * c + 4 * q4) = acc[c];
             if (q4 == 0) {
-                a.part_ml[2 * r] = m_run;
+                a.part_ml[2 * r] = base;
                 a.part_ml[2 * r + 1] = l;
             }
             if (t0 == 0) {                          // begun here: its last unit's slice ends it
