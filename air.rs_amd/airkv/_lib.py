@@ -27,6 +27,7 @@ AIR_KV_E_STATE = -5
 
 F32, BF16, INT8, FP8 = 0, 1, 2, 3
 LAYOUT_HEAD_MAJOR, LAYOUT_TOKEN_MAJOR = 0, 1
+ROTARY_HALF, ROTARY_PAIRS = 0, 1
 
 
 class AirKvError(RuntimeError):
@@ -118,6 +119,11 @@ SIGNATURES = {
     "air_paged_diff_prefill_workspace_size": (_int, [_P, _i32, _i32, _i32, ctypes.POINTER(_SZ)]),
     "air_paged_diff_prefill": (_int, [_P, _P, _P, _i32, _i32, _P, _i32, _P, _i32, _i32, _P, _P, _i32, _i32,
                                       ctypes.c_float, _P, ctypes.c_float, ctypes.c_float, _P, _SZ, _P, _i32]),
+    "air_rotary_frequencies": (_int, [_i32, ctypes.c_double, _i32, ctypes.c_double, ctypes.c_double, ctypes.c_double,
+                                      ctypes.c_double, _P, ctypes.POINTER(ctypes.c_float)]),
+    "air_kv_append_rotary": (_int, [_P, _P, _P, _i64, _i32, _P, _i64, _P, _i64, _i32, _P, _P, _i32, _P, _i32, _i32,
+                                    ctypes.c_float, _P, _i32]),
+    "air_kv_rotate": (_int, [_P, _P, _P, _i32, _i32, _P, _P, _P, _i32, _P, _i32, _i32]),
     "air_kv_session_create": (_int, [_P, ctypes.POINTER(_P), _i32, ctypes.POINTER(_P)]),
     "air_kv_session_destroy": (_int, [_P]),
     "air_kv_session_fork": (_int, [_P, ctypes.POINTER(_P)]),

@@ -12,7 +12,7 @@ import ctypes
 import numpy as np
 
 from . import _lib
-from ._lib import BF16, F32, FP8, INT8, LAYOUT_HEAD_MAJOR, PoolDesc
+from ._lib import BF16, F32, FP8, INT8, LAYOUT_HEAD_MAJOR, ROTARY_HALF, ROTARY_PAIRS, PoolDesc
 
 ELEM_BYTES = {F32: 4, BF16: 2, INT8: 1, FP8: 1}
 PAGE_NP_DTYPE = {F32: np.float32, BF16: np.uint16, INT8: np.int8, FP8: np.uint8}
@@ -57,6 +57,23 @@ def _dev(t, dtype, what, shape=None):
     if shape is not None and t.shape != shape:
         raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {shape}")
     return t.data_ptr()
+
+
+def _dev_rows(t, dtype, what, shape):
+    """(address, row stride) of t, a device tensor [tokens, heads, head_dim] whose rows are dense
+    but may lie apart (a slice of a projection's output)."""
+    torch = _torch()
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{what} must be a CUDA/HIP torch tensor")
+    if t.dtype is not dtype:
+        raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {shape}")
+    n, heads, d = shape
+    row, head, one = t.stride()
+    if one != 1 or (heads > 1 and head != d):
+        raise ValueError(f"{what} must have dense rows")
+    return t.data_ptr(), row if n > 1 else heads * d
 
 
 def _workspace(nbytes, stream):
@@ -460,6 +477,75 @@ class KvPool:
                 block_tables.shape[0], block_tables.shape[1], ctypes.c_void_p(out_k.data_ptr()),
                 ctypes.c_void_p(out_v.data_ptr()), out_dtype, layout)
         return _launcher(fn, args, "air_kv_gather", (block_tables, seq_lens, out_offsets, out_k, out_v, stream))
+
+    # -- rotary positions ---------------------------------------------------------
+
+    def _rotary_args(self, inv_freq, interleaved):
+        return (_dev(inv_freq, _torch().float32, "inv_freq", (inv_freq.numel(),)), 2 * inv_freq.numel(),
+                ROTARY_PAIRS if interleaved else ROTARY_HALF)
+
+    def _append_rotary_args(self, q, k, v, slot_mapping, positions, inv_freq, q_out, interleaved, magnitude, stream):
+        torch = _torch()
+        n, it = k.shape[0], k.dtype
+        if it is not torch.float32 and it is not torch.bfloat16:
+            raise TypeError("q, k and v must be float32 or bfloat16")
+        kv = (n, self.n_kv_heads, self.head_dim)
+        kp, ks = _dev_rows(k, it, "k", kv)
+        vp, vs = _dev_rows(v, it, "v", kv)
+        sp = _dev(slot_mapping, torch.int64, "slot_mapping", (n,))
+        pp = _dev(positions, torch.int32, "positions", (n,))
+        if q is None:
+            if q_out is not None:
+                raise ValueError("q_out without q")
+            qp, qs, heads, op, odt = None, 0, 0, None, F32
+        else:
+            heads = q.shape[1]
+            qp, qs = _dev_rows(q, it, "q", (n, heads, self.head_dim))
+            if q_out is None:
+                q_out = torch.empty(n, heads, self.head_dim, dtype=it, device=q.device)
+            _, odt = self._act_dtypes(it, q_out.dtype)
+            op = _dev(q_out, q_out.dtype, "q_out", (n, heads, self.head_dim))
+        args = (self.handle, _stream_ptr(stream), qp, qs, heads, kp, ks, vp, vs, F32 if it is torch.float32 else BF16, sp, pp, n,
+                *self._rotary_args(inv_freq, interleaved), magnitude, op, odt)
+        return args, q_out
+
+    def append_rotary(self, q, k, v, slot_mapping, positions, inv_freq, q_out=None, interleaved=False, magnitude=1.0,
+                      stream=None):
+        """Append with rotary positions (air_kv_append_rotary): queries [n, n_q_heads, head_dim] and keys [n,
+        n_kv_heads, head_dim] turn by their tokens' positions (int32 [n]), keys and values go to their slots as
+        append writes them.  q, k, v are float32 or bfloat16, each token's rows dense (slices of one projection
+        will do); inv_freq float32 [rot_dim / 2] on the device, as rotary.frequencies gives them.  Returns q_out
+        (default: a new tensor of q's type, on the current stream; it may be q itself).  q may be None."""
+        if q is not None and q_out is None and stream is not None:
+            raise ValueError("a call on another stream needs q_out")
+        args, q_out = self._append_rotary_args(q, k, v, slot_mapping, positions, inv_freq, q_out, interleaved, magnitude, stream)
+        _lib.check(_lib.load().air_kv_append_rotary(*args), "air_kv_append_rotary")
+        return q_out
+
+    def bind_append_rotary(self, q, k, v, slot_mapping, positions, inv_freq, q_out, interleaved=False, magnitude=1.0,
+                           stream=None):
+        """Validate once, return a zero-argument launcher of append_rotary."""
+        if q is not None and (q_out is None or q_out.data_ptr() == q.data_ptr()):
+            raise ValueError("a bound append needs a q_out of its own")
+        self.append_rotary(q, k, v, slot_mapping, positions, inv_freq, q_out, interleaved, magnitude, stream)
+        args, _ = self._append_rotary_args(q, k, v, slot_mapping, positions, inv_freq, q_out, interleaved, magnitude, stream)
+        return _launcher(_lib.load().air_kv_append_rotary, args, "air_kv_append_rotary",
+                         (q, k, v, slot_mapping, positions, inv_freq, q_out, stream))
+
+    def rotate(self, block_tables, from_pos, cu, inv_freq, to_pos=None, interleaved=False, stream=None):
+        """Turn cached keys to other positions in their pages (air_kv_rotate): token i of sequence b, turned for
+        position from_pos[cu[b] + i], leaves turned for to_pos[cu[b] + i] (default: i, its place).  After
+        compact(tables, lens, keep, cu_keep): rotate(tables, keep, cu_keep, inv_freq).  The blocks written belong
+        to that sequence alone."""
+        torch = _torch()
+        tables_at = _dev(block_tables, torch.int32, "block_tables")
+        batch, max_blocks = block_tables.shape
+        total = from_pos.shape[0]
+        from_at = _dev(from_pos, torch.int32, "from_pos", (total,))
+        to_at = None if to_pos is None else _dev(to_pos, torch.int32, "to_pos", (total,))
+        cu_at = _dev(cu, torch.int32, "cu", (batch + 1,))
+        _lib.check(_lib.load().air_kv_rotate(self.handle, _stream_ptr(stream), tables_at, batch, max_blocks, from_at, to_at,
+                                             cu_at, total, *self._rotary_args(inv_freq, interleaved)), "air_kv_rotate")
 
     def copy_blocks(self, src, dst, stream=None):
         torch = _torch()

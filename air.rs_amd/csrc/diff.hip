@@ -6,36 +6,17 @@
 #include "host/status.hpp"
 #include "kernels/diff_common.hpp"
 #include "kernels/diff_prefill.hpp"
+#include "on_device.hpp"
 #include "pool.hpp"
 
 using airkv::fail;
+using airkv::OnDevice;
 
 namespace {
 
 int hip_fail(hipError_t e, const char *what) {
     return fail(AIR_KV_E_HIP, "%s: %s", what, hipGetErrorString(e));
 }
-
-// The pool's device is the current one while this lives.
-class OnDevice {
-public:
-    explicit OnDevice(int device) {
-        status_ = hipGetDevice(&before_);
-        if (status_ == hipSuccess && before_ != device) {
-            status_ = hipSetDevice(device);
-            changed_ = status_ == hipSuccess;
-        }
-    }
-    ~OnDevice() {
-        if (changed_) (void)hipSetDevice(before_);
-    }
-    hipError_t status() const { return status_; }
-
-private:
-    int before_ = 0;
-    bool changed_ = false;
-    hipError_t status_;
-};
 
 // The pool and the heads of a differential call.
 int check_shape(const air_kv_pool *p, int32_t n_q_heads) {

@@ -65,6 +65,14 @@ hipError_t launch_copy_blocks(const air_kv_pool &pool, hipStream_t s, const int3
 hipError_t launch_compact(const air_kv_pool &pool, hipStream_t s, const int32_t *tables, const int32_t *lens,
                           int32_t batch, int32_t max_blocks, const int32_t *keep, const int32_t *cu_keep,
                           int32_t total_keep);
+// (rotary positions: kernels/kv_rotary.hip)
+hipError_t launch_append_rotary(const air_kv_pool &pool, hipStream_t s, const void *q, int64_t q_stride, int32_t n_q_heads,
+                                const void *k, int64_t k_stride, const void *v, int64_t v_stride, int32_t in_dtype,
+                                const int64_t *slots, const int32_t *positions, int32_t n_tokens, const float *inv_freq,
+                                int32_t rot_dim, int32_t layout, float magnitude, void *q_out, int32_t q_out_dtype);
+hipError_t launch_rotate(const air_kv_pool &pool, hipStream_t s, const int32_t *tables, int32_t batch, int32_t max_blocks,
+                         const int32_t *from, const int32_t *to, const int32_t *cu, int32_t total, const float *inv_freq,
+                         int32_t rot_dim, int32_t layout);
 hipError_t launch_stage_blocks(const air_kv_pool &pool, hipStream_t s, const int32_t *ids, int32_t n,
                                void *staging, bool to_staging);
 size_t wire_block_bytes(const air_kv_pool &pool);

@@ -15,7 +15,7 @@ HEADER = os.path.join(ROOT, "include", "air_kv.h")
 OUT = os.path.join(HERE, "airkv-sys", "src", "lib.rs")
 
 SCALARS = {"int": "c_int", "int32_t": "i32", "int64_t": "i64", "uint32_t": "u32", "uint16_t": "u16",
-           "uint64_t": "u64", "uint8_t": "u8", "int8_t": "i8", "size_t": "usize", "float": "f32",
+           "uint64_t": "u64", "uint8_t": "u8", "int8_t": "i8", "size_t": "usize", "float": "f32", "double": "f64",
            "void": "c_void", "char": "c_char"}
 
 

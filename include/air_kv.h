@@ -445,6 +445,78 @@ int air_paged_diff_prefill(air_kv_pool *pool, void *stream, const void *q, int32
                            int32_t out_dtype);
 
 /* ------------------------------------------------------------------------ */
+/* Rotary positions                                                          */
+/* ------------------------------------------------------------------------ */
+
+/* No counterpart among the reference's cache interfaces (its models rotate queries
+ * and keys before they append).  The first rot_dim elements of a head (a multiple
+ * of 8, at most head_dim) are rot_dim / 2 pairs (x, y); at position p, pair i turns
+ * by p * inv_freq[i]:
+ *   (x, y) -> (x c - y s, x s + y c),  c, s = magnitude * cos, sin of the angle
+ * The angle is held in 64 bits, c and s are rounded to f32 once, and so is each
+ * product and sum.  inv_freq is f32 [rot_dim / 2] on the device. */
+#define AIR_ROTARY_HALF 0  /* pair i is elements i and i + rot_dim / 2 */
+#define AIR_ROTARY_PAIRS 1 /* pair i is elements 2i and 2i + 1 */
+
+/* Frequencies for a model's base, as trained or scaled for contexts longer than it
+ * was trained on, into host memory (f32 [rot_dim / 2]), and the magnitude to use
+ * with them.  With f_i = base^(-2i / rot_dim), w_i = 2 pi / f_i, L = trained_len:
+ *   PLAIN   f_i
+ *   LINEAR  f_i / factor
+ *   BASE    those of the base  base * factor^(rot_dim / (rot_dim - 2))  (rot_dim > 2)
+ *   BANDS   f_i where w_i < L / high, f_i / factor where w_i > L / low, between them
+ *           (1 - t) f_i / factor + t f_i,  t = (L / w_i - low) / (high - low)
+ *   RAMP    (1 - t) f_i + t f_i / factor,  t = (i - a) / (b - a) clamped to [0, 1],
+ *           a = floor(turns(high)), b = ceil(turns(low)) clamped to [0, rot_dim - 1]
+ *           (b = a + 0.001 where they meet), turns(n) = rot_dim ln(L / (2 pi n)) /
+ *           (2 ln base): pairs that turn more than high times over L keep their
+ *           frequency; magnitude 0.1 ln(factor) + 1
+ * factor >= 1; BANDS and RAMP need trained_len > 0 and 0 < low < high. */
+#define AIR_ROTARY_PLAIN 0
+#define AIR_ROTARY_LINEAR 1
+#define AIR_ROTARY_BASE 2
+#define AIR_ROTARY_BANDS 3
+#define AIR_ROTARY_RAMP 4
+int air_rotary_frequencies(int32_t rot_dim, double base, int32_t scaling, double factor, double trained_len,
+                           double low, double high, float *inv_freq, float *magnitude);
+
+/* A step's rows on their way to attention: queries and keys of token t turn by
+ * positions[t] (int32, device; any value), and keys and values go to slot
+ * slot_mapping[t] exactly as air_kv_append writes such f32 rows (rounded, or
+ * quantized with a scale per scale_group elements).  Rows of q are
+ * [n_q_heads][head_dim], of k and v [n_kv_heads][head_dim], as in_dtype
+ * (AIR_KV_F32 or AIR_KV_BF16), from one token to the next q_stride, k_stride and
+ * v_stride elements apart (slices of one projection's output, say); pointers and
+ * strides are multiples of 16 bytes.  q_out is [n_tokens][n_q_heads][head_dim] as
+ * q_out_dtype, 16-byte aligned; it may be q itself where that is dense and of that
+ * type, and overlaps no input else.  n_q_heads may be 0 (q and q_out unused).
+ * Slots below 0 are skipped, slots beyond the pool skipped and counted
+ * (air_kv_pool_error_count); their queries are written all the same.  No slot may
+ * be listed twice. */
+int air_kv_append_rotary(air_kv_pool *pool, void *stream, const void *q, int64_t q_stride, int32_t n_q_heads,
+                         const void *k, int64_t k_stride, const void *v, int64_t v_stride, int32_t in_dtype,
+                         const int64_t *slot_mapping, const int32_t *positions, int32_t n_tokens,
+                         const float *inv_freq, int32_t rot_dim, int32_t layout, float magnitude, void *q_out,
+                         int32_t q_out_dtype);
+
+/* Cached keys to other positions, in their pages: what air_kv_compact leaves to do
+ * where keys were appended with rotary positions.  The tokens 0, 1, ... of sequence
+ * b, n of them for its n entries from[cu[b] .. cu[b + 1]) (int32, device), hold keys
+ * turned for positions `from`, and leave turned for `to` (laid out alike; NULL: their
+ * place in the sequence).  After air_kv_compact(..., keep, cu_keep, ...) that is
+ * air_kv_rotate(..., keep, NULL, cu_keep, ...).  A key is read (1-byte pages:
+ * dequantized), turned by to - from, and stored again (1-byte pages: the scale groups
+ * that hold a turned element are quantized anew); tokens with to == from keep their
+ * bytes, and values are not touched.  cu is int32 [batch + 1] (device) over total
+ * entries; sequences whose range does not lie in [0, total] are left alone and
+ * counted; tokens behind their table or in blocks outside the pool are skipped and
+ * counted.  No other sequence may hold a block that is written (copy-on-write
+ * first), nor may one sequence be listed twice. */
+int air_kv_rotate(air_kv_pool *pool, void *stream, const int32_t *block_tables, int32_t batch, int32_t max_blocks,
+                  const int32_t *from, const int32_t *to, const int32_t *cu, int32_t total, const float *inv_freq,
+                  int32_t rot_dim, int32_t layout);
+
+/* ------------------------------------------------------------------------ */
 /* SessionKvCache over pages                                                 */
 /* ------------------------------------------------------------------------ */
 
