@@ -119,6 +119,9 @@ SIGNATURES = {
     "air_paged_diff_prefill_workspace_size": (_int, [_P, _i32, _i32, _i32, ctypes.POINTER(_SZ)]),
     "air_paged_diff_prefill": (_int, [_P, _P, _P, _i32, _i32, _P, _i32, _P, _i32, _i32, _P, _P, _i32, _i32,
                                       ctypes.c_float, _P, ctypes.c_float, ctypes.c_float, _P, _SZ, _P, _i32]),
+    "air_paged_cross_workspace_size": (_int, [_P, _i32, _i32, _i32, ctypes.POINTER(_SZ)]),
+    "air_paged_cross": (_int, [_P, _P, _P, _i32, _i32, _P, _i32, _i32, _P, _P, _i32, _i32, ctypes.c_float, _P, _SZ,
+                               _P, _i32]),
     "air_rotary_frequencies": (_int, [_i32, ctypes.c_double, _i32, ctypes.c_double, ctypes.c_double, ctypes.c_double,
                                       ctypes.c_double, _P, ctypes.POINTER(ctypes.c_float)]),
     "air_kv_append_rotary": (_int, [_P, _P, _P, _i64, _i32, _P, _i64, _P, _i64, _i32, _P, _P, _i32, _P, _i32, _i32,

@@ -478,6 +478,53 @@ class KvPool:
                 ctypes.c_void_p(out_v.data_ptr()), out_dtype, layout)
         return _launcher(fn, args, "air_kv_gather", (block_tables, seq_lens, out_offsets, out_k, out_v, stream))
 
+    # -- cross attention ----------------------------------------------------------
+
+    def cross_workspace_size(self, n_q_heads, batch, max_q_len):
+        out = ctypes.c_size_t()
+        _lib.check(_lib.load().air_paged_cross_workspace_size(self.handle, n_q_heads, batch, max_q_len, ctypes.byref(out)),
+                   "air_paged_cross_workspace_size")
+        return out.value
+
+    def new_cross_workspace(self, n_q_heads, batch, max_q_len, stream=None):
+        """A workspace to keep, for calls on `stream` (None: the current one)."""
+        return _workspace(self.cross_workspace_size(n_q_heads, batch, max_q_len), stream)
+
+    def _cross_args(self, q, cu_q, block_tables, seq_lens, out, max_q_len, scale, workspace, stream):
+        torch = _torch()
+        total_q, n_q, d = shape = q.shape
+        if d != self.head_dim:
+            raise ValueError("q head_dim differs from the pool")
+        qt, ot = q.dtype, out.dtype
+        qdt, odt = self._act_dtypes(qt, ot)
+        q_at = _dev(q, qt, "q")
+        out_at = _dev(out, ot, "out", shape)
+        tables_at = _dev(block_tables, torch.int32, "block_tables")
+        batch, max_blocks = block_tables.shape[:2]
+        lens_at = _dev(seq_lens, torch.int32, "seq_lens", (batch,))
+        cu_at = _dev(cu_q, torch.int32, "cu_q", (batch + 1,))
+        most = 0 if max_q_len is None else max_q_len
+        if workspace is None:
+            workspace = self.new_cross_workspace(n_q, batch, most, stream)
+        ws_at = _dev(workspace, workspace.dtype, "workspace")
+        return (self.handle, _stream_ptr(stream), q_at, qdt, n_q, cu_at, total_q, most, tables_at, lens_at, batch, max_blocks,
+                self._scale if scale is None else scale, ws_at, workspace.nbytes, out_at, odt), workspace
+
+    def paged_cross(self, q, cu_q, block_tables, seq_lens, out, max_q_len=None, scale=None, workspace=None, stream=None):
+        """Cross attention (air_paged_cross): each sequence's cu_q[b+1] - cu_q[b] rows of q [total_q][n_q][d] see
+        all of its seq_lens[b] cached tokens.  max_q_len, the most rows of a sequence, is a hint (nothing is read
+        back without it)."""
+        args, _ws = self._cross_args(q, cu_q, block_tables, seq_lens, out, max_q_len, scale, workspace, stream)
+        _lib.check(_lib.load().air_paged_cross(*args), "air_paged_cross")
+        return out
+
+    def bind_cross(self, q, cu_q, block_tables, seq_lens, out, max_q_len=None, scale=None, workspace=None, stream=None):
+        """Validate once, return a zero-argument launcher of paged_cross."""
+        args, ws = self._cross_args(q, cu_q, block_tables, seq_lens, out, max_q_len, scale, workspace, stream)
+        fn = _lib.load().air_paged_cross
+        _lib.check(fn(*args), "air_paged_cross")
+        return _launcher(fn, args, "air_paged_cross", (q, cu_q, block_tables, seq_lens, out, ws, stream))
+
     # -- rotary positions ---------------------------------------------------------
 
     def _rotary_args(self, inv_freq, interleaved):

@@ -1,0 +1,561 @@
+// The kernel of cross attention over pages (formulas and work division: paged_cross.hpp), for
+// paged_cross_16.hip and paged_cross_f32.hip.
+//
+// A wave holds 32 rows and walks keys 32 at a time, once, with a running base and sum:
+//   S   = K . Q^T      v_mfma_f32_32x32x16_bf16, lane (n, h) holds 16 of the 32 keys of row n
+//   O^T += V^T . P^T   the same instruction; its contraction takes the keys in the order in
+//                      which the lanes hold P, so P never moves
+// Operands are bf16 parts: KP of keys and values, QP of queries and probabilities (1: rounded to
+// bf16, 3: all 24 bits of an f32), of which products with i + j < 3 are formed.  Keys and
+// values are staged in LDS as rows, 16 (keys) and 64 (values) bytes apart modulo 256, so that
+// neither the rows' reads nor the values' transposing reads meet in a bank; a tile is loaded
+// two ahead into registers and staged one ahead where two buffers fit.
+//
+// WK waves share 32 rows and take a tile's keys in turn (few rows), or each wave has rows of its
+// own (WK = 1).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "codecs.hpp"
+#include "paged_cross.hpp"
+
+namespace airkv {
+
+typedef float cross_f32x16 __attribute__((ext_vector_type(16)));
+typedef float cross_f32x4 __attribute__((ext_vector_type(4)));
+typedef float cross_f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 cross_bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 cross_bf16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t cross_u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t cross_u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kCrossLds = 149 * 1024;              // of a CU's 160 KB, for the tiles
+constexpr int kCrossBuffer = 0x00020000;           // a raw buffer's last word
+constexpr int kCrossNowhere = 0x40000000;          // an offset outside of every buffer: reads zeros
+
+// Rows of keys and of values in LDS, bytes apart.
+constexpr int cross_k_stride(int d) { return 2 * d + 16; }
+constexpr int cross_v_stride(int d) { return 2 * d + (2 * d / 64 % 2 ? 0 : 64); }
+constexpr int cross_tile_bytes(int d, int parts, int keys) { return keys * parts * (cross_k_stride(d) + cross_v_stride(d)); }
+// Waves of a workgroup: queries in three parts and their sums leave room for one wave a SIMD.
+constexpr int cross_waves(int d, int qp) { return qp == 3 && d >= 96 ? 4 : 8; }
+// Waves that share rows: as many as have room for 32 keys each.
+constexpr int cross_wk(int d, int kp, int qp, bool few) {
+    int wk = few ? cross_waves(d, qp) : 1;
+    while (wk > 1 && cross_tile_bytes(d, kp, 32 * wk) > kCrossLds) wk /= 2;
+    return wk;
+}
+// Keys of a tile that one wave takes, in 32s.
+constexpr int cross_sub(int d, int kp, int wk) { return wk == 1 && cross_tile_bytes(d, kp, 64) <= kCrossLds ? 2 : 1; }
+
+__device__ __forceinline__ cross_f32x16 cross_mfma(cross_u32x4 a, cross_u32x4 b, cross_f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(cross_bf16x8, a), __builtin_bit_cast(cross_bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t cross_bf16_pair(float x, float y) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((cross_f32x2{x, y}), cross_bf16x2));
+}
+// x, y as bf16 parts whose sum they are, 8 bits each, cut off rather than rounded (the largest
+// float stays finite).
+__device__ __forceinline__ void cross_split(float x, float y, uint32_t (&p)[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        p[i] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+        x -= __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+        y -= __uint_as_float(__float_as_uint(y) & 0xFFFF0000u);
+    }
+}
+template <int P> __device__ __forceinline__ void cross_parts(float x, float y, uint32_t (&p)[P]) {
+    if constexpr (P == 3) cross_split(x, y, p);
+    else p[0] = cross_bf16_pair(x, y);
+}
+// The values of the four 1-byte codes in w times their scale.
+__device__ __forceinline__ cross_f32x4 cross_codes(bool fp8, uint32_t w, float s) {
+    if (fp8) {
+        const cross_f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+        return cross_f32x4{lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
+    }
+    return cross_f32x4{(float)(int8_t)w * s, (float)(int8_t)(w >> 8) * s, (float)(int8_t)(w >> 16) * s, (float)(int8_t)(w >> 24) * s};
+}
+// Over lanes l and l ^ 32.
+__device__ __forceinline__ float cross_max32(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float cross_sum32(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ int64_t cross_uniform(int64_t x) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+// Four outputs of a row from element `at` on.
+__device__ __forceinline__ void cross_store4(const CrossArgs &a, int64_t at, cross_f32x4 x) {
+    if (a.out_dtype == AIR_KV_F32) *reinterpret_cast<cross_f32x4 *>((float *)a.out + at) = x;
+    else *reinterpret_cast<cross_u32x2 *>((uint16_t *)a.out + at) = cross_u32x2{cross_bf16_pair(x[0], x[1]), cross_bf16_pair(x[2], x[3])};
+}
+
+// WIDE: f32 or 1-byte pages (a.dtype says which), else bf16 ones.
+template <int D, bool WIDE, int QP, bool FEW>
+struct CrossShape {
+    static constexpr int KP = WIDE && QP == 3 ? 3 : 1;
+    static constexpr int WAVES = cross_waves(D, QP), WK = cross_wk(D, KP, QP, FEW), SUB = cross_sub(D, KP, WK);
+    static constexpr int ROWS = 32 * (WAVES / WK), TK = 32 * WK * SUB;
+    static constexpr int TILE = cross_tile_bytes(D, KP, TK), NB = 2 * TILE <= kCrossLds ? 2 : 1;
+};
+
+template <int D, bool WIDE, int QP, bool FEW>
+__global__ __launch_bounds__((CrossShape<D, WIDE, QP, FEW>::WAVES * 64))
+__attribute__((amdgpu_waves_per_eu(CrossShape<D, WIDE, QP, FEW>::WAVES / 4, CrossShape<D, WIDE, QP, FEW>::WAVES / 4)))
+void paged_cross_kernel(CrossArgs a) {
+    typedef CrossShape<D, WIDE, QP, FEW> S;
+    constexpr int KP = S::KP, WAVES = S::WAVES, WK = S::WK, SUB = S::SUB, ROWS = S::ROWS, TK = S::TK, NB = S::NB, THREADS = 64 * WAVES;
+    constexpr int KST = cross_k_stride(D), VST = cross_v_stride(D);
+    constexpr int KPLANE = TK * KST, VPLANE = TK * VST, VAT = KP * KPLANE;    // a part's rows; where values begin
+    constexpr int KS = D / 16, CT = D / 32;            // steps of the first product, 32-column tiles of the second
+    // Staging: a wave's pass covers WR rows of one 16-key half of the keys or the values, LPR
+    // lanes a row (a power of two: some idle where D / 8 is none), 8 elements a lane.
+    constexpr int LPR = D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32, WR = 64 / LPR, NP = 2 * TK / (WAVES * WR);
+    static_assert(NP >= 1 && 2 * TK % (WAVES * WR) == 0 && TK % WR == 0, "whole passes");
+    constexpr int JOIN = WAVES * 64 * 16 * 4;          // bytes of a column tile of every wave's sums, at a block's end
+    constexpr int MEM = NB * S::TILE > JOIN || WK == 1 ? NB * S::TILE : JOIN;
+    constexpr int CR = MEM / JOIN < CT ? MEM / JOIN : CT;      // column tiles joined at once (WK > 1)
+    __shared__ int64_t s_pre[kCrossBatch + 1];
+    __shared__ int64_t s_sum[WAVES];
+    __shared__ int32_t s_ok[NB][TK / 16];              // whether the tile's 16-key halves are in the pool
+    __shared__ float2 s_ml[WAVES][32];
+    __shared__ __align__(16) uint8_t s_mem[MEM];
+
+    const int tid = threadIdx.x, lane = tid & 63, hf = lane >> 5, r32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rg = wave / WK, wk = wave % WK;          // 32 rows; which keys of a tile
+    // workgroups of one K/V head take every heads-th place: with eight heads, one XCD's (its L2
+    // then sees one head's keys and values)
+    const int head = blockIdx.x % a.heads, w = blockIdx.x / a.heads;
+    const int64_t cell = (int64_t)head * a.slices + w;
+
+    // sequences without work here: rows of refused ones (counted) and of empty ones are zeros
+    for (int b = w; b < a.batch; b += a.slices) {
+        const CrossSeq s = cross_seq(a, b);
+        if (s.ok && (s.len || !s.rows)) continue;
+        if (!s.ok && head == 0 && tid == 0) atomicAdd(a.errors, 1ull);
+        const int32_t r0 = a.cu[b], r1 = a.cu[b + 1];
+        if (r0 < 0 || r1 > a.total_q || r1 < r0) continue;
+        const int64_t n = (int64_t)(r1 - r0) * a.group * (D / 4);
+        for (int64_t i = tid; i < n; i += THREADS) {
+            const int64_t row = i / (D / 4), c = i % (D / 4) * 4;
+            cross_store4(a, ((r0 + row / a.group) * a.q_heads + head * a.group + row % a.group) * D + c, cross_f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+        }
+    }
+    // units before each sequence
+    {
+        const int per = (a.batch + THREADS - 1) / THREADS, lo = min(tid * per, a.batch), hi = min(lo + per, a.batch);
+        int64_t mine = 0;
+        for (int b = lo; b < hi; ++b) {
+            const int64_t u = cross_units<ROWS, TK>(cross_seq(a, b));
+            s_pre[b + 1] = u;
+            mine += u;
+        }
+        int64_t incl = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t y = __shfl_up(incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 63) s_sum[wave] = incl;
+        if (tid == 0) s_pre[0] = 0;
+        __syncthreads();
+        int64_t run = incl - mine;
+        for (int i = 0; i < wave; ++i) run += s_sum[i];
+        for (int b = lo; b < hi; ++b) {
+            run += s_pre[b + 1];
+            s_pre[b + 1] = run;
+        }
+        __syncthreads();
+    }
+    const int64_t units = cross_uniform(s_pre[a.batch]);
+    int64_t chunk = (units + a.slices - 1) / a.slices;
+    chunk = chunk < a.least ? a.least : chunk;
+    int64_t u = w * chunk;
+    const int64_t end = u + chunk < units ? u + chunk : units;
+    int4 begun = {0, 0, 0, 0};
+
+    // this lane's place in every pass
+    const int p_c = lane % LPR, p_row0 = wave * WR;    // (of pass 0, among keys' and values' 2 TK rows)
+    const bool p_in = p_c < D / 8;
+    const int esize = !WIDE ? 2 : a.dtype == AIR_KV_F32 ? 4 : 1;
+    const int p_off = p_in ? (lane / LPR * D + 8 * p_c) * esize : kCrossNowhere;
+    const int nsc = WIDE && a.dtype != AIR_KV_F32 ? D >> a.sg_log2 : 0;
+    const int p_sc = p_in ? (lane / LPR * nsc + (8 * p_c >> a.sg_log2)) * 4 : kCrossNowhere;
+
+    int b = 0;
+    if (u < end) {
+        int lo = 0, hi = a.batch;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (s_pre[mid] <= u) lo = mid;
+            else hi = mid;
+        }
+        b = __builtin_amdgcn_readfirstlane(lo);
+    }
+    while (u < end) {
+        while (cross_uniform(s_pre[b + 1]) <= u) ++b;
+        CrossSeq sq = cross_seq(a, b);
+        sq.row0 = __builtin_amdgcn_readfirstlane(sq.row0);
+        sq.rows = __builtin_amdgcn_readfirstlane(sq.rows);
+        sq.len = __builtin_amdgcn_readfirstlane(sq.len);
+        const int nt = cross_tiles<ROWS, TK>(sq);
+        const int64_t in = u - cross_uniform(s_pre[b]);
+        const int blk = (int)(in / (nt + kCrossExtra)), at = (int)(in - (int64_t)blk * (nt + kCrossExtra));
+        const int64_t left = nt + kCrossExtra - at, mine = end - u < left ? end - u : left;
+        // a block's first kCrossExtra units are its beginning
+        const int t0 = at < kCrossExtra ? 0 : at - kCrossExtra;
+        const int t1 = at + (int)mine < kCrossExtra ? 0 : at + (int)mine - kCrossExtra;
+        u += mine;
+        if (t0 == t1) continue;                        // the slice ends before the block's first tile
+        const bool whole = t0 == 0 && t1 == nt;
+        const int tiles = t1 - t0;
+        const int64_t key0 = (int64_t)t0 * TK;
+        const int32_t *table = a.tables + (int64_t)b * a.max_blocks;
+
+        const int row = blk * ROWS + 32 * rg + r32;    // of the sequence's at this K/V head
+        const bool live = row < sq.rows, any = blk * ROWS + 32 * rg < sq.rows;
+        const int row_at = live ? row : sq.rows - 1;
+        const int64_t io = ((int64_t)(sq.row0 + row_at / a.group) * a.q_heads + head * a.group + row_at % a.group) * D;
+
+        // Q^T as the B operand: lane (n, h) holds elements 16 s + 8 h .. +8 of row n
+        cross_u32x4 qf[QP][KS];
+        if (a.q_dtype == AIR_KV_BF16) {
+            const uint16_t *q = (const uint16_t *)a.q + io + 8 * hf;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                qf[0][s] = *reinterpret_cast<const cross_u32x4 *>(q + 16 * s);
+#pragma unroll
+                for (int p = 1; p < QP; ++p) qf[p][s] = cross_u32x4{0, 0, 0, 0};
+            }
+        } else {
+            const float *q = (const float *)a.q + io + 8 * hf;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const cross_f32x4 x = *reinterpret_cast<const cross_f32x4 *>(q + 16 * s + 4 * i);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        uint32_t p[QP];
+                        cross_parts<QP>(x[2 * j], x[2 * j + 1], p);
+#pragma unroll
+                        for (int k = 0; k < QP; ++k) qf[k][s][2 * i + j] = p[k];
+                    }
+                }
+        }
+        cross_f32x16 acc[CT];
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
+        // Probabilities are held 2^(score - base), the base kDown above every score so far: 2^24 of
+        // them sum to 1 at most, so that values near the largest float do too.  A base is taken
+        // kSlack further up, so that it seldom changes: where a score passes lim.
+        constexpr float kDown = 24.0f, kSlack = 4.0f, kFar = 0x1p20f;
+        float base = -INFINITY, lim = -INFINITY, l_run = 0.0f;
+
+        struct Raw {                                   // a tile on its way
+            cross_u32x4 w[NP][WIDE ? 2 : 1];
+            float s[WIDE ? NP : 1];
+        } raw;
+        // lane h: the entry of a tile's half h, read a tile before it is needed, and its block
+        int32_t entry = 0, window = -1;
+        auto fetch = [&](int t) __attribute__((always_inline)) {
+            const int64_t key = key0 + (int64_t)t * TK + 16 * lane;
+            entry = lane < TK / 16 && key < sq.len ? table[key >> a.bs_log2] : 0;
+        };
+        auto look_up = [&](int t) __attribute__((always_inline)) {
+            const int64_t key = key0 + (int64_t)t * TK + 16 * lane;
+            const bool there = lane < TK / 16 && key < sq.len, out = there && (entry < 0 || entry >= a.num_blocks);
+            window = out || !there ? -1 : entry;
+            // counted once: by the first block of rows at the first head
+            if (head == 0 && blk == 0 && wave == 0) {
+                const int n = __popcll(__ballot(out && (key & ((1 << a.bs_log2) - 1)) == 0));
+                if (n && lane == 0) atomicAdd(a.errors, (unsigned long long)n);
+            }
+            fetch(t + 1);
+        };
+        auto load_tile = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int r = p_row0 + i * WAVES * WR, val = r / TK, at = r % TK;            // (of the wave)
+                const int32_t e = __builtin_amdgcn_readlane(window, at / 16);
+                const int64_t rest = sq.len - (key0 + (int64_t)t * TK + at);
+                const int have = e < 0 || rest <= 0 ? 0 : rest < WR ? (int)rest : WR;
+                const int64_t prow = (((int64_t)(e < 0 ? 0 : e) * a.heads + head) << a.bs_log2) + (at & ((1 << a.bs_log2) - 1));
+                const uint8_t *pages = (const uint8_t *)(val ? a.v_pages : a.k_pages) + prow * (D * esize);
+                // rows past the sequence's end lie outside of the buffer: zeros
+                const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)pages, (short)0, have * D * esize, kCrossBuffer);
+                if constexpr (!WIDE) {
+                    raw.w[i][0] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off, 0, 0));
+                } else if (a.dtype == AIR_KV_F32) {
+                    raw.w[i][0] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off, 0, 0));
+                    raw.w[i][1] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + 16, 0, 0));
+                } else {
+                    const cross_u32x2 x = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, p_off, 0, 0));
+                    raw.w[i][0][0] = x[0];
+                    raw.w[i][0][1] = x[1];
+                    const float *scales = (val ? a.v_scales : a.k_scales) + prow * nsc;
+                    const __amdgpu_buffer_rsrc_t ss = __builtin_amdgcn_make_buffer_rsrc((void *)scales, (short)0, have * nsc * 4, kCrossBuffer);
+                    raw.s[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ss, p_sc, 0, 0));
+                }
+            }
+        };
+        auto write_tile = [&](int t) __attribute__((always_inline)) {
+            uint8_t *mem = s_mem + t % NB * S::TILE;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int r = p_row0 + i * WAVES * WR, val = r / TK, at = r % TK + lane / LPR;
+                uint8_t *to = mem + (val ? VAT + at * VST : at * KST) + 16 * p_c;
+                const int plane = val ? VPLANE : KPLANE;
+                if constexpr (!WIDE) {
+                    if (p_in) *reinterpret_cast<cross_u32x4 *>(to) = raw.w[i][0];
+                } else {
+                    float x[8];
+                    if (a.dtype == AIR_KV_F32) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(raw.w[i][j / 4][j % 4]);
+                    } else {
+                        const cross_f32x4 lo = cross_codes(a.dtype == AIR_KV_FP8, raw.w[i][0][0], raw.s[i]);
+                        const cross_f32x4 hi = cross_codes(a.dtype == AIR_KV_FP8, raw.w[i][0][1], raw.s[i]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) { x[j] = lo[j]; x[4 + j] = hi[j]; }
+                    }
+                    cross_u32x4 y[KP];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t p[KP];
+                        cross_parts<KP>(x[2 * j], x[2 * j + 1], p);
+#pragma unroll
+                        for (int k = 0; k < KP; ++k) y[k][j] = p[k];
+                    }
+#pragma unroll
+                    for (int k = 0; k < KP; ++k)
+                        if (p_in) *reinterpret_cast<cross_u32x4 *>(to + k * plane) = y[k];
+                }
+            }
+            if (wave == 0 && lane < TK / 16) s_ok[t % NB][lane] = window >= 0;
+        };
+
+        __syncthreads();                               // the buffers of the block before are free
+        fetch(0);
+        look_up(0);
+        load_tile(0);
+        write_tile(0);
+        if (1 < tiles) {
+            look_up(1);
+            load_tile(1);
+        }
+        __syncthreads();
+        for (int t = 0; t < tiles; ++t) {
+            if (NB == 2 && t + 1 < tiles) {
+                write_tile(t + 1);
+                if (t + 2 < tiles) {
+                    look_up(t + 2);
+                    load_tile(t + 2);
+                }
+            }
+            if (any) {
+                const uint8_t *mem = s_mem + t % NB * S::TILE;
+#pragma unroll
+                for (int sub = 0; sub < SUB; ++sub) {
+                    const int k0 = 32 * (wk * SUB + sub);              // the keys' rows in the tile
+                    const int64_t rest = sq.len - (key0 + (int64_t)t * TK + k0);
+                    if (rest <= 0) continue;
+                    cross_f32x16 sc;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        cross_u32x4 kf[KP];
+#pragma unroll
+                        for (int p = 0; p < KP; ++p)
+                            kf[p] = *reinterpret_cast<const cross_u32x4 *>(mem + p * KPLANE + (k0 + r32) * KST + 32 * s + 16 * hf);
+#pragma unroll
+                        for (int i = 0; i < KP; ++i)
+#pragma unroll
+                            for (int j = 0; j < QP; ++j)
+                                if (i + j < 3) sc = cross_mfma(kf[i], qf[j][s], sc);
+                    }
+                    // keys past the end and of blocks outside the pool
+                    const int ok0 = __builtin_amdgcn_readfirstlane(s_ok[t % NB][k0 / 16]);
+                    const int ok1 = __builtin_amdgcn_readfirstlane(s_ok[t % NB][k0 / 16 + 1]);
+                    uint32_t mask = rest < 32 ? (1u << (int)rest) - 1 : ~0u;
+                    mask &= (ok0 ? 0x0000FFFFu : 0u) | (ok1 ? 0xFFFF0000u : 0u);
+                    if (mask != ~0u) {
+                        const uint32_t m = mask >> (4 * hf);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sc[i] = (m >> (8 * (i / 4) + i % 4)) & 1 ? sc[i] : -INFINITY;
+                    }
+                    float ft = a.scale_log2;
+                    float top = sc[0];
+#pragma unroll
+                    for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
+                    top = cross_max32(top) * ft;
+                    if (__ballot(top > lim) != 0ull) {
+                        // (scores past 2^20, which f32 holds in steps of an eighth and more, are each rounded as
+                        // the largest was, so that their distances from the base are exact)
+                        const float cap = __builtin_fabsf(base) < kFar ? base - kDown : base;
+                        const float now = top > cap ? top + (__builtin_fabsf(top) < kFar ? kDown + kSlack : 0.0f) : base;
+                        const float alpha = base == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(base - now);
+                        l_run *= alpha;
+#pragma unroll
+                        for (int c = 0; c < CT; ++c) acc[c] *= alpha;
+                        base = now;
+                        const bool far = !(__builtin_fabsf(base) < kFar) && base != -INFINITY;
+                        lim = far ? -INFINITY : base - kDown;
+                        if (__ballot(far) != 0ull) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) sc[i] *= ft;
+                            ft = 1.0f;
+                        }
+                    }
+                    const float from = base == -INFINITY ? 0.0f : base;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], ft, -from));
+                    cross_u32x4 p[QP][2];
+#pragma unroll
+                    for (int s = 0; s < 2; ++s)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t x[QP];
+                            cross_parts<QP>(sc[8 * s + 2 * j], sc[8 * s + 2 * j + 1], x);
+#pragma unroll
+                            for (int k = 0; k < QP; ++k) p[k][s][j] = x[k];
+                        }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) l_run += sc[i];
+                    // V^T as the A operand: lane (m, h) takes keys 16 s + 8 b + 4 h .. +4 of column m, b = 0, 1.
+                    // Within each 16-lane group, lane j of a transposing read receives element j % 4 of the 8
+                    // bytes that lanes 4 k + j / 4 address, k = 0 .. 3: lane i points at key i / 4 of the four
+                    // and columns 4 (i % 4) of the group's sixteen.
+                    const uint8_t *v0 = mem + VAT + (k0 + 4 * hf + ((lane & 15) >> 2)) * VST + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+#pragma unroll
+                    for (int c = 0; c < CT; ++c)
+#pragma unroll
+                        for (int s = 0; s < 2; ++s)
+#pragma unroll
+                            for (int i = 0; i < KP; ++i) {
+                                typedef short s16x4 __attribute__((ext_vector_type(4)));
+                                const uint8_t *v = v0 + i * VPLANE + 64 * c + 16 * s * VST;
+                                const cross_u32x2 x = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                          (__attribute__((address_space(3))) s16x4 *)v));
+                                const cross_u32x2 y = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                          (__attribute__((address_space(3))) s16x4 *)(v + 8 * VST)));
+                                const cross_u32x4 vf = {x[0], x[1], y[0], y[1]};
+#pragma unroll
+                                for (int j = 0; j < QP; ++j)
+                                    if (i + j < 3) acc[c] = cross_mfma(vf, p[j][s], acc[c]);
+                            }
+                }
+            }
+            __syncthreads();
+            if (NB == 1 && t + 1 < tiles) {
+                write_tile(t + 1);
+                if (t + 2 < tiles) {
+                    look_up(t + 2);
+                    load_tile(t + 2);
+                }
+                __syncthreads();
+            }
+        }
+
+        // lane (n, h): columns 32 c + 8 (i / 4) + 4 h + i % 4 of row n in acc[c][i]
+        float l = cross_sum32(l_run);
+        const int64_t slot = 2 * cell + (t0 == 0 ? 1 : 0);
+        const int64_t prow = slot * ROWS + 32 * rg + r32;
+        if constexpr (WK == 1) {
+            // no key at all (every block outside the pool): zeros
+            const float k = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+            if (whole ? live : any) {
+#pragma unroll
+                for (int c = 0; c < CT; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const cross_f32x4 x = {acc[c][4 * i] * k, acc[c][4 * i + 1] * k, acc[c][4 * i + 2] * k, acc[c][4 * i + 3] * k};
+                        const int col = 32 * c + 8 * i + 4 * hf;
+                        if (whole) cross_store4(a, io + col, x);
+                        else *reinterpret_cast<cross_f32x4 *>(a.part_o + prow * D + col) = x;
+                    }
+                if (!whole && hf == 0) a.part_ml[prow] = make_float2(base, l);
+            }
+        } else {
+            // the waves of one row group: their bases' largest, then their sums, CR column tiles at a
+            // time, four columns (c, i) of all of them to one wave
+            if (hf == 0) s_ml[wave][r32] = make_float2(base, l);
+            __syncthreads();
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < WK; ++i) top = fmaxf(top, s_ml[rg * WK + i][r32].x);
+            l = 0.0f;
+#pragma unroll
+            for (int i = 0; i < WK; ++i) {
+                const float2 ml = s_ml[rg * WK + i][r32];
+                l += ml.x == -INFINITY ? ml.y : ml.y * __builtin_amdgcn_exp2f(ml.x - top);
+            }
+            const float alpha = base == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(base - top);
+            const float k = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+            cross_f32x4 *x = reinterpret_cast<cross_f32x4 *>(s_mem) + lane;
+#pragma unroll
+            for (int c0 = 0; c0 < CT; c0 += CR) {
+                if (c0) __syncthreads();
+#pragma unroll
+                for (int c = c0; c < c0 + CR && c < CT; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        x[((wave * CR + c - c0) * 4 + i) * 64] = cross_f32x4{acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]} * alpha;
+                __syncthreads();
+                const int quads = 4 * (CT - c0 < CR ? CT - c0 : CR);
+                for (int g = wk; g < quads; g += WK) {
+                    cross_f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int i = 0; i < WK; ++i) y += x[((rg * WK + i) * CR * 4 + g) * 64];
+                    const int col = 32 * (c0 + g / 4) + 8 * (g % 4) + 4 * hf;
+                    if (whole) {
+                        if (live) cross_store4(a, io + col, y * k);
+                    } else if (any) {
+                        *reinterpret_cast<cross_f32x4 *>(a.part_o + prow * D + col) = y;
+                    }
+                }
+            }
+            if (!whole && any && hf == 0 && wk == 0) a.part_ml[prow] = make_float2(top, l);
+        }
+        if (!whole && t0 == 0) {                       // begun here: its last unit's slice ends it
+            const int64_t last = u - mine - at + nt + kCrossExtra - 1;
+            begun = int4{b, blk, (int)(last / chunk - w + 1), 0};
+        }
+    }
+    if (tid == 0) a.desc[cell] = begun;
+}
+
+template <int QP, bool WIDE, bool FEW> hipError_t launch_cross_shape(const CrossArgs &a, int d, hipStream_t s) {
+    const dim3 grid((unsigned)(a.slices * a.heads));
+    switch (d) {
+#define AIRKV_CROSS(D) \
+    case D: hipLaunchKernelGGL((paged_cross_kernel<D, WIDE, QP, FEW>), grid, dim3(CrossShape<D, WIDE, QP, FEW>::WAVES * 64), 0, s, a); break;
+        AIRKV_CROSS(32) AIRKV_CROSS(64) AIRKV_CROSS(96) AIRKV_CROSS(128)
+        AIRKV_CROSS(160) AIRKV_CROSS(192) AIRKV_CROSS(224) AIRKV_CROSS(256)
+#undef AIRKV_CROSS
+    }
+    return hipGetLastError();
+}
+
+template <int QP, bool WIDE, bool FEW> int cross_rows_shape(int d) {
+    switch (d) {
+#define AIRKV_CROSS(D) case D: return CrossShape<D, WIDE, QP, FEW>::ROWS;
+        AIRKV_CROSS(32) AIRKV_CROSS(64) AIRKV_CROSS(96) AIRKV_CROSS(128)
+        AIRKV_CROSS(160) AIRKV_CROSS(192) AIRKV_CROSS(224) AIRKV_CROSS(256)
+#undef AIRKV_CROSS
+    }
+    return 0;
+}
+
+}  // namespace airkv

@@ -73,6 +73,11 @@ hipError_t launch_append_rotary(const air_kv_pool &pool, hipStream_t s, const vo
 hipError_t launch_rotate(const air_kv_pool &pool, hipStream_t s, const int32_t *tables, int32_t batch, int32_t max_blocks,
                          const int32_t *from, const int32_t *to, const int32_t *cu, int32_t total, const float *inv_freq,
                          int32_t rot_dim, int32_t layout);
+// (cross attention: kernels/paged_cross.hip)
+size_t cross_workspace(const air_kv_pool &pool);
+hipError_t launch_cross(const air_kv_pool &pool, hipStream_t s, const void *q, int32_t q_dtype, int32_t n_q_heads,
+                        const int32_t *cu, int32_t total_q, int32_t max_q_len, const int32_t *tables, const int32_t *lens,
+                        int32_t batch, int32_t max_blocks, float scale, void *workspace, void *out, int32_t out_dtype);
 hipError_t launch_stage_blocks(const air_kv_pool &pool, hipStream_t s, const int32_t *ids, int32_t n,
                                void *staging, bool to_staging);
 size_t wire_block_bytes(const air_kv_pool &pool);

@@ -118,6 +118,8 @@ extern "C" {
     pub fn air_paged_diff_decode(pool: *mut air_kv_pool, stream: *mut c_void, q: *const c_void, q_dtype: i32, n_q_heads: i32, lambda: *const f32, lambda_per_row: i32, block_tables: *const i32, seq_lens: *const i32, batch: i32, max_blocks: i32, scale: f32, max_splits: i32, norm_weight: *const f32, norm_eps: f32, out_scale: f32, workspace: *mut c_void, ws_bytes: usize, out: *mut c_void, out_dtype: i32) -> c_int;
     pub fn air_paged_diff_prefill_workspace_size(pool: *const air_kv_pool, n_q_heads: i32, batch: i32, max_q_len: i32, bytes: *mut usize) -> c_int;
     pub fn air_paged_diff_prefill(pool: *mut air_kv_pool, stream: *mut c_void, q: *const c_void, q_dtype: i32, n_q_heads: i32, lambda: *const f32, lambda_per_row: i32, cu_q: *const i32, total_q: i32, max_q_len: i32, block_tables: *const i32, seq_lens: *const i32, batch: i32, max_blocks: i32, scale: f32, norm_weight: *const f32, norm_eps: f32, out_scale: f32, workspace: *mut c_void, ws_bytes: usize, out: *mut c_void, out_dtype: i32) -> c_int;
+    pub fn air_paged_cross_workspace_size(pool: *const air_kv_pool, n_q_heads: i32, batch: i32, max_q_len: i32, bytes: *mut usize) -> c_int;
+    pub fn air_paged_cross(pool: *mut air_kv_pool, stream: *mut c_void, q: *const c_void, q_dtype: i32, n_q_heads: i32, cu_q: *const i32, total_q: i32, max_q_len: i32, block_tables: *const i32, seq_lens: *const i32, batch: i32, max_blocks: i32, scale: f32, workspace: *mut c_void, ws_bytes: usize, out: *mut c_void, out_dtype: i32) -> c_int;
     pub fn air_rotary_frequencies(rot_dim: i32, base: f64, scaling: i32, factor: f64, trained_len: f64, low: f64, high: f64, inv_freq: *mut f32, magnitude: *mut f32) -> c_int;
     pub fn air_kv_append_rotary(pool: *mut air_kv_pool, stream: *mut c_void, q: *const c_void, q_stride: i64, n_q_heads: i32, k: *const c_void, k_stride: i64, v: *const c_void, v_stride: i64, in_dtype: i32, slot_mapping: *const i64, positions: *const i32, n_tokens: i32, inv_freq: *const f32, rot_dim: i32, layout: i32, magnitude: f32, q_out: *mut c_void, q_out_dtype: i32) -> c_int;
     pub fn air_kv_rotate(pool: *mut air_kv_pool, stream: *mut c_void, block_tables: *const i32, batch: i32, max_blocks: i32, from: *const i32, to: *const i32, cu: *const i32, total: i32, inv_freq: *const f32, rot_dim: i32, layout: i32) -> c_int;

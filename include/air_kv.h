@@ -445,6 +445,42 @@ int air_paged_diff_prefill(air_kv_pool *pool, void *stream, const void *q, int32
                            int32_t out_dtype);
 
 /* ------------------------------------------------------------------------ */
+/* Cross attention over pages                                                */
+/* ------------------------------------------------------------------------ */
+
+/* No counterpart in the reference's cache interfaces.  A decoder's rows attend to an
+ * encoder's states, cached like any sequence (air_kv_append): row r of sequence b,
+ * r from cu_q[b] to cu_q[b + 1] - 1, sees all of the sequence's seq_lens[b] tokens,
+ *   out[r][h] = softmax(scale * q[r][h] . K[h / group]^T) . V[h / group]
+ * whatever the number of rows (one token, a prompt, the beams of a sequence): there
+ * is no order between rows and tokens.  Arguments, pools and refusals are those of
+ * air_paged_prefill: q and out [total_q][n_q_heads][head_dim] as q_dtype and out_dtype
+ * (16-byte aligned), any group, any head_dim of a pool; max_q_len is a hint (an upper
+ * bound of a sequence's rows; 0: not known), under which few rows take their
+ * sequence's keys side by side.  A sequence whose rows do not lie in [0, total_q] or
+ * whose seq_len lies outside [0, max_blocks * block_size] is counted
+ * (air_kv_pool_error_count) and its rows (where they lie in [0, total_q]) are
+ * zero-filled; rows of a sequence of length 0 are zeros; rows of no sequence stay as
+ * they were.  Out-of-pool table entries are counted and their tokens left out (of
+ * all of a sequence's: zeros).  Rows of different sequences must not overlap.
+ *
+ * Scores, sums and outputs are held in 32 bits.  bf16 queries with bf16 outputs on
+ * BF16, INT8 and FP8 pools take products of bf16 values (probabilities, and the
+ * keys and values of 1-byte pages, rounded once); everything else keeps f32
+ * precision, where what lies below 2^-133 of an f32 or 1-byte page's value is cut
+ * off.  Probabilities below 2^-98 of a row's largest count as 0, and so may what
+ * values below 2^-98 add.  Keys and values that are not finite give NaN where they reach.
+ * The workspace (16-byte aligned, at least air_paged_cross_workspace_size bytes, no
+ * initialisation needed) holds the parts of blocks of rows that several workgroups
+ * share; calls that share one must be ordered (same stream). */
+int air_paged_cross_workspace_size(const air_kv_pool *pool, int32_t n_q_heads, int32_t batch, int32_t max_q_len,
+                                   size_t *bytes);
+int air_paged_cross(air_kv_pool *pool, void *stream, const void *q, int32_t q_dtype, int32_t n_q_heads,
+                    const int32_t *cu_q, int32_t total_q, int32_t max_q_len, const int32_t *block_tables,
+                    const int32_t *seq_lens, int32_t batch, int32_t max_blocks, float scale, void *workspace,
+                    size_t ws_bytes, void *out, int32_t out_dtype);
+
+/* ------------------------------------------------------------------------ */
 /* Rotary positions                                                          */
 /* ------------------------------------------------------------------------ */
 
