@@ -25,11 +25,13 @@ __global__ __launch_bounds__(kMergeThreads) void cross_merge_kernel(CrossArgs a,
     const int32_t r0 = a.cu[it.x];
     const int32_t row = it.y * rows + r;
     if (row >= (a.cu[it.x + 1] - r0) * a.group || col >= d) return;
+    // the mean of the values so far, its weight l under `base` (a mean stays within its values' range,
+    // where a sum of values near the largest or the smallest floats would not)
     float base = -INFINITY, l = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     constexpr int kBatch = 4;
     for (int p0 = 0; p0 < it.z; p0 += kBatch) {
-        float2 ml[kBatch];
+        float4 ml[kBatch];
         f32x4 x[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
@@ -40,18 +42,18 @@ __global__ __launch_bounds__(kMergeThreads) void cross_merge_kernel(CrossArgs a,
         }
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            // (a piece without a key in the pool has base -inf and sum 0)
-            if (p0 + i >= it.z || (ml[i].x == -INFINITY && ml[i].y == 0.0f)) continue;
+            // (a piece without a key in the pool has sum 0)
+            if (p0 + i >= it.z || ml[i].y == 0.0f) continue;
             const float top = fmaxf(base, ml[i].x);
-            const float was = base == top ? 1.0f : __builtin_amdgcn_exp2f(base - top), is = ml[i].x == top ? 1.0f : __builtin_amdgcn_exp2f(ml[i].x - top);
-            l = l * was + ml[i].y * is;
-            o = o * was + x[i] * is;
+            const float was = base == top ? l : l * __builtin_amdgcn_exp2f(base - top);
+            const float is = ml[i].x == top ? 1.0f : __builtin_amdgcn_exp2f(ml[i].x - top);
+            l = was + ml[i].y * is;
+            const float k = 1.0f / l;
+            o = o * (was * k) + x[i] * (is * k) * ml[i].z;
             base = top;
         }
     }
-    const float k = l == 0.0f ? 0.0f : 1.0f / l;
     const int64_t at = ((int64_t)(r0 + row / a.group) * a.q_heads + blockIdx.z * a.group + row % a.group) * d + col;
-    o *= k;
     if (a.out_dtype == AIR_KV_F32)
         *reinterpret_cast<f32x4 *>((float *)a.out + at) = o;
     else
@@ -82,7 +84,7 @@ int slices_of(const air_kv_pool &p) { return std::max(1, p.cus / p.desc.n_kv_hea
 
 size_t bytes_of(const air_kv_pool &p, int rows) {
     const size_t cells = (size_t)p.desc.n_kv_heads * slices_of(p), slots = 2 * cells * rows;
-    return align256(cells * sizeof(int4)) + align256(slots * sizeof(float2)) + slots * p.desc.head_dim * 4;
+    return align256(cells * sizeof(int4)) + align256(slots * sizeof(float4)) + slots * p.desc.head_dim * 4;
 }
 
 }  // namespace
@@ -130,8 +132,8 @@ hipError_t launch_cross(const air_kv_pool &p, hipStream_t s, const void *q, int3
     char *ws = (char *)workspace;
     a.desc = (int4 *)ws;
     ws += align256(cells * sizeof(int4));
-    a.part_ml = (float2 *)ws;
-    ws += align256(slots * sizeof(float2));
+    a.part_ml = (float4 *)ws;
+    ws += align256(slots * sizeof(float4));
     a.part_o = (float *)ws;
     for (int32_t b0 = 0; b0 < batch; b0 += kCrossBatch) {
         a.batch = std::min(batch - b0, kCrossBatch);

@@ -36,9 +36,9 @@ struct CrossArgs {
     int32_t least;                     // units a slice holds at least
     // cut blocks: per (K/V head, slice) the block it begins and does not end, {sequence, block,
     // pieces}; two piece slots each, 2w for a block begun before and 2w + 1 for one that goes
-    // on: [slot][row] of (base, sum), and of head_dim sums
+    // on: [slot][row] of (base, sum, the sums' unit), and of head_dim sums
     int4 *desc;
-    float2 *part_ml;
+    float4 *part_ml;
     float *part_o;
 };
 

@@ -5,13 +5,13 @@
 namespace airkv {
 
 hipError_t launch_cross_f32(const CrossArgs &a, int head_dim, bool few, hipStream_t s) {
-    if (a.dtype == AIR_KV_BF16) return few ? launch_cross_shape<3, false, true>(a, head_dim, s) : launch_cross_shape<3, false, false>(a, head_dim, s);
-    return few ? launch_cross_shape<3, true, true>(a, head_dim, s) : launch_cross_shape<3, true, false>(a, head_dim, s);
+    if (a.dtype == AIR_KV_BF16) return few ? launch_cross_shape<kParts, true>(a, head_dim, s) : launch_cross_shape<kParts, false>(a, head_dim, s);
+    return few ? launch_cross_shape<kWide, true>(a, head_dim, s) : launch_cross_shape<kWide, false>(a, head_dim, s);
 }
 
 int cross_rows_f32(int head_dim, bool few, bool wide) {
-    if (wide) return few ? cross_rows_shape<3, true, true>(head_dim) : cross_rows_shape<3, true, false>(head_dim);
-    return few ? cross_rows_shape<3, false, true>(head_dim) : cross_rows_shape<3, false, false>(head_dim);
+    if (wide) return few ? cross_rows_shape<kWide, true>(head_dim) : cross_rows_shape<kWide, false>(head_dim);
+    return few ? cross_rows_shape<kParts, true>(head_dim) : cross_rows_shape<kParts, false>(head_dim);
 }
 
 }  // namespace airkv

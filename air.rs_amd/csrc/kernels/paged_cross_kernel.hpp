@@ -5,11 +5,17 @@
 //   S   = K . Q^T      v_mfma_f32_32x32x16_bf16, lane (n, h) holds 16 of the 32 keys of row n
 //   O^T += V^T . P^T   the same instruction; its contraction takes the keys in the order in
 //                      which the lanes hold P, so P never moves
-// Operands are bf16 parts: KP of keys and values, QP of queries and probabilities (1: rounded to
-// bf16, 3: all 24 bits of an f32), of which products with i + j < 3 are formed.  Keys and
-// values are staged in LDS as rows, 16 (keys) and 64 (values) bytes apart modulo 256, so that
-// neither the rows' reads nor the values' transposing reads meet in a bank; a tile is loaded
-// two ahead into registers and staged one ahead where two buffers fit.
+// Operands by kind (CrossKind):
+//   kBf16   bf16 queries over bf16 pages: probabilities are rounded to bf16
+//   kCodes  bf16 queries over 1-byte pages: everything as f16 (11 bits), under powers of two: of a
+//           query row's, of a tile's keys (from the largest scale of those that are not all zeros,
+//           known a barrier before the tile is staged) and of the values' (the smallest so far)
+//   kParts  f32 precision over bf16 pages, kWide over f32 and 1-byte ones: bf16 parts that hold all
+//           24 bits, of queries and probabilities and (kWide) of keys and values; products with
+//           i + j < 3 are formed
+// Keys and values are staged in LDS as rows, 16 (keys) and 64 (values) bytes apart modulo 256, so
+// that neither the rows' reads nor the values' transposing reads meet in a bank; a tile is
+// loaded two ahead into registers and staged one ahead where two buffers fit.
 //
 // WK waves share 32 rows and take a tile's keys in turn (few rows), or each wave has rows of its
 // own (WK = 1).
@@ -28,8 +34,12 @@ typedef float cross_f32x4 __attribute__((ext_vector_type(4)));
 typedef float cross_f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 cross_bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 cross_bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 cross_f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 cross_f16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t cross_u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t cross_u32x2 __attribute__((ext_vector_type(2)));
+
+enum CrossKind { kBf16, kCodes, kParts, kWide };
 
 constexpr int kCrossLds = 149 * 1024;              // of a CU's 160 KB, for the tiles
 constexpr int kCrossBuffer = 0x00020000;           // a raw buffer's last word
@@ -50,8 +60,14 @@ constexpr int cross_wk(int d, int kp, int qp, bool few) {
 // Keys of a tile that one wave takes, in 32s.
 constexpr int cross_sub(int d, int kp, int wk) { return wk == 1 && cross_tile_bytes(d, kp, 64) <= kCrossLds ? 2 : 1; }
 
-__device__ __forceinline__ cross_f32x16 cross_mfma(cross_u32x4 a, cross_u32x4 b, cross_f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(cross_bf16x8, a), __builtin_bit_cast(cross_bf16x8, b), c, 0, 0, 0);
+template <bool F16> __device__ __forceinline__ cross_f32x16 cross_mfma(cross_u32x4 a, cross_u32x4 b, cross_f32x16 c) {
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(cross_f16x8, a), __builtin_bit_cast(cross_f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(cross_bf16x8, a), __builtin_bit_cast(cross_bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t cross_f16_pair(float x, float y) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((cross_f32x2{x, y}), cross_f16x2));
 }
 __device__ __forceinline__ uint32_t cross_bf16_pair(float x, float y) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((cross_f32x2{x, y}), cross_bf16x2));
@@ -66,10 +82,14 @@ __device__ __forceinline__ void cross_split(float x, float y, uint32_t (&p)[3]) 
         y -= __uint_as_float(__float_as_uint(y) & 0xFFFF0000u);
     }
 }
-template <int P> __device__ __forceinline__ void cross_parts(float x, float y, uint32_t (&p)[P]) {
+// x, y as P parts: three, or one rounded to f16 or bf16.
+template <bool F16, int P> __device__ __forceinline__ void cross_parts(float x, float y, uint32_t (&p)[P]) {
     if constexpr (P == 3) cross_split(x, y, p);
-    else p[0] = cross_bf16_pair(x, y);
+    else p[0] = F16 ? cross_f16_pair(x, y) : cross_bf16_pair(x, y);
 }
+// 2^e, e clamped to the normal numbers; the exponent of a normal number.
+__device__ __forceinline__ float cross_pow2(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
+__device__ __forceinline__ int cross_exponent(float x) { return (int)((__float_as_uint(x) >> 23) & 0xFF) - 127; }
 // The values of the four 1-byte codes in w times their scale.
 __device__ __forceinline__ cross_f32x4 cross_codes(bool fp8, uint32_t w, float s) {
     if (fp8) {
@@ -97,21 +117,21 @@ __device__ __forceinline__ void cross_store4(const CrossArgs &a, int64_t at, cro
     else *reinterpret_cast<cross_u32x2 *>((uint16_t *)a.out + at) = cross_u32x2{cross_bf16_pair(x[0], x[1]), cross_bf16_pair(x[2], x[3])};
 }
 
-// WIDE: f32 or 1-byte pages (a.dtype says which), else bf16 ones.
-template <int D, bool WIDE, int QP, bool FEW>
+template <int D, CrossKind KIND, bool FEW>
 struct CrossShape {
-    static constexpr int KP = WIDE && QP == 3 ? 3 : 1;
+    static constexpr int KP = KIND == kWide ? 3 : 1, QP = KIND == kParts || KIND == kWide ? 3 : 1;
     static constexpr int WAVES = cross_waves(D, QP), WK = cross_wk(D, KP, QP, FEW), SUB = cross_sub(D, KP, WK);
     static constexpr int ROWS = 32 * (WAVES / WK), TK = 32 * WK * SUB;
     static constexpr int TILE = cross_tile_bytes(D, KP, TK), NB = 2 * TILE <= kCrossLds ? 2 : 1;
 };
 
-template <int D, bool WIDE, int QP, bool FEW>
-__global__ __launch_bounds__((CrossShape<D, WIDE, QP, FEW>::WAVES * 64))
-__attribute__((amdgpu_waves_per_eu(CrossShape<D, WIDE, QP, FEW>::WAVES / 4, CrossShape<D, WIDE, QP, FEW>::WAVES / 4)))
+template <int D, CrossKind KIND, bool FEW>
+__global__ __launch_bounds__((CrossShape<D, KIND, FEW>::WAVES * 64))
+__attribute__((amdgpu_waves_per_eu(CrossShape<D, KIND, FEW>::WAVES / 4, CrossShape<D, KIND, FEW>::WAVES / 4)))
 void paged_cross_kernel(CrossArgs a) {
-    typedef CrossShape<D, WIDE, QP, FEW> S;
-    constexpr int KP = S::KP, WAVES = S::WAVES, WK = S::WK, SUB = S::SUB, ROWS = S::ROWS, TK = S::TK, NB = S::NB, THREADS = 64 * WAVES;
+    typedef CrossShape<D, KIND, FEW> S;
+    constexpr bool F16 = KIND == kCodes;
+    constexpr int KP = S::KP, QP = S::QP, WAVES = S::WAVES, WK = S::WK, SUB = S::SUB, ROWS = S::ROWS, TK = S::TK, NB = S::NB, THREADS = 64 * WAVES;
     constexpr int KST = cross_k_stride(D), VST = cross_v_stride(D);
     constexpr int KPLANE = TK * KST, VPLANE = TK * VST, VAT = KP * KPLANE;    // a part's rows; where values begin
     constexpr int KS = D / 16, CT = D / 32;            // steps of the first product, 32-column tiles of the second
@@ -124,7 +144,8 @@ void paged_cross_kernel(CrossArgs a) {
     constexpr int CR = MEM / JOIN < CT ? MEM / JOIN : CT;      // column tiles joined at once (WK > 1)
     __shared__ int64_t s_pre[kCrossBatch + 1];
     __shared__ int64_t s_sum[WAVES];
-    __shared__ int32_t s_ok[NB][TK / 16];              // whether the tile's 16-key halves are in the pool
+    __shared__ int32_t s_ok[4][TK / 16];               // whether a tile's 16-key halves are in the pool
+    __shared__ uint32_t s_top[3][2];                   // a tile's largest scale of keys and of values, as bits
     __shared__ float2 s_ml[WAVES][32];
     __shared__ __align__(16) uint8_t s_mem[MEM];
 
@@ -185,9 +206,9 @@ void paged_cross_kernel(CrossArgs a) {
     // this lane's place in every pass
     const int p_c = lane % LPR, p_row0 = wave * WR;    // (of pass 0, among keys' and values' 2 TK rows)
     const bool p_in = p_c < D / 8;
-    const int esize = !WIDE ? 2 : a.dtype == AIR_KV_F32 ? 4 : 1;
+    const int esize = KIND == kCodes ? 1 : KIND != kWide ? 2 : a.dtype == AIR_KV_F32 ? 4 : 1;
     const int p_off = p_in ? (lane / LPR * D + 8 * p_c) * esize : kCrossNowhere;
-    const int nsc = WIDE && a.dtype != AIR_KV_F32 ? D >> a.sg_log2 : 0;
+    const int nsc = KIND == kCodes || (KIND == kWide && a.dtype != AIR_KV_F32) ? D >> a.sg_log2 : 0;
     const int p_sc = p_in ? (lane / LPR * nsc + (8 * p_c >> a.sg_log2)) * 4 : kCrossNowhere;
 
     int b = 0;
@@ -227,7 +248,8 @@ void paged_cross_kernel(CrossArgs a) {
 
         // Q^T as the B operand: lane (n, h) holds elements 16 s + 8 h .. +8 of row n
         cross_u32x4 qf[QP][KS];
-        if (a.q_dtype == AIR_KV_BF16) {
+        int qe = 0;                                    // (kCodes: the power of two they are under)
+        if (KIND == kBf16 || KIND == kCodes || a.q_dtype == AIR_KV_BF16) {
             const uint16_t *q = (const uint16_t *)a.q + io + 8 * hf;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
@@ -245,11 +267,28 @@ void paged_cross_kernel(CrossArgs a) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         uint32_t p[QP];
-                        cross_parts<QP>(x[2 * j], x[2 * j + 1], p);
+                        cross_parts<F16, QP>(x[2 * j], x[2 * j + 1], p);
 #pragma unroll
                         for (int k = 0; k < QP; ++k) qf[k][s][2 * i + j] = p[k];
                     }
                 }
+        }
+        if constexpr (F16) {
+            // the row's largest element to [2^4, 2^5): bf16's 8 bits are exact in f16 down to 2^-11
+            float top = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    top = fmaxf(top, fmaxf(__builtin_fabsf(__uint_as_float(qf[0][s][j] << 16)),
+                                           __builtin_fabsf(__uint_as_float(qf[0][s][j] & 0xFFFF0000u))));
+            const float fq = cross_pow2(4 - cross_exponent(cross_max32(top)));
+            qe = cross_exponent(fq);
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    qf[0][s][j] = cross_f16_pair(__uint_as_float(qf[0][s][j] << 16) * fq, __uint_as_float(qf[0][s][j] & 0xFFFF0000u) * fq);
         }
         cross_f32x16 acc[CT];
 #pragma unroll
@@ -257,15 +296,17 @@ void paged_cross_kernel(CrossArgs a) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
         // Probabilities are held 2^(score - base), the base kDown above every score so far: 2^24 of
-        // them sum to 1 at most, so that values near the largest float do too.  A base is taken
-        // kSlack further up, so that it seldom changes: where a score passes lim.
-        constexpr float kDown = 24.0f, kSlack = 4.0f, kFar = 0x1p20f;
+        // them sum to 1 at most, so that values near the largest float do too.  (f16 ones up to
+        // 2^15, so that they keep 11 bits down to 2^-25 of the largest; values are below 2^15 there.)
+        // A base is taken kSlack further up, so that it seldom changes: where a score passes lim.
+        constexpr float kDown = F16 ? -15.0f : 24.0f, kSlack = 4.0f, kFar = 0x1p20f;
         float base = -INFINITY, lim = -INFINITY, l_run = 0.0f;
 
         struct Raw {                                   // a tile on its way
-            cross_u32x4 w[NP][WIDE ? 2 : 1];
-            float s[WIDE ? NP : 1];
-        } raw;
+            cross_u32x4 w[NP][KIND == kWide ? 2 : 1];
+            float s[KIND == kWide || KIND == kCodes ? NP : 1];
+        } raw, next;                                   // (next: kCodes with two buffers, a tile further ahead)
+        float fk = 1.0f, fk_next = 1.0f, fv = 0.0f, fv_next = 0.0f;    // kCodes: powers of two (0: no value yet)
         // lane h: the entry of a tile's half h, read a tile before it is needed, and its block
         int32_t entry = 0, window = -1;
         auto fetch = [&](int t) __attribute__((always_inline)) {
@@ -274,16 +315,17 @@ void paged_cross_kernel(CrossArgs a) {
         };
         auto look_up = [&](int t) __attribute__((always_inline)) {
             const int64_t key = key0 + (int64_t)t * TK + 16 * lane;
-            const bool there = lane < TK / 16 && key < sq.len, out = there && (entry < 0 || entry >= a.num_blocks);
+            const bool there = t < tiles && lane < TK / 16 && key < sq.len, out = there && (entry < 0 || entry >= a.num_blocks);
             window = out || !there ? -1 : entry;
             // counted once: by the first block of rows at the first head
             if (head == 0 && blk == 0 && wave == 0) {
                 const int n = __popcll(__ballot(out && (key & ((1 << a.bs_log2) - 1)) == 0));
                 if (n && lane == 0) atomicAdd(a.errors, (unsigned long long)n);
             }
+            if (wave == 0 && lane < TK / 16) s_ok[t % 4][lane] = window >= 0;
             fetch(t + 1);
         };
-        auto load_tile = [&](int t) __attribute__((always_inline)) {
+        auto load_tile = [&](int t, Raw &raw) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const int r = p_row0 + i * WAVES * WR, val = r / TK, at = r % TK;            // (of the wave)
@@ -294,38 +336,74 @@ void paged_cross_kernel(CrossArgs a) {
                 const uint8_t *pages = (const uint8_t *)(val ? a.v_pages : a.k_pages) + prow * (D * esize);
                 // rows past the sequence's end lie outside of the buffer: zeros
                 const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)pages, (short)0, have * D * esize, kCrossBuffer);
-                if constexpr (!WIDE) {
+                if constexpr (KIND == kBf16 || KIND == kParts) {
                     raw.w[i][0] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off, 0, 0));
-                } else if (a.dtype == AIR_KV_F32) {
-                    raw.w[i][0] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off, 0, 0));
-                    raw.w[i][1] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + 16, 0, 0));
-                } else {
+                } else if (KIND == kCodes || a.dtype != AIR_KV_F32) {
                     const cross_u32x2 x = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, p_off, 0, 0));
                     raw.w[i][0][0] = x[0];
                     raw.w[i][0][1] = x[1];
                     const float *scales = (val ? a.v_scales : a.k_scales) + prow * nsc;
                     const __amdgpu_buffer_rsrc_t ss = __builtin_amdgcn_make_buffer_rsrc((void *)scales, (short)0, have * nsc * 4, kCrossBuffer);
                     raw.s[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ss, p_sc, 0, 0));
+                } else if constexpr (KIND == kWide) {
+                    raw.w[i][0] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off, 0, 0));
+                    raw.w[i][1] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + 16, 0, 0));
+                }
+            }
+        };
+        // kCodes: the largest finite scales of tile t, of all waves.  (The scale 1 that the append gives a
+        // group of zeros does not count: lanes whose codes are zeros leave theirs out.)
+        auto mark = [&](int t, const Raw &raw) __attribute__((always_inline)) {
+            if constexpr (F16) {
+                const uint32_t sign = a.dtype == AIR_KV_FP8 ? 0x7F7F7F7Fu : ~0u;
+                float k = 0.0f, v = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    const float x = __builtin_fabsf(raw.s[i]);
+                    const float y = x < INFINITY && ((raw.w[i][0][0] | raw.w[i][0][1]) & sign) ? x : 0.0f;
+                    if ((p_row0 + i * WAVES * WR) / TK) v = fmaxf(v, y);
+                    else k = fmaxf(k, y);
+                }
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    k = fmaxf(k, __shfl_xor(k, o));
+                    v = fmaxf(v, __shfl_xor(v, o));
+                }
+                k = cross_max32(k);
+                v = cross_max32(v);
+                if (lane == 0) {
+                    atomicMax(&s_top[t % 3][0], __float_as_uint(k));
+                    atomicMax(&s_top[t % 3][1], __float_as_uint(v));
                 }
             }
         };
         auto write_tile = [&](int t) __attribute__((always_inline)) {
             uint8_t *mem = s_mem + t % NB * S::TILE;
+            if constexpr (F16) {
+                // codes are at most 448 (2^9): the largest value to 2^13 at most
+                const float k = __uint_as_float(__builtin_amdgcn_readfirstlane(s_top[t % 3][0]));
+                const float v = __uint_as_float(__builtin_amdgcn_readfirstlane(s_top[t % 3][1]));
+                fk_next = k == 0.0f ? 1.0f : cross_pow2(3 - cross_exponent(k));
+                // values: kept as long as the largest stays below 2^15; it never grows
+                const float want = cross_pow2(3 - cross_exponent(v));
+                fv_next = v == 0.0f ? fv_next : fv_next == 0.0f || fv_next > 4.0f * want ? want : fv_next;
+            }
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const int r = p_row0 + i * WAVES * WR, val = r / TK, at = r % TK + lane / LPR;
                 uint8_t *to = mem + (val ? VAT + at * VST : at * KST) + 16 * p_c;
                 const int plane = val ? VPLANE : KPLANE;
-                if constexpr (!WIDE) {
+                if constexpr (KIND == kBf16 || KIND == kParts) {
                     if (p_in) *reinterpret_cast<cross_u32x4 *>(to) = raw.w[i][0];
                 } else {
                     float x[8];
-                    if (a.dtype == AIR_KV_F32) {
+                    if (KIND == kWide && a.dtype == AIR_KV_F32) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(raw.w[i][j / 4][j % 4]);
+                        for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(raw.w[i][KIND == kWide ? j / 4 : 0][j % 4]);
                     } else {
-                        const cross_f32x4 lo = cross_codes(a.dtype == AIR_KV_FP8, raw.w[i][0][0], raw.s[i]);
-                        const cross_f32x4 hi = cross_codes(a.dtype == AIR_KV_FP8, raw.w[i][0][1], raw.s[i]);
+                        const float sc = F16 ? raw.s[i] * (val ? fv_next : fk_next) : raw.s[i];
+                        const cross_f32x4 lo = cross_codes(a.dtype == AIR_KV_FP8, raw.w[i][0][0], sc);
+                        const cross_f32x4 hi = cross_codes(a.dtype == AIR_KV_FP8, raw.w[i][0][1], sc);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) { x[j] = lo[j]; x[4 + j] = hi[j]; }
                     }
@@ -333,7 +411,7 @@ void paged_cross_kernel(CrossArgs a) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint32_t p[KP];
-                        cross_parts<KP>(x[2 * j], x[2 * j + 1], p);
+                        cross_parts<F16, KP>(x[2 * j], x[2 * j + 1], p);
 #pragma unroll
                         for (int k = 0; k < KP; ++k) y[k][j] = p[k];
                     }
@@ -342,27 +420,67 @@ void paged_cross_kernel(CrossArgs a) {
                         if (p_in) *reinterpret_cast<cross_u32x4 *>(to + k * plane) = y[k];
                 }
             }
-            if (wave == 0 && lane < TK / 16) s_ok[t % NB][lane] = window >= 0;
+        };
+        // What comes between two tiles' products, t the one at hand: tile t + 1 into its buffer, t + 2
+        // on its way (kCodes with two buffers: t + 2 marked, t + 3 on its way).
+        auto stage = [&](int t) __attribute__((always_inline)) {
+            write_tile(t + 1);
+            if (t + 2 >= tiles) return;
+            if constexpr (F16 && NB == 2) {
+                raw = next;
+                if (t + 3 < tiles) {
+                    look_up(t + 3);
+                    load_tile(t + 3, next);
+                }
+                mark(t + 2, raw);
+            } else {
+                look_up(t + 2);
+                load_tile(t + 2, raw);
+            }
         };
 
-        __syncthreads();                               // the buffers of the block before are free
         fetch(0);
+        __syncthreads();                               // the buffers of the block before are free
+        if (F16 && tid < 6) s_top[tid / 2][tid % 2] = 0;
         look_up(0);
-        load_tile(0);
+        load_tile(0, raw);
+        if (F16 && NB == 2 && 1 < tiles) {
+            look_up(1);
+            load_tile(1, next);
+        }
+        if constexpr (F16) {
+            __syncthreads();
+            mark(0, raw);
+            __syncthreads();
+        }
         write_tile(0);
         if (1 < tiles) {
-            look_up(1);
-            load_tile(1);
+            if constexpr (F16 && NB == 2) {
+                raw = next;
+                if (2 < tiles) {
+                    look_up(2);
+                    load_tile(2, next);
+                }
+                mark(1, raw);
+            } else {
+                look_up(1);
+                load_tile(1, raw);
+            }
         }
         __syncthreads();
         for (int t = 0; t < tiles; ++t) {
-            if (NB == 2 && t + 1 < tiles) {
-                write_tile(t + 1);
-                if (t + 2 < tiles) {
-                    look_up(t + 2);
-                    load_tile(t + 2);
+            if constexpr (F16) {
+                // (a power of two that changes: the sums so far are brought under it)
+                fk = fk_next;
+                if (fv != fv_next) {
+                    const float by = fv == 0.0f ? 1.0f : fv_next / fv;
+#pragma unroll
+                    for (int c = 0; c < CT; ++c) acc[c] *= by;
+                    fv = fv_next;
                 }
+                if (tid < 2) s_top[t % 3][tid] = 0;
             }
+            if (NB == 2 && t + 1 < tiles) stage(t);
             if (any) {
                 const uint8_t *mem = s_mem + t % NB * S::TILE;
 #pragma unroll
@@ -383,11 +501,11 @@ void paged_cross_kernel(CrossArgs a) {
                         for (int i = 0; i < KP; ++i)
 #pragma unroll
                             for (int j = 0; j < QP; ++j)
-                                if (i + j < 3) sc = cross_mfma(kf[i], qf[j][s], sc);
+                                if (i + j < 3) sc = cross_mfma<F16>(kf[i], qf[j][s], sc);
                     }
                     // keys past the end and of blocks outside the pool
-                    const int ok0 = __builtin_amdgcn_readfirstlane(s_ok[t % NB][k0 / 16]);
-                    const int ok1 = __builtin_amdgcn_readfirstlane(s_ok[t % NB][k0 / 16 + 1]);
+                    const int ok0 = __builtin_amdgcn_readfirstlane(s_ok[t % 4][k0 / 16]);
+                    const int ok1 = __builtin_amdgcn_readfirstlane(s_ok[t % 4][k0 / 16 + 1]);
                     uint32_t mask = rest < 32 ? (1u << (int)rest) - 1 : ~0u;
                     mask &= (ok0 ? 0x0000FFFFu : 0u) | (ok1 ? 0xFFFF0000u : 0u);
                     if (mask != ~0u) {
@@ -395,7 +513,10 @@ void paged_cross_kernel(CrossArgs a) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) sc[i] = (m >> (8 * (i / 4) + i % 4)) & 1 ? sc[i] : -INFINITY;
                     }
+                    // (neither 0 nor infinite: a masked score, -inf, times 0 would be NaN, and so would 0 times
+                    // infinity)
                     float ft = a.scale_log2;
+                    if constexpr (F16) ft = fminf(fmaxf(__builtin_amdgcn_ldexpf(ft, -(qe + cross_exponent(fk))), 0x1p-126f), 0x1.fffffep127f);
                     float top = sc[0];
 #pragma unroll
                     for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
@@ -427,7 +548,7 @@ void paged_cross_kernel(CrossArgs a) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             uint32_t x[QP];
-                            cross_parts<QP>(sc[8 * s + 2 * j], sc[8 * s + 2 * j + 1], x);
+                            cross_parts<F16, QP>(sc[8 * s + 2 * j], sc[8 * s + 2 * j + 1], x);
 #pragma unroll
                             for (int k = 0; k < QP; ++k) p[k][s][j] = x[k];
                         }
@@ -453,23 +574,21 @@ void paged_cross_kernel(CrossArgs a) {
                                 const cross_u32x4 vf = {x[0], x[1], y[0], y[1]};
 #pragma unroll
                                 for (int j = 0; j < QP; ++j)
-                                    if (i + j < 3) acc[c] = cross_mfma(vf, p[j][s], acc[c]);
+                                    if (i + j < 3) acc[c] = cross_mfma<F16>(vf, p[j][s], acc[c]);
                             }
                 }
             }
+            if (NB == 1 && t + 1 < tiles) mark(t + 1, raw);
             __syncthreads();
             if (NB == 1 && t + 1 < tiles) {
-                write_tile(t + 1);
-                if (t + 2 < tiles) {
-                    look_up(t + 2);
-                    load_tile(t + 2);
-                }
+                stage(t);
                 __syncthreads();
             }
         }
 
         // lane (n, h): columns 32 c + 8 (i / 4) + 4 h + i % 4 of row n in acc[c][i]
         float l = cross_sum32(l_run);
+        const float unit = F16 && fv != 0.0f ? 1.0f / fv : 1.0f;       // of the sums (pieces' stay under it)
         const int64_t slot = 2 * cell + (t0 == 0 ? 1 : 0);
         const int64_t prow = slot * ROWS + 32 * rg + r32;
         if constexpr (WK == 1) {
@@ -480,12 +599,13 @@ void paged_cross_kernel(CrossArgs a) {
                 for (int c = 0; c < CT; ++c)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const cross_f32x4 x = {acc[c][4 * i] * k, acc[c][4 * i + 1] * k, acc[c][4 * i + 2] * k, acc[c][4 * i + 3] * k};
+                        cross_f32x4 x = cross_f32x4{acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]} * k;
+                        if (F16 && whole) x *= unit;
                         const int col = 32 * c + 8 * i + 4 * hf;
                         if (whole) cross_store4(a, io + col, x);
                         else *reinterpret_cast<cross_f32x4 *>(a.part_o + prow * D + col) = x;
                     }
-                if (!whole && hf == 0) a.part_ml[prow] = make_float2(base, l);
+                if (!whole && hf == 0) a.part_ml[prow] = make_float4(base, l, unit, 0.0f);
             }
         } else {
             // the waves of one row group: their bases' largest, then their sums, CR column tiles at a
@@ -518,15 +638,17 @@ void paged_cross_kernel(CrossArgs a) {
                     cross_f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int i = 0; i < WK; ++i) y += x[((rg * WK + i) * CR * 4 + g) * 64];
+                    y *= k;
+                    if (F16 && whole) y *= unit;
                     const int col = 32 * (c0 + g / 4) + 8 * (g % 4) + 4 * hf;
                     if (whole) {
-                        if (live) cross_store4(a, io + col, y * k);
+                        if (live) cross_store4(a, io + col, y);
                     } else if (any) {
                         *reinterpret_cast<cross_f32x4 *>(a.part_o + prow * D + col) = y;
                     }
                 }
             }
-            if (!whole && any && hf == 0 && wk == 0) a.part_ml[prow] = make_float2(top, l);
+            if (!whole && any && hf == 0 && wk == 0) a.part_ml[prow] = make_float4(top, l, unit, 0.0f);
         }
         if (!whole && t0 == 0) {                       // begun here: its last unit's slice ends it
             const int64_t last = u - mine - at + nt + kCrossExtra - 1;
@@ -536,11 +658,11 @@ void paged_cross_kernel(CrossArgs a) {
     if (tid == 0) a.desc[cell] = begun;
 }
 
-template <int QP, bool WIDE, bool FEW> hipError_t launch_cross_shape(const CrossArgs &a, int d, hipStream_t s) {
+template <CrossKind KIND, bool FEW> hipError_t launch_cross_shape(const CrossArgs &a, int d, hipStream_t s) {
     const dim3 grid((unsigned)(a.slices * a.heads));
     switch (d) {
 #define AIRKV_CROSS(D) \
-    case D: hipLaunchKernelGGL((paged_cross_kernel<D, WIDE, QP, FEW>), grid, dim3(CrossShape<D, WIDE, QP, FEW>::WAVES * 64), 0, s, a); break;
+    case D: hipLaunchKernelGGL((paged_cross_kernel<D, KIND, FEW>), grid, dim3(CrossShape<D, KIND, FEW>::WAVES * 64), 0, s, a); break;
         AIRKV_CROSS(32) AIRKV_CROSS(64) AIRKV_CROSS(96) AIRKV_CROSS(128)
         AIRKV_CROSS(160) AIRKV_CROSS(192) AIRKV_CROSS(224) AIRKV_CROSS(256)
 #undef AIRKV_CROSS
@@ -548,9 +670,9 @@ template <int QP, bool WIDE, bool FEW> hipError_t launch_cross_shape(const Cross
     return hipGetLastError();
 }
 
-template <int QP, bool WIDE, bool FEW> int cross_rows_shape(int d) {
+template <CrossKind KIND, bool FEW> int cross_rows_shape(int d) {
     switch (d) {
-#define AIRKV_CROSS(D) case D: return CrossShape<D, WIDE, QP, FEW>::ROWS;
+#define AIRKV_CROSS(D) case D: return CrossShape<D, KIND, FEW>::ROWS;
         AIRKV_CROSS(32) AIRKV_CROSS(64) AIRKV_CROSS(96) AIRKV_CROSS(128)
         AIRKV_CROSS(160) AIRKV_CROSS(192) AIRKV_CROSS(224) AIRKV_CROSS(256)
 #undef AIRKV_CROSS

@@ -465,8 +465,10 @@ int air_paged_diff_prefill(air_kv_pool *pool, void *stream, const void *q, int32
  * all of a sequence's: zeros).  Rows of different sequences must not overlap.
  *
  * Scores, sums and outputs are held in 32 bits.  bf16 queries with bf16 outputs on
- * BF16, INT8 and FP8 pools take products of bf16 values (probabilities, and the
- * keys and values of 1-byte pages, rounded once); everything else keeps f32
+ * BF16 pools round probabilities to bf16; on INT8 and FP8 pools they round
+ * probabilities, keys and values to 11 bits, and no finer than 2^-35 of a row's
+ * largest probability, 2^-37 of the largest key of its 32 to 256 neighbours and
+ * of the largest value so far.  Everything else keeps f32
  * precision, where what lies below 2^-133 of an f32 or 1-byte page's value is cut
  * off.  Probabilities below 2^-98 of a row's largest count as 0, and so may what
  * values below 2^-98 add.  Keys and values that are not finite give NaN where they reach.

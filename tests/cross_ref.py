@@ -27,7 +27,8 @@ def values(pool, snapshot, scale_group, fp8_table):
 def cross(q, cu, k, v, tables, lens, scale, bs, precise, rounded_pages, out_type):
     """(out, bound) for rows q [rows, heads, d] in 64 bits; out is NaN and bound infinite for rows of no sequence.
 
-    precise: f32 precision, else products of bf16 values; rounded_pages: those of 1-byte pages, rounded to bf16.
+    precise: f32 precision, else probabilities rounded to bf16; rounded_pages: those of 1-byte pages, rounded to f32
+    or, with their probabilities, to f16.
     The bound: a score errs by what its products and their sum do, a probability by that times two (its own score
     and the row's sum) and its rounding, an output by its probabilities', its values' and its sum's errors, and by its
     own rounding."""
@@ -36,7 +37,7 @@ def cross(q, cu, k, v, tables, lens, scale, bs, precise, rounded_pages, out_type
     g = heads // kv
     out = torch.full(q.shape, math.nan, dtype=torch.float64)
     bound = torch.full(q.shape, math.inf, dtype=torch.float64)
-    u = HALF_STEP["bf16"]
+    u = 2.0 ** -11 if rounded_pages else HALF_STEP["bf16"]
     f = 2.0 ** -24
     # products that are left out of two split values (their parts are below 2^-7 and 2^-15 of them)
     split = 2.0 ** -21 if precise else 0.0

@@ -185,8 +185,33 @@ def test_large_values(dtype, io):
     small = torch.randn(c.pool.num_blocks * 16, 1, 64, device="cuda")
     c.pool.append(small, big, torch.arange(c.pool.num_blocks * 16, device="cuda"))
     for hint in (1, 33):
-        out = c.call(max_q_len=hint)
-        assert torch.isfinite(out).all() and ((out / 3.0e38 - 1).abs() < 2.0 ** -7).all()
+        for c.out in (c.out, torch.empty_like(c.out, dtype=torch.bfloat16)):
+            out = c.call(max_q_len=hint).float()
+            assert torch.isfinite(out).all() and ((out / 3.0e38 - 1).abs() < 2.0 ** -7).all()
+
+
+@pytest.mark.parametrize("dtype", [airkv.INT8, airkv.FP8])
+@pytest.mark.parametrize("k_size,v_size", [(1.0, 1.0), (1e20, 1e30), (1e-20, 1e-30), (3e4, 3e-5), (1.0, 3e36), (1e-30, 1e-36)])
+def test_codes_of_many_sizes(dtype, k_size, v_size):
+    """16-bit products over 1-byte pages: tokens whose keys and values differ by powers of two, in
+    units far from 1, rows of queries too; a token of zeros."""
+    torch = torch_mod()
+    c = Case(dtype, 64, 2, 2, 16, [700, 33, 9], [33, 3, 1], seed=11)
+    n = c.pool.num_blocks * 16
+    gen = torch.Generator(device="cuda").manual_seed(3)
+
+    def rows(size, lo, hi):
+        x = torch.randn(n, 2, 64, generator=gen, device="cuda")
+        return x * torch.exp2(torch.randint(lo, hi + 1, (n, 1, 1), generator=gen, device="cuda").float()) * size
+    k, v = rows(k_size, -9, 1), rows(v_size, -8, 4)
+    k[5] = 0.0
+    v[6] = 0.0
+    c.pool.append(k, v, torch.arange(n, device="cuda"))
+    c.q = (c.q.float() * torch.exp2(torch.arange(len(c.q), device="cuda").float() % 13 - 9)[:, None, None]).bfloat16()
+    scale = c.scale / k_size
+    for hint in (1, 33):
+        c.out.fill_(7.0)
+        c.check(f"hint {hint}", scale=scale, max_q_len=hint)
 
 
 def test_not_finite():
