@@ -15,77 +15,120 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kMergeThreads = 256;
 
-// The rows of one cut block: a row's pieces folded in order, four columns a lane.
-template <int LANES>
+// A mean of values and its weight l under `base`: what a row's pieces are folded to.  (A mean stays
+// within its values' range, where a sum of values near the largest or the smallest floats would not.)
+struct Fold {
+    float base, l;
+    f32x4 o;
+    __device__ __forceinline__ void add(float b, float w, f32x4 mean) {
+        if (w == 0.0f) return;                         // (no key in the pool)
+        const float top = fmaxf(base, b);
+        const float was = base == top ? l : l * __builtin_amdgcn_exp2f(base - top);
+        const float is = b == top ? w : w * __builtin_amdgcn_exp2f(b - top);
+        l = was + is;
+        const float k = 1.0f / l;
+        o = o * (was * k) + mean * (is * k);
+        base = top;
+    }
+};
+
+// The rows of one cut block, rows blockIdx.x, + gridDim.x, ... : LANES lanes of four columns fold
+// every GROUPS-th piece, then the groups' results, in order.
+template <int LANES, int GROUPS>
 __global__ __launch_bounds__(kMergeThreads) void cross_merge_kernel(CrossArgs a, int rows, int d) {
+    constexpr int PER = kMergeThreads / (LANES * GROUPS);      // rows at a time
     const int64_t cell = (int64_t)blockIdx.z * a.slices + blockIdx.y;
     const int4 it = a.desc[cell];
     if (it.z == 0) return;
-    const int r = blockIdx.x * (kMergeThreads / LANES) + threadIdx.x / LANES, col = threadIdx.x % LANES * 4;
+    __shared__ f32x4 s_o[GROUPS][kMergeThreads / GROUPS];
+    __shared__ float2 s_bl[GROUPS][kMergeThreads / GROUPS];
+    const int lane = threadIdx.x % LANES, g = threadIdx.x / LANES % GROUPS, pr = threadIdx.x / (LANES * GROUPS);
+    const int col = lane * 4, place = pr * LANES + lane;
     const int32_t r0 = a.cu[it.x];
-    const int32_t row = it.y * rows + r;
-    if (row >= (a.cu[it.x + 1] - r0) * a.group || col >= d) return;
-    // the mean of the values so far, its weight l under `base` (a mean stays within its values' range,
-    // where a sum of values near the largest or the smallest floats would not)
-    float base = -INFINITY, l = 0.0f;
-    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int kBatch = 4;
-    for (int p0 = 0; p0 < it.z; p0 += kBatch) {
-        float4 ml[kBatch];
-        f32x4 x[kBatch];
+    const int32_t here = (a.cu[it.x + 1] - r0) * a.group - it.y * rows;        // rows of the block
+    const int many = here < rows ? here : rows;
+    for (int first = blockIdx.x * PER; first < many; first += gridDim.x * PER) {
+        const int r = first + pr;
+        const bool mine = r < many && col < d;
+        Fold f = {-INFINITY, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
+        if (mine) {
+            constexpr int kBatch = 4;
+            for (int p0 = g; p0 < it.z; p0 += kBatch * GROUPS) {
+                float4 ml[kBatch];
+                f32x4 x[kBatch];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int p = p0 + i < it.z ? p0 + i : p0;
-            const int64_t at = (2 * (cell + p) + (p == 0 ? 1 : 0)) * rows + r;
-            ml[i] = a.part_ml[at];
-            x[i] = *reinterpret_cast<const f32x4 *>(a.part_o + at * d + col);
-        }
+                for (int i = 0; i < kBatch; ++i) {
+                    const int p = p0 + i * GROUPS < it.z ? p0 + i * GROUPS : p0;
+                    const int64_t at = (2 * (cell + p) + (p == 0 ? 1 : 0)) * rows + r;
+                    ml[i] = a.part_ml[at];
+                    x[i] = *reinterpret_cast<const f32x4 *>(a.part_o + at * d + col);
+                }
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            // (a piece without a key in the pool has sum 0)
-            if (p0 + i >= it.z || ml[i].y == 0.0f) continue;
-            const float top = fmaxf(base, ml[i].x);
-            const float was = base == top ? l : l * __builtin_amdgcn_exp2f(base - top);
-            const float is = ml[i].x == top ? 1.0f : __builtin_amdgcn_exp2f(ml[i].x - top);
-            l = was + ml[i].y * is;
-            const float k = 1.0f / l;
-            o = o * (was * k) + x[i] * (is * k) * ml[i].z;
-            base = top;
+                for (int i = 0; i < kBatch; ++i)
+                    if (p0 + i * GROUPS < it.z) f.add(ml[i].x, ml[i].y, x[i] * (1.0f / ml[i].y) * ml[i].z);
+            }
         }
+        if constexpr (GROUPS > 1) {
+            s_o[g][place] = f.o;
+            s_bl[g][place] = make_float2(f.base, f.l);
+            __syncthreads();
+            if (g == 0) {
+                f = {-INFINITY, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
+                for (int i = 0; i < GROUPS; ++i) f.add(s_bl[i][place].x, s_bl[i][place].y, s_o[i][place]);
+            }
+            __syncthreads();
+        }
+        if (!mine || g) continue;
+        const int32_t row = it.y * rows + r;
+        const int64_t at = ((int64_t)(r0 + row / a.group) * a.q_heads + blockIdx.z * a.group + row % a.group) * d + col;
+        if (a.out_dtype == AIR_KV_F32)
+            *reinterpret_cast<f32x4 *>((float *)a.out + at) = f.o;
+        else
+            *reinterpret_cast<u32x2 *>((uint16_t *)a.out + at) = u32x2{(uint32_t)bf16_rne(f.o[0]) | ((uint32_t)bf16_rne(f.o[1]) << 16),
+                                                                       (uint32_t)bf16_rne(f.o[2]) | ((uint32_t)bf16_rne(f.o[3]) << 16)};
     }
-    const int64_t at = ((int64_t)(r0 + row / a.group) * a.q_heads + blockIdx.z * a.group + row % a.group) * d + col;
-    if (a.out_dtype == AIR_KV_F32)
-        *reinterpret_cast<f32x4 *>((float *)a.out + at) = o;
-    else
-        *reinterpret_cast<u32x2 *>((uint16_t *)a.out + at) = u32x2{(uint32_t)bf16_rne(o[0]) | ((uint32_t)bf16_rne(o[1]) << 16),
-                                                                   (uint32_t)bf16_rne(o[2]) | ((uint32_t)bf16_rne(o[3]) << 16)};
 }
 
-hipError_t launch_merge(const CrossArgs &a, int rows, int d, hipStream_t s) {
+// few: blocks of at most `most` rows, of which each takes a workgroup (sequences of many pieces).
+hipError_t launch_merge(const CrossArgs &a, CrossBlocks blocks, int d, bool few, int64_t most, hipStream_t s) {
     if (a.slices < 2) return hipSuccess;               // nothing is cut
     const int lanes = d <= 32 ? 8 : d <= 64 ? 16 : d <= 128 ? 32 : 64;
-    const int per = kMergeThreads / lanes;
-    const dim3 grid((unsigned)((rows + per - 1) / per), (unsigned)a.slices, (unsigned)a.heads);
-    if (lanes == 8) hipLaunchKernelGGL(cross_merge_kernel<8>, grid, dim3(kMergeThreads), 0, s, a, rows, d);
-    else if (lanes == 16) hipLaunchKernelGGL(cross_merge_kernel<16>, grid, dim3(kMergeThreads), 0, s, a, rows, d);
-    else if (lanes == 32) hipLaunchKernelGGL(cross_merge_kernel<32>, grid, dim3(kMergeThreads), 0, s, a, rows, d);
-    else hipLaunchKernelGGL(cross_merge_kernel<64>, grid, dim3(kMergeThreads), 0, s, a, rows, d);
+    const int per = few ? 1 : kMergeThreads / lanes;
+    const int64_t rows = few ? std::min<int64_t>(std::max<int64_t>(most, 1), blocks.rows) : blocks.rows;
+    const dim3 grid((unsigned)((rows + per - 1) / per), (unsigned)a.slices, (unsigned)a.heads), threads(kMergeThreads);
+    if (few) {
+        if (lanes == 8) hipLaunchKernelGGL((cross_merge_kernel<8, 32>), grid, threads, 0, s, a, blocks.rows, d);
+        else if (lanes == 16) hipLaunchKernelGGL((cross_merge_kernel<16, 16>), grid, threads, 0, s, a, blocks.rows, d);
+        else if (lanes == 32) hipLaunchKernelGGL((cross_merge_kernel<32, 8>), grid, threads, 0, s, a, blocks.rows, d);
+        else hipLaunchKernelGGL((cross_merge_kernel<64, 4>), grid, threads, 0, s, a, blocks.rows, d);
+    } else {
+        if (lanes == 8) hipLaunchKernelGGL((cross_merge_kernel<8, 1>), grid, threads, 0, s, a, blocks.rows, d);
+        else if (lanes == 16) hipLaunchKernelGGL((cross_merge_kernel<16, 1>), grid, threads, 0, s, a, blocks.rows, d);
+        else if (lanes == 32) hipLaunchKernelGGL((cross_merge_kernel<32, 1>), grid, threads, 0, s, a, blocks.rows, d);
+        else hipLaunchKernelGGL((cross_merge_kernel<64, 1>), grid, threads, 0, s, a, blocks.rows, d);
+    }
     return hipGetLastError();
 }
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-int rows_of(const air_kv_pool &p, bool half, bool few) {
-    return half ? cross_rows_16(p.desc.head_dim, few) : cross_rows_f32(p.desc.head_dim, few, p.desc.dtype != AIR_KV_BF16);
+CrossBlocks blocks_of(const air_kv_pool &p, bool half, bool few) {
+    return half ? cross_blocks_16(p.desc.head_dim, p.desc.dtype != AIR_KV_BF16, few)
+                : cross_blocks_f32(p.desc.head_dim, p.desc.dtype != AIR_KV_BF16, few);
 }
 
-// Slices per K/V head: the CUs' share; one workgroup is resident on a CU.
-int slices_of(const air_kv_pool &p) { return std::max(1, p.cus / p.desc.n_kv_heads); }
+// Slices per K/V head: its share of the workgroups that are resident.
+int slices_of(const air_kv_pool &p, CrossBlocks blocks) { return std::max(1, p.cus * blocks.groups / p.desc.n_kv_heads); }
 
-size_t bytes_of(const air_kv_pool &p, int rows) {
-    const size_t cells = (size_t)p.desc.n_kv_heads * slices_of(p), slots = 2 * cells * rows;
-    return align256(cells * sizeof(int4)) + align256(slots * sizeof(float4)) + slots * p.desc.head_dim * 4;
-}
+struct Workspace {
+    size_t ml, o, bytes;           // where the pieces' parts begin, and its end
+    Workspace(const air_kv_pool &p, CrossBlocks blocks) {
+        const size_t cells = (size_t)p.desc.n_kv_heads * slices_of(p, blocks), slots = 2 * cells * blocks.rows;
+        ml = align256(cells * sizeof(int4));
+        o = ml + align256(slots * sizeof(float4));
+        bytes = o + slots * p.desc.head_dim * 4;
+    }
+};
 
 }  // namespace
 
@@ -93,7 +136,7 @@ size_t cross_workspace(const air_kv_pool &p) {
     size_t most = 0;
     for (int half = 0; half < 2; ++half)
         for (int few = 0; few < 2; ++few)
-            if (!half || p.desc.dtype != AIR_KV_F32) most = std::max(most, bytes_of(p, rows_of(p, half, few)));
+            if (!half || p.desc.dtype != AIR_KV_F32) most = std::max(most, Workspace(p, blocks_of(p, half, few)).bytes);
     return most;
 }
 
@@ -102,10 +145,11 @@ hipError_t launch_cross(const air_kv_pool &p, hipStream_t s, const void *q, int3
                         int32_t max_blocks, float scale, void *workspace, void *out, int32_t out_dtype) {
     const bool half = p.desc.dtype != AIR_KV_F32 && q_dtype == AIR_KV_BF16 && out_dtype == AIR_KV_BF16;
     const int d = p.desc.head_dim, group = n_q_heads / p.desc.n_kv_heads;
-    const int64_t most = (int64_t)(max_q_len ? max_q_len : (total_q + batch - 1) / batch) * group;
+    const int64_t most = (int64_t)(max_q_len ? max_q_len : ((int64_t)total_q + batch - 1) / batch) * group;
     // rows of one wave: its keys go to the others
     const bool few = most <= 32;
-    const int rows = rows_of(p, half, few);
+    const CrossBlocks blocks = blocks_of(p, half, few);
+    const Workspace ws(p, blocks);
     CrossArgs a{};
     a.q = q;
     a.out = out;
@@ -126,22 +170,18 @@ hipError_t launch_cross(const air_kv_pool &p, hipStream_t s, const void *q, int3
     a.k_scales = p.k_scales;
     a.v_scales = p.v_scales;
     a.errors = p.errors;
-    a.slices = slices_of(p);
+    a.slices = slices_of(p, blocks);
     a.least = 3;
-    const size_t cells = (size_t)a.heads * a.slices, slots = 2 * cells * rows;
-    char *ws = (char *)workspace;
-    a.desc = (int4 *)ws;
-    ws += align256(cells * sizeof(int4));
-    a.part_ml = (float4 *)ws;
-    ws += align256(slots * sizeof(float4));
-    a.part_o = (float *)ws;
+    a.desc = (int4 *)workspace;
+    a.part_ml = (float4 *)((char *)workspace + ws.ml);
+    a.part_o = (float *)((char *)workspace + ws.o);
     for (int32_t b0 = 0; b0 < batch; b0 += kCrossBatch) {
         a.batch = std::min(batch - b0, kCrossBatch);
         a.cu = cu + b0;
         a.tables = tables + (int64_t)b0 * max_blocks;
         a.lens = lens + b0;
         hipError_t e = half ? launch_cross_16(a, d, few, s) : launch_cross_f32(a, d, few, s);
-        if (e == hipSuccess) e = launch_merge(a, rows, d, s);
+        if (e == hipSuccess) e = launch_merge(a, blocks, d, few, most, s);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;

@@ -17,7 +17,7 @@
 
 namespace airkv {
 
-constexpr int kCrossBatch = 1024;      // sequences per launch (the host splits larger batches)
+constexpr int kCrossBatch = 512;       // sequences per launch (the host splits larger batches)
 constexpr int kCrossExtra = 1;
 
 struct CrossArgs {
@@ -64,10 +64,13 @@ template <int ROWS, int TK> __device__ __forceinline__ int64_t cross_units(const
     return tiles ? ((int64_t)s.rows + ROWS - 1) / ROWS * (tiles + kCrossExtra) : 0;
 }
 
+// Rows of a block, and workgroups that are resident on a CU.
+struct CrossBlocks {
+    int rows, groups;
+};
+CrossBlocks cross_blocks_16(int head_dim, bool codes, bool few);
+CrossBlocks cross_blocks_f32(int head_dim, bool wide, bool few);
 hipError_t launch_cross_16(const CrossArgs &a, int head_dim, bool few, hipStream_t s);
 hipError_t launch_cross_f32(const CrossArgs &a, int head_dim, bool few, hipStream_t s);
-// Rows of a block of these kernels.
-int cross_rows_16(int head_dim, bool few);
-int cross_rows_f32(int head_dim, bool few, bool wide);
 
 }  // namespace airkv

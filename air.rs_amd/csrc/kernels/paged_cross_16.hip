@@ -9,9 +9,9 @@ hipError_t launch_cross_16(const CrossArgs &a, int head_dim, bool few, hipStream
     return few ? launch_cross_shape<kCodes, true>(a, head_dim, s) : launch_cross_shape<kCodes, false>(a, head_dim, s);
 }
 
-int cross_rows_16(int head_dim, bool few) {
-    // (both kinds stage two bytes an element: the same shape)
-    return few ? cross_rows_shape<kBf16, true>(head_dim) : cross_rows_shape<kBf16, false>(head_dim);
+CrossBlocks cross_blocks_16(int head_dim, bool codes, bool few) {
+    if (codes) return few ? cross_blocks_shape<kCodes, true>(head_dim) : cross_blocks_shape<kCodes, false>(head_dim);
+    return few ? cross_blocks_shape<kBf16, true>(head_dim) : cross_blocks_shape<kBf16, false>(head_dim);
 }
 
 }  // namespace airkv

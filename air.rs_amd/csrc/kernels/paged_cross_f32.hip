@@ -9,9 +9,9 @@ hipError_t launch_cross_f32(const CrossArgs &a, int head_dim, bool few, hipStrea
     return few ? launch_cross_shape<kWide, true>(a, head_dim, s) : launch_cross_shape<kWide, false>(a, head_dim, s);
 }
 
-int cross_rows_f32(int head_dim, bool few, bool wide) {
-    if (wide) return few ? cross_rows_shape<kWide, true>(head_dim) : cross_rows_shape<kWide, false>(head_dim);
-    return few ? cross_rows_shape<kParts, true>(head_dim) : cross_rows_shape<kParts, false>(head_dim);
+CrossBlocks cross_blocks_f32(int head_dim, bool wide, bool few) {
+    if (wide) return few ? cross_blocks_shape<kWide, true>(head_dim) : cross_blocks_shape<kWide, false>(head_dim);
+    return few ? cross_blocks_shape<kParts, true>(head_dim) : cross_blocks_shape<kParts, false>(head_dim);
 }
 
 }  // namespace airkv

@@ -13,18 +13,20 @@
 //   kParts  f32 precision over bf16 pages, kWide over f32 and 1-byte ones: bf16 parts that hold all
 //           24 bits, of queries and probabilities and (kWide) of keys and values; products with
 //           i + j < 3 are formed
-// Keys and values are staged in LDS as rows, 16 (keys) and 64 (values) bytes apart modulo 256, so
-// that neither the rows' reads nor the values' transposing reads meet in a bank; a tile is
-// loaded two ahead into registers and staged one ahead where two buffers fit.
+// Keys and values are staged in LDS as rows, padded or their 16-byte chunks placed so that neither
+// the rows' reads nor the values' transposing reads meet in a bank.
 //
-// WK waves share 32 rows and take a tile's keys in turn (few rows), or each wave has rows of its
-// own (WK = 1).
+// Many rows (WK = 1): each wave has 32 rows of its own and all take the same keys; a tile is
+// loaded two ahead into registers and staged one ahead where two buffers fit.  Few rows: WK waves
+// share 32 rows and each takes 32 keys of a tile.  Where all of a workgroup's waves do, each stages
+// its own keys, and none waits for another until the block ends (PRIVATE).
 #pragma once
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include "codecs.hpp"
+#include "decode_slices.hpp"
 #include "paged_cross.hpp"
 
 namespace airkv {
@@ -41,24 +43,30 @@ typedef uint32_t cross_u32x2 __attribute__((ext_vector_type(2)));
 
 enum CrossKind { kBf16, kCodes, kParts, kWide };
 
-constexpr int kCrossLds = 149 * 1024;              // of a CU's 160 KB, for the tiles
 constexpr int kCrossBuffer = 0x00020000;           // a raw buffer's last word
 constexpr int kCrossNowhere = 0x40000000;          // an offset outside of every buffer: reads zeros
 
-// Rows of keys and of values in LDS, bytes apart.
+// Rows of keys and of values in LDS, bytes apart.  Keys: 16 bytes more than a whole number of
+// 256, or as good.  Values are read four rows at a time, 64 bytes of each: where a row is a whole
+// number of 256 bytes, the chunks of row r are placed 64 (r % 4) bytes away (exclusive or).
 constexpr int cross_k_stride(int d) { return 2 * d + 16; }
-constexpr int cross_v_stride(int d) { return 2 * d + (2 * d / 64 % 2 ? 0 : 64); }
+constexpr bool cross_v_xor(int d) { return 2 * d % 256 == 0; }
+constexpr int cross_v_stride(int d) { return cross_v_xor(d) || 2 * d / 64 % 2 ? 2 * d : 2 * d + 64; }
 constexpr int cross_tile_bytes(int d, int parts, int keys) { return keys * parts * (cross_k_stride(d) + cross_v_stride(d)); }
-// Waves of a workgroup: queries in three parts and their sums leave room for one wave a SIMD.
-constexpr int cross_waves(int d, int qp) { return qp == 3 && d >= 96 ? 4 : 8; }
+// Waves of a workgroup, and workgroups a CU: registers leave room for four waves a SIMD (small
+// heads), two, or (queries in three parts and their sums, the largest heads) one.
+constexpr int cross_waves(int d, int qp, bool few) { return few || (qp == 3 ? d >= 96 : d >= 192) ? 4 : 8; }
+constexpr int cross_groups(int d, int qp, bool few) { return few ? (d <= (qp == 3 ? 64 : 128) ? 2 : 1) : qp == 1 && d <= 64 ? 2 : 1; }
+// What a workgroup's tiles may take of a CU's 160 KB.
+constexpr int cross_lds(int groups) { return 160 * 1024 / groups - 7 * 1024; }
 // Waves that share rows: as many as have room for 32 keys each.
 constexpr int cross_wk(int d, int kp, int qp, bool few) {
-    int wk = few ? cross_waves(d, qp) : 1;
-    while (wk > 1 && cross_tile_bytes(d, kp, 32 * wk) > kCrossLds) wk /= 2;
+    int wk = few ? cross_waves(d, qp, few) : 1;
+    while (wk > 1 && cross_tile_bytes(d, kp, 32 * wk) > cross_lds(1)) wk /= 2;
     return wk;
 }
 // Keys of a tile that one wave takes, in 32s.
-constexpr int cross_sub(int d, int kp, int wk) { return wk == 1 && cross_tile_bytes(d, kp, 64) <= kCrossLds ? 2 : 1; }
+constexpr int cross_sub(int d, int kp, int wk) { return wk == 1 && cross_tile_bytes(d, kp, 64) <= cross_lds(1) ? 2 : 1; }
 
 template <bool F16> __device__ __forceinline__ cross_f32x16 cross_mfma(cross_u32x4 a, cross_u32x4 b, cross_f32x16 c) {
     if constexpr (F16)
@@ -90,6 +98,16 @@ template <bool F16, int P> __device__ __forceinline__ void cross_parts(float x, 
 // 2^e, e clamped to the normal numbers; the exponent of a normal number.
 __device__ __forceinline__ float cross_pow2(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 __device__ __forceinline__ int cross_exponent(float x) { return (int)((__float_as_uint(x) >> 23) & 0xFF) - 127; }
+// The sum of a pair and c; ones: cross_ones (an inline constant would not be read as a pair).
+template <bool F16> __device__ __forceinline__ uint32_t cross_ones() {
+    uint32_t x = F16 ? 0x3C003C00u : 0x3F803F80u;
+    asm("" : "+s"(x));
+    return x;
+}
+template <bool F16> __device__ __forceinline__ float cross_add_pair(uint32_t p, uint32_t ones, float c) {
+    if constexpr (F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(cross_f16x2, p), __builtin_bit_cast(cross_f16x2, ones), c, false);
+    else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(cross_bf16x2, p), __builtin_bit_cast(cross_bf16x2, ones), c, false);
+}
 // The values of the four 1-byte codes in w times their scale.
 __device__ __forceinline__ cross_f32x4 cross_codes(bool fp8, uint32_t w, float s) {
     if (fp8) {
@@ -98,14 +116,9 @@ __device__ __forceinline__ cross_f32x4 cross_codes(bool fp8, uint32_t w, float s
     }
     return cross_f32x4{(float)(int8_t)w * s, (float)(int8_t)(w >> 8) * s, (float)(int8_t)(w >> 16) * s, (float)(int8_t)(w >> 24) * s};
 }
-// Over lanes l and l ^ 32.
-__device__ __forceinline__ float cross_max32(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float cross_sum32(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+// The largest of the wave's lanes' x >= 0.
+__device__ __forceinline__ float cross_wave_max(float x) {
+    return __uint_as_float(__builtin_amdgcn_readlane(wave_scan((int)__float_as_uint(x), [](int a, int b) { return a > b ? a : b; }), 63));
 }
 __device__ __forceinline__ int64_t cross_uniform(int64_t x) {
     const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
@@ -120,25 +133,30 @@ __device__ __forceinline__ void cross_store4(const CrossArgs &a, int64_t at, cro
 template <int D, CrossKind KIND, bool FEW>
 struct CrossShape {
     static constexpr int KP = KIND == kWide ? 3 : 1, QP = KIND == kParts || KIND == kWide ? 3 : 1;
-    static constexpr int WAVES = cross_waves(D, QP), WK = cross_wk(D, KP, QP, FEW), SUB = cross_sub(D, KP, WK);
+    static constexpr int WAVES = cross_waves(D, QP, FEW), WK = cross_wk(D, KP, QP, FEW), SUB = cross_sub(D, KP, WK);
+    static constexpr bool PRIVATE = FEW && WK == WAVES;
     static constexpr int ROWS = 32 * (WAVES / WK), TK = 32 * WK * SUB;
-    static constexpr int TILE = cross_tile_bytes(D, KP, TK), NB = 2 * TILE <= kCrossLds ? 2 : 1;
+    static constexpr int TILE = cross_tile_bytes(D, KP, TK);
+    static constexpr int GROUPS = cross_groups(D, QP, FEW) == 2 && TILE <= cross_lds(2) ? 2 : 1;
+    static constexpr int NB = !PRIVATE && 2 * TILE <= cross_lds(GROUPS) ? 2 : 1;
+    static constexpr int WAVES_SIMD = WAVES / 4 * GROUPS;
 };
 
 template <int D, CrossKind KIND, bool FEW>
 __global__ __launch_bounds__((CrossShape<D, KIND, FEW>::WAVES * 64))
-__attribute__((amdgpu_waves_per_eu(CrossShape<D, KIND, FEW>::WAVES / 4, CrossShape<D, KIND, FEW>::WAVES / 4)))
+__attribute__((amdgpu_waves_per_eu(CrossShape<D, KIND, FEW>::WAVES_SIMD, CrossShape<D, KIND, FEW>::WAVES_SIMD)))
 void paged_cross_kernel(CrossArgs a) {
     typedef CrossShape<D, KIND, FEW> S;
-    constexpr bool F16 = KIND == kCodes;
+    constexpr bool F16 = KIND == kCodes, PRIVATE = S::PRIVATE;
     constexpr int KP = S::KP, QP = S::QP, WAVES = S::WAVES, WK = S::WK, SUB = S::SUB, ROWS = S::ROWS, TK = S::TK, NB = S::NB, THREADS = 64 * WAVES;
     constexpr int KST = cross_k_stride(D), VST = cross_v_stride(D);
     constexpr int KPLANE = TK * KST, VPLANE = TK * VST, VAT = KP * KPLANE;    // a part's rows; where values begin
     constexpr int KS = D / 16, CT = D / 32;            // steps of the first product, 32-column tiles of the second
-    // Staging: a wave's pass covers WR rows of one 16-key half of the keys or the values, LPR
-    // lanes a row (a power of two: some idle where D / 8 is none), 8 elements a lane.
-    constexpr int LPR = D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32, WR = 64 / LPR, NP = 2 * TK / (WAVES * WR);
-    static_assert(NP >= 1 && 2 * TK % (WAVES * WR) == 0 && TK % WR == 0, "whole passes");
+    // Staging: a wave takes SH of the tile's 16-key halves of keys or values, WR rows a pass, LPR lanes
+    // a row (a power of two: some idle where D / 8 is none), 8 elements a lane.
+    constexpr int LPR = D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32, WR = 64 / LPR, NPH = 16 / WR;
+    constexpr int SH = 2 * TK / 16 / WAVES, NP = SH * NPH;
+    static_assert(SH >= 1 && SH * WAVES * 16 == 2 * TK && (SH == 1 || SH % 2 == 0), "whole halves");
     constexpr int JOIN = WAVES * 64 * 16 * 4;          // bytes of a column tile of every wave's sums, at a block's end
     constexpr int MEM = NB * S::TILE > JOIN || WK == 1 ? NB * S::TILE : JOIN;
     constexpr int CR = MEM / JOIN < CT ? MEM / JOIN : CT;      // column tiles joined at once (WK > 1)
@@ -146,7 +164,7 @@ void paged_cross_kernel(CrossArgs a) {
     __shared__ int64_t s_sum[WAVES];
     __shared__ int32_t s_ok[4][TK / 16];               // whether a tile's 16-key halves are in the pool
     __shared__ uint32_t s_top[3][2];                   // a tile's largest scale of keys and of values, as bits
-    __shared__ float2 s_ml[WAVES][32];
+    __shared__ float4 s_ml[WAVES][32];
     __shared__ __align__(16) uint8_t s_mem[MEM];
 
     const int tid = threadIdx.x, lane = tid & 63, hf = lane >> 5, r32 = lane & 31;
@@ -204,13 +222,21 @@ void paged_cross_kernel(CrossArgs a) {
     int4 begun = {0, 0, 0, 0};
 
     // this lane's place in every pass
-    const int p_c = lane % LPR, p_row0 = wave * WR;    // (of pass 0, among keys' and values' 2 TK rows)
+    const int p_c = lane % LPR;
     const bool p_in = p_c < D / 8;
     const int esize = KIND == kCodes ? 1 : KIND != kWide ? 2 : a.dtype == AIR_KV_F32 ? 4 : 1;
     const int p_off = p_in ? (lane / LPR * D + 8 * p_c) * esize : kCrossNowhere;
     const int nsc = KIND == kCodes || (KIND == kWide && a.dtype != AIR_KV_F32) ? D >> a.sg_log2 : 0;
     const int p_sc = p_in ? (lane / LPR * nsc + (8 * p_c >> a.sg_log2)) * 4 : kCrossNowhere;
 
+    // half j of this wave's: of values (else keys), and which of the tile's
+    auto of_values = [&](int j) __attribute__((always_inline)) { return SH == 1 ? wave >= WAVES / 2 : j >= SH / 2; };
+    auto half_of = [&](int j) __attribute__((always_inline)) { return SH == 1 ? wave % (WAVES / 2) : wave * (SH / 2) + j % (SH / 2); };
+
+    const uint32_t ones = cross_ones<F16>();
+    // A SIMD has waves i and i + 4 of a workgroup: the second goes first, so that the two get out of
+    // phase and one's products run beside the other's arithmetic.
+    if (!FEW && wave >= 4) __builtin_amdgcn_s_setprio(1);
     int b = 0;
     if (u < end) {
         int lo = 0, hi = a.batch;
@@ -282,7 +308,7 @@ void paged_cross_kernel(CrossArgs a) {
                 for (int j = 0; j < 4; ++j)
                     top = fmaxf(top, fmaxf(__builtin_fabsf(__uint_as_float(qf[0][s][j] << 16)),
                                            __builtin_fabsf(__uint_as_float(qf[0][s][j] & 0xFFFF0000u))));
-            const float fq = cross_pow2(4 - cross_exponent(cross_max32(top)));
+            const float fq = cross_pow2(4 - cross_exponent(max_x32(top)));
             qe = cross_exponent(fq);
 #pragma unroll
             for (int s = 0; s < KS; ++s)
@@ -322,76 +348,79 @@ void paged_cross_kernel(CrossArgs a) {
                 const int n = __popcll(__ballot(out && (key & ((1 << a.bs_log2) - 1)) == 0));
                 if (n && lane == 0) atomicAdd(a.errors, (unsigned long long)n);
             }
-            if (wave == 0 && lane < TK / 16) s_ok[t % 4][lane] = window >= 0;
+            if (!PRIVATE && wave == 0 && lane < TK / 16) s_ok[t % 4][lane] = window >= 0;
             fetch(t + 1);
         };
         auto load_tile = [&](int t, Raw &raw) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const int r = p_row0 + i * WAVES * WR, val = r / TK, at = r % TK;            // (of the wave)
-                const int32_t e = __builtin_amdgcn_readlane(window, at / 16);
-                const int64_t rest = sq.len - (key0 + (int64_t)t * TK + at);
-                const int have = e < 0 || rest <= 0 ? 0 : rest < WR ? (int)rest : WR;
-                const int64_t prow = (((int64_t)(e < 0 ? 0 : e) * a.heads + head) << a.bs_log2) + (at & ((1 << a.bs_log2) - 1));
+            for (int j = 0; j < SH; ++j) {
+                const int half = half_of(j);
+                const bool val = of_values(j);
+                const int32_t e = __builtin_amdgcn_readlane(window, half);
+                const int64_t rest = sq.len - (key0 + (int64_t)t * TK + 16 * half);
+                const int have = e < 0 || rest <= 0 ? 0 : rest < 16 ? (int)rest : 16;
+                const int64_t prow = (((int64_t)(e < 0 ? 0 : e) * a.heads + head) << a.bs_log2) + (16 * half & ((1 << a.bs_log2) - 1));
                 const uint8_t *pages = (const uint8_t *)(val ? a.v_pages : a.k_pages) + prow * (D * esize);
                 // rows past the sequence's end lie outside of the buffer: zeros
                 const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)pages, (short)0, have * D * esize, kCrossBuffer);
-                if constexpr (KIND == kBf16 || KIND == kParts) {
-                    raw.w[i][0] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off, 0, 0));
-                } else if (KIND == kCodes || a.dtype != AIR_KV_F32) {
-                    const cross_u32x2 x = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, p_off, 0, 0));
-                    raw.w[i][0][0] = x[0];
-                    raw.w[i][0][1] = x[1];
-                    const float *scales = (val ? a.v_scales : a.k_scales) + prow * nsc;
-                    const __amdgpu_buffer_rsrc_t ss = __builtin_amdgcn_make_buffer_rsrc((void *)scales, (short)0, have * nsc * 4, kCrossBuffer);
-                    raw.s[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ss, p_sc, 0, 0));
-                } else if constexpr (KIND == kWide) {
-                    raw.w[i][0] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off, 0, 0));
-                    raw.w[i][1] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + 16, 0, 0));
+                const float *scales = (val ? a.v_scales : a.k_scales) + prow * nsc;
+                const __amdgpu_buffer_rsrc_t ss = __builtin_amdgcn_make_buffer_rsrc((void *)scales, (short)0, have * nsc * 4, kCrossBuffer);
+#pragma unroll
+                for (int k = 0; k < NPH; ++k) {
+                    const int i = j * NPH + k;
+                    if constexpr (KIND == kBf16 || KIND == kParts) {
+                        raw.w[i][0] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + k * WR * D * 2, 0, 0));
+                    } else if (KIND == kCodes || a.dtype != AIR_KV_F32) {
+                        const cross_u32x2 x = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, p_off + k * WR * D, 0, 0));
+                        raw.w[i][0][0] = x[0];
+                        raw.w[i][0][1] = x[1];
+                        raw.s[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ss, p_sc + k * WR * nsc * 4, 0, 0));
+                    } else if constexpr (KIND == kWide) {
+                        raw.w[i][0] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + k * WR * D * 4, 0, 0));
+                        raw.w[i][1] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + k * WR * D * 4 + 16, 0, 0));
+                    }
                 }
             }
         };
-        // kCodes: the largest finite scales of tile t, of all waves.  (The scale 1 that the append gives a
-        // group of zeros does not count: lanes whose codes are zeros leave theirs out.)
-        auto mark = [&](int t, const Raw &raw) __attribute__((always_inline)) {
+        // kCodes: the largest finite scales of tile t (PRIVATE: of this wave's part), and the powers of two
+        // they ask for.  (The scale 1 that the append gives a group of zeros does not count: lanes whose
+        // codes are zeros leave theirs out.)
+        auto mark = [&](int t, const Raw &raw, float &k, float &v) __attribute__((always_inline)) {
             if constexpr (F16) {
                 const uint32_t sign = a.dtype == AIR_KV_FP8 ? 0x7F7F7F7Fu : ~0u;
-                float k = 0.0f, v = 0.0f;
+                k = v = 0.0f;
 #pragma unroll
                 for (int i = 0; i < NP; ++i) {
                     const float x = __builtin_fabsf(raw.s[i]);
                     const float y = x < INFINITY && ((raw.w[i][0][0] | raw.w[i][0][1]) & sign) ? x : 0.0f;
-                    if ((p_row0 + i * WAVES * WR) / TK) v = fmaxf(v, y);
+                    if (of_values(i / NPH)) v = fmaxf(v, y);
                     else k = fmaxf(k, y);
                 }
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    k = fmaxf(k, __shfl_xor(k, o));
-                    v = fmaxf(v, __shfl_xor(v, o));
-                }
-                k = cross_max32(k);
-                v = cross_max32(v);
-                if (lane == 0) {
-                    atomicMax(&s_top[t % 3][0], __float_as_uint(k));
-                    atomicMax(&s_top[t % 3][1], __float_as_uint(v));
+                if (SH > 1 || !of_values(0)) k = cross_wave_max(k);
+                if (SH > 1 || of_values(0)) v = cross_wave_max(v);
+                if (!PRIVATE && lane == 0) {
+                    if (SH > 1 || !of_values(0)) atomicMax(&s_top[t % 3][0], __float_as_uint(k));
+                    if (SH > 1 || of_values(0)) atomicMax(&s_top[t % 3][1], __float_as_uint(v));
                 }
             }
         };
-        auto write_tile = [&](int t) __attribute__((always_inline)) {
+        auto powers = [&](float k, float v) __attribute__((always_inline)) {
+            // codes are at most 448 (2^9): the largest value to 2^13 at most
+            fk_next = k == 0.0f ? 1.0f : cross_pow2(3 - cross_exponent(k));
+            // values: kept as long as the largest stays below 2^15; it never grows
+            const float want = cross_pow2(3 - cross_exponent(v));
+            fv_next = v == 0.0f ? fv_next : fv_next == 0.0f || fv_next > 4.0f * want ? want : fv_next;
+        };
+        auto write_tile = [&](int t, const Raw &raw) __attribute__((always_inline)) {
             uint8_t *mem = s_mem + t % NB * S::TILE;
-            if constexpr (F16) {
-                // codes are at most 448 (2^9): the largest value to 2^13 at most
-                const float k = __uint_as_float(__builtin_amdgcn_readfirstlane(s_top[t % 3][0]));
-                const float v = __uint_as_float(__builtin_amdgcn_readfirstlane(s_top[t % 3][1]));
-                fk_next = k == 0.0f ? 1.0f : cross_pow2(3 - cross_exponent(k));
-                // values: kept as long as the largest stays below 2^15; it never grows
-                const float want = cross_pow2(3 - cross_exponent(v));
-                fv_next = v == 0.0f ? fv_next : fv_next == 0.0f || fv_next > 4.0f * want ? want : fv_next;
-            }
+            if constexpr (F16 && !PRIVATE)
+                powers(__uint_as_float(__builtin_amdgcn_readfirstlane(s_top[t % 3][0])), __uint_as_float(__builtin_amdgcn_readfirstlane(s_top[t % 3][1])));
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
-                const int r = p_row0 + i * WAVES * WR, val = r / TK, at = r % TK + lane / LPR;
-                uint8_t *to = mem + (val ? VAT + at * VST : at * KST) + 16 * p_c;
+                const bool val = of_values(i / NPH);
+                const int at = 16 * half_of(i / NPH) + i % NPH * WR + lane / LPR;
+                const int chunk = val && cross_v_xor(D) ? p_c ^ ((at & 3) << 2) : p_c;
+                uint8_t *to = mem + (val ? VAT + at * VST : at * KST) + 16 * chunk;
                 const int plane = val ? VPLANE : KPLANE;
                 if constexpr (KIND == kBf16 || KIND == kParts) {
                     if (p_in) *reinterpret_cast<cross_u32x4 *>(to) = raw.w[i][0];
@@ -421,10 +450,11 @@ void paged_cross_kernel(CrossArgs a) {
                 }
             }
         };
-        // What comes between two tiles' products, t the one at hand: tile t + 1 into its buffer, t + 2
-        // on its way (kCodes with two buffers: t + 2 marked, t + 3 on its way).
+        float mk = 0.0f, mv = 0.0f;
+        // Many rows: what comes between two tiles' products, t the one at hand: tile t + 1 into its
+        // buffer, t + 2 on its way (kCodes with two buffers: t + 2 marked, t + 3 on its way).
         auto stage = [&](int t) __attribute__((always_inline)) {
-            write_tile(t + 1);
+            write_tile(t + 1, raw);
             if (t + 2 >= tiles) return;
             if constexpr (F16 && NB == 2) {
                 raw = next;
@@ -432,7 +462,7 @@ void paged_cross_kernel(CrossArgs a) {
                     look_up(t + 3);
                     load_tile(t + 3, next);
                 }
-                mark(t + 2, raw);
+                mark(t + 2, raw, mk, mv);
             } else {
                 look_up(t + 2);
                 load_tile(t + 2, raw);
@@ -441,34 +471,54 @@ void paged_cross_kernel(CrossArgs a) {
 
         fetch(0);
         __syncthreads();                               // the buffers of the block before are free
-        if (F16 && tid < 6) s_top[tid / 2][tid % 2] = 0;
         look_up(0);
         load_tile(0, raw);
-        if (F16 && NB == 2 && 1 < tiles) {
-            look_up(1);
-            load_tile(1, next);
-        }
-        if constexpr (F16) {
-            __syncthreads();
-            mark(0, raw);
-            __syncthreads();
-        }
-        write_tile(0);
-        if (1 < tiles) {
-            if constexpr (F16 && NB == 2) {
-                raw = next;
-                if (2 < tiles) {
-                    look_up(2);
-                    load_tile(2, next);
-                }
-                mark(1, raw);
-            } else {
+        if constexpr (!PRIVATE) {
+            if (F16 && tid < 6) s_top[tid / 2][tid % 2] = 0;
+            if (F16 && NB == 2 && 1 < tiles) {
                 look_up(1);
-                load_tile(1, raw);
+                load_tile(1, next);
             }
+            if constexpr (F16) {
+                __syncthreads();
+                mark(0, raw, mk, mv);
+                __syncthreads();
+            }
+            write_tile(0, raw);
+            if (1 < tiles) {
+                if constexpr (F16 && NB == 2) {
+                    raw = next;
+                    if (2 < tiles) {
+                        look_up(2);
+                        load_tile(2, next);
+                    }
+                    mark(1, raw, mk, mv);
+                } else {
+                    look_up(1);
+                    load_tile(1, raw);
+                }
+            }
+            __syncthreads();
         }
-        __syncthreads();
         for (int t = 0; t < tiles; ++t) {
+            int ok = 3;                                // PRIVATE: whether this wave's halves are in the pool
+            if constexpr (PRIVATE) {
+                ok = (__builtin_amdgcn_readlane(window, 2 * wave) >= 0 ? 1 : 0) | (__builtin_amdgcn_readlane(window, 2 * wave + 1) >= 0 ? 2 : 0);
+                if constexpr (F16) {
+                    mark(t, raw, mk, mv);
+                    powers(mk, mv);
+                }
+                // (a wave's LDS accesses are in order: the tile before has been read)
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                write_tile(t, raw);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                if (t + 1 < tiles) {
+                    look_up(t + 1);
+                    load_tile(t + 1, raw);
+                }
+            }
             if constexpr (F16) {
                 // (a power of two that changes: the sums so far are brought under it)
                 fk = fk_next;
@@ -478,9 +528,9 @@ void paged_cross_kernel(CrossArgs a) {
                     for (int c = 0; c < CT; ++c) acc[c] *= by;
                     fv = fv_next;
                 }
-                if (tid < 2) s_top[t % 3][tid] = 0;
+                if (!PRIVATE && tid < 2) s_top[t % 3][tid] = 0;
             }
-            if (NB == 2 && t + 1 < tiles) stage(t);
+            if (!PRIVATE && NB == 2 && t + 1 < tiles) stage(t);
             if (any) {
                 const uint8_t *mem = s_mem + t % NB * S::TILE;
 #pragma unroll
@@ -504,11 +554,12 @@ void paged_cross_kernel(CrossArgs a) {
                                 if (i + j < 3) sc = cross_mfma<F16>(kf[i], qf[j][s], sc);
                     }
                     // keys past the end and of blocks outside the pool
-                    const int ok0 = __builtin_amdgcn_readfirstlane(s_ok[t % 4][k0 / 16]);
-                    const int ok1 = __builtin_amdgcn_readfirstlane(s_ok[t % 4][k0 / 16 + 1]);
+                    if constexpr (!PRIVATE)
+                        ok = __builtin_amdgcn_readfirstlane(s_ok[t % 4][k0 / 16] + 2 * s_ok[t % 4][k0 / 16 + 1]);
                     uint32_t mask = rest < 32 ? (1u << (int)rest) - 1 : ~0u;
-                    mask &= (ok0 ? 0x0000FFFFu : 0u) | (ok1 ? 0xFFFF0000u : 0u);
+                    mask &= (ok & 1 ? 0x0000FFFFu : 0u) | (ok & 2 ? 0xFFFF0000u : 0u);
                     if (mask != ~0u) {
+                        asm volatile("");              // (a branch: selects would cost every tile 60 instructions)
                         const uint32_t m = mask >> (4 * hf);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) sc[i] = (m >> (8 * (i / 4) + i % 4)) & 1 ? sc[i] : -INFINITY;
@@ -520,7 +571,7 @@ void paged_cross_kernel(CrossArgs a) {
                     float top = sc[0];
 #pragma unroll
                     for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
-                    top = cross_max32(top) * ft;
+                    top = max_x32(top) * ft;
                     if (__ballot(top > lim) != 0ull) {
                         // (scores past 2^20, which f32 holds in steps of an eighth and more, are each rounded as
                         // the largest was, so that their distances from the base are exact)
@@ -552,13 +603,20 @@ void paged_cross_kernel(CrossArgs a) {
 #pragma unroll
                             for (int k = 0; k < QP; ++k) p[k][s][j] = x[k];
                         }
+                    // (16-bit ones are summed as they were rounded)
+                    if constexpr (QP == 3) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) l_run += sc[i];
+                        for (int i = 0; i < 16; ++i) l_run += sc[i];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) l_run = cross_add_pair<F16>(p[0][i / 4][i % 4], ones, l_run);
+                    }
                     // V^T as the A operand: lane (m, h) takes keys 16 s + 8 b + 4 h .. +4 of column m, b = 0, 1.
                     // Within each 16-lane group, lane j of a transposing read receives element j % 4 of the 8
                     // bytes that lanes 4 k + j / 4 address, k = 0 .. 3: lane i points at key i / 4 of the four
                     // and columns 4 (i % 4) of the group's sixteen.
-                    const uint8_t *v0 = mem + VAT + (k0 + 4 * hf + ((lane & 15) >> 2)) * VST + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+                    const int vr = 4 * hf + ((lane & 15) >> 2);
+                    const uint8_t *v0 = mem + VAT + (k0 + vr) * VST + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
 #pragma unroll
                     for (int c = 0; c < CT; ++c)
 #pragma unroll
@@ -566,7 +624,8 @@ void paged_cross_kernel(CrossArgs a) {
 #pragma unroll
                             for (int i = 0; i < KP; ++i) {
                                 typedef short s16x4 __attribute__((ext_vector_type(4)));
-                                const uint8_t *v = v0 + i * VPLANE + 64 * c + 16 * s * VST;
+                                const int cc = cross_v_xor(D) ? 64 * (c ^ (vr & 3)) : 64 * c;
+                                const uint8_t *v = v0 + i * VPLANE + cc + 16 * s * VST;
                                 const cross_u32x2 x = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                                           (__attribute__((address_space(3))) s16x4 *)v));
                                 const cross_u32x2 y = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -578,17 +637,20 @@ void paged_cross_kernel(CrossArgs a) {
                             }
                 }
             }
-            if (NB == 1 && t + 1 < tiles) mark(t + 1, raw);
-            __syncthreads();
-            if (NB == 1 && t + 1 < tiles) {
-                stage(t);
+            if constexpr (!PRIVATE) {
+                if (NB == 1 && t + 1 < tiles) mark(t + 1, raw, mk, mv);
                 __syncthreads();
+                if (NB == 1 && t + 1 < tiles) {
+                    stage(t);
+                    __syncthreads();
+                }
             }
         }
+        if constexpr (PRIVATE) __syncthreads();
 
         // lane (n, h): columns 32 c + 8 (i / 4) + 4 h + i % 4 of row n in acc[c][i]
-        float l = cross_sum32(l_run);
-        const float unit = F16 && fv != 0.0f ? 1.0f / fv : 1.0f;       // of the sums (pieces' stay under it)
+        float l = sum_x32(l_run);
+        float unit = F16 && fv != 0.0f ? 1.0f / fv : 1.0f;     // of the sums (pieces' stay under it)
         const int64_t slot = 2 * cell + (t0 == 0 ? 1 : 0);
         const int64_t prow = slot * ROWS + 32 * rg + r32;
         if constexpr (WK == 1) {
@@ -610,18 +672,24 @@ void paged_cross_kernel(CrossArgs a) {
         } else {
             // the waves of one row group: their bases' largest, then their sums, CR column tiles at a
             // time, four columns (c, i) of all of them to one wave
-            if (hf == 0) s_ml[wave][r32] = make_float2(base, l);
+            if (hf == 0) s_ml[wave][r32] = make_float4(base, l, fv, 0.0f);
             __syncthreads();
-            float top = -INFINITY;
+            float top = -INFINITY, least = 0.0f;       // (the smallest power of two of the values': the largest unit)
 #pragma unroll
-            for (int i = 0; i < WK; ++i) top = fmaxf(top, s_ml[rg * WK + i][r32].x);
+            for (int i = 0; i < WK; ++i) {
+                const float4 ml = s_ml[rg * WK + i][r32];
+                top = fmaxf(top, ml.x);
+                least = ml.z != 0.0f && (least == 0.0f || ml.z < least) ? ml.z : least;
+            }
             l = 0.0f;
 #pragma unroll
             for (int i = 0; i < WK; ++i) {
-                const float2 ml = s_ml[rg * WK + i][r32];
+                const float4 ml = s_ml[rg * WK + i][r32];
                 l += ml.x == -INFINITY ? ml.y : ml.y * __builtin_amdgcn_exp2f(ml.x - top);
             }
-            const float alpha = base == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(base - top);
+            float alpha = base == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(base - top);
+            if (F16 && fv != 0.0f) alpha *= least / fv;
+            if (F16) unit = least != 0.0f ? 1.0f / least : 1.0f;
             const float k = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
             cross_f32x4 *x = reinterpret_cast<cross_f32x4 *>(s_mem) + lane;
 #pragma unroll
@@ -670,14 +738,14 @@ template <CrossKind KIND, bool FEW> hipError_t launch_cross_shape(const CrossArg
     return hipGetLastError();
 }
 
-template <CrossKind KIND, bool FEW> int cross_rows_shape(int d) {
+template <CrossKind KIND, bool FEW> CrossBlocks cross_blocks_shape(int d) {
     switch (d) {
-#define AIRKV_CROSS(D) case D: return CrossShape<D, KIND, FEW>::ROWS;
+#define AIRKV_CROSS(D) case D: return {CrossShape<D, KIND, FEW>::ROWS, CrossShape<D, KIND, FEW>::GROUPS};
         AIRKV_CROSS(32) AIRKV_CROSS(64) AIRKV_CROSS(96) AIRKV_CROSS(128)
         AIRKV_CROSS(160) AIRKV_CROSS(192) AIRKV_CROSS(224) AIRKV_CROSS(256)
 #undef AIRKV_CROSS
     }
-    return 0;
+    return {0, 0};
 }
 
 }  // namespace airkv
