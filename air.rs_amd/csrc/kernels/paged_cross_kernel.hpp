@@ -25,6 +25,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "codecs.hpp"
 #include "decode_slices.hpp"
 #include "paged_cross.hpp"
@@ -55,8 +57,9 @@ constexpr int cross_v_stride(int d) { return cross_v_xor(d) || 2 * d / 64 % 2 ? 
 constexpr int cross_tile_bytes(int d, int parts, int keys) { return keys * parts * (cross_k_stride(d) + cross_v_stride(d)); }
 // Waves of a workgroup, and workgroups a CU: registers leave room for four waves a SIMD (small
 // heads), two, or (queries in three parts and their sums, the largest heads) one.
+constexpr bool cross_pipe(int d, int qp, bool few) { return !few && qp == 1 && d <= 128; }
 constexpr int cross_waves(int d, int qp, bool few) { return few || (qp == 3 ? d >= 96 : d >= 192) ? 4 : 8; }
-constexpr int cross_groups(int d, int qp, bool few) { return few ? (d <= (qp == 3 ? 64 : 128) ? 2 : 1) : qp == 1 && d <= 64 ? 2 : 1; }
+constexpr int cross_groups(int d, int qp, bool few) { return few ? (d <= (qp == 3 ? 64 : 128) ? 2 : 1) : 1; }
 // What a workgroup's tiles may take of a CU's 160 KB.
 constexpr int cross_lds(int groups) { return 160 * 1024 / groups - 7 * 1024; }
 // Waves that share rows: as many as have room for 32 keys each.
@@ -134,11 +137,12 @@ template <int D, CrossKind KIND, bool FEW>
 struct CrossShape {
     static constexpr int KP = KIND == kWide ? 3 : 1, QP = KIND == kParts || KIND == kWide ? 3 : 1;
     static constexpr int WAVES = cross_waves(D, QP, FEW), WK = cross_wk(D, KP, QP, FEW), SUB = cross_sub(D, KP, WK);
-    static constexpr bool PRIVATE = FEW && WK == WAVES;
-    static constexpr int ROWS = 32 * (WAVES / WK), TK = 32 * WK * SUB;
+    static constexpr bool PRIVATE = FEW && WK == WAVES, PIPE = cross_pipe(D, QP, FEW);
+    static constexpr int RT = 1;                       // 32s of rows a wave
+    static constexpr int ROWS = 32 * RT * (WAVES / WK), TK = 32 * WK * SUB;
     static constexpr int TILE = cross_tile_bytes(D, KP, TK);
     static constexpr int GROUPS = cross_groups(D, QP, FEW) == 2 && TILE <= cross_lds(2) ? 2 : 1;
-    static constexpr int NB = !PRIVATE && 2 * TILE <= cross_lds(GROUPS) ? 2 : 1;
+    static constexpr int NB = PIPE ? 3 : !PRIVATE && 2 * TILE <= cross_lds(GROUPS) ? 2 : 1;
     static constexpr int WAVES_SIMD = WAVES / 4 * GROUPS;
 };
 
@@ -147,8 +151,8 @@ __global__ __launch_bounds__((CrossShape<D, KIND, FEW>::WAVES * 64))
 __attribute__((amdgpu_waves_per_eu(CrossShape<D, KIND, FEW>::WAVES_SIMD, CrossShape<D, KIND, FEW>::WAVES_SIMD)))
 void paged_cross_kernel(CrossArgs a) {
     typedef CrossShape<D, KIND, FEW> S;
-    constexpr bool F16 = KIND == kCodes, PRIVATE = S::PRIVATE;
-    constexpr int KP = S::KP, QP = S::QP, WAVES = S::WAVES, WK = S::WK, SUB = S::SUB, ROWS = S::ROWS, TK = S::TK, NB = S::NB, THREADS = 64 * WAVES;
+    constexpr bool F16 = KIND == kCodes, PRIVATE = S::PRIVATE, PIPE = S::PIPE;
+    constexpr int KP = S::KP, QP = S::QP, WAVES = S::WAVES, WK = S::WK, SUB = S::SUB, ROWS = S::ROWS, TK = S::TK, NB = S::NB, RT = S::RT, THREADS = 64 * WAVES;
     constexpr int KST = cross_k_stride(D), VST = cross_v_stride(D);
     constexpr int KPLANE = TK * KST, VPLANE = TK * VST, VAT = KP * KPLANE;    // a part's rows; where values begin
     constexpr int KS = D / 16, CT = D / 32;            // steps of the first product, 32-column tiles of the second
@@ -162,7 +166,7 @@ void paged_cross_kernel(CrossArgs a) {
     constexpr int CR = MEM / JOIN < CT ? MEM / JOIN : CT;      // column tiles joined at once (WK > 1)
     __shared__ int64_t s_pre[kCrossBatch + 1];
     __shared__ int64_t s_sum[WAVES];
-    __shared__ int32_t s_ok[4][TK / 16];               // whether a tile's 16-key halves are in the pool
+    __shared__ int32_t s_ok[8][TK / 16];               // whether a tile's 16-key halves are in the pool
     __shared__ uint32_t s_top[3][2];                   // a tile's largest scale of keys and of values, as bits
     __shared__ float4 s_ml[WAVES][32];
     __shared__ __align__(16) uint8_t s_mem[MEM];
@@ -236,7 +240,7 @@ void paged_cross_kernel(CrossArgs a) {
     const uint32_t ones = cross_ones<F16>();
     // A SIMD has waves i and i + 4 of a workgroup: the second goes first, so that the two get out of
     // phase and one's products run beside the other's arithmetic.
-    if (!FEW && wave >= 4) __builtin_amdgcn_s_setprio(1);
+    if (WAVES == 8 && wave >= 4) __builtin_amdgcn_s_setprio(1);
     int b = 0;
     if (u < end) {
         int lo = 0, hi = a.batch;
@@ -267,66 +271,84 @@ void paged_cross_kernel(CrossArgs a) {
         const int64_t key0 = (int64_t)t0 * TK;
         const int32_t *table = a.tables + (int64_t)b * a.max_blocks;
 
-        const int row = blk * ROWS + 32 * rg + r32;    // of the sequence's at this K/V head
-        const bool live = row < sq.rows, any = blk * ROWS + 32 * rg < sq.rows;
-        const int row_at = live ? row : sq.rows - 1;
-        const int64_t io = ((int64_t)(sq.row0 + row_at / a.group) * a.q_heads + head * a.group + row_at % a.group) * D;
+        // rows 32 (RT rg + r) .. +31 of the block
+        const bool any = blk * ROWS + 32 * RT * rg < sq.rows;
+        bool live[RT];
+        int64_t io[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const int row = blk * ROWS + 32 * (RT * rg + r) + r32;             // of the sequence's at this K/V head
+            live[r] = row < sq.rows;
+            const int row_at = live[r] ? row : sq.rows - 1;
+            io[r] = ((int64_t)(sq.row0 + row_at / a.group) * a.q_heads + head * a.group + row_at % a.group) * D;
+        }
 
         // Q^T as the B operand: lane (n, h) holds elements 16 s + 8 h .. +8 of row n
-        cross_u32x4 qf[QP][KS];
-        int qe = 0;                                    // (kCodes: the power of two they are under)
-        if (KIND == kBf16 || KIND == kCodes || a.q_dtype == AIR_KV_BF16) {
-            const uint16_t *q = (const uint16_t *)a.q + io + 8 * hf;
+        cross_u32x4 qf[RT][QP][KS];
+        int qe[RT];                                    // (kCodes: the power of two they are under)
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                qf[0][s] = *reinterpret_cast<const cross_u32x4 *>(q + 16 * s);
+        for (int r = 0; r < RT; ++r) {
+            qe[r] = 0;
+            if (KIND == kBf16 || KIND == kCodes || a.q_dtype == AIR_KV_BF16) {
+                const uint16_t *q = (const uint16_t *)a.q + io[r] + 8 * hf;
 #pragma unroll
-                for (int p = 1; p < QP; ++p) qf[p][s] = cross_u32x4{0, 0, 0, 0};
-            }
-        } else {
-            const float *q = (const float *)a.q + io + 8 * hf;
+                for (int s = 0; s < KS; ++s) {
+                    qf[r][0][s] = *reinterpret_cast<const cross_u32x4 *>(q + 16 * s);
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const cross_f32x4 x = *reinterpret_cast<const cross_f32x4 *>(q + 16 * s + 4 * i);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        uint32_t p[QP];
-                        cross_parts<F16, QP>(x[2 * j], x[2 * j + 1], p);
-#pragma unroll
-                        for (int k = 0; k < QP; ++k) qf[k][s][2 * i + j] = p[k];
-                    }
+                    for (int p = 1; p < QP; ++p) qf[r][p][s] = cross_u32x4{0, 0, 0, 0};
                 }
+            } else {
+                const float *q = (const float *)a.q + io[r] + 8 * hf;
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const cross_f32x4 x = *reinterpret_cast<const cross_f32x4 *>(q + 16 * s + 4 * i);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            uint32_t p[QP];
+                            cross_parts<F16, QP>(x[2 * j], x[2 * j + 1], p);
+#pragma unroll
+                            for (int k = 0; k < QP; ++k) qf[r][k][s][2 * i + j] = p[k];
+                        }
+                    }
+            }
+            if constexpr (F16) {
+                // the row's largest element to [2^4, 2^5): bf16's 8 bits are exact in f16 down to 2^-11
+                float top = 0.0f;
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        top = fmaxf(top, fmaxf(__builtin_fabsf(__uint_as_float(qf[r][0][s][j] << 16)),
+                                               __builtin_fabsf(__uint_as_float(qf[r][0][s][j] & 0xFFFF0000u))));
+                const float fq = cross_pow2(4 - cross_exponent(max_x32(top)));
+                qe[r] = cross_exponent(fq);
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        qf[r][0][s][j] = cross_f16_pair(__uint_as_float(qf[r][0][s][j] << 16) * fq, __uint_as_float(qf[r][0][s][j] & 0xFFFF0000u) * fq);
+            }
         }
-        if constexpr (F16) {
-            // the row's largest element to [2^4, 2^5): bf16's 8 bits are exact in f16 down to 2^-11
-            float top = 0.0f;
+        cross_f32x16 acc[RT][CT];
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    top = fmaxf(top, fmaxf(__builtin_fabsf(__uint_as_float(qf[0][s][j] << 16)),
-                                           __builtin_fabsf(__uint_as_float(qf[0][s][j] & 0xFFFF0000u))));
-            const float fq = cross_pow2(4 - cross_exponent(max_x32(top)));
-            qe = cross_exponent(fq);
+            for (int c = 0; c < CT; ++c)
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    qf[0][s][j] = cross_f16_pair(__uint_as_float(qf[0][s][j] << 16) * fq, __uint_as_float(qf[0][s][j] & 0xFFFF0000u) * fq);
-        }
-        cross_f32x16 acc[CT];
-#pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
+                for (int i = 0; i < 16; ++i) acc[r][c][i] = 0.0f;
         // Probabilities are held 2^(score - base), the base kDown above every score so far: 2^24 of
         // them sum to 1 at most, so that values near the largest float do too.  (f16 ones up to
         // 2^15, so that they keep 11 bits down to 2^-25 of the largest; values are below 2^15 there.)
         // A base is taken kSlack further up, so that it seldom changes: where a score passes lim.
         constexpr float kDown = F16 ? -15.0f : 24.0f, kSlack = 4.0f, kFar = 0x1p20f;
-        float base = -INFINITY, lim = -INFINITY, l_run = 0.0f;
+        float base[RT], lim[RT], l_run[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            base[r] = lim[r] = -INFINITY;
+            l_run[r] = 0.0f;
+        }
 
         struct Raw {                                   // a tile on its way
             cross_u32x4 w[NP][KIND == kWide ? 2 : 1];
@@ -348,7 +370,7 @@ void paged_cross_kernel(CrossArgs a) {
                 const int n = __popcll(__ballot(out && (key & ((1 << a.bs_log2) - 1)) == 0));
                 if (n && lane == 0) atomicAdd(a.errors, (unsigned long long)n);
             }
-            if (!PRIVATE && wave == 0 && lane < TK / 16) s_ok[t % 4][lane] = window >= 0;
+            if (!PRIVATE && wave == 0 && lane < TK / 16) s_ok[t % 8][lane] = window >= 0;
             fetch(t + 1);
         };
         auto load_tile = [&](int t, Raw &raw) __attribute__((always_inline)) {
@@ -456,7 +478,7 @@ void paged_cross_kernel(CrossArgs a) {
         auto stage = [&](int t) __attribute__((always_inline)) {
             write_tile(t + 1, raw);
             if (t + 2 >= tiles) return;
-            if constexpr (F16 && NB == 2) {
+            if constexpr (F16 && NB >= 2) {
                 raw = next;
                 if (t + 3 < tiles) {
                     look_up(t + 3);
@@ -475,7 +497,7 @@ void paged_cross_kernel(CrossArgs a) {
         load_tile(0, raw);
         if constexpr (!PRIVATE) {
             if (F16 && tid < 6) s_top[tid / 2][tid % 2] = 0;
-            if (F16 && NB == 2 && 1 < tiles) {
+            if (F16 && NB >= 2 && 1 < tiles) {
                 look_up(1);
                 load_tile(1, next);
             }
@@ -486,7 +508,7 @@ void paged_cross_kernel(CrossArgs a) {
             }
             write_tile(0, raw);
             if (1 < tiles) {
-                if constexpr (F16 && NB == 2) {
+                if constexpr (F16 && NB >= 2) {
                     raw = next;
                     if (2 < tiles) {
                         look_up(2);
@@ -500,179 +522,356 @@ void paged_cross_kernel(CrossArgs a) {
             }
             __syncthreads();
         }
-        for (int t = 0; t < tiles; ++t) {
-            int ok = 3;                                // PRIVATE: whether this wave's halves are in the pool
-            if constexpr (PRIVATE) {
-                ok = (__builtin_amdgcn_readlane(window, 2 * wave) >= 0 ? 1 : 0) | (__builtin_amdgcn_readlane(window, 2 * wave + 1) >= 0 ? 2 : 0);
-                if constexpr (F16) {
-                    mark(t, raw, mk, mv);
-                    powers(mk, mv);
-                }
-                // (a wave's LDS accesses are in order: the tile before has been read)
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                write_tile(t, raw);
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                if (t + 1 < tiles) {
-                    look_up(t + 1);
-                    load_tile(t + 1, raw);
+        // ---- a step's parts: 32 keys, those of a buffer `mem` from row k0 on
+
+        auto scores = [&](const uint8_t *mem, int k0, cross_f32x16 (&sc)[RT]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sc[r][i] = 0.0f;
+            int ln = lane;
+            asm volatile("" : "+v"(ln));
+            const uint8_t *k = mem + (k0 + (ln & 31)) * KST + 16 * (ln >> 5);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                cross_u32x4 kf[KP];
+#pragma unroll
+                for (int p = 0; p < KP; ++p) kf[p] = *reinterpret_cast<const cross_u32x4 *>(k + p * KPLANE + 32 * s);
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int i = 0; i < KP; ++i)
+#pragma unroll
+                        for (int j = 0; j < QP; ++j)
+                            if (i + j < 3) sc[r] = cross_mfma<F16>(kf[i], qf[r][j][s], sc[r]);
+            }
+        };
+        auto tops = [&](const cross_f32x16 (&sc)[RT], float (&top)[RT]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                float x = sc[r][0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) x = fmaxf(x, sc[r][i]);
+                top[r] = max_x32(x);
+            }
+        };
+        // keys past the end (rest are left) and of blocks outside the pool (ok: a bit for each half)
+        auto hide = [&](int64_t rest, int ok, cross_f32x16 (&sc)[RT], float (&top)[RT]) __attribute__((always_inline)) {
+            uint32_t mask = rest >= 32 ? ~0u : rest <= 0 ? 0u : (1u << (int)rest) - 1;
+            mask &= (ok & 1 ? 0x0000FFFFu : 0u) | (ok & 2 ? 0xFFFF0000u : 0u);
+            if (__builtin_expect(mask != ~0u, 0)) {
+                asm volatile("");                      // (a branch: selects would cost every tile 60 instructions)
+                const uint32_t m = mask >> (4 * hf);
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sc[r][i] = (m >> (8 * (i / 4) + i % 4)) & 1 ? sc[r][i] : -INFINITY;
+                tops(sc, top);
+            }
+        };
+        // Another base for rows whose largest score passes lim; what is behind has to be multiplied by
+        // alpha then (the return value: for some row).
+        auto rebase = [&](cross_f32x16 (&sc)[RT], const float (&top)[RT], float (&ft)[RT], float (&alpha)[RT]) __attribute__((always_inline)) -> bool {
+            bool past = false;
+#pragma unroll
+            for (int r = 0; r < RT; ++r) past |= top[r] * ft[r] > lim[r];
+            if (__builtin_expect(__ballot(past) == 0ull, 1)) return false;
+            asm volatile("");
+            bool far = false;
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const float x = top[r] * ft[r];
+                const float cap = __builtin_fabsf(base[r]) < kFar ? base[r] - kDown : base[r];
+                const float now = x > cap ? x + (__builtin_fabsf(x) < kFar ? kDown + kSlack : 0.0f) : base[r];
+                alpha[r] = base[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(base[r] - now);
+                l_run[r] *= alpha[r];
+                base[r] = now;
+                const bool is_far = !(__builtin_fabsf(now) < kFar) && now != -INFINITY;
+                lim[r] = is_far ? -INFINITY : now - kDown;
+                far |= is_far;
+            }
+            // (scores past 2^20, which f32 holds in steps of an eighth and more, are each rounded as
+            // the largest was, so that their distances from the base are exact)
+            if (__ballot(far) != 0ull) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    sc[r] *= ft[r];
+                    ft[r] = 1.0f;
                 }
             }
-            if constexpr (F16) {
-                // (a power of two that changes: the sums so far are brought under it)
-                fk = fk_next;
-                if (fv != fv_next) {
-                    const float by = fv == 0.0f ? 1.0f : fv_next / fv;
+            return true;
+        };
+        auto scale_sums = [&](const float (&by)[RT]) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int c = 0; c < CT; ++c) acc[c] *= by;
-                    fv = fv_next;
-                }
-                if (!PRIVATE && tid < 2) s_top[t % 3][tid] = 0;
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int c = 0; c < CT; ++c) acc[r][c] *= by[r];
+        };
+        auto scale_all = [&](float by) __attribute__((always_inline)) {
+            float b[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) b[r] = by;
+            scale_sums(b);
+        };
+        // what products are multiplied by.  (Neither 0 nor infinite: a masked score, -inf, times 0 would be NaN,
+        // and so would 0 times infinity.)
+        auto factors = [&](float fk, float (&ft)[RT]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                ft[r] = a.scale_log2;
+                if constexpr (F16) ft[r] = fminf(fmaxf(__builtin_amdgcn_ldexpf(ft[r], -(qe[r] + cross_exponent(fk))), 0x1p-126f), 0x1.fffffep127f);
             }
-            if (!PRIVATE && NB == 2 && t + 1 < tiles) stage(t);
-            if (any) {
-                const uint8_t *mem = s_mem + t % NB * S::TILE;
+        };
+        auto probabilities = [&](cross_f32x16 (&sc)[RT], const float (&ft)[RT], cross_u32x4 (&p)[RT][QP][2]) __attribute__((always_inline)) {
 #pragma unroll
-                for (int sub = 0; sub < SUB; ++sub) {
-                    const int k0 = 32 * (wk * SUB + sub);              // the keys' rows in the tile
-                    const int64_t rest = sq.len - (key0 + (int64_t)t * TK + k0);
-                    if (rest <= 0) continue;
-                    cross_f32x16 sc;
+            for (int r = 0; r < RT; ++r) {
+                const float from = base[r] == -INFINITY ? 0.0f : base[r];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
+                for (int i = 0; i < 16; ++i) sc[r][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][i], ft[r], -from));
 #pragma unroll
-                    for (int s = 0; s < KS; ++s) {
-                        cross_u32x4 kf[KP];
+                for (int s = 0; s < 2; ++s)
 #pragma unroll
-                        for (int p = 0; p < KP; ++p)
-                            kf[p] = *reinterpret_cast<const cross_u32x4 *>(mem + p * KPLANE + (k0 + r32) * KST + 32 * s + 16 * hf);
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t x[QP];
+                        cross_parts<F16, QP>(sc[r][8 * s + 2 * j], sc[r][8 * s + 2 * j + 1], x);
 #pragma unroll
-                        for (int i = 0; i < KP; ++i)
+                        for (int k = 0; k < QP; ++k) p[r][k][s][j] = x[k];
+                        // (16-bit ones are summed as they were rounded)
+                        if constexpr (QP == 1) l_run[r] = cross_add_pair<F16>(x[0], ones, l_run[r]);
+                        else l_run[r] += sc[r][8 * s + 2 * j] + sc[r][8 * s + 2 * j + 1];
+                    }
+            }
+        };
+        // V^T as the A operand: lane (m, h) takes keys 16 s + 8 b + 4 h .. +4 of column m, b = 0, 1.
+        // Within each 16-lane group, lane j of a transposing read receives element j % 4 of the 8
+        // bytes that lanes 4 k + j / 4 address, k = 0 .. 3: lane i points at key i / 4 of the four
+        // and columns 4 (i % 4) of the group's sixteen.
+        auto values = [&](const uint8_t *mem, int k0, const cross_u32x4 (&p)[RT][QP][2]) __attribute__((always_inline)) {
+            int ln = lane;                             // (its addresses are not kept in registers from step to step)
+            asm volatile("" : "+v"(ln));
+            const int vr = 4 * (ln >> 5) + ((ln & 15) >> 2);
+            const uint8_t *v0 = mem + VAT + (k0 + vr) * VST + 32 * ((ln >> 4) & 1) + 8 * (ln & 3);
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int i = 0; i < KP; ++i) {
+                        typedef short s16x4 __attribute__((ext_vector_type(4)));
+                        const int cc = cross_v_xor(D) ? 64 * (c ^ (vr & 3)) : 64 * c;
+                        const uint8_t *v = v0 + i * VPLANE + cc + 16 * s * VST;
+                        const cross_u32x2 x = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                  (__attribute__((address_space(3))) s16x4 *)v));
+                        const cross_u32x2 y = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                  (__attribute__((address_space(3))) s16x4 *)(v + 8 * VST)));
+                        const cross_u32x4 vf = {x[0], x[1], y[0], y[1]};
+#pragma unroll
+                        for (int r = 0; r < RT; ++r)
 #pragma unroll
                             for (int j = 0; j < QP; ++j)
-                                if (i + j < 3) sc = cross_mfma<F16>(kf[i], qf[j][s], sc);
+                                if (i + j < 3) acc[r][c] = cross_mfma<F16>(vf, p[r][j][s], acc[r][c]);
                     }
-                    // keys past the end and of blocks outside the pool
-                    if constexpr (!PRIVATE)
-                        ok = __builtin_amdgcn_readfirstlane(s_ok[t % 4][k0 / 16] + 2 * s_ok[t % 4][k0 / 16 + 1]);
-                    uint32_t mask = rest < 32 ? (1u << (int)rest) - 1 : ~0u;
-                    mask &= (ok & 1 ? 0x0000FFFFu : 0u) | (ok & 2 ? 0xFFFF0000u : 0u);
-                    if (mask != ~0u) {
-                        asm volatile("");              // (a branch: selects would cost every tile 60 instructions)
-                        const uint32_t m = mask >> (4 * hf);
+        };
+
+        if constexpr (PIPE) {
+            // A step's probabilities are computed beside the next step's scores and the one before's
+            // values, so that products and arithmetic, about as much of either, run at once.  A tile is
+            // two steps; the next tile is staged beside the first and there at a barrier before the second.
+            static_assert(RT == 1 && QP == 1 && KP == 1 && KS == 2 * CT && NB == 3, "one row tile, 16-bit parts");
+            cross_f32x16 sa[RT], sb[RT];
+            cross_u32x4 pa[2], pb[2];
+            float top[RT];
+            float fv_t = fv_next;                      // kCodes: of the tile whose values come next
+            // (this lane's places in a buffer: keys, values of four column tiles)
+            const int k_at = r32 * KST + 16 * hf, vr = 4 * hf + ((lane & 15) >> 2);
+            int v_at[4];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) sc[i] = (m >> (8 * (i / 4) + i % 4)) & 1 ? sc[i] : -INFINITY;
+            for (int c = 0; c < 4; ++c)
+                v_at[c] = VAT + vr * VST + 32 * ((lane >> 4) & 1) + 8 * (lane & 3) + 64 * (cross_v_xor(D) ? c ^ (vr & 3) : c);
+            // A step from its scores in sc: p; the next step's scores, of the keys from row k0 of buffer kb, in
+            // sn; the sums of the step before, its probabilities q and the values from row v0 of buffer vb.
+            auto step = [&](cross_f32x16 (&sc)[RT], cross_f32x16 (&sn)[RT], cross_u32x4 (&p)[2], const cross_u32x4 (&q)[2], int kb, int k0, int vb,
+                            int v0, int64_t rest, int ok, float fk) __attribute__((always_inline)) {
+                hide(rest, ok, sc, top);
+                float ft[RT], alpha[RT];
+                factors(fk, ft);
+                const bool changed = rebase(sc, top, ft, alpha);
+                // what follows is in the order in which it shall run: a product, then arithmetic that is done
+                // while it runs, fragments read three products ahead
+                constexpr int AHEAD = 3, N = KS + 2 * CT;
+                typedef const __attribute__((address_space(3))) uint8_t *lds_t;
+                const lds_t k = (lds_t)s_mem + kb * S::TILE + k0 * KST + k_at;
+                lds_t v[CT < 4 ? CT : 4];
+#pragma unroll
+                for (int c = 0; c < CT && c < 4; ++c) v[c] = (lds_t)s_mem + vb * S::TILE + v0 * VST + v_at[c];
+                cross_u32x4 f[N];
+                auto read = [&](int i) __attribute__((always_inline)) {
+                    typedef short s16x4 __attribute__((ext_vector_type(4)));
+                    if (i < KS) {
+                        f[i] = *reinterpret_cast<const __attribute__((address_space(3))) cross_u32x4 *>(k + 32 * i);
+                    } else if (i < N) {
+                        const int c = (i - KS) / 2, at = 256 * (c / 4) + 16 * ((i - KS) % 2) * VST;
+                        const cross_u32x2 x = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                  (__attribute__((address_space(3))) s16x4 *)(v[c % 4] + at)));
+                        const cross_u32x2 y = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                  (__attribute__((address_space(3))) s16x4 *)(v[c % 4] + at + 8 * VST)));
+                        f[i] = cross_u32x4{x[0], x[1], y[0], y[1]};
                     }
-                    // (neither 0 nor infinite: a masked score, -inf, times 0 would be NaN, and so would 0 times
-                    // infinity)
-                    float ft = a.scale_log2;
-                    if constexpr (F16) ft = fminf(fmaxf(__builtin_amdgcn_ldexpf(ft, -(qe + cross_exponent(fk))), 0x1p-126f), 0x1.fffffep127f);
-                    float top = sc[0];
+                };
+                const float from = base[0] == -INFINITY ? 0.0f : base[0];
+                auto pair = [&](int i) __attribute__((always_inline)) {
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[0][2 * i], ft[0], -from));
+                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[0][2 * i + 1], ft[0], -from));
+                    p[i / 4][i % 4] = F16 ? cross_f16_pair(x, y) : cross_bf16_pair(x, y);
+                    l_run[0] = cross_add_pair<F16>(p[i / 4][i % 4], ones, l_run[0]);
+                };
 #pragma unroll
-                    for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
-                    top = max_x32(top) * ft;
-                    if (__ballot(top > lim) != 0ull) {
-                        // (scores past 2^20, which f32 holds in steps of an eighth and more, are each rounded as
-                        // the largest was, so that their distances from the base are exact)
-                        const float cap = __builtin_fabsf(base) < kFar ? base - kDown : base;
-                        const float now = top > cap ? top + (__builtin_fabsf(top) < kFar ? kDown + kSlack : 0.0f) : base;
-                        const float alpha = base == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(base - now);
-                        l_run *= alpha;
+                for (int i = 0; i < 16; ++i) sn[0][i] = 0.0f;
 #pragma unroll
-                        for (int c = 0; c < CT; ++c) acc[c] *= alpha;
-                        base = now;
-                        const bool far = !(__builtin_fabsf(base) < kFar) && base != -INFINITY;
-                        lim = far ? -INFINITY : base - kDown;
-                        if (__ballot(far) != 0ull) {
+                for (int i = 0; i < AHEAD; ++i) read(i);
+                __builtin_amdgcn_sched_barrier(0);
+                int done = 0;
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) sc[i] *= ft;
-                            ft = 1.0f;
-                        }
-                    }
-                    const float from = base == -INFINITY ? 0.0f : base;
+                for (int i = 0; i < N; ++i) {
+                    read(i + AHEAD);
+                    if (i < KS) sn[0] = cross_mfma<F16>(f[i], qf[0][0][i], sn[0]);
+                    else acc[0][(i - KS) / 2] = cross_mfma<F16>(f[i], q[(i - KS) % 2], acc[0][(i - KS) / 2]);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], ft, -from));
-                    cross_u32x4 p[QP][2];
-#pragma unroll
-                    for (int s = 0; s < 2; ++s)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint32_t x[QP];
-                            cross_parts<F16, QP>(sc[8 * s + 2 * j], sc[8 * s + 2 * j + 1], x);
-#pragma unroll
-                            for (int k = 0; k < QP; ++k) p[k][s][j] = x[k];
-                        }
-                    // (16-bit ones are summed as they were rounded)
-                    if constexpr (QP == 3) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) l_run += sc[i];
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) l_run = cross_add_pair<F16>(p[0][i / 4][i % 4], ones, l_run);
-                    }
-                    // V^T as the A operand: lane (m, h) takes keys 16 s + 8 b + 4 h .. +4 of column m, b = 0, 1.
-                    // Within each 16-lane group, lane j of a transposing read receives element j % 4 of the 8
-                    // bytes that lanes 4 k + j / 4 address, k = 0 .. 3: lane i points at key i / 4 of the four
-                    // and columns 4 (i % 4) of the group's sixteen.
-                    const int vr = 4 * hf + ((lane & 15) >> 2);
-                    const uint8_t *v0 = mem + VAT + (k0 + vr) * VST + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-#pragma unroll
-                    for (int c = 0; c < CT; ++c)
-#pragma unroll
-                        for (int s = 0; s < 2; ++s)
-#pragma unroll
-                            for (int i = 0; i < KP; ++i) {
-                                typedef short s16x4 __attribute__((ext_vector_type(4)));
-                                const int cc = cross_v_xor(D) ? 64 * (c ^ (vr & 3)) : 64 * c;
-                                const uint8_t *v = v0 + i * VPLANE + cc + 16 * s * VST;
-                                const cross_u32x2 x = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                          (__attribute__((address_space(3))) s16x4 *)v));
-                                const cross_u32x2 y = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                          (__attribute__((address_space(3))) s16x4 *)(v + 8 * VST)));
-                                const cross_u32x4 vf = {x[0], x[1], y[0], y[1]};
-#pragma unroll
-                                for (int j = 0; j < QP; ++j)
-                                    if (i + j < 3) acc[c] = cross_mfma<F16>(vf, p[j][s], acc[c]);
-                            }
+                    for (; done < 8 * (i + 1) / N; ++done) pair(done);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-            }
-            if constexpr (!PRIVATE) {
-                if (NB == 1 && t + 1 < tiles) mark(t + 1, raw, mk, mv);
+                tops(sn, top);
+                // (here, and not where they are used: behind a branch)
+                asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(l_run[0]));
+                if (__builtin_expect(changed, 0)) {
+                    asm volatile("");                  // (a branch: no products by 1)
+                    scale_sums(alpha);
+                }
+            };
+            auto in_pool = [&](int t, int half) __attribute__((always_inline)) {
+                return __builtin_amdgcn_readfirstlane(s_ok[t % 8][half] + 2 * s_ok[t % 8][half + 1]);
+            };
+            // (the step before the first: probabilities of 0, of values that are there)
+            pb[0] = pb[1] = cross_u32x4{0, 0, 0, 0};
+            scores(s_mem, 0, sa);
+            tops(sa, top);
+            int before = 0, at = 0;                    // buffers of tiles t - 1 and t
+            for (int t = 0; t < tiles; ++t) {
+                const int next = at == 2 ? 0 : at + 1;
+                const int64_t rest = sq.len - (key0 + (int64_t)t * TK);
+                step(sa, sb, pa, pb, at, 32, before, 32, rest, in_pool(t, 0), fk_next);
+                if constexpr (F16) {
+                    fk = fk_next;
+                    fv_t = fv_next;
+                    if (tid < 2) s_top[t % 3][tid] = 0;
+                }
+                if (t + 1 < tiles) stage(t);
                 __syncthreads();
-                if (NB == 1 && t + 1 < tiles) {
-                    stage(t);
+                if constexpr (F16) {
+                    // (a power of two that changes: the sums so far are brought under it)
+                    if (__builtin_expect(fv != fv_t, 0)) {
+                        scale_all(fv == 0.0f ? 1.0f : fv_t / fv);
+                        fv = fv_t;
+                    }
+                }
+                step(sb, sa, pb, pa, next, 0, at, 0, rest - 32, in_pool(t, 2), fk);
+                before = at;
+                at = next;
+            }
+            // (the last tile's second half)
+            cross_u32x4 p[RT][QP][2] = {{{pb[0], pb[1]}}};
+            values(s_mem + before * S::TILE, 32, p);
+            __syncthreads();
+        } else {
+            for (int t = 0; t < tiles; ++t) {
+                int ok = 3;                            // whether this wave's halves are in the pool
+                if constexpr (PRIVATE) {
+                    ok = (__builtin_amdgcn_readlane(window, 2 * wave) >= 0 ? 1 : 0) | (__builtin_amdgcn_readlane(window, 2 * wave + 1) >= 0 ? 2 : 0);
+                    if constexpr (F16) {
+                        mark(t, raw, mk, mv);
+                        powers(mk, mv);
+                    }
+                    // (a wave's LDS accesses are in order: the tile before has been read)
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+                    write_tile(t, raw);
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+                    if (t + 1 < tiles) {
+                        look_up(t + 1);
+                        load_tile(t + 1, raw);
+                    }
+                }
+                if constexpr (F16) {
+                    fk = fk_next;
+                    if (fv != fv_next) {
+                        scale_all(fv == 0.0f ? 1.0f : fv_next / fv);
+                        fv = fv_next;
+                    }
+                    if (!PRIVATE && tid < 2) s_top[t % 3][tid] = 0;
+                }
+                if (!PRIVATE && NB == 2 && t + 1 < tiles) stage(t);
+                if (any) {
+                    const uint8_t *mem = s_mem + t % NB * S::TILE;
+#pragma unroll
+                    for (int sub = 0; sub < SUB; ++sub) {
+                        const int k0 = 32 * (wk * SUB + sub);          // the keys' rows in the tile
+                        const int64_t rest = sq.len - (key0 + (int64_t)t * TK + k0);
+                        if (rest <= 0) continue;
+                        cross_f32x16 sc[RT];
+                        cross_u32x4 p[RT][QP][2];
+                        float top[RT], ft[RT], alpha[RT];
+                        scores(mem, k0, sc);
+                        tops(sc, top);
+                        if constexpr (!PRIVATE) ok = __builtin_amdgcn_readfirstlane(s_ok[t % 8][k0 / 16] + 2 * s_ok[t % 8][k0 / 16 + 1]);
+                        hide(rest, ok, sc, top);
+                        factors(fk, ft);
+                        if (rebase(sc, top, ft, alpha)) scale_sums(alpha);
+                        probabilities(sc, ft, p);
+                        values(mem, k0, p);
+                    }
+                }
+                if constexpr (!PRIVATE) {
+                    if (NB == 1 && t + 1 < tiles) mark(t + 1, raw, mk, mv);
                     __syncthreads();
+                    if (NB == 1 && t + 1 < tiles) {
+                        stage(t);
+                        __syncthreads();
+                    }
                 }
             }
+            if constexpr (PRIVATE) __syncthreads();
         }
-        if constexpr (PRIVATE) __syncthreads();
 
         // lane (n, h): columns 32 c + 8 (i / 4) + 4 h + i % 4 of row n in acc[c][i]
-        float l = sum_x32(l_run);
         float unit = F16 && fv != 0.0f ? 1.0f / fv : 1.0f;     // of the sums (pieces' stay under it)
         const int64_t slot = 2 * cell + (t0 == 0 ? 1 : 0);
-        const int64_t prow = slot * ROWS + 32 * rg + r32;
         if constexpr (WK == 1) {
-            // no key at all (every block outside the pool): zeros
-            const float k = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-            if (whole ? live : any) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const float l = sum_x32(l_run[r]);
+                const int64_t prow = slot * ROWS + 32 * (RT * rg + r) + r32;
+                // no key at all (every block outside the pool): zeros
+                const float k = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+                if (whole ? !live[r] : !any) continue;
 #pragma unroll
                 for (int c = 0; c < CT; ++c)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        cross_f32x4 x = cross_f32x4{acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]} * k;
+                        cross_f32x4 x = cross_f32x4{acc[r][c][4 * i], acc[r][c][4 * i + 1], acc[r][c][4 * i + 2], acc[r][c][4 * i + 3]} * k;
                         if (F16 && whole) x *= unit;
                         const int col = 32 * c + 8 * i + 4 * hf;
-                        if (whole) cross_store4(a, io + col, x);
+                        if (whole) cross_store4(a, io[r] + col, x);
                         else *reinterpret_cast<cross_f32x4 *>(a.part_o + prow * D + col) = x;
                     }
-                if (!whole && hf == 0) a.part_ml[prow] = make_float4(base, l, unit, 0.0f);
+                if (!whole && hf == 0) a.part_ml[prow] = make_float4(base[r], l, unit, 0.0f);
             }
         } else {
             // the waves of one row group: their bases' largest, then their sums, CR column tiles at a
             // time, four columns (c, i) of all of them to one wave
-            if (hf == 0) s_ml[wave][r32] = make_float4(base, l, fv, 0.0f);
+            float l = sum_x32(l_run[0]);
+            const int64_t prow = slot * ROWS + 32 * rg + r32;
+            if (hf == 0) s_ml[wave][r32] = make_float4(base[0], l, fv, 0.0f);
             __syncthreads();
             float top = -INFINITY, least = 0.0f;       // (the smallest power of two of the values': the largest unit)
 #pragma unroll
@@ -687,7 +886,7 @@ void paged_cross_kernel(CrossArgs a) {
                 const float4 ml = s_ml[rg * WK + i][r32];
                 l += ml.x == -INFINITY ? ml.y : ml.y * __builtin_amdgcn_exp2f(ml.x - top);
             }
-            float alpha = base == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(base - top);
+            float alpha = base[0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(base[0] - top);
             if (F16 && fv != 0.0f) alpha *= least / fv;
             if (F16) unit = least != 0.0f ? 1.0f / least : 1.0f;
             const float k = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
@@ -699,7 +898,7 @@ void paged_cross_kernel(CrossArgs a) {
                 for (int c = c0; c < c0 + CR && c < CT; ++c)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        x[((wave * CR + c - c0) * 4 + i) * 64] = cross_f32x4{acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]} * alpha;
+                        x[((wave * CR + c - c0) * 4 + i) * 64] = cross_f32x4{acc[0][c][4 * i], acc[0][c][4 * i + 1], acc[0][c][4 * i + 2], acc[0][c][4 * i + 3]} * alpha;
                 __syncthreads();
                 const int quads = 4 * (CT - c0 < CR ? CT - c0 : CR);
                 for (int g = wk; g < quads; g += WK) {
@@ -710,7 +909,7 @@ void paged_cross_kernel(CrossArgs a) {
                     if (F16 && whole) y *= unit;
                     const int col = 32 * (c0 + g / 4) + 8 * (g % 4) + 4 * hf;
                     if (whole) {
-                        if (live) cross_store4(a, io + col, y);
+                        if (live[0]) cross_store4(a, io[0] + col, y);
                     } else if (any) {
                         *reinterpret_cast<cross_f32x4 *>(a.part_o + prow * D + col) = y;
                     }
