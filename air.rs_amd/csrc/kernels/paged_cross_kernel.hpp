@@ -58,8 +58,8 @@ constexpr int cross_tile_bytes(int d, int parts, int keys) { return keys * parts
 // Waves of a workgroup, and workgroups a CU: registers leave room for four waves a SIMD (small
 // heads), two, or (queries in three parts and their sums, the largest heads) one.
 constexpr bool cross_pipe(int d, int qp, bool few) { return !few && qp == 1 && d <= 128; }
-constexpr int cross_waves(int d, int qp, bool few) { return few || (qp == 3 ? d >= 96 : d >= 192) ? 4 : 8; }
-constexpr int cross_groups(int d, int qp, bool few) { return few ? (d <= (qp == 3 ? 64 : 128) ? 2 : 1) : 1; }
+constexpr int cross_waves(int d, int qp, bool few) { return few || (cross_pipe(d, qp, few) && d <= 64) || (qp == 3 ? d >= 96 : d >= 192) ? 4 : 8; }
+constexpr int cross_groups(int d, int qp, bool few) { return few ? (d <= (qp == 3 ? 64 : 128) ? 2 : 1) : cross_pipe(d, qp, few) && d <= 64 ? 2 : 1; }
 // What a workgroup's tiles may take of a CU's 160 KB.
 constexpr int cross_lds(int groups) { return 160 * 1024 / groups - 7 * 1024; }
 // Waves that share rows: as many as have room for 32 keys each.
