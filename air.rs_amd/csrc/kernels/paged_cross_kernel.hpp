@@ -46,6 +46,7 @@ typedef uint32_t cross_u32x2 __attribute__((ext_vector_type(2)));
 enum CrossKind { kBf16, kCodes, kParts, kWide };
 
 constexpr int kCrossBuffer = 0x00020000;           // a raw buffer's last word
+constexpr int kCrossStream = 2;                    // non-temporal: pages are read once
 constexpr int kCrossNowhere = 0x40000000;          // an offset outside of every buffer: reads zeros
 
 // Rows of keys and of values in LDS, bytes apart.  Keys: 16 bytes more than a whole number of
@@ -111,13 +112,19 @@ template <bool F16> __device__ __forceinline__ float cross_add_pair(uint32_t p, 
     if constexpr (F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(cross_f16x2, p), __builtin_bit_cast(cross_f16x2, ones), c, false);
     else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(cross_bf16x2, p), __builtin_bit_cast(cross_bf16x2, ones), c, false);
 }
-// The values of the four 1-byte codes in w times their scale.
-__device__ __forceinline__ cross_f32x4 cross_codes(bool fp8, uint32_t w, float s) {
-    if (fp8) {
+// The values of the four 1-byte codes in w times their scale.  SMALL: |s| is below 2^100; int8 codes
+// then take two instructions each, (code + 128) s - 128 s in one step (128 s is exact, and the
+// unsigned byte's conversion takes it from its place).
+template <int DT, bool SMALL> __device__ __forceinline__ cross_f32x4 cross_codes(uint32_t w, float s) {
+    if constexpr (DT == AIR_KV_FP8) {
         const cross_f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
         return cross_f32x4{lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
-    }
-    return cross_f32x4{(float)(int8_t)w * s, (float)(int8_t)(w >> 8) * s, (float)(int8_t)(w >> 16) * s, (float)(int8_t)(w >> 24) * s};
+    } else if constexpr (SMALL) {
+        const uint32_t u = w ^ 0x80808080u;
+        const float off = -128.0f * s;
+        return cross_f32x4{__builtin_fmaf((float)(u & 0xFFu), s, off), __builtin_fmaf((float)((u >> 8) & 0xFFu), s, off),
+                           __builtin_fmaf((float)((u >> 16) & 0xFFu), s, off), __builtin_fmaf((float)(u >> 24), s, off)};
+    } else return cross_f32x4{(float)(int8_t)w * s, (float)(int8_t)(w >> 8) * s, (float)(int8_t)(w >> 16) * s, (float)(int8_t)(w >> 24) * s};
 }
 // The largest of the wave's lanes' x >= 0.
 __device__ __forceinline__ float cross_wave_max(float x) {
@@ -161,6 +168,7 @@ void paged_cross_kernel(CrossArgs a) {
     constexpr int LPR = D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32, WR = 64 / LPR, NPH = 16 / WR;
     constexpr int SH = 2 * TK / 16 / WAVES, NP = SH * NPH;
     static_assert(SH >= 1 && SH * WAVES * 16 == 2 * TK && (SH == 1 || SH % 2 == 0), "whole halves");
+    constexpr int kOnce = FEW ? kCrossStream : 0;
     constexpr int JOIN = WAVES * 64 * 16 * 4;          // bytes of a column tile of every wave's sums, at a block's end
     constexpr int MEM = NB * S::TILE > JOIN || WK == 1 ? NB * S::TILE : JOIN;
     constexpr int CR = MEM / JOIN < CT ? MEM / JOIN : CT;      // column tiles joined at once (WK > 1)
@@ -391,15 +399,15 @@ void paged_cross_kernel(CrossArgs a) {
                 for (int k = 0; k < NPH; ++k) {
                     const int i = j * NPH + k;
                     if constexpr (KIND == kBf16 || KIND == kParts) {
-                        raw.w[i][0] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + k * WR * D * 2, 0, 0));
+                        raw.w[i][0] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + k * WR * D * 2, 0, kOnce));
                     } else if (KIND == kCodes || a.dtype != AIR_KV_F32) {
-                        const cross_u32x2 x = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, p_off + k * WR * D, 0, 0));
+                        const cross_u32x2 x = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, p_off + k * WR * D, 0, kOnce));
                         raw.w[i][0][0] = x[0];
                         raw.w[i][0][1] = x[1];
                         raw.s[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ss, p_sc + k * WR * nsc * 4, 0, 0));
                     } else if constexpr (KIND == kWide) {
-                        raw.w[i][0] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + k * WR * D * 4, 0, 0));
-                        raw.w[i][1] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + k * WR * D * 4 + 16, 0, 0));
+                        raw.w[i][0] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + k * WR * D * 4, 0, kOnce));
+                        raw.w[i][1] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + k * WR * D * 4 + 16, 0, kOnce));
                     }
                 }
             }
@@ -437,40 +445,48 @@ void paged_cross_kernel(CrossArgs a) {
             uint8_t *mem = s_mem + t % NB * S::TILE;
             if constexpr (F16 && !PRIVATE)
                 powers(__uint_as_float(__builtin_amdgcn_readfirstlane(s_top[t % 3][0])), __uint_as_float(__builtin_amdgcn_readfirstlane(s_top[t % 3][1])));
+            // (the type is asked for once a tile)
+            auto rows = [&](auto type) __attribute__((always_inline)) {
+                constexpr int DT = decltype(type)::value;
 #pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const bool val = of_values(i / NPH);
-                const int at = 16 * half_of(i / NPH) + i % NPH * WR + lane / LPR;
-                const int chunk = val && cross_v_xor(D) ? p_c ^ ((at & 3) << 2) : p_c;
-                uint8_t *to = mem + (val ? VAT + at * VST : at * KST) + 16 * chunk;
-                const int plane = val ? VPLANE : KPLANE;
-                if constexpr (KIND == kBf16 || KIND == kParts) {
-                    if (p_in) *reinterpret_cast<cross_u32x4 *>(to) = raw.w[i][0];
-                } else {
-                    float x[8];
-                    if (KIND == kWide && a.dtype == AIR_KV_F32) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(raw.w[i][KIND == kWide ? j / 4 : 0][j % 4]);
-                    } else {
-                        const float sc = F16 ? raw.s[i] * (val ? fv_next : fk_next) : raw.s[i];
-                        const cross_f32x4 lo = cross_codes(a.dtype == AIR_KV_FP8, raw.w[i][0][0], sc);
-                        const cross_f32x4 hi = cross_codes(a.dtype == AIR_KV_FP8, raw.w[i][0][1], sc);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) { x[j] = lo[j]; x[4 + j] = hi[j]; }
-                    }
+                for (int i = 0; i < NP; ++i) {
+                    const bool val = of_values(i / NPH);
+                    const int at = 16 * half_of(i / NPH) + i % NPH * WR + lane / LPR;
+                    const int chunk = val && cross_v_xor(D) ? p_c ^ ((at & 3) << 2) : p_c;
+                    uint8_t *to = mem + (val ? VAT + at * VST : at * KST) + 16 * chunk;
+                    const int plane = val ? VPLANE : KPLANE;
                     cross_u32x4 y[KP];
+                    if constexpr (DT == AIR_KV_BF16) {
+                        y[0] = raw.w[i][0];
+                    } else {
+                        float x[8];
+                        if constexpr (DT == AIR_KV_F32) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t p[KP];
-                        cross_parts<F16, KP>(x[2 * j], x[2 * j + 1], p);
+                            for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(raw.w[i][KIND == kWide ? j / 4 : 0][j % 4]);
+                        } else {
+                            // (scales of groups of zeros were left out: theirs may be any size)
+                            const float sc = F16 ? __builtin_amdgcn_fmed3f(raw.s[i] * (val ? fv_next : fk_next), -0x1p100f, 0x1p100f) : raw.s[i];
+                            const cross_f32x4 lo = cross_codes<DT, F16>(raw.w[i][0][0], sc), hi = cross_codes<DT, F16>(raw.w[i][0][1], sc);
 #pragma unroll
-                        for (int k = 0; k < KP; ++k) y[k][j] = p[k];
+                            for (int j = 0; j < 4; ++j) { x[j] = lo[j]; x[4 + j] = hi[j]; }
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t p[KP];
+                            cross_parts<F16, KP>(x[2 * j], x[2 * j + 1], p);
+#pragma unroll
+                            for (int k = 0; k < KP; ++k) y[k][j] = p[k];
+                        }
                     }
 #pragma unroll
                     for (int k = 0; k < KP; ++k)
                         if (p_in) *reinterpret_cast<cross_u32x4 *>(to + k * plane) = y[k];
                 }
-            }
+            };
+            if constexpr (KIND == kBf16 || KIND == kParts) rows(std::integral_constant<int, AIR_KV_BF16>{});
+            else if (KIND == kWide && a.dtype == AIR_KV_F32) rows(std::integral_constant<int, AIR_KV_F32>{});
+            else if (a.dtype == AIR_KV_INT8) rows(std::integral_constant<int, AIR_KV_INT8>{});
+            else rows(std::integral_constant<int, AIR_KV_FP8>{});
         };
         float mk = 0.0f, mv = 0.0f;
         // Many rows: what comes between two tiles' products, t the one at hand: tile t + 1 into its
