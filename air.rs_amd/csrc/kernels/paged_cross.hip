@@ -171,7 +171,7 @@ hipError_t launch_cross(const air_kv_pool &p, hipStream_t s, const void *q, int3
     a.v_scales = p.v_scales;
     a.errors = p.errors;
     a.slices = slices_of(p, blocks);
-    a.least = 3;
+    a.least = 1;
     a.desc = (int4 *)workspace;
     a.part_ml = (float4 *)((char *)workspace + ws.ml);
     a.part_o = (float *)((char *)workspace + ws.o);

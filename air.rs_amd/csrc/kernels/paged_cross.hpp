@@ -4,7 +4,7 @@
 // sequence's cached tokens:
 //   s[t] = scale * q . K[t],  out = sum_t exp(s[t] - max s) V[t] / sum_t exp(s[t] - max s)
 // A sequence's rows at one K/V head (token after token, query head after query head) are cut
-// into blocks, a block's keys into tiles.  A block counts as kCrossExtra units (what its
+// into blocks, a block's keys into tiles.  A block counts as `extra` units (what its
 // beginning and end cost beside a tile) and one for each tile; the K/V head's units, sequence
 // after sequence, block after block, are cut into equal slices, one workgroup each.  A block
 // that several slices hold is joined by a second kernel, piece after piece in order.
@@ -18,7 +18,9 @@
 namespace airkv {
 
 constexpr int kCrossBatch = 512;       // sequences per launch (the host splits larger batches)
-constexpr int kCrossExtra = 1;
+// what a block's beginning and end cost beside a tile (many rows, 16-bit: 1, 3, 6: 279, 269, 267 us
+// for int8 chunks, 93, 91, 92 for small heads; few rows: 111, 114, 113)
+constexpr int cross_extra(bool few) { return few ? 1 : 3; }
 
 struct CrossArgs {
     const void *q;                     // [total_q][q_heads][head_dim]
@@ -58,10 +60,10 @@ __device__ __forceinline__ CrossSeq cross_seq(const CrossArgs &a, int b) {
 }
 
 // ROWS rows a block, TK keys a tile.
-template <int ROWS, int TK> __device__ __forceinline__ int32_t cross_tiles(const CrossSeq &s) { return (int32_t)(((int64_t)s.len + TK - 1) / TK); }
-template <int ROWS, int TK> __device__ __forceinline__ int64_t cross_units(const CrossSeq &s) {
-    const int64_t tiles = cross_tiles<ROWS, TK>(s);
-    return tiles ? ((int64_t)s.rows + ROWS - 1) / ROWS * (tiles + kCrossExtra) : 0;
+template <int TK> __device__ __forceinline__ int32_t cross_tiles(const CrossSeq &s) { return (int32_t)(((int64_t)s.len + TK - 1) / TK); }
+template <int ROWS, int TK, int EXTRA> __device__ __forceinline__ int64_t cross_units(const CrossSeq &s) {
+    const int64_t tiles = cross_tiles<TK>(s);
+    return tiles ? ((int64_t)s.rows + ROWS - 1) / ROWS * (tiles + EXTRA) : 0;
 }
 
 // Rows of a block, and workgroups that are resident on a CU.

@@ -168,6 +168,7 @@ void paged_cross_kernel(CrossArgs a) {
     constexpr int LPR = D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32, WR = 64 / LPR, NPH = 16 / WR;
     constexpr int SH = 2 * TK / 16 / WAVES, NP = SH * NPH;
     static_assert(SH >= 1 && SH * WAVES * 16 == 2 * TK && (SH == 1 || SH % 2 == 0), "whole halves");
+    constexpr int EXTRA = cross_extra(FEW);
     constexpr int kOnce = FEW ? kCrossStream : 0;
     constexpr int JOIN = WAVES * 64 * 16 * 4;          // bytes of a column tile of every wave's sums, at a block's end
     constexpr int MEM = NB * S::TILE > JOIN || WK == 1 ? NB * S::TILE : JOIN;
@@ -187,25 +188,15 @@ void paged_cross_kernel(CrossArgs a) {
     const int head = blockIdx.x % a.heads, w = blockIdx.x / a.heads;
     const int64_t cell = (int64_t)head * a.slices + w;
 
-    // sequences without work here: rows of refused ones (counted) and of empty ones are zeros
-    for (int b = w; b < a.batch; b += a.slices) {
-        const CrossSeq s = cross_seq(a, b);
-        if (s.ok && (s.len || !s.rows)) continue;
-        if (!s.ok && head == 0 && tid == 0) atomicAdd(a.errors, 1ull);
-        const int32_t r0 = a.cu[b], r1 = a.cu[b + 1];
-        if (r0 < 0 || r1 > a.total_q || r1 < r0) continue;
-        const int64_t n = (int64_t)(r1 - r0) * a.group * (D / 4);
-        for (int64_t i = tid; i < n; i += THREADS) {
-            const int64_t row = i / (D / 4), c = i % (D / 4) * 4;
-            cross_store4(a, ((r0 + row / a.group) * a.q_heads + head * a.group + row % a.group) * D + c, cross_f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-        }
-    }
     // units before each sequence
+    int idle = 0;                                      // whether some sequence has rows and no work
     {
         const int per = (a.batch + THREADS - 1) / THREADS, lo = min(tid * per, a.batch), hi = min(lo + per, a.batch);
         int64_t mine = 0;
         for (int b = lo; b < hi; ++b) {
-            const int64_t u = cross_units<ROWS, TK>(cross_seq(a, b));
+            const CrossSeq s = cross_seq(a, b);
+            const int64_t u = cross_units<ROWS, TK, EXTRA>(s);
+            idle |= !s.ok || (s.rows && !s.len);
             s_pre[b + 1] = u;
             mine += u;
         }
@@ -217,7 +208,7 @@ void paged_cross_kernel(CrossArgs a) {
         }
         if (lane == 63) s_sum[wave] = incl;
         if (tid == 0) s_pre[0] = 0;
-        __syncthreads();
+        idle = __syncthreads_or(idle);
         int64_t run = incl - mine;
         for (int i = 0; i < wave; ++i) run += s_sum[i];
         for (int b = lo; b < hi; ++b) {
@@ -225,6 +216,21 @@ void paged_cross_kernel(CrossArgs a) {
             s_pre[b + 1] = run;
         }
         __syncthreads();
+    }
+    // sequences without work: rows of refused ones (counted) and of empty ones are zeros
+    if (idle) {
+        for (int b = w; b < a.batch; b += a.slices) {
+            const CrossSeq s = cross_seq(a, b);
+            if (s.ok && (s.len || !s.rows)) continue;
+            if (!s.ok && head == 0 && tid == 0) atomicAdd(a.errors, 1ull);
+            const int32_t r0 = a.cu[b], r1 = a.cu[b + 1];
+            if (r0 < 0 || r1 > a.total_q || r1 < r0) continue;
+            const int64_t n = (int64_t)(r1 - r0) * a.group * (D / 4);
+            for (int64_t i = tid; i < n; i += THREADS) {
+                const int64_t row = i / (D / 4), c = i % (D / 4) * 4;
+                cross_store4(a, ((r0 + row / a.group) * a.q_heads + head * a.group + row % a.group) * D + c, cross_f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+            }
+        }
     }
     const int64_t units = cross_uniform(s_pre[a.batch]);
     int64_t chunk = (units + a.slices - 1) / a.slices;
@@ -265,13 +271,13 @@ void paged_cross_kernel(CrossArgs a) {
         sq.row0 = __builtin_amdgcn_readfirstlane(sq.row0);
         sq.rows = __builtin_amdgcn_readfirstlane(sq.rows);
         sq.len = __builtin_amdgcn_readfirstlane(sq.len);
-        const int nt = cross_tiles<ROWS, TK>(sq);
+        const int nt = cross_tiles<TK>(sq);
         const int64_t in = u - cross_uniform(s_pre[b]);
-        const int blk = (int)(in / (nt + kCrossExtra)), at = (int)(in - (int64_t)blk * (nt + kCrossExtra));
-        const int64_t left = nt + kCrossExtra - at, mine = end - u < left ? end - u : left;
-        // a block's first kCrossExtra units are its beginning
-        const int t0 = at < kCrossExtra ? 0 : at - kCrossExtra;
-        const int t1 = at + (int)mine < kCrossExtra ? 0 : at + (int)mine - kCrossExtra;
+        const int blk = (int)(in / (nt + EXTRA)), at = (int)(in - (int64_t)blk * (nt + EXTRA));
+        const int64_t left = nt + EXTRA - at, mine = end - u < left ? end - u : left;
+        // a block's first EXTRA units are its beginning
+        const int t0 = at < EXTRA ? 0 : at - EXTRA;
+        const int t1 = at + (int)mine < EXTRA ? 0 : at + (int)mine - EXTRA;
         u += mine;
         if (t0 == t1) continue;                        // the slice ends before the block's first tile
         const bool whole = t0 == 0 && t1 == nt;
@@ -934,7 +940,7 @@ void paged_cross_kernel(CrossArgs a) {
             if (!whole && any && hf == 0 && wk == 0) a.part_ml[prow] = make_float4(top, l, unit, 0.0f);
         }
         if (!whole && t0 == 0) {                       // begun here: its last unit's slice ends it
-            const int64_t last = u - mine - at + nt + kCrossExtra - 1;
+            const int64_t last = u - mine - at + nt + EXTRA - 1;
             begun = int4{b, blk, (int)(last / chunk - w + 1), 0};
         }
     }
