@@ -40,41 +40,56 @@ struct Rotary {
     float magnitude;
 };
 
-// Four elements of an activation row.
-template <bool HALF> __device__ __forceinline__ void load4(const void *p, int64_t at, float (&x)[4]) {
-    if constexpr (HALF) {
-        const u32x2 w = *reinterpret_cast<const u32x2 *>((const uint16_t *)p + at);
+// Four elements as they lie in memory (bf16 or f32), and as f32.
+template <bool HALF> struct Four;
+template <> struct Four<true> {
+    u32x2 w;
+    __device__ __forceinline__ void load(const void *p, int64_t at) { w = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>((const uint16_t *)p + at)); }
+    __device__ __forceinline__ void get(float *x) const {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             x[2 * j] = __uint_as_float(w[j] << 16);
             x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
         }
-    } else {
-        const f32x4 w = *reinterpret_cast<const f32x4 *>((const float *)p + at);
+    }
+};
+template <> struct Four<false> {
+    f32x4 w;
+    __device__ __forceinline__ void load(const void *p, int64_t at) { w = *reinterpret_cast<const f32x4 *>((const float *)p + at); }
+    __device__ __forceinline__ void get(float *x) const {
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = w[j];
     }
+};
+
+// 8 f32 to a page or an output of type DT, as store_row_chunk; bf16 by the hardware's rounding (to
+// nearest even, a NaN stays one), where bf16_rne's branches cost more than all else.
+template <int DT>
+__device__ __forceinline__ void store8(const float (&x)[8], void *pages, float *scales, int64_t elem, int64_t scale_idx, bool lead, int lanes) {
+    if constexpr (DT == AIR_KV_BF16) {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        u32x4 w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x[2 * j], x[2 * j + 1]}), bf16x2));
+        *reinterpret_cast<u32x4 *>((uint16_t *)pages + elem) = w;
+    } else {
+        store_row_chunk<DT>(x, pages, scales, elem, scale_idx, lead, lanes, true);
+    }
 }
 
-// The 8 elements x from element e on of a row, turned; four(at, y) gives the row's elements
-// at .. at + 3.
-template <typename F>
-__device__ __forceinline__ void turn8(float (&x)[8], const Rotary &r, const float2 *cs, int e, F four) {
-    float z[2][4], y[2][4];
-    if (!r.pairs) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (e + 4 * i < r.rot) four(rotary_partner(e + 4 * i, r.rot / 2), y[i]);
-    }
+// The 8 elements x from element e on of a row, turned; y their partners (half layout).
+__device__ __forceinline__ void turn8(float (&x)[8], const float (&y)[2][4], const Rotary &r, const float2 *cs, int e) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         if (e + 4 * i >= r.rot) continue;
+        float z[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) z[i][j] = x[4 * i + j];
-        if (r.pairs) rotary_pairs4(z[i], cs, e + 4 * i);
-        else rotary_half4(z[i], y[i], cs, e + 4 * i, r.rot / 2);
+        for (int j = 0; j < 4; ++j) z[j] = x[4 * i + j];
+        if (r.pairs) rotary_pairs4(z, cs, e + 4 * i);
+        else rotary_half4(z, y[i], cs, e + 4 * i, r.rot / 2);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[4 * i + j] = z[i][j];
+        for (int j = 0; j < 4; ++j) x[4 * i + j] = z[j];
     }
 }
 
@@ -90,54 +105,78 @@ struct AppendArgs {
     int32_t per_part;                               // rows (heads of q, k and v) of a workgroup
 };
 
-// One token and per_part of its rows (query heads, then key heads, then value heads).
+// One token and per_part of its rows (query heads, then key heads, then value heads).  A row is
+// read before the one before it is stored; the angles are computed while the first is on its way.
 template <int DT, bool IN16, bool OUT16>
 __global__ __launch_bounds__(kThreads) void append_rotary_kernel(AppendArgs a) {
     __shared__ float2 s_cs[kMaxPairs];
     const int64_t t = blockIdx.x;
     const int tid = threadIdx.x, d = a.p.head_dim;
-    const int e = (tid & ((1 << a.p.lanes_log2) - 1)) * 8;
-    const int position = a.positions[t];
-    const int64_t slot = a.slots[t];
-    if (tid < a.r.rot / 2) s_cs[tid] = rotary_turn(position, a.r.inv_freq[tid], a.r.magnitude);
-    if (blockIdx.y == 0 && tid == 0 && slot >= a.p.num_blocks << a.p.bs_log2) atomicAdd(a.p.errors, 1ull);
-    const bool kept = slot >= 0 && slot < a.p.num_blocks << a.p.bs_log2;
+    const int e = (tid & ((1 << a.p.lanes_log2) - 1)) * 8, step = kThreads >> a.p.lanes_log2;
     const int all = a.q_heads + 2 * a.p.heads;
     const int end = min(all, (int)(blockIdx.y + 1) * a.per_part);
+    struct Row {
+        Four<IN16> own[2], partner[2];
+    };
+    auto load = [&](int row, Row &x) __attribute__((always_inline)) {
+        if (row >= end || e >= d) return;
+        const bool q = row < a.q_heads, k = !q && row < a.q_heads + a.p.heads;
+        const void *src = q ? a.q : k ? a.k : a.v;
+        const int h = q ? row : k ? row - a.q_heads : row - a.q_heads - a.p.heads;
+        const int64_t from = t * (q ? a.q_stride : k ? a.k_stride : a.v_stride) + (int64_t)h * d;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x.own[i].load(src, from + e + 4 * i);
+        if ((q || k) && !a.r.pairs) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (e + 4 * i < a.r.rot) x.partner[i].load(src, from + rotary_partner(e + 4 * i, a.r.rot / 2));
+        }
+    };
+    int row = blockIdx.y * a.per_part + (tid >> a.p.lanes_log2);
+    const int64_t slot = a.slots[t];
+    const int position = a.positions[t];
+    Row now, next;
+    load(row, now);
+    const bool kept = slot >= 0 && slot < a.p.num_blocks << a.p.bs_log2;
+    if (blockIdx.y == 0 && tid == 0 && slot >= a.p.num_blocks << a.p.bs_log2) atomicAdd(a.p.errors, 1ull);
+    if (tid < a.r.rot / 2) s_cs[tid] = rotary_turn(position, a.r.inv_freq[tid], a.r.magnitude);
     __syncthreads();
     if (e >= d) return;
-    for (int row = blockIdx.y * a.per_part + (tid >> a.p.lanes_log2); row < end; row += kThreads >> a.p.lanes_log2) {
+    constexpr bool QUANT = DT == AIR_KV_INT8 || DT == AIR_KV_FP8;      // (their codes need the registers)
+    for (; row < end; row += step) {
+        if (!QUANT) load(row + step, next);
         const int kind = row < a.q_heads ? 0 : row < a.q_heads + a.p.heads ? 1 : 2;
-        if (kind && !kept) continue;
-        const int h = kind == 0 ? row : kind == 1 ? row - a.q_heads : row - a.q_heads - a.p.heads;
-        const void *src = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-        const int64_t from = t * (kind == 0 ? a.q_stride : kind == 1 ? a.k_stride : a.v_stride) + (int64_t)h * d;
-        float x[8];
-        {
-            float lo[4], hi[4];
-            load4<IN16>(src, from + e, lo);
-            load4<IN16>(src, from + e + 4, hi);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { x[j] = lo[j]; x[4 + j] = hi[j]; }
-        }
-        if (kind < 2) turn8(x, a.r, s_cs, e, [&](int at, float (&y)[4]) { load4<IN16>(src, from + at, y); });
-        if (kind == 0) {
-            const int64_t to = (t * a.q_heads + h) * d + e;
-            if constexpr (OUT16) store_row_chunk<AIR_KV_BF16>(x, a.q_out, nullptr, to, 0, false, 1, true);
-            else store_row_chunk<AIR_KV_F32>(x, a.q_out, nullptr, to, 0, false, 1, true);
-        } else {
-            const int64_t dst = (((slot >> a.p.bs_log2) * a.p.heads + h) << a.p.bs_log2) + (slot & ((1 << a.p.bs_log2) - 1));
-            int lanes = 1;
-            int64_t sc = 0;
-            bool lead = false;
-            if constexpr (DT == AIR_KV_INT8 || DT == AIR_KV_FP8) {
-                lanes = 1 << (a.p.sg_log2 - 3);
-                sc = dst * (d >> a.p.sg_log2) + (e >> a.p.sg_log2);
-                lead = ((e >> 3) & (lanes - 1)) == 0;
+        if (kind == 0 || kept) {
+            float x[8], y[2][4];
+            now.own[0].get(x);
+            now.own[1].get(x + 4);
+            if (kind < 2) {
+                if (!a.r.pairs) {
+                    now.partner[0].get(y[0]);
+                    now.partner[1].get(y[1]);
+                }
+                turn8(x, y, a.r, s_cs, e);
             }
-            store_row_chunk<DT>(x, kind == 1 ? a.p.k_pages : a.p.v_pages, kind == 1 ? a.p.k_scales : a.p.v_scales, dst * d + e,
-                                sc, lead, lanes, true);
+            if (kind == 0) {
+                const int64_t to = (t * a.q_heads + row) * d + e;
+                if constexpr (OUT16) store8<AIR_KV_BF16>(x, a.q_out, nullptr, to, 0, false, 1);
+                else store8<AIR_KV_F32>(x, a.q_out, nullptr, to, 0, false, 1);
+            } else {
+                const int h = kind == 1 ? row - a.q_heads : row - a.q_heads - a.p.heads;
+                const int64_t dst = (((slot >> a.p.bs_log2) * a.p.heads + h) << a.p.bs_log2) + (slot & ((1 << a.p.bs_log2) - 1));
+                int lanes = 1;
+                int64_t sc = 0;
+                bool lead = false;
+                if constexpr (DT == AIR_KV_INT8 || DT == AIR_KV_FP8) {
+                    lanes = 1 << (a.p.sg_log2 - 3);
+                    sc = dst * (d >> a.p.sg_log2) + (e >> a.p.sg_log2);
+                    lead = ((e >> 3) & (lanes - 1)) == 0;
+                }
+                store8<DT>(x, kind == 1 ? a.p.k_pages : a.p.v_pages, kind == 1 ? a.p.k_scales : a.p.v_scales, dst * d + e, sc, lead, lanes);
+            }
         }
+        if (QUANT) load(row + step, now);
+        else now = next;
     }
 }
 
@@ -146,9 +185,13 @@ template <int DT>
 __device__ __forceinline__ void cached4(const void *pages, const float *scales, int64_t row, int d, int sg_log2, int e, float (&x)[4]) {
     const int64_t at = row * d + e;
     if constexpr (DT == AIR_KV_F32) {
-        load4<false>(pages, at, x);
+        Four<false> f;
+        f.load(pages, at);
+        f.get(x);
     } else if constexpr (DT == AIR_KV_BF16) {
-        load4<true>(pages, at, x);
+        Four<true> f;
+        f.load(pages, at);
+        f.get(x);
     } else {
         const uint32_t w = *reinterpret_cast<const uint32_t *>((const uint8_t *)pages + at);
         const float s = scales[row * (d >> sg_log2) + (e >> sg_log2)];
@@ -204,6 +247,7 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
         }
         if (tid < kRun) s_by[tid] = by;
         if (!__syncthreads_or(by != 0)) continue;      // (also: the rows of the run before are done)
+#pragma unroll 1
         for (int i = tid; i < here * half; i += kThreads) {
             const int k = i / half;
             s_cs[i] = rotary_turn(s_by[k], a.r.inv_freq[i - k * half], 1.0f);
@@ -226,12 +270,92 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
                 four(e + 4, hi);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) { x[j] = lo[j]; x[4 + j] = hi[j]; }
-                turn8(x, a.r, s_cs + k * half, e, four);
+                float y[2][4];
+                if (!a.r.pairs) {
+#pragma unroll
+                    for (int p = 0; p < 2; ++p)
+                        if (e + 4 * p < a.r.rot) four(rotary_partner(e + 4 * p, half), y[p]);
+                }
+                turn8(x, y, a.r, s_cs + k * half, e);
                 const int64_t sc = QUANT ? row * (d >> a.p.sg_log2) + (e >> a.p.sg_log2) : 0;
-                store_row_chunk<DT>(x, a.p.k_pages, a.p.k_scales, row * d + e, sc, ((e >> 3) & (lanes - 1)) == 0, lanes, true);
+                store8<DT>(x, a.p.k_pages, a.p.k_scales, row * d + e, sc, ((e >> 3) & (lanes - 1)) == 0, lanes);
             }
         }
         __syncthreads();
+    }
+}
+
+// The same where a row is floats and rot a multiple of 16: a lane owns 8 elements and their 8
+// partners (or 16 neighbours) of one token's rows, so nothing is read twice, and the pairs' c and s
+// stay in its registers from head to head.  A row is read before the one before it is stored.
+template <bool HALF, bool PAIRS>
+__global__ __launch_bounds__(kThreads) void rotate_floats_kernel(RotateArgs a) {
+    __shared__ float2 s_cs[kRun * kMaxPairs];
+    const int b = blockIdx.x, tid = threadIdx.x, d = a.p.head_dim, half = a.r.rot / 2;
+    const int c0 = a.cu[b], c1 = a.cu[b + 1];
+    if (c0 < 0 || c1 > a.total || c1 < c0) {
+        if (blockIdx.y == 0 && tid == 0) atomicAdd(a.p.errors, 1ull);
+        return;
+    }
+    const int n = c1 - c0;
+    int lanes_log2 = 0;                                // of a row, 16 elements each
+    while (16 << lanes_log2 < a.r.rot) ++lanes_log2;
+    const int part = tid & ((1 << lanes_log2) - 1), k = (tid >> lanes_log2) % kRun;
+    const int group = tid >> lanes_log2 >> 4, groups = kThreads >> lanes_log2 >> 4;        // of heads
+    const int e0 = PAIRS ? 16 * part : 8 * part, e1 = PAIRS ? e0 + 8 : e0 + half;
+    const int stride = (int)gridDim.y * kRun;
+    for (int64_t at = (int64_t)blockIdx.y * kRun; at < n; at += stride) {
+        const int64_t index = at >> a.p.bs_log2;
+        const int32_t block = index < a.max_blocks ? a.tables[(int64_t)b * a.max_blocks + index] : -1;
+        const int here = n - at < kRun ? (int)(n - at) : kRun;
+        auto turn = [&](int i) __attribute__((always_inline)) -> int64_t {     // of token i of the run
+            const int64_t j = c0 + at + i;
+            return i < here ? (a.to ? (int64_t)a.to[j] : at + i) - a.from[j] : 0;
+        };
+        const int64_t by = turn(k);
+        if (block < 0 || block >= a.p.num_blocks) {
+            if (tid == 0) atomicAdd(a.p.errors, (unsigned long long)here);
+            continue;
+        }
+        const bool mine = by != 0 && 16 * part < a.r.rot;
+        const int64_t row = (((int64_t)block * a.p.heads << a.p.bs_log2) + (at & ((1 << a.p.bs_log2) - 1)) + k) * d;
+        Four<HALF> now[4], next[4];
+        auto load = [&](int h, Four<HALF> (&x)[4]) __attribute__((always_inline)) {
+            if (!mine || h >= a.p.heads) return;
+            const int64_t from = row + ((int64_t)h << a.p.bs_log2) * d;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i].load(a.p.k_pages, from + (i < 2 ? e0 + 4 * i : e1 + 4 * (i - 2)));
+        };
+        load(group, now);
+        if (!__syncthreads_or(by != 0)) continue;      // (also: the angles of the run before are used)
+        // (lanes a row hold 8 pairs each)
+#pragma unroll 1                                       // (unrolled, it takes the registers of the rows on their way)
+        for (int i = tid; i < kRun << (lanes_log2 + 3); i += kThreads) {
+            const int token = i >> (lanes_log2 + 3), pair = i & ((8 << lanes_log2) - 1);
+            if (pair < half) s_cs[token * half + pair] = rotary_turn(turn(token), a.r.inv_freq[pair], 1.0f);
+        }
+        __syncthreads();
+        if (!mine) continue;
+        float2 cs[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) cs[j] = s_cs[k * half + 8 * part + j];
+#pragma unroll 1
+        for (int h = group; h < a.p.heads; h += groups) {
+            load(h + groups, next);
+            float x[2][8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) now[i].get(x[i / 2] + 4 * (i % 2));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {              // pair j: elements j of both halves, or neighbours
+                if constexpr (PAIRS) rotary_pair(x[j / 4][2 * (j % 4)], x[j / 4][2 * (j % 4) + 1], cs[j]);
+                else rotary_pair(x[0][j], x[1][j], cs[j]);
+            }
+            const int64_t to = row + ((int64_t)h << a.p.bs_log2) * d;
+            store8<HALF ? AIR_KV_BF16 : AIR_KV_F32>(x[0], a.p.k_pages, nullptr, to + e0, 0, false, 1);
+            store8<HALF ? AIR_KV_BF16 : AIR_KV_F32>(x[1], a.p.k_pages, nullptr, to + e1, 0, false, 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) now[i] = next[i];
+        }
     }
 }
 
@@ -315,6 +439,17 @@ hipError_t launch_rotate(const air_kv_pool &p, hipStream_t s, const int32_t *tab
     // runs are dealt to workgroups; eight a CU are resident
     const int64_t runs = ((int64_t)total + kRun - 1) / kRun, most = std::max<int64_t>(1, (8LL * p.cus + batch - 1) / batch);
     const dim3 grid((unsigned)batch, (unsigned)std::max<int64_t>(1, std::min(runs, most)));
+    if (rot_dim % 16 == 0 && !dtype_quantized(p.desc.dtype)) {
+        const bool bf16 = p.desc.dtype == AIR_KV_BF16;
+        if (a.r.pairs) {
+            if (bf16) hipLaunchKernelGGL((rotate_floats_kernel<true, true>), grid, dim3(kThreads), 0, s, a);
+            else hipLaunchKernelGGL((rotate_floats_kernel<false, true>), grid, dim3(kThreads), 0, s, a);
+        } else {
+            if (bf16) hipLaunchKernelGGL((rotate_floats_kernel<true, false>), grid, dim3(kThreads), 0, s, a);
+            else hipLaunchKernelGGL((rotate_floats_kernel<false, false>), grid, dim3(kThreads), 0, s, a);
+        }
+        return hipGetLastError();
+    }
     switch (p.desc.dtype) {
     case AIR_KV_F32: hipLaunchKernelGGL(rotate_kernel<AIR_KV_F32>, grid, dim3(kThreads), 0, s, a); break;
     case AIR_KV_BF16: hipLaunchKernelGGL(rotate_kernel<AIR_KV_BF16>, grid, dim3(kThreads), 0, s, a); break;

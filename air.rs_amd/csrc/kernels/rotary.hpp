@@ -18,31 +18,32 @@ namespace airkv {
 // pi / 2 has no bits below 2^-52 and lies within 1 of the angle, so the first difference is
 // exact, and the second takes what pi / 2 has beyond.  On [-pi / 4, pi / 4] the Taylor sums
 // to r^17 and r^16 are within 2^-57 and 2^-58 of sine and cosine.
+//
+// rotary_scalar: a coefficient in scalar registers, which leaves the vector ones to rows on their way
+// (as literals they took 34, held from loop to loop).
+__device__ __forceinline__ double rotary_scalar(double x) {
+    asm("" : "+s"(x));
+    return x;
+}
 __device__ __forceinline__ float2 rotary_turn(int64_t position, float inv_freq, float magnitude) {
+    constexpr double kSin[8] = {-1.0 / 6.0, 1.0 / 120.0, -1.0 / 5040.0, 1.0 / 362880.0, -1.0 / 39916800.0,
+                                1.0 / 6227020800.0, -1.0 / 1307674368000.0, 1.0 / 355687428096000.0};
+    constexpr double kCos[8] = {-0.5, 1.0 / 24.0, -1.0 / 720.0, 1.0 / 40320.0, -1.0 / 3628800.0,
+                                1.0 / 479001600.0, -1.0 / 87178291200.0, 1.0 / 20922789888000.0};
     const double angle = (double)position * (double)inv_freq;
     const double k = __builtin_rint(angle * 0x1.45f306dc9c883p-1);
     double r = __builtin_fma(-k, 0x1.921fb54442d18p+0, angle);
     r = __builtin_fma(-k, 0x1.1a62633145c07p-54, r);
     const double z = r * r;
-    double s = 1.0 / 355687428096000.0;                                // 1 / 17!
-    s = __builtin_fma(s, z, -1.0 / 1307674368000.0);
-    s = __builtin_fma(s, z, 1.0 / 6227020800.0);
-    s = __builtin_fma(s, z, -1.0 / 39916800.0);
-    s = __builtin_fma(s, z, 1.0 / 362880.0);
-    s = __builtin_fma(s, z, -1.0 / 5040.0);
-    s = __builtin_fma(s, z, 1.0 / 120.0);
-    s = __builtin_fma(s, z, -1.0 / 6.0);
+    double s = kSin[7], c = kCos[7];
+#pragma unroll
+    for (int i = 6; i >= 0; --i) {
+        s = __builtin_fma(s, z, rotary_scalar(kSin[i]));
+        c = __builtin_fma(c, z, rotary_scalar(kCos[i]));
+    }
     s = __builtin_fma(s * z, r, r);
-    double c = 1.0 / 20922789888000.0;                                 // 1 / 16!
-    c = __builtin_fma(c, z, -1.0 / 87178291200.0);
-    c = __builtin_fma(c, z, 1.0 / 479001600.0);
-    c = __builtin_fma(c, z, -1.0 / 3628800.0);
-    c = __builtin_fma(c, z, 1.0 / 40320.0);
-    c = __builtin_fma(c, z, -1.0 / 720.0);
-    c = __builtin_fma(c, z, 1.0 / 24.0);
-    c = __builtin_fma(c, z, -0.5);
     c = __builtin_fma(c, z, 1.0);
-    // k mod 4 (k is below 2^55 or so; past it every k is a multiple of 4)
+    // k mod 4 (past 2^55 or so every k is a multiple of 4)
     const int quarter = (int)(k - 4.0 * __builtin_floor(k * 0.25));
     const double cq = quarter & 1 ? -s : c, sq = quarter & 1 ? c : s;
     const double m = quarter & 2 ? -(double)magnitude : (double)magnitude;
@@ -54,9 +55,16 @@ __device__ __forceinline__ float2 rotary_turn(int64_t position, float inv_freq, 
 // first or all second elements.
 __device__ __forceinline__ int rotary_partner(int e, int half) { return e < half ? e + half : e - half; }
 
+// One pair.  Products and sums round one by one: what a 1-byte page's codes are made from is defined
+// bit for bit.
+__device__ __forceinline__ void rotary_pair(float &x, float &y, float2 cs) {
+#pragma clang fp contract(off)
+    const float xc = x * cs.x, ys = y * cs.y, xs = x * cs.y, yc = y * cs.x;
+    x = xc - ys;
+    y = xs + yc;
+}
 // Four elements x of a row from element e on, turned; y their partners (half layout), cs the
-// pairs' (c, s).  Products and sums round one by one: what a 1-byte page's codes are made
-// from is defined bit for bit.
+// pairs' (c, s).
 __device__ __forceinline__ void rotary_half4(float (&x)[4], const float (&y)[4], const float2 *cs, int e, int half) {
 #pragma clang fp contract(off)
     const bool second = e >= half;
@@ -68,14 +76,8 @@ __device__ __forceinline__ void rotary_half4(float (&x)[4], const float (&y)[4],
     }
 }
 __device__ __forceinline__ void rotary_pairs4(float (&x)[4], const float2 *cs, int e) {
-#pragma clang fp contract(off)
 #pragma unroll
-    for (int j = 0; j < 4; j += 2) {
-        const float2 p = cs[(e + j) / 2];
-        const float ac = x[j] * p.x, bs = x[j + 1] * p.y, as = x[j] * p.y, bc = x[j + 1] * p.x;
-        x[j] = ac - bs;
-        x[j + 1] = as + bc;
-    }
+    for (int j = 0; j < 4; j += 2) rotary_pair(x[j], x[j + 1], cs[(e + j) / 2]);
 }
 
 }  // namespace airkv

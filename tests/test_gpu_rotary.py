@@ -144,6 +144,30 @@ def test_append_bad_slots_and_values():
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dtype", [airkv.BF16, airkv.F32, airkv.INT8, airkv.FP8])
+def test_values_are_appends(dtype):
+    """Values (and what of keys does not turn) are stored as append stores them, whatever they are:
+    NaN of any payload, infinities, subnormals, halfway cases."""
+    torch = torch_mod()
+    r = np.random.default_rng(1)
+    n, d = 64, 64
+    bits = r.integers(0, 1 << 32, (n, 2, d), np.uint64).astype(np.uint32)
+    bits[0::4] |= 0x7F800000
+    bits[1::4] &= 0x807FFFFF
+    bits[2::4, :, ::2] = (bits[2::4, :, ::2] & 0xFFFF0000) | 0x8000
+    x = _dev(bits.view(np.float32))
+    two = [airkv.KvPool(n // 16, 16, 2, d, dtype) for _ in range(2)]
+    slots = torch.arange(n, device="cuda")
+    f = _dev(ref.frequencies(8))
+    two[0].append(x, x, slots)
+    two[1].append_rotary(None, x, x, slots, torch.zeros(n, dtype=torch.int32, device="cuda"), f)
+    a, b = two[0].snapshot(), two[1].snapshot()
+    assert np.array_equal(a[1].view(np.uint8), b[1].view(np.uint8))
+    if a[3] is not None:
+        assert np.array_equal(a[3].view(np.uint32), b[3].view(np.uint32))
+    assert np.array_equal(a[0][..., 32:].view(np.uint8), b[0][..., 32:].view(np.uint8))
+
+
 # ---- rotate -----------------------------------------------------------------
 
 def _filled(dtype, d, kv, bs, group, lens, seed, spare=2):
