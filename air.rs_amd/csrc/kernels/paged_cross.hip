@@ -181,7 +181,7 @@ hipError_t launch_cross(const air_kv_pool &p, hipStream_t s, const void *q, int3
         a.tables = tables + (int64_t)b0 * max_blocks;
         a.lens = lens + b0;
         hipError_t e = half ? launch_cross_16(a, d, few, s) : launch_cross_f32(a, d, few, s);
-        if (e == hipSuccess) e = launch_merge(a, blocks, d, few, most, s);
+        if (e == hipSuccess) e = launch_merge(a, blocks, d, blocks.few, most, s);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;

@@ -66,9 +66,11 @@ template <int ROWS, int TK, int EXTRA> __device__ __forceinline__ int64_t cross_
     return tiles ? ((int64_t)s.rows + ROWS - 1) / ROWS * (tiles + EXTRA) : 0;
 }
 
-// Rows of a block, and workgroups that are resident on a CU.
+// Rows of a block, workgroups that are resident on a CU, and whether a block's waves share its
+// rows (asked for with `few`; without it where a tile's values have no room beside the others').
 struct CrossBlocks {
     int rows, groups;
+    bool few;
 };
 CrossBlocks cross_blocks_16(int head_dim, bool codes, bool few);
 CrossBlocks cross_blocks_f32(int head_dim, bool wide, bool few);

@@ -10,16 +10,17 @@
 //   kCodes  bf16 queries over 1-byte pages: everything as f16 (11 bits), under powers of two: of a
 //           query row's, of a tile's keys (from the largest scale of those that are not all zeros,
 //           known a barrier before the tile is staged) and of the values' (the smallest so far)
-//   kParts  f32 precision over bf16 pages, kWide over f32 and 1-byte ones: bf16 parts that hold all
-//           24 bits, of queries and probabilities and (kWide) of keys and values; products with
+//   kParts  f32 precision over bf16 pages, kFloats over f32 and kWide over 1-byte ones: bf16 parts
+//           that hold all 24 bits, of queries and probabilities and (not kParts) of keys and values; products with
 //           i + j < 3 are formed
 // Keys and values are staged in LDS as rows, padded or their 16-byte chunks placed so that neither
 // the rows' reads nor the values' transposing reads meet in a bank.
 //
-// Many rows (WK = 1): each wave has 32 rows of its own and all take the same keys; a tile is
-// loaded two ahead into registers and staged one ahead where two buffers fit.  Few rows: WK waves
-// share 32 rows and each takes 32 keys of a tile.  Where all of a workgroup's waves do, each stages
-// its own keys, and none waits for another until the block ends (PRIVATE).
+// Many rows: each wave has 32 rows of its own and all take the same keys; a tile is loaded two
+// ahead into registers and staged one ahead where two buffers fit.  Few rows (PRIVATE): a
+// workgroup's waves share 32 rows, each takes 32 keys of a tile and stages them itself, and none waits
+// for another until the block ends.  SPLIT: values take the keys' place when the scores are there, half
+// the LDS (all but kCodes, whose values' scales are looked through beside the keys').
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -43,7 +44,7 @@ typedef _Float16 cross_f16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t cross_u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t cross_u32x2 __attribute__((ext_vector_type(2)));
 
-enum CrossKind { kBf16, kCodes, kParts, kWide };
+enum CrossKind { kBf16, kCodes, kParts, kFloats, kWide };
 
 constexpr int kCrossBuffer = 0x00020000;           // a raw buffer's last word
 constexpr int kCrossStream = 2;                    // non-temporal: pages are read once
@@ -63,14 +64,16 @@ constexpr int cross_waves(int d, int qp, bool few) { return few || (cross_pipe(d
 constexpr int cross_groups(int d, int qp, bool few) { return few ? (d <= (qp == 3 ? 64 : 128) ? 2 : 1) : cross_pipe(d, qp, few) && d <= 64 ? 2 : 1; }
 // What a workgroup's tiles may take of a CU's 160 KB.
 constexpr int cross_lds(int groups) { return 160 * 1024 / groups - 7 * 1024; }
-// Waves that share rows: as many as have room for 32 keys each.
-constexpr int cross_wk(int d, int kp, int qp, bool few) {
-    int wk = few ? cross_waves(d, qp, few) : 1;
-    while (wk > 1 && cross_tile_bytes(d, kp, 32 * wk) > cross_lds(1)) wk /= 2;
-    return wk;
+// What 32 keys, and then their values (split) or both, take of a wave that stages its own; whether
+// there is room for all, in LDS and (three parts) in registers.
+constexpr int cross_region(int d, int parts, bool split) {
+    return !split ? cross_tile_bytes(d, parts, 32) : 32 * parts * (cross_k_stride(d) > cross_v_stride(d) ? cross_k_stride(d) : cross_v_stride(d));
+}
+constexpr bool cross_private(int d, int parts, int qp, bool few, bool split) {
+    return few && (parts == 1 || d <= 128) && cross_waves(d, qp, few) * cross_region(d, parts, split) <= cross_lds(1);
 }
 // Keys of a tile that one wave takes, in 32s.
-constexpr int cross_sub(int d, int kp, int wk) { return wk == 1 && cross_tile_bytes(d, kp, 64) <= cross_lds(1) ? 2 : 1; }
+constexpr int cross_sub(int d, int kp) { return cross_tile_bytes(d, kp, 64) <= cross_lds(1) ? 2 : 1; }
 
 template <bool F16> __device__ __forceinline__ cross_f32x16 cross_mfma(cross_u32x4 a, cross_u32x4 b, cross_f32x16 c) {
     if constexpr (F16)
@@ -142,12 +145,12 @@ __device__ __forceinline__ void cross_store4(const CrossArgs &a, int64_t at, cro
 
 template <int D, CrossKind KIND, bool FEW>
 struct CrossShape {
-    static constexpr int KP = KIND == kWide ? 3 : 1, QP = KIND == kParts || KIND == kWide ? 3 : 1;
-    static constexpr int WAVES = cross_waves(D, QP, FEW), WK = cross_wk(D, KP, QP, FEW), SUB = cross_sub(D, KP, WK);
-    static constexpr bool PRIVATE = FEW && WK == WAVES, PIPE = cross_pipe(D, QP, FEW);
-    static constexpr int RT = 1;                       // 32s of rows a wave
-    static constexpr int ROWS = 32 * RT * (WAVES / WK), TK = 32 * WK * SUB;
-    static constexpr int TILE = cross_tile_bytes(D, KP, TK);
+    static constexpr int KP = KIND == kFloats || KIND == kWide ? 3 : 1, QP = KIND == kParts ? 3 : KP;
+    static constexpr int WAVES = cross_waves(D, QP, FEW);
+    static constexpr bool SPLIT = KIND != kCodes, PRIVATE = cross_private(D, KP, QP, FEW, SPLIT), PIPE = cross_pipe(D, QP, FEW);
+    static constexpr int WK = PRIVATE ? WAVES : 1, SUB = PRIVATE ? 1 : cross_sub(D, KP);       // waves that share rows; 32s of a tile's keys of one
+    static constexpr int ROWS = 32 * (WAVES / WK), TK = 32 * WK * SUB;
+    static constexpr int REGION = cross_region(D, KP, SPLIT), TILE = PRIVATE ? WAVES * REGION : cross_tile_bytes(D, KP, TK);
     static constexpr int GROUPS = cross_groups(D, QP, FEW) == 2 && TILE <= cross_lds(2) ? 2 : 1;
     static constexpr int NB = PIPE ? 3 : !PRIVATE && 2 * TILE <= cross_lds(GROUPS) ? 2 : 1;
     static constexpr int WAVES_SIMD = WAVES / 4 * GROUPS;
@@ -158,10 +161,11 @@ __global__ __launch_bounds__((CrossShape<D, KIND, FEW>::WAVES * 64))
 __attribute__((amdgpu_waves_per_eu(CrossShape<D, KIND, FEW>::WAVES_SIMD, CrossShape<D, KIND, FEW>::WAVES_SIMD)))
 void paged_cross_kernel(CrossArgs a) {
     typedef CrossShape<D, KIND, FEW> S;
-    constexpr bool F16 = KIND == kCodes, PRIVATE = S::PRIVATE, PIPE = S::PIPE;
-    constexpr int KP = S::KP, QP = S::QP, WAVES = S::WAVES, WK = S::WK, SUB = S::SUB, ROWS = S::ROWS, TK = S::TK, NB = S::NB, RT = S::RT, THREADS = 64 * WAVES;
+    constexpr bool F16 = KIND == kCodes, PRIVATE = S::PRIVATE, SPLIT = S::SPLIT, PIPE = S::PIPE;
+    constexpr int KP = S::KP, QP = S::QP, WAVES = S::WAVES, WK = S::WK, SUB = S::SUB, ROWS = S::ROWS, TK = S::TK, NB = S::NB, RT = 1, THREADS = 64 * WAVES;
     constexpr int KST = cross_k_stride(D), VST = cross_v_stride(D);
-    constexpr int KPLANE = TK * KST, VPLANE = TK * VST, VAT = KP * KPLANE;    // a part's rows; where values begin
+    constexpr int STAGED = PRIVATE ? 32 : TK;          // keys side by side
+    constexpr int KPLANE = STAGED * KST, VPLANE = STAGED * VST, VAT = PRIVATE && SPLIT ? 0 : KP * KPLANE;      // a part's rows; where values begin
     constexpr int KS = D / 16, CT = D / 32;            // steps of the first product, 32-column tiles of the second
     // Staging: a wave takes SH of the tile's 16-key halves of keys or values, WR rows a pass, LPR lanes
     // a row (a power of two: some idle where D / 8 is none), 8 elements a lane.
@@ -242,9 +246,10 @@ void paged_cross_kernel(CrossArgs a) {
     // this lane's place in every pass
     const int p_c = lane % LPR;
     const bool p_in = p_c < D / 8;
-    const int esize = KIND == kCodes ? 1 : KIND != kWide ? 2 : a.dtype == AIR_KV_F32 ? 4 : 1;
+    constexpr bool CODES = KIND == kCodes || KIND == kWide;
+    constexpr int esize = CODES ? 1 : KIND == kFloats ? 4 : 2;
     const int p_off = p_in ? (lane / LPR * D + 8 * p_c) * esize : kCrossNowhere;
-    const int nsc = KIND == kCodes || (KIND == kWide && a.dtype != AIR_KV_F32) ? D >> a.sg_log2 : 0;
+    const int nsc = CODES ? D >> a.sg_log2 : 0;
     const int p_sc = p_in ? (lane / LPR * nsc + (8 * p_c >> a.sg_log2)) * 4 : kCrossNowhere;
 
     // half j of this wave's: of values (else keys), and which of the tile's
@@ -365,8 +370,8 @@ void paged_cross_kernel(CrossArgs a) {
         }
 
         struct Raw {                                   // a tile on its way
-            cross_u32x4 w[NP][KIND == kWide ? 2 : 1];
-            float s[KIND == kWide || KIND == kCodes ? NP : 1];
+            cross_u32x4 w[NP][KIND == kFloats ? 2 : 1];
+            float s[CODES ? NP : 1];
         } raw, next;                                   // (next: kCodes with two buffers, a tile further ahead)
         float fk = 1.0f, fk_next = 1.0f, fv = 0.0f, fv_next = 0.0f;    // kCodes: powers of two (0: no value yet)
         // lane h: the entry of a tile's half h, read a tile before it is needed, and its block
@@ -387,9 +392,17 @@ void paged_cross_kernel(CrossArgs a) {
             if (!PRIVATE && wave == 0 && lane < TK / 16) s_ok[t % 8][lane] = window >= 0;
             fetch(t + 1);
         };
-        auto load_tile = [&](int t, Raw &raw) __attribute__((always_inline)) {
+        // a tile's keys and values, or one of them (SPLIT)
+        constexpr std::integral_constant<int, 0> kBoth{};
+        constexpr std::integral_constant<int, 1> kKeys{};
+        constexpr std::integral_constant<int, 2> kValues{};
+        auto skip = [&](int j, auto part) __attribute__((always_inline)) {
+            return decltype(part)::value && of_values(j) != (decltype(part)::value == 2);
+        };
+        auto load_tile = [&](int t, Raw &raw, auto part) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < SH; ++j) {
+                if (skip(j, part)) continue;
                 const int half = half_of(j);
                 const bool val = of_values(j);
                 const int32_t e = __builtin_amdgcn_readlane(window, half);
@@ -406,12 +419,12 @@ void paged_cross_kernel(CrossArgs a) {
                     const int i = j * NPH + k;
                     if constexpr (KIND == kBf16 || KIND == kParts) {
                         raw.w[i][0] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + k * WR * D * 2, 0, kOnce));
-                    } else if (KIND == kCodes || a.dtype != AIR_KV_F32) {
+                    } else if constexpr (CODES) {
                         const cross_u32x2 x = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, p_off + k * WR * D, 0, kOnce));
                         raw.w[i][0][0] = x[0];
                         raw.w[i][0][1] = x[1];
                         raw.s[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ss, p_sc + k * WR * nsc * 4, 0, 0));
-                    } else if constexpr (KIND == kWide) {
+                    } else {
                         raw.w[i][0] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + k * WR * D * 4, 0, kOnce));
                         raw.w[i][1] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + k * WR * D * 4 + 16, 0, kOnce));
                     }
@@ -440,24 +453,27 @@ void paged_cross_kernel(CrossArgs a) {
                 }
             }
         };
-        auto powers = [&](float k, float v) __attribute__((always_inline)) {
-            // codes are at most 448 (2^9): the largest value to 2^13 at most
-            fk_next = k == 0.0f ? 1.0f : cross_pow2(3 - cross_exponent(k));
-            // values: kept as long as the largest stays below 2^15; it never grows
+        // codes are at most 448 (2^9): the largest value to 2^13 at most
+        auto keys_power = [&](float k) __attribute__((always_inline)) { fk_next = k == 0.0f ? 1.0f : cross_pow2(3 - cross_exponent(k)); };
+        auto values_power = [&](float v) __attribute__((always_inline)) {
+            // (kept as long as the largest stays below 2^15; it never grows)
             const float want = cross_pow2(3 - cross_exponent(v));
             fv_next = v == 0.0f ? fv_next : fv_next == 0.0f || fv_next > 4.0f * want ? want : fv_next;
         };
-        auto write_tile = [&](int t, const Raw &raw) __attribute__((always_inline)) {
-            uint8_t *mem = s_mem + t % NB * S::TILE;
-            if constexpr (F16 && !PRIVATE)
-                powers(__uint_as_float(__builtin_amdgcn_readfirstlane(s_top[t % 3][0])), __uint_as_float(__builtin_amdgcn_readfirstlane(s_top[t % 3][1])));
-            // (the type is asked for once a tile)
+        auto write_tile = [&](int t, const Raw &raw, auto part) __attribute__((always_inline)) {
+            uint8_t *mem = PRIVATE ? s_mem + wave * S::REGION : s_mem + t % NB * S::TILE;
+            if constexpr (F16 && !PRIVATE) {
+                keys_power(__uint_as_float(__builtin_amdgcn_readfirstlane(s_top[t % 3][0])));
+                values_power(__uint_as_float(__builtin_amdgcn_readfirstlane(s_top[t % 3][1])));
+            }
+            // (the type is asked for once a tile; kWide asks at each chunk: all of a tile's, twice over, do not fit the registers)
             auto rows = [&](auto type) __attribute__((always_inline)) {
                 constexpr int DT = decltype(type)::value;
 #pragma unroll
                 for (int i = 0; i < NP; ++i) {
+                    if (skip(i / NPH, part)) continue;
                     const bool val = of_values(i / NPH);
-                    const int at = 16 * half_of(i / NPH) + i % NPH * WR + lane / LPR;
+                    const int at = 16 * (PRIVATE ? i / NPH % (SH > 1 ? SH / 2 : 1) : half_of(i / NPH)) + i % NPH * WR + lane / LPR;
                     const int chunk = val && cross_v_xor(D) ? p_c ^ ((at & 3) << 2) : p_c;
                     uint8_t *to = mem + (val ? VAT + at * VST : at * KST) + 16 * chunk;
                     const int plane = val ? VPLANE : KPLANE;
@@ -468,11 +484,20 @@ void paged_cross_kernel(CrossArgs a) {
                         float x[8];
                         if constexpr (DT == AIR_KV_F32) {
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(raw.w[i][KIND == kWide ? j / 4 : 0][j % 4]);
+                            for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(raw.w[i][KIND == kFloats ? j / 4 : 0][j % 4]);
                         } else {
                             // (scales of groups of zeros were left out: theirs may be any size)
                             const float sc = F16 ? __builtin_amdgcn_fmed3f(raw.s[i] * (val ? fv_next : fk_next), -0x1p100f, 0x1p100f) : raw.s[i];
-                            const cross_f32x4 lo = cross_codes<DT, F16>(raw.w[i][0][0], sc), hi = cross_codes<DT, F16>(raw.w[i][0][1], sc);
+                            uint32_t w0 = raw.w[i][0][0], w1 = raw.w[i][0][1];
+                            asm volatile("" : "+v"(w0), "+v"(w1));     // (not taken apart while on its way: four registers for one)
+                            cross_f32x4 lo, hi;
+                            if (KIND == kWide && a.dtype == AIR_KV_INT8) {
+                                lo = cross_codes<AIR_KV_INT8, F16>(w0, sc);
+                                hi = cross_codes<AIR_KV_INT8, F16>(w1, sc);
+                            } else {
+                                lo = cross_codes<DT, F16>(w0, sc);
+                                hi = cross_codes<DT, F16>(w1, sc);
+                            }
 #pragma unroll
                             for (int j = 0; j < 4; ++j) { x[j] = lo[j]; x[4 + j] = hi[j]; }
                         }
@@ -487,59 +512,61 @@ void paged_cross_kernel(CrossArgs a) {
 #pragma unroll
                     for (int k = 0; k < KP; ++k)
                         if (p_in) *reinterpret_cast<cross_u32x4 *>(to + k * plane) = y[k];
+                    // (parts of several chunks at once would not fit the registers)
+                    if constexpr (KP == 3) __builtin_amdgcn_sched_barrier(0);
                 }
             };
             if constexpr (KIND == kBf16 || KIND == kParts) rows(std::integral_constant<int, AIR_KV_BF16>{});
-            else if (KIND == kWide && a.dtype == AIR_KV_F32) rows(std::integral_constant<int, AIR_KV_F32>{});
-            else if (a.dtype == AIR_KV_INT8) rows(std::integral_constant<int, AIR_KV_INT8>{});
+            else if constexpr (KIND == kFloats) rows(std::integral_constant<int, AIR_KV_F32>{});
+            else if (KIND == kCodes && a.dtype == AIR_KV_INT8) rows(std::integral_constant<int, AIR_KV_INT8>{});
             else rows(std::integral_constant<int, AIR_KV_FP8>{});
         };
         float mk = 0.0f, mv = 0.0f;
         // Many rows: what comes between two tiles' products, t the one at hand: tile t + 1 into its
         // buffer, t + 2 on its way (kCodes with two buffers: t + 2 marked, t + 3 on its way).
         auto stage = [&](int t) __attribute__((always_inline)) {
-            write_tile(t + 1, raw);
+            write_tile(t + 1, raw, kBoth);
             if (t + 2 >= tiles) return;
             if constexpr (F16 && NB >= 2) {
                 raw = next;
                 if (t + 3 < tiles) {
                     look_up(t + 3);
-                    load_tile(t + 3, next);
+                    load_tile(t + 3, next, kBoth);
                 }
                 mark(t + 2, raw, mk, mv);
             } else {
                 look_up(t + 2);
-                load_tile(t + 2, raw);
+                load_tile(t + 2, raw, kBoth);
             }
         };
 
         fetch(0);
         __syncthreads();                               // the buffers of the block before are free
         look_up(0);
-        load_tile(0, raw);
+        load_tile(0, raw, kBoth);
         if constexpr (!PRIVATE) {
             if (F16 && tid < 6) s_top[tid / 2][tid % 2] = 0;
             if (F16 && NB >= 2 && 1 < tiles) {
                 look_up(1);
-                load_tile(1, next);
+                load_tile(1, next, kBoth);
             }
             if constexpr (F16) {
                 __syncthreads();
                 mark(0, raw, mk, mv);
                 __syncthreads();
             }
-            write_tile(0, raw);
+            write_tile(0, raw, kBoth);
             if (1 < tiles) {
                 if constexpr (F16 && NB >= 2) {
                     raw = next;
                     if (2 < tiles) {
                         look_up(2);
-                        load_tile(2, next);
+                        load_tile(2, next, kBoth);
                     }
                     mark(1, raw, mk, mv);
                 } else {
                     look_up(1);
-                    load_tile(1, raw);
+                    load_tile(1, raw, kBoth);
                 }
             }
             __syncthreads();
@@ -804,65 +831,91 @@ void paged_cross_kernel(CrossArgs a) {
             cross_u32x4 p[RT][QP][2] = {{{pb[0], pb[1]}}};
             values(s_mem + before * S::TILE, 32, p);
             __syncthreads();
-        } else {
+        } else if constexpr (PRIVATE) {
+            uint8_t *mem = s_mem + wave * S::REGION;
+            // (a wave's LDS accesses are in order: what was there has been read)
+            auto ordered = [&]() __attribute__((always_inline)) {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            };
             for (int t = 0; t < tiles; ++t) {
-                int ok = 3;                            // whether this wave's halves are in the pool
-                if constexpr (PRIVATE) {
-                    ok = (__builtin_amdgcn_readlane(window, 2 * wave) >= 0 ? 1 : 0) | (__builtin_amdgcn_readlane(window, 2 * wave + 1) >= 0 ? 2 : 0);
-                    if constexpr (F16) {
-                        mark(t, raw, mk, mv);
-                        powers(mk, mv);
-                    }
-                    // (a wave's LDS accesses are in order: the tile before has been read)
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                    __builtin_amdgcn_wave_barrier();
-                    write_tile(t, raw);
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                    __builtin_amdgcn_wave_barrier();
-                    if (t + 1 < tiles) {
-                        look_up(t + 1);
-                        load_tile(t + 1, raw);
+                // whether this wave's halves are in the pool
+                const int ok = (__builtin_amdgcn_readlane(window, 2 * wave) >= 0 ? 1 : 0) | (__builtin_amdgcn_readlane(window, 2 * wave + 1) >= 0 ? 2 : 0);
+                const int64_t rest = sq.len - (key0 + (int64_t)t * TK + 32 * wave);
+                cross_u32x4 p[RT][QP][2];
+                if constexpr (F16) {
+                    mark(t, raw, mk, mv);
+                    keys_power(mk);
+                    values_power(mv);
+                    // (a power of two that changes: the sums so far are brought under it)
+                    if (fv != fv_next) {
+                        scale_all(fv == 0.0f ? 1.0f : fv_next / fv);
+                        fv = fv_next;
                     }
                 }
+                constexpr auto kFirst = std::conditional_t<SPLIT, decltype(kKeys), decltype(kBoth)>{};
+                ordered();
+                write_tile(t, raw, kFirst);
+                ordered();
+                if (t + 1 < tiles) {
+                    look_up(t + 1);
+                    load_tile(t + 1, raw, kFirst);
+                }
+                if (rest > 0) {
+                    cross_f32x16 sc[RT];
+                    float top[RT], ft[RT], alpha[RT];
+                    scores(mem, 0, sc);
+                    tops(sc, top);
+                    hide(rest, ok, sc, top);
+                    factors(fk_next, ft);
+                    if (rebase(sc, top, ft, alpha)) scale_sums(alpha);
+                    probabilities(sc, ft, p);
+                }
+                if constexpr (SPLIT) {
+                    ordered();
+                    write_tile(t, raw, kValues);
+                    ordered();
+                    if (t + 1 < tiles) load_tile(t + 1, raw, kValues);
+                }
+                if (rest > 0) values(mem, 0, p);
+            }
+            __syncthreads();
+        } else {
+            for (int t = 0; t < tiles; ++t) {
                 if constexpr (F16) {
                     fk = fk_next;
                     if (fv != fv_next) {
                         scale_all(fv == 0.0f ? 1.0f : fv_next / fv);
                         fv = fv_next;
                     }
-                    if (!PRIVATE && tid < 2) s_top[t % 3][tid] = 0;
+                    if (tid < 2) s_top[t % 3][tid] = 0;
                 }
-                if (!PRIVATE && NB == 2 && t + 1 < tiles) stage(t);
+                if (NB == 2 && t + 1 < tiles) stage(t);
                 if (any) {
                     const uint8_t *mem = s_mem + t % NB * S::TILE;
 #pragma unroll
                     for (int sub = 0; sub < SUB; ++sub) {
-                        const int k0 = 32 * (wk * SUB + sub);          // the keys' rows in the tile
-                        const int64_t rest = sq.len - (key0 + (int64_t)t * TK + k0);
+                        const int64_t rest = sq.len - (key0 + (int64_t)t * TK + 32 * sub);
                         if (rest <= 0) continue;
                         cross_f32x16 sc[RT];
                         cross_u32x4 p[RT][QP][2];
                         float top[RT], ft[RT], alpha[RT];
-                        scores(mem, k0, sc);
+                        scores(mem, 32 * sub, sc);
                         tops(sc, top);
-                        if constexpr (!PRIVATE) ok = __builtin_amdgcn_readfirstlane(s_ok[t % 8][k0 / 16] + 2 * s_ok[t % 8][k0 / 16 + 1]);
-                        hide(rest, ok, sc, top);
+                        hide(rest, __builtin_amdgcn_readfirstlane(s_ok[t % 8][2 * sub] + 2 * s_ok[t % 8][2 * sub + 1]), sc, top);
                         factors(fk, ft);
                         if (rebase(sc, top, ft, alpha)) scale_sums(alpha);
                         probabilities(sc, ft, p);
-                        values(mem, k0, p);
+                        values(mem, 32 * sub, p);
                     }
                 }
-                if constexpr (!PRIVATE) {
-                    if (NB == 1 && t + 1 < tiles) mark(t + 1, raw, mk, mv);
+                if (NB == 1 && t + 1 < tiles) mark(t + 1, raw, mk, mv);
+                __syncthreads();
+                if (NB == 1 && t + 1 < tiles) {
+                    stage(t);
                     __syncthreads();
-                    if (NB == 1 && t + 1 < tiles) {
-                        stage(t);
-                        __syncthreads();
-                    }
                 }
             }
-            if constexpr (PRIVATE) __syncthreads();
         }
 
         // lane (n, h): columns 32 c + 8 (i / 4) + 4 h + i % 4 of row n in acc[c][i]
@@ -951,7 +1004,11 @@ template <CrossKind KIND, bool FEW> hipError_t launch_cross_shape(const CrossArg
     const dim3 grid((unsigned)(a.slices * a.heads));
     switch (d) {
 #define AIRKV_CROSS(D) \
-    case D: hipLaunchKernelGGL((paged_cross_kernel<D, KIND, FEW>), grid, dim3(CrossShape<D, KIND, FEW>::WAVES * 64), 0, s, a); break;
+    case D: { \
+        constexpr bool F = FEW && CrossShape<D, KIND, true>::PRIVATE; \
+        hipLaunchKernelGGL((paged_cross_kernel<D, KIND, F>), grid, dim3(CrossShape<D, KIND, F>::WAVES * 64), 0, s, a); \
+        break; \
+    }
         AIRKV_CROSS(32) AIRKV_CROSS(64) AIRKV_CROSS(96) AIRKV_CROSS(128)
         AIRKV_CROSS(160) AIRKV_CROSS(192) AIRKV_CROSS(224) AIRKV_CROSS(256)
 #undef AIRKV_CROSS
@@ -961,12 +1018,16 @@ template <CrossKind KIND, bool FEW> hipError_t launch_cross_shape(const CrossArg
 
 template <CrossKind KIND, bool FEW> CrossBlocks cross_blocks_shape(int d) {
     switch (d) {
-#define AIRKV_CROSS(D) case D: return {CrossShape<D, KIND, FEW>::ROWS, CrossShape<D, KIND, FEW>::GROUPS};
+#define AIRKV_CROSS(D) \
+    case D: { \
+        constexpr bool F = FEW && CrossShape<D, KIND, true>::PRIVATE; \
+        return {CrossShape<D, KIND, F>::ROWS, CrossShape<D, KIND, F>::GROUPS, F}; \
+    }
         AIRKV_CROSS(32) AIRKV_CROSS(64) AIRKV_CROSS(96) AIRKV_CROSS(128)
         AIRKV_CROSS(160) AIRKV_CROSS(192) AIRKV_CROSS(224) AIRKV_CROSS(256)
 #undef AIRKV_CROSS
     }
-    return {0, 0};
+    return {0, 0, false};
 }
 
 }  // namespace airkv
