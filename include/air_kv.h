@@ -462,12 +462,13 @@ int air_paged_diff_prefill(air_kv_pool *pool, void *stream, const void *q, int32
  * (air_kv_pool_error_count) and its rows (where they lie in [0, total_q]) are
  * zero-filled; rows of a sequence of length 0 are zeros; rows of no sequence stay as
  * they were.  Out-of-pool table entries are counted and their tokens left out (of
- * all of a sequence's: zeros).  Rows of different sequences must not overlap.
+ * all of a sequence's: zeros).  Rows of different sequences must not overlap; out may
+ * be q itself where both have one type, and overlaps it nowhere else.
  *
  * Scores, sums and outputs are held in 32 bits.  bf16 queries with bf16 outputs on
  * BF16 pools round probabilities to bf16; on INT8 and FP8 pools they round
  * probabilities, keys and values to 11 bits, and no finer than 2^-35 of a row's
- * largest probability, 2^-37 of the largest key of its 32 to 256 neighbours and
+ * largest probability, 2^-37 of the largest key among its 32 or 64 neighbours and
  * of the largest value so far.  Everything else keeps f32
  * precision, where what lies below 2^-133 of an f32 or 1-byte page's value is cut
  * off.  Probabilities below 2^-98 of a row's largest count as 0, and so may what
