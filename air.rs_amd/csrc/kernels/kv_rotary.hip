@@ -5,6 +5,12 @@
 // 1-byte pages are then made by the same lanes and code.  Rows take a power of two of lanes,
 // so that a row lies in one wave: its lanes load what they turn, their own elements and the
 // partners', before any of them stores, and a row may be written where it was read.
+//
+// Both move bytes: an append reads and writes each row once (8192 tokens of 32 + 16 heads of 128, bf16:
+// 44.8 us, 4.5 TB/s; int8 pages 47.8), a rotation reads and writes the keys alone (4 sequences of 16000
+// tokens, 8 heads of 128, bf16 50.7 us, f32 79 us; a copy of 2 GiB reaches 4.9 TB/s read and written).
+// A position costs rot_dim / 2 angles in 64 bits, computed once a token, in a workgroup's LDS, while the
+// first rows are on their way.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -287,9 +293,12 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
 
 // The same where a row is floats and rot a multiple of 16: a lane owns 8 elements and their 8
 // partners (or 16 neighbours) of one token's rows, so nothing is read twice, and the pairs' c and s
-// stay in its registers from head to head.  A row is read before the one before it is stored.
+// stay in its registers from head to head.  (4 sequences of 16000 tokens: bf16 50.7 us, with the kernel
+// above 86; f32 79 and 86.)  ROWS rows are on their way before the first is stored, as many as leave four
+// waves a SIMD (bf16 / f32: 1 and 1 rows 55.7 / 80, 2 and 1 51.9 / 79, 4 and 2 48.5 / 81 but 131 in place of
+// 129 us for sequences whose keys no cache holds, and one f32 sequence 23.7 in place of 21.2).
 template <bool HALF, bool PAIRS>
-__global__ __launch_bounds__(kThreads) void rotate_floats_kernel(RotateArgs a) {
+__global__ __launch_bounds__(kThreads, 4) void rotate_floats_kernel(RotateArgs a) {
     __shared__ float2 s_cs[kRun * kMaxPairs];
     const int b = blockIdx.x, tid = threadIdx.x, d = a.p.head_dim, half = a.r.rot / 2;
     const int c0 = a.cu[b], c1 = a.cu[b + 1];
@@ -303,6 +312,7 @@ __global__ __launch_bounds__(kThreads) void rotate_floats_kernel(RotateArgs a) {
     const int part = tid & ((1 << lanes_log2) - 1), k = (tid >> lanes_log2) % kRun;
     const int group = tid >> lanes_log2 >> 4, groups = kThreads >> lanes_log2 >> 4;        // of heads
     const int e0 = PAIRS ? 16 * part : 8 * part, e1 = PAIRS ? e0 + 8 : e0 + half;
+    constexpr int ROWS = HALF ? 2 : 1;                 // on their way
     const int stride = (int)gridDim.y * kRun;
     for (int64_t at = (int64_t)blockIdx.y * kRun; at < n; at += stride) {
         const int64_t index = at >> a.p.bs_log2;
@@ -319,14 +329,15 @@ __global__ __launch_bounds__(kThreads) void rotate_floats_kernel(RotateArgs a) {
         }
         const bool mine = by != 0 && 16 * part < a.r.rot;
         const int64_t row = (((int64_t)block * a.p.heads << a.p.bs_log2) + (at & ((1 << a.p.bs_log2) - 1)) + k) * d;
-        Four<HALF> now[4], next[4];
+        Four<HALF> x[ROWS][4];
         auto load = [&](int h, Four<HALF> (&x)[4]) __attribute__((always_inline)) {
             if (!mine || h >= a.p.heads) return;
             const int64_t from = row + ((int64_t)h << a.p.bs_log2) * d;
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i].load(a.p.k_pages, from + (i < 2 ? e0 + 4 * i : e1 + 4 * (i - 2)));
         };
-        load(group, now);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) load(group + r * groups, x[r]);
         if (!__syncthreads_or(by != 0)) continue;      // (also: the angles of the run before are used)
         // (lanes a row hold 8 pairs each)
 #pragma unroll 1                                       // (unrolled, it takes the registers of the rows on their way)
@@ -340,21 +351,24 @@ __global__ __launch_bounds__(kThreads) void rotate_floats_kernel(RotateArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) cs[j] = s_cs[k * half + 8 * part + j];
 #pragma unroll 1
-        for (int h = group; h < a.p.heads; h += groups) {
-            load(h + groups, next);
-            float x[2][8];
+        for (int h0 = group; h0 < a.p.heads; h0 += ROWS * groups) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) now[i].get(x[i / 2] + 4 * (i % 2));
+            for (int r = 0; r < ROWS; ++r) {
+                const int h = h0 + r * groups;
+                if (h >= a.p.heads) break;
+                float y[2][8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {              // pair j: elements j of both halves, or neighbours
-                if constexpr (PAIRS) rotary_pair(x[j / 4][2 * (j % 4)], x[j / 4][2 * (j % 4) + 1], cs[j]);
-                else rotary_pair(x[0][j], x[1][j], cs[j]);
+                for (int i = 0; i < 4; ++i) x[r][i].get(y[i / 2] + 4 * (i % 2));
+                load(h + ROWS * groups, x[r]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {          // pair j: elements j of both halves, or neighbours
+                    if constexpr (PAIRS) rotary_pair(y[j / 4][2 * (j % 4)], y[j / 4][2 * (j % 4) + 1], cs[j]);
+                    else rotary_pair(y[0][j], y[1][j], cs[j]);
+                }
+                const int64_t to = row + ((int64_t)h << a.p.bs_log2) * d;
+                store8<HALF ? AIR_KV_BF16 : AIR_KV_F32>(y[0], a.p.k_pages, nullptr, to + e0, 0, false, 1);
+                store8<HALF ? AIR_KV_BF16 : AIR_KV_F32>(y[1], a.p.k_pages, nullptr, to + e1, 0, false, 1);
             }
-            const int64_t to = row + ((int64_t)h << a.p.bs_log2) * d;
-            store8<HALF ? AIR_KV_BF16 : AIR_KV_F32>(x[0], a.p.k_pages, nullptr, to + e0, 0, false, 1);
-            store8<HALF ? AIR_KV_BF16 : AIR_KV_F32>(x[1], a.p.k_pages, nullptr, to + e1, 0, false, 1);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) now[i] = next[i];
         }
     }
 }
@@ -399,9 +413,10 @@ hipError_t launch_append_rotary(const air_kv_pool &p, hipStream_t s, const void 
     a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride;
     a.q_heads = n_q_heads;
     const int all = n_q_heads + 2 * p.desc.n_kv_heads, pass = kThreads >> a.p.lanes_log2;
-    // few tokens: a pass of rows per workgroup, until the CUs have two each
+    // few tokens: a pass of rows per workgroup, until the CUs have two each (bf16, us, split and whole: 64
+    // tokens 3.0, 4.4; 512: 4.9, 5.7; 1024: 7.9, 8.1; 4096: 26.7, 25.3; int8, 1024: 9.1, 8.7)
     int parts = (all + pass - 1) / pass;
-    if (n_tokens >= 2 * p.cus) parts = 1;
+    if (n_tokens > 2 * p.cus) parts = 1;
     a.per_part = (all + parts - 1) / parts;
     const bool in16 = in_dtype == AIR_KV_BF16, out16 = q_out_dtype == AIR_KV_BF16;
     const int64_t in = in16 ? 2 : 4, out = out16 ? 2 : 4;
@@ -436,8 +451,9 @@ hipError_t launch_rotate(const air_kv_pool &p, hipStream_t s, const int32_t *tab
     a.cu = cu;
     a.max_blocks = max_blocks;
     a.total = total;
-    // runs are dealt to workgroups; eight a CU are resident
-    const int64_t runs = ((int64_t)total + kRun - 1) / kRun, most = std::max<int64_t>(1, (8LL * p.cus + batch - 1) / batch);
+    // runs are dealt to workgroups, 16 a CU (bf16, us: one sequence of 16000 tokens 16.1 with 8, 15.4 with 16
+    // and 64; 4 of 16000: 51.9, 50.7, 50.7; four a CU are resident)
+    const int64_t runs = ((int64_t)total + kRun - 1) / kRun, most = std::max<int64_t>(1, (16LL * p.cus + batch - 1) / batch);
     const dim3 grid((unsigned)batch, (unsigned)std::max<int64_t>(1, std::min(runs, most)));
     if (rot_dim % 16 == 0 && !dtype_quantized(p.desc.dtype)) {
         const bool bf16 = p.desc.dtype == AIR_KV_BF16;
