@@ -146,8 +146,11 @@ hipError_t launch_cross(const air_kv_pool &p, hipStream_t s, const void *q, int3
     const bool half = p.desc.dtype != AIR_KV_F32 && q_dtype == AIR_KV_BF16 && out_dtype == AIR_KV_BF16;
     const int d = p.desc.head_dim, group = n_q_heads / p.desc.n_kv_heads;
     const int64_t most = (int64_t)(max_q_len ? max_q_len : ((int64_t)total_q + batch - 1) / batch) * group;
-    // rows of one wave: its keys go to the others
-    const bool few = most <= 32;
+    // Few rows: a block's waves share its 32 rows, each with keys of its own, where that makes two blocks at
+    // most, one for f32 precision and large heads.  (Shared and not, us, 32 sequences of 2000 tokens, 8 heads of
+    // 128: 32 rows bf16 67, 90, fp8 64, 114, f32 126, 237; 64 rows 64, 93, 73, 118, 252, 248, f32 heads of 64 99, 128,
+    // of 160 478, 329; 128 rows bf16 139, 95, fp8 139, 118.)
+    const bool few = most <= (half || d <= 128 ? 64 : 32);
     const CrossBlocks blocks = blocks_of(p, half, few);
     const Workspace ws(p, blocks);
     CrossArgs a{};
@@ -171,7 +174,6 @@ hipError_t launch_cross(const air_kv_pool &p, hipStream_t s, const void *q, int3
     a.v_scales = p.v_scales;
     a.errors = p.errors;
     a.slices = slices_of(p, blocks);
-    a.least = 1;
     a.desc = (int4 *)workspace;
     a.part_ml = (float4 *)((char *)workspace + ws.ml);
     a.part_o = (float *)((char *)workspace + ws.o);

@@ -35,7 +35,6 @@ struct CrossArgs {
     const float *k_scales, *v_scales;
     unsigned long long *errors;
     int32_t slices;                    // per K/V head
-    int32_t least;                     // units a slice holds at least
     // cut blocks: per (K/V head, slice) the block it begins and does not end, {sequence, block,
     // pieces}; two piece slots each, 2w for a block begun before and 2w + 1 for one that goes
     // on: [slot][row] of (base, sum, the sums' unit), and of head_dim sums

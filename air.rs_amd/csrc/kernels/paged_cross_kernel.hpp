@@ -16,6 +16,12 @@
 // Keys and values are staged in LDS as rows, padded or their 16-byte chunks placed so that neither
 // the rows' reads nor the values' transposing reads meet in a bank.
 //
+// Many rows (16-bit products, heads up to 128) are bound by the products and the arithmetic between them,
+// about as much of either: a step's exponentials run beside the next step's scores and the last one's
+// values (8192 states, 4096 tokens of 32 heads of 128: 558 us, 985 TFLOP/s; one after the other 577 to 597).
+// Few rows are bound by the pages' reads (64 tokens, 512 to 4096 states, 8 heads of 128, bf16: 109 us, 5.2
+// TB/s; one f32 token over each of 32 sequences 110 us, 4.8; 1-byte pages 3.4, by their conversion).
+//
 // Many rows: each wave has 32 rows of its own and all take the same keys; a tile is loaded two
 // ahead into registers and staged one ahead where two buffers fit.  Few rows (PRIVATE): a
 // workgroup's waves share 32 rows, each takes 32 keys of a tile and stages them itself, and none waits
@@ -47,7 +53,7 @@ typedef uint32_t cross_u32x2 __attribute__((ext_vector_type(2)));
 enum CrossKind { kBf16, kCodes, kParts, kFloats, kWide };
 
 constexpr int kCrossBuffer = 0x00020000;           // a raw buffer's last word
-constexpr int kCrossStream = 2;                    // non-temporal: pages are read once
+constexpr int kCrossStream = 2;                    // non-temporal: pages are read once (64 single tokens 125 -> 111 us)
 constexpr int kCrossNowhere = 0x40000000;          // an offset outside of every buffer: reads zeros
 
 // Rows of keys and of values in LDS, bytes apart.  Keys: 16 bytes more than a whole number of
@@ -57,20 +63,23 @@ constexpr int cross_k_stride(int d) { return 2 * d + 16; }
 constexpr bool cross_v_xor(int d) { return 2 * d % 256 == 0; }
 constexpr int cross_v_stride(int d) { return cross_v_xor(d) || 2 * d / 64 % 2 ? 2 * d : 2 * d + 64; }
 constexpr int cross_tile_bytes(int d, int parts, int keys) { return keys * parts * (cross_k_stride(d) + cross_v_stride(d)); }
-// Waves of a workgroup, and workgroups a CU: registers leave room for four waves a SIMD (small
-// heads), two, or (queries in three parts and their sums, the largest heads) one.
+// Waves of a workgroup, and workgroups a CU: registers leave room for two waves a SIMD, or (queries in
+// three parts and their sums, the largest heads) one.  Two workgroups of four waves do not wait at each
+// other's barriers, but stage every tile twice: few rows stage their own in any case (heads of 64, two in
+// place of one: 104 -> 92 us; three, where registers allow them, 92), many rows gain from it at small heads.
 constexpr bool cross_pipe(int d, int qp, bool few) { return !few && qp == 1 && d <= 128; }
 constexpr int cross_waves(int d, int qp, bool few) { return few || (cross_pipe(d, qp, few) && d <= 64) || (qp == 3 ? d >= 96 : d >= 192) ? 4 : 8; }
 constexpr int cross_groups(int d, int qp, bool few) { return few ? (d <= (qp == 3 ? 64 : 128) ? 2 : 1) : cross_pipe(d, qp, few) && d <= 64 ? 2 : 1; }
 // What a workgroup's tiles may take of a CU's 160 KB.
 constexpr int cross_lds(int groups) { return 160 * 1024 / groups - 7 * 1024; }
 // What 32 keys, and then their values (split) or both, take of a wave that stages its own; whether
-// there is room for all, in LDS and (three parts) in registers.
+// there is room for all.  (Where registers do not suffice it pays still: f32 rows over bf16 heads of 192
+// 101 us with 75 spilled, 171 with waves that share a tile.)
 constexpr int cross_region(int d, int parts, bool split) {
     return !split ? cross_tile_bytes(d, parts, 32) : 32 * parts * (cross_k_stride(d) > cross_v_stride(d) ? cross_k_stride(d) : cross_v_stride(d));
 }
 constexpr bool cross_private(int d, int parts, int qp, bool few, bool split) {
-    return few && (parts == 1 || d <= 128) && cross_waves(d, qp, few) * cross_region(d, parts, split) <= cross_lds(1);
+    return few && cross_waves(d, qp, few) * cross_region(d, parts, split) <= cross_lds(1);
 }
 // Keys of a tile that one wave takes, in 32s.
 constexpr int cross_sub(int d, int kp) { return cross_tile_bytes(d, kp, 64) <= cross_lds(1) ? 2 : 1; }
@@ -237,8 +246,7 @@ void paged_cross_kernel(CrossArgs a) {
         }
     }
     const int64_t units = cross_uniform(s_pre[a.batch]);
-    int64_t chunk = (units + a.slices - 1) / a.slices;
-    chunk = chunk < a.least ? a.least : chunk;
+    const int64_t chunk = (units + a.slices - 1) / a.slices;
     int64_t u = w * chunk;
     const int64_t end = u + chunk < units ? u + chunk : units;
     int4 begun = {0, 0, 0, 0};
