@@ -171,7 +171,7 @@ __attribute__((amdgpu_waves_per_eu(CrossShape<D, KIND, FEW>::WAVES_SIMD, CrossSh
 void paged_cross_kernel(CrossArgs a) {
     typedef CrossShape<D, KIND, FEW> S;
     constexpr bool F16 = KIND == kCodes, PRIVATE = S::PRIVATE, SPLIT = S::SPLIT, PIPE = S::PIPE;
-    constexpr int KP = S::KP, QP = S::QP, WAVES = S::WAVES, WK = S::WK, SUB = S::SUB, ROWS = S::ROWS, TK = S::TK, NB = S::NB, RT = 1, THREADS = 64 * WAVES;
+    constexpr int KP = S::KP, QP = S::QP, WAVES = S::WAVES, WK = S::WK, SUB = S::SUB, ROWS = S::ROWS, TK = S::TK, NB = S::NB, THREADS = 64 * WAVES;
     constexpr int KST = cross_k_stride(D), VST = cross_v_stride(D);
     constexpr int STAGED = PRIVATE ? 32 : TK;          // keys side by side
     constexpr int KPLANE = STAGED * KST, VPLANE = STAGED * VST, VAT = PRIVATE && SPLIT ? 0 : KP * KPLANE;      // a part's rows; where values begin
@@ -298,84 +298,68 @@ void paged_cross_kernel(CrossArgs a) {
         const int64_t key0 = (int64_t)t0 * TK;
         const int32_t *table = a.tables + (int64_t)b * a.max_blocks;
 
-        // rows 32 (RT rg + r) .. +31 of the block
-        const bool any = blk * ROWS + 32 * RT * rg < sq.rows;
-        bool live[RT];
-        int64_t io[RT];
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            const int row = blk * ROWS + 32 * (RT * rg + r) + r32;             // of the sequence's at this K/V head
-            live[r] = row < sq.rows;
-            const int row_at = live[r] ? row : sq.rows - 1;
-            io[r] = ((int64_t)(sq.row0 + row_at / a.group) * a.q_heads + head * a.group + row_at % a.group) * D;
-        }
+        // rows 32 rg .. +31 of the block
+        const bool any = blk * ROWS + 32 * rg < sq.rows;
+        const int row = blk * ROWS + 32 * rg + r32;    // of the sequence's at this K/V head
+        const bool live = row < sq.rows;
+        const int row_at = live ? row : sq.rows - 1;
+        const int64_t io = ((int64_t)(sq.row0 + row_at / a.group) * a.q_heads + head * a.group + row_at % a.group) * D;
 
         // Q^T as the B operand: lane (n, h) holds elements 16 s + 8 h .. +8 of row n
-        cross_u32x4 qf[RT][QP][KS];
-        int qe[RT];                                    // (kCodes: the power of two they are under)
+        cross_u32x4 qf[QP][KS];
+        int qe = 0;                                    // (kCodes: the power of two they are under)
+        if (KIND == kBf16 || KIND == kCodes || a.q_dtype == AIR_KV_BF16) {
+            const uint16_t *q = (const uint16_t *)a.q + io + 8 * hf;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            qe[r] = 0;
-            if (KIND == kBf16 || KIND == kCodes || a.q_dtype == AIR_KV_BF16) {
-                const uint16_t *q = (const uint16_t *)a.q + io[r] + 8 * hf;
+            for (int s = 0; s < KS; ++s) {
+                qf[0][s] = *reinterpret_cast<const cross_u32x4 *>(q + 16 * s);
 #pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    qf[r][0][s] = *reinterpret_cast<const cross_u32x4 *>(q + 16 * s);
+                for (int p = 1; p < QP; ++p) qf[p][s] = cross_u32x4{0, 0, 0, 0};
+            }
+        } else {
+            const float *q = (const float *)a.q + io + 8 * hf;
 #pragma unroll
-                    for (int p = 1; p < QP; ++p) qf[r][p][s] = cross_u32x4{0, 0, 0, 0};
-                }
-            } else {
-                const float *q = (const float *)a.q + io[r] + 8 * hf;
+            for (int s = 0; s < KS; ++s)
 #pragma unroll
-                for (int s = 0; s < KS; ++s)
+                for (int i = 0; i < 2; ++i) {
+                    const cross_f32x4 x = *reinterpret_cast<const cross_f32x4 *>(q + 16 * s + 4 * i);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const cross_f32x4 x = *reinterpret_cast<const cross_f32x4 *>(q + 16 * s + 4 * i);
+                    for (int j = 0; j < 2; ++j) {
+                        uint32_t p[QP];
+                        cross_parts<F16, QP>(x[2 * j], x[2 * j + 1], p);
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            uint32_t p[QP];
-                            cross_parts<F16, QP>(x[2 * j], x[2 * j + 1], p);
-#pragma unroll
-                            for (int k = 0; k < QP; ++k) qf[r][k][s][2 * i + j] = p[k];
-                        }
+                        for (int k = 0; k < QP; ++k) qf[k][s][2 * i + j] = p[k];
                     }
-            }
-            if constexpr (F16) {
-                // the row's largest element to [2^4, 2^5): bf16's 8 bits are exact in f16 down to 2^-11
-                float top = 0.0f;
-#pragma unroll
-                for (int s = 0; s < KS; ++s)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        top = fmaxf(top, fmaxf(__builtin_fabsf(__uint_as_float(qf[r][0][s][j] << 16)),
-                                               __builtin_fabsf(__uint_as_float(qf[r][0][s][j] & 0xFFFF0000u))));
-                const float fq = cross_pow2(4 - cross_exponent(max_x32(top)));
-                qe[r] = cross_exponent(fq);
-#pragma unroll
-                for (int s = 0; s < KS; ++s)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        qf[r][0][s][j] = cross_f16_pair(__uint_as_float(qf[r][0][s][j] << 16) * fq, __uint_as_float(qf[r][0][s][j] & 0xFFFF0000u) * fq);
-            }
+                }
         }
-        cross_f32x16 acc[RT][CT];
+        if constexpr (F16) {
+            // the row's largest element to [2^4, 2^5): bf16's 8 bits are exact in f16 down to 2^-11
+            float top = 0.0f;
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+            for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int c = 0; c < CT; ++c)
+                for (int j = 0; j < 4; ++j)
+                    top = fmaxf(top, fmaxf(__builtin_fabsf(__uint_as_float(qf[0][s][j] << 16)),
+                                           __builtin_fabsf(__uint_as_float(qf[0][s][j] & 0xFFFF0000u))));
+            const float fq = cross_pow2(4 - cross_exponent(max_x32(top)));
+            qe = cross_exponent(fq);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[r][c][i] = 0.0f;
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    qf[0][s][j] = cross_f16_pair(__uint_as_float(qf[0][s][j] << 16) * fq, __uint_as_float(qf[0][s][j] & 0xFFFF0000u) * fq);
+        }
+        cross_f32x16 acc[CT];
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
         // Probabilities are held 2^(score - base), the base kDown above every score so far: 2^24 of
         // them sum to 1 at most, so that values near the largest float do too.  (f16 ones up to
         // 2^15, so that they keep 11 bits down to 2^-25 of the largest; values are below 2^15 there.)
         // A base is taken kSlack further up, so that it seldom changes: where a score passes lim.
         constexpr float kDown = F16 ? -15.0f : 24.0f, kSlack = 4.0f, kFar = 0x1p20f;
-        float base[RT], lim[RT], l_run[RT];
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            base[r] = lim[r] = -INFINITY;
-            l_run[r] = 0.0f;
-        }
+        float base = -INFINITY, lim = -INFINITY, l_run = 0.0f;
 
         struct Raw {                                   // a tile on its way
             cross_u32x4 w[NP][KIND == kFloats ? 2 : 1];
@@ -581,11 +565,9 @@ void paged_cross_kernel(CrossArgs a) {
         }
         // ---- a step's parts: 32 keys, those of a buffer `mem` from row k0 on
 
-        auto scores = [&](const uint8_t *mem, int k0, cross_f32x16 (&sc)[RT]) __attribute__((always_inline)) {
+        auto scores = [&](const uint8_t *mem, int k0, cross_f32x16 &sc) __attribute__((always_inline)) {
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) sc[r][i] = 0.0f;
+            for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
             int ln = lane;
             asm volatile("" : "+v"(ln));
             const uint8_t *k = mem + (k0 + (ln & 31)) * KST + 16 * (ln >> 5);
@@ -595,115 +577,84 @@ void paged_cross_kernel(CrossArgs a) {
 #pragma unroll
                 for (int p = 0; p < KP; ++p) kf[p] = *reinterpret_cast<const cross_u32x4 *>(k + p * KPLANE + 32 * s);
 #pragma unroll
-                for (int r = 0; r < RT; ++r)
+                for (int i = 0; i < KP; ++i)
 #pragma unroll
-                    for (int i = 0; i < KP; ++i)
-#pragma unroll
-                        for (int j = 0; j < QP; ++j)
-                            if (i + j < 3) sc[r] = cross_mfma<F16>(kf[i], qf[r][j][s], sc[r]);
+                    for (int j = 0; j < QP; ++j)
+                        if (i + j < 3) sc = cross_mfma<F16>(kf[i], qf[j][s], sc);
             }
         };
-        auto tops = [&](const cross_f32x16 (&sc)[RT], float (&top)[RT]) __attribute__((always_inline)) {
+        auto tops = [&](const cross_f32x16 &sc, float &top) __attribute__((always_inline)) {
+            float x = sc[0];
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                float x = sc[r][0];
-#pragma unroll
-                for (int i = 1; i < 16; ++i) x = fmaxf(x, sc[r][i]);
-                top[r] = max_x32(x);
-            }
+            for (int i = 1; i < 16; ++i) x = fmaxf(x, sc[i]);
+            top = max_x32(x);
         };
         // keys past the end (rest are left) and of blocks outside the pool (ok: a bit for each half)
-        auto hide = [&](int64_t rest, int ok, cross_f32x16 (&sc)[RT], float (&top)[RT]) __attribute__((always_inline)) {
+        auto hide = [&](int64_t rest, int ok, cross_f32x16 &sc, float &top) __attribute__((always_inline)) {
             uint32_t mask = rest >= 32 ? ~0u : rest <= 0 ? 0u : (1u << (int)rest) - 1;
             mask &= (ok & 1 ? 0x0000FFFFu : 0u) | (ok & 2 ? 0xFFFF0000u : 0u);
             if (__builtin_expect(mask != ~0u, 0)) {
                 asm volatile("");                      // (a branch: selects would cost every tile 60 instructions)
                 const uint32_t m = mask >> (4 * hf);
 #pragma unroll
-                for (int r = 0; r < RT; ++r)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) sc[r][i] = (m >> (8 * (i / 4) + i % 4)) & 1 ? sc[r][i] : -INFINITY;
+                for (int i = 0; i < 16; ++i) sc[i] = (m >> (8 * (i / 4) + i % 4)) & 1 ? sc[i] : -INFINITY;
                 tops(sc, top);
             }
         };
         // Another base for rows whose largest score passes lim; what is behind has to be multiplied by
         // alpha then (the return value: for some row).
-        auto rebase = [&](cross_f32x16 (&sc)[RT], const float (&top)[RT], float (&ft)[RT], float (&alpha)[RT]) __attribute__((always_inline)) -> bool {
-            bool past = false;
-#pragma unroll
-            for (int r = 0; r < RT; ++r) past |= top[r] * ft[r] > lim[r];
+        auto rebase = [&](cross_f32x16 &sc, float top, float &ft, float &alpha) __attribute__((always_inline)) -> bool {
+            const bool past = top * ft > lim;
             if (__builtin_expect(__ballot(past) == 0ull, 1)) return false;
             asm volatile("");
-            bool far = false;
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const float x = top[r] * ft[r];
-                const float cap = __builtin_fabsf(base[r]) < kFar ? base[r] - kDown : base[r];
-                const float now = x > cap ? x + (__builtin_fabsf(x) < kFar ? kDown + kSlack : 0.0f) : base[r];
-                alpha[r] = base[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(base[r] - now);
-                l_run[r] *= alpha[r];
-                base[r] = now;
-                const bool is_far = !(__builtin_fabsf(now) < kFar) && now != -INFINITY;
-                lim[r] = is_far ? -INFINITY : now - kDown;
-                far |= is_far;
-            }
+            const float x = top * ft;
+            const float cap = __builtin_fabsf(base) < kFar ? base - kDown : base;
+            const float now = x > cap ? x + (__builtin_fabsf(x) < kFar ? kDown + kSlack : 0.0f) : base;
+            alpha = base == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(base - now);
+            l_run *= alpha;
+            base = now;
+            const bool far = !(__builtin_fabsf(now) < kFar) && now != -INFINITY;
+            lim = far ? -INFINITY : now - kDown;
             // (scores past 2^20, which f32 holds in steps of an eighth and more, are each rounded as
             // the largest was, so that their distances from the base are exact)
             if (__ballot(far) != 0ull) {
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    sc[r] *= ft[r];
-                    ft[r] = 1.0f;
-                }
+                sc *= ft;
+                ft = 1.0f;
             }
             return true;
         };
-        auto scale_sums = [&](const float (&by)[RT]) __attribute__((always_inline)) {
+        auto scale_sums = [&](float by) __attribute__((always_inline)) {
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int c = 0; c < CT; ++c) acc[r][c] *= by[r];
-        };
-        auto scale_all = [&](float by) __attribute__((always_inline)) {
-            float b[RT];
-#pragma unroll
-            for (int r = 0; r < RT; ++r) b[r] = by;
-            scale_sums(b);
+            for (int c = 0; c < CT; ++c) acc[c] *= by;
         };
         // what products are multiplied by.  (Neither 0 nor infinite: a masked score, -inf, times 0 would be NaN,
         // and so would 0 times infinity.)
-        auto factors = [&](float fk, float (&ft)[RT]) __attribute__((always_inline)) {
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                ft[r] = a.scale_log2;
-                if constexpr (F16) ft[r] = fminf(fmaxf(__builtin_amdgcn_ldexpf(ft[r], -(qe[r] + cross_exponent(fk))), 0x1p-126f), 0x1.fffffep127f);
-            }
+        auto factors = [&](float fk, float &ft) __attribute__((always_inline)) {
+            ft = a.scale_log2;
+            if constexpr (F16) ft = fminf(fmaxf(__builtin_amdgcn_ldexpf(ft, -(qe + cross_exponent(fk))), 0x1p-126f), 0x1.fffffep127f);
         };
-        auto probabilities = [&](cross_f32x16 (&sc)[RT], const float (&ft)[RT], cross_u32x4 (&p)[RT][QP][2]) __attribute__((always_inline)) {
+        auto probabilities = [&](cross_f32x16 &sc, float ft, cross_u32x4 (&p)[QP][2]) __attribute__((always_inline)) {
+            const float from = base == -INFINITY ? 0.0f : base;
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const float from = base[r] == -INFINITY ? 0.0f : base[r];
+            for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], ft, -from));
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sc[r][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r][i], ft[r], -from));
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int s = 0; s < 2; ++s)
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t x[QP];
+                    cross_parts<F16, QP>(sc[8 * s + 2 * j], sc[8 * s + 2 * j + 1], x);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t x[QP];
-                        cross_parts<F16, QP>(sc[r][8 * s + 2 * j], sc[r][8 * s + 2 * j + 1], x);
-#pragma unroll
-                        for (int k = 0; k < QP; ++k) p[r][k][s][j] = x[k];
-                        // (16-bit ones are summed as they were rounded)
-                        if constexpr (QP == 1) l_run[r] = cross_add_pair<F16>(x[0], ones, l_run[r]);
-                        else l_run[r] += sc[r][8 * s + 2 * j] + sc[r][8 * s + 2 * j + 1];
-                    }
-            }
+                    for (int k = 0; k < QP; ++k) p[k][s][j] = x[k];
+                    // (16-bit ones are summed as they were rounded)
+                    if constexpr (QP == 1) l_run = cross_add_pair<F16>(x[0], ones, l_run);
+                    else l_run += sc[8 * s + 2 * j] + sc[8 * s + 2 * j + 1];
+                }
         };
         // V^T as the A operand: lane (m, h) takes keys 16 s + 8 b + 4 h .. +4 of column m, b = 0, 1.
         // Within each 16-lane group, lane j of a transposing read receives element j % 4 of the 8
         // bytes that lanes 4 k + j / 4 address, k = 0 .. 3: lane i points at key i / 4 of the four
         // and columns 4 (i % 4) of the group's sixteen.
-        auto values = [&](const uint8_t *mem, int k0, const cross_u32x4 (&p)[RT][QP][2]) __attribute__((always_inline)) {
+        auto values = [&](const uint8_t *mem, int k0, const cross_u32x4 (&p)[QP][2]) __attribute__((always_inline)) {
             int ln = lane;                             // (its addresses are not kept in registers from step to step)
             asm volatile("" : "+v"(ln));
             const int vr = 4 * (ln >> 5) + ((ln & 15) >> 2);
@@ -723,10 +674,8 @@ void paged_cross_kernel(CrossArgs a) {
                                                   (__attribute__((address_space(3))) s16x4 *)(v + 8 * VST)));
                         const cross_u32x4 vf = {x[0], x[1], y[0], y[1]};
 #pragma unroll
-                        for (int r = 0; r < RT; ++r)
-#pragma unroll
-                            for (int j = 0; j < QP; ++j)
-                                if (i + j < 3) acc[r][c] = cross_mfma<F16>(vf, p[r][j][s], acc[r][c]);
+                        for (int j = 0; j < QP; ++j)
+                            if (i + j < 3) acc[c] = cross_mfma<F16>(vf, p[j][s], acc[c]);
                     }
         };
 
@@ -734,10 +683,10 @@ void paged_cross_kernel(CrossArgs a) {
             // A step's probabilities are computed beside the next step's scores and the one before's
             // values, so that products and arithmetic, about as much of either, run at once.  A tile is
             // two steps; the next tile is staged beside the first and there at a barrier before the second.
-            static_assert(RT == 1 && QP == 1 && KP == 1 && KS == 2 * CT && NB == 3, "one row tile, 16-bit parts");
-            cross_f32x16 sa[RT], sb[RT];
+            static_assert(QP == 1 && KP == 1 && KS == 2 * CT && NB == 3, "16-bit parts");
+            cross_f32x16 sa, sb;
             cross_u32x4 pa[2], pb[2];
-            float top[RT];
+            float top;
             float fv_t = fv_next;                      // kCodes: of the tile whose values come next
             // (this lane's places in a buffer: keys, values of four column tiles)
             const int k_at = r32 * KST + 16 * hf, vr = 4 * hf + ((lane & 15) >> 2);
@@ -747,10 +696,10 @@ void paged_cross_kernel(CrossArgs a) {
                 v_at[c] = VAT + vr * VST + 32 * ((lane >> 4) & 1) + 8 * (lane & 3) + 64 * (cross_v_xor(D) ? c ^ (vr & 3) : c);
             // A step from its scores in sc: p; the next step's scores, of the keys from row k0 of buffer kb, in
             // sn; the sums of the step before, its probabilities q and the values from row v0 of buffer vb.
-            auto step = [&](cross_f32x16 (&sc)[RT], cross_f32x16 (&sn)[RT], cross_u32x4 (&p)[2], const cross_u32x4 (&q)[2], int kb, int k0, int vb,
+            auto step = [&](cross_f32x16 &sc, cross_f32x16 &sn, cross_u32x4 (&p)[2], const cross_u32x4 (&q)[2], int kb, int k0, int vb,
                             int v0, int64_t rest, int ok, float fk) __attribute__((always_inline)) {
                 hide(rest, ok, sc, top);
-                float ft[RT], alpha[RT];
+                float ft, alpha;
                 factors(fk, ft);
                 const bool changed = rebase(sc, top, ft, alpha);
                 // what follows is in the order in which it shall run: a product, then arithmetic that is done
@@ -775,15 +724,15 @@ void paged_cross_kernel(CrossArgs a) {
                         f[i] = cross_u32x4{x[0], x[1], y[0], y[1]};
                     }
                 };
-                const float from = base[0] == -INFINITY ? 0.0f : base[0];
+                const float from = base == -INFINITY ? 0.0f : base;
                 auto pair = [&](int i) __attribute__((always_inline)) {
-                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[0][2 * i], ft[0], -from));
-                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[0][2 * i + 1], ft[0], -from));
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * i], ft, -from));
+                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * i + 1], ft, -from));
                     p[i / 4][i % 4] = F16 ? cross_f16_pair(x, y) : cross_bf16_pair(x, y);
-                    l_run[0] = cross_add_pair<F16>(p[i / 4][i % 4], ones, l_run[0]);
+                    l_run = cross_add_pair<F16>(p[i / 4][i % 4], ones, l_run);
                 };
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sn[0][i] = 0.0f;
+                for (int i = 0; i < 16; ++i) sn[i] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < AHEAD; ++i) read(i);
                 __builtin_amdgcn_sched_barrier(0);
@@ -791,15 +740,15 @@ void paged_cross_kernel(CrossArgs a) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     read(i + AHEAD);
-                    if (i < KS) sn[0] = cross_mfma<F16>(f[i], qf[0][0][i], sn[0]);
-                    else acc[0][(i - KS) / 2] = cross_mfma<F16>(f[i], q[(i - KS) % 2], acc[0][(i - KS) / 2]);
+                    if (i < KS) sn = cross_mfma<F16>(f[i], qf[0][i], sn);
+                    else acc[(i - KS) / 2] = cross_mfma<F16>(f[i], q[(i - KS) % 2], acc[(i - KS) / 2]);
 #pragma unroll
                     for (; done < 8 * (i + 1) / N; ++done) pair(done);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 tops(sn, top);
                 // (here, and not where they are used: behind a branch)
-                asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(l_run[0]));
+                asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(l_run));
                 if (__builtin_expect(changed, 0)) {
                     asm volatile("");                  // (a branch: no products by 1)
                     scale_sums(alpha);
@@ -827,7 +776,7 @@ void paged_cross_kernel(CrossArgs a) {
                 if constexpr (F16) {
                     // (a power of two that changes: the sums so far are brought under it)
                     if (__builtin_expect(fv != fv_t, 0)) {
-                        scale_all(fv == 0.0f ? 1.0f : fv_t / fv);
+                        scale_sums(fv == 0.0f ? 1.0f : fv_t / fv);
                         fv = fv_t;
                     }
                 }
@@ -836,7 +785,7 @@ void paged_cross_kernel(CrossArgs a) {
                 at = next;
             }
             // (the last tile's second half)
-            cross_u32x4 p[RT][QP][2] = {{{pb[0], pb[1]}}};
+            cross_u32x4 p[QP][2] = {{pb[0], pb[1]}};
             values(s_mem + before * S::TILE, 32, p);
             __syncthreads();
         } else if constexpr (PRIVATE) {
@@ -850,14 +799,14 @@ void paged_cross_kernel(CrossArgs a) {
                 // whether this wave's halves are in the pool
                 const int ok = (__builtin_amdgcn_readlane(window, 2 * wave) >= 0 ? 1 : 0) | (__builtin_amdgcn_readlane(window, 2 * wave + 1) >= 0 ? 2 : 0);
                 const int64_t rest = sq.len - (key0 + (int64_t)t * TK + 32 * wave);
-                cross_u32x4 p[RT][QP][2];
+                cross_u32x4 p[QP][2];
                 if constexpr (F16) {
                     mark(t, raw, mk, mv);
                     keys_power(mk);
                     values_power(mv);
                     // (a power of two that changes: the sums so far are brought under it)
                     if (fv != fv_next) {
-                        scale_all(fv == 0.0f ? 1.0f : fv_next / fv);
+                        scale_sums(fv == 0.0f ? 1.0f : fv_next / fv);
                         fv = fv_next;
                     }
                 }
@@ -870,8 +819,8 @@ void paged_cross_kernel(CrossArgs a) {
                     load_tile(t + 1, raw, kFirst);
                 }
                 if (rest > 0) {
-                    cross_f32x16 sc[RT];
-                    float top[RT], ft[RT], alpha[RT];
+                    cross_f32x16 sc;
+                    float top, ft, alpha;
                     scores(mem, 0, sc);
                     tops(sc, top);
                     hide(rest, ok, sc, top);
@@ -893,7 +842,7 @@ void paged_cross_kernel(CrossArgs a) {
                 if constexpr (F16) {
                     fk = fk_next;
                     if (fv != fv_next) {
-                        scale_all(fv == 0.0f ? 1.0f : fv_next / fv);
+                        scale_sums(fv == 0.0f ? 1.0f : fv_next / fv);
                         fv = fv_next;
                     }
                     if (tid < 2) s_top[t % 3][tid] = 0;
@@ -905,9 +854,9 @@ void paged_cross_kernel(CrossArgs a) {
                     for (int sub = 0; sub < SUB; ++sub) {
                         const int64_t rest = sq.len - (key0 + (int64_t)t * TK + 32 * sub);
                         if (rest <= 0) continue;
-                        cross_f32x16 sc[RT];
-                        cross_u32x4 p[RT][QP][2];
-                        float top[RT], ft[RT], alpha[RT];
+                        cross_f32x16 sc;
+                        cross_u32x4 p[QP][2];
+                        float top, ft, alpha;
                         scores(mem, 32 * sub, sc);
                         tops(sc, top);
                         hide(rest, __builtin_amdgcn_readfirstlane(s_ok[t % 8][2 * sub] + 2 * s_ok[t % 8][2 * sub + 1]), sc, top);
@@ -930,31 +879,29 @@ void paged_cross_kernel(CrossArgs a) {
         float unit = F16 && fv != 0.0f ? 1.0f / fv : 1.0f;     // of the sums (pieces' stay under it)
         const int64_t slot = 2 * cell + (t0 == 0 ? 1 : 0);
         if constexpr (WK == 1) {
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const float l = sum_x32(l_run[r]);
-                const int64_t prow = slot * ROWS + 32 * (RT * rg + r) + r32;
-                // no key at all (every block outside the pool): zeros
-                const float k = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-                if (whole ? !live[r] : !any) continue;
+            const float l = sum_x32(l_run);
+            const int64_t prow = slot * ROWS + 32 * rg + r32;
+            // no key at all (every block outside the pool): zeros
+            const float k = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+            if (whole ? live : any) {
 #pragma unroll
                 for (int c = 0; c < CT; ++c)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        cross_f32x4 x = cross_f32x4{acc[r][c][4 * i], acc[r][c][4 * i + 1], acc[r][c][4 * i + 2], acc[r][c][4 * i + 3]} * k;
+                        cross_f32x4 x = cross_f32x4{acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]} * k;
                         if (F16 && whole) x *= unit;
                         const int col = 32 * c + 8 * i + 4 * hf;
-                        if (whole) cross_store4(a, io[r] + col, x);
+                        if (whole) cross_store4(a, io + col, x);
                         else *reinterpret_cast<cross_f32x4 *>(a.part_o + prow * D + col) = x;
                     }
-                if (!whole && hf == 0) a.part_ml[prow] = make_float4(base[r], l, unit, 0.0f);
+                if (!whole && hf == 0) a.part_ml[prow] = make_float4(base, l, unit, 0.0f);
             }
         } else {
             // the waves of one row group: their bases' largest, then their sums, CR column tiles at a
             // time, four columns (c, i) of all of them to one wave
-            float l = sum_x32(l_run[0]);
+            float l = sum_x32(l_run);
             const int64_t prow = slot * ROWS + 32 * rg + r32;
-            if (hf == 0) s_ml[wave][r32] = make_float4(base[0], l, fv, 0.0f);
+            if (hf == 0) s_ml[wave][r32] = make_float4(base, l, fv, 0.0f);
             __syncthreads();
             float top = -INFINITY, least = 0.0f;       // (the smallest power of two of the values': the largest unit)
 #pragma unroll
@@ -969,7 +916,7 @@ void paged_cross_kernel(CrossArgs a) {
                 const float4 ml = s_ml[rg * WK + i][r32];
                 l += ml.x == -INFINITY ? ml.y : ml.y * __builtin_amdgcn_exp2f(ml.x - top);
             }
-            float alpha = base[0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(base[0] - top);
+            float alpha = base == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(base - top);
             if (F16 && fv != 0.0f) alpha *= least / fv;
             if (F16) unit = least != 0.0f ? 1.0f / least : 1.0f;
             const float k = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
@@ -981,7 +928,7 @@ void paged_cross_kernel(CrossArgs a) {
                 for (int c = c0; c < c0 + CR && c < CT; ++c)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        x[((wave * CR + c - c0) * 4 + i) * 64] = cross_f32x4{acc[0][c][4 * i], acc[0][c][4 * i + 1], acc[0][c][4 * i + 2], acc[0][c][4 * i + 3]} * alpha;
+                        x[((wave * CR + c - c0) * 4 + i) * 64] = cross_f32x4{acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]} * alpha;
                 __syncthreads();
                 const int quads = 4 * (CT - c0 < CR ? CT - c0 : CR);
                 for (int g = wk; g < quads; g += WK) {
@@ -992,7 +939,7 @@ void paged_cross_kernel(CrossArgs a) {
                     if (F16 && whole) y *= unit;
                     const int col = 32 * (c0 + g / 4) + 8 * (g % 4) + 4 * hf;
                     if (whole) {
-                        if (live[0]) cross_store4(a, io[0] + col, y);
+                        if (live) cross_store4(a, io + col, y);
                     } else if (any) {
                         *reinterpret_cast<cross_f32x4 *>(a.part_o + prow * D + col) = y;
                     }
