@@ -66,7 +66,7 @@ template <int ROWS, int TK, int EXTRA> __device__ __forceinline__ int64_t cross_
 }
 
 // Rows of a block, workgroups that are resident on a CU, and whether a block's waves share its
-// rows (asked for with `few`; without it where a tile's values have no room beside the others').
+// rows (asked for with `few`, and so where LDS has room for keys of each wave's own).
 struct CrossBlocks {
     int rows, groups;
     bool few;
