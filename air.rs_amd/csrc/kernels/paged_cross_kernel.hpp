@@ -478,8 +478,10 @@ void paged_cross_kernel(CrossArgs a) {
 #pragma unroll
                             for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(raw.w[i][KIND == kFloats ? j / 4 : 0][j % 4]);
                         } else {
-                            // (scales of groups of zeros were left out: theirs may be any size)
-                            const float sc = F16 ? __builtin_amdgcn_fmed3f(raw.s[i] * (val ? fv_next : fk_next), -0x1p100f, 0x1p100f) : raw.s[i];
+                            // (scales of groups of zeros were left out: theirs may be any size; one that is not finite
+                            // leaves NaN, 0 * s, to all of its group, zero codes too)
+                            const float sc = F16 ? __builtin_fmaf(raw.s[i], 0.0f, __builtin_amdgcn_fmed3f(raw.s[i] * (val ? fv_next : fk_next), -0x1p100f, 0x1p100f))
+                                                 : raw.s[i];
                             uint32_t w0 = raw.w[i][0][0], w1 = raw.w[i][0][1];
                             asm volatile("" : "+v"(w0), "+v"(w1));     // (not taken apart while on its way: four registers for one)
                             cross_f32x4 lo, hi;
