@@ -6,7 +6,9 @@
 //   O^T += V^T . P^T   the same instruction; its contraction takes the keys in the order in
 //                      which the lanes hold P, so P never moves
 // Operands by kind (CrossKind):
-//   kBf16   bf16 queries over bf16 pages: probabilities are rounded to bf16
+//   kBf16   bf16 queries over bf16 pages.  Probabilities of bf16's 8 bits would err about as much as the output's
+//           rounding (2.3e-3 of its norm with both, 1.7e-3 with 11 bits or more): many rows round them to f16
+//           and multiply values as f16 (CONVERT), few rows take them in two bf16 parts, 16 bits
 //   kCodes  bf16 queries over 1-byte pages: everything as f16 (11 bits), under powers of two: of a
 //           query row's, of a tile's keys (from the largest scale of those that are not all zeros,
 //           known a barrier before the tile is staged) and of the values' (the smallest so far)
@@ -18,7 +20,7 @@
 //
 // Many rows (16-bit products, heads up to 128) are bound by the products and the arithmetic between them,
 // about as much of either: a step's exponentials run beside the next step's scores and the last one's
-// values (8192 states, 4096 tokens of 32 heads of 128: 558 us, 985 TFLOP/s; one after the other 577 to 597).
+// values (8192 states, 4096 tokens of 32 heads of 128: 590 us, 930 TFLOP/s).
 // Few rows are bound by the pages' reads (64 tokens, 512 to 4096 states, 8 heads of 128, bf16: 109 us, 5.2
 // TB/s; one f32 token over each of 32 sequences 110 us, 4.8; 1-byte pages 3.4, by their conversion).
 //
@@ -106,23 +108,25 @@ __device__ __forceinline__ void cross_split(float x, float y, uint32_t (&p)[3]) 
         y -= __uint_as_float(__float_as_uint(y) & 0xFFFF0000u);
     }
 }
-// x, y as P parts: three, or one rounded to f16 or bf16.
-template <bool F16, int P> __device__ __forceinline__ void cross_parts(float x, float y, uint32_t (&p)[P]) {
+// x, y as P parts: three, two bf16 ones (rounded, and what that leaves: 16 bits), or one f16 one.
+template <int P> __device__ __forceinline__ void cross_parts(float x, float y, uint32_t (&p)[P]) {
     if constexpr (P == 3) cross_split(x, y, p);
-    else p[0] = F16 ? cross_f16_pair(x, y) : cross_bf16_pair(x, y);
+    else if constexpr (P == 2) {
+        p[0] = cross_bf16_pair(x, y);
+        p[1] = cross_bf16_pair(x - __uint_as_float(p[0] << 16), y - __uint_as_float(p[0] & 0xFFFF0000u));
+    } else p[0] = cross_f16_pair(x, y);
 }
 // 2^e, e clamped to the normal numbers; the exponent of a normal number.
 __device__ __forceinline__ float cross_pow2(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 __device__ __forceinline__ int cross_exponent(float x) { return (int)((__float_as_uint(x) >> 23) & 0xFF) - 127; }
-// The sum of a pair and c; ones: cross_ones (an inline constant would not be read as a pair).
-template <bool F16> __device__ __forceinline__ uint32_t cross_ones() {
-    uint32_t x = F16 ? 0x3C003C00u : 0x3F803F80u;
+// The sum of a pair of f16 and c; ones: cross_ones (an inline constant would not be read as a pair).
+__device__ __forceinline__ uint32_t cross_ones() {
+    uint32_t x = 0x3C003C00u;
     asm("" : "+s"(x));
     return x;
 }
-template <bool F16> __device__ __forceinline__ float cross_add_pair(uint32_t p, uint32_t ones, float c) {
-    if constexpr (F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(cross_f16x2, p), __builtin_bit_cast(cross_f16x2, ones), c, false);
-    else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(cross_bf16x2, p), __builtin_bit_cast(cross_bf16x2, ones), c, false);
+__device__ __forceinline__ float cross_add_pair(uint32_t p, uint32_t ones, float c) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(cross_f16x2, p), __builtin_bit_cast(cross_f16x2, ones), c, false);
 }
 // The values of the four 1-byte codes in w times their scale.  SMALL: |s| is below 2^100; int8 codes
 // then take two instructions each, (code + 128) s - 128 s in one step (128 s is exact, and the
@@ -163,6 +167,11 @@ struct CrossShape {
     static constexpr int GROUPS = cross_groups(D, QP, FEW) == 2 && TILE <= cross_lds(2) ? 2 : 1;
     static constexpr int NB = PIPE ? 3 : !PRIVATE && 2 * TILE <= cross_lds(GROUPS) ? 2 : 1;
     static constexpr int WAVES_SIMD = WAVES / 4 * GROUPS;
+    // Values of bf16 pages as f16, under a power of two, converted once for a block's rows.  (8192 states of 128: bf16
+    // probabilities 560 us, f16 ones 590, in two bf16 parts with products of both 736; 2000 states, heads of 160 / 256:
+    // 116 / 275, 121 / 309, 149 / 321.  Few rows, bound by the pages, lose nothing to the parts.)
+    static constexpr bool CONVERT = KIND == kBf16 && !PRIVATE;
+    static constexpr int PP = KIND == kBf16 && !CONVERT ? 2 : QP;      // parts of probabilities
 };
 
 template <int D, CrossKind KIND, bool FEW>
@@ -170,8 +179,8 @@ __global__ __launch_bounds__((CrossShape<D, KIND, FEW>::WAVES * 64))
 __attribute__((amdgpu_waves_per_eu(CrossShape<D, KIND, FEW>::WAVES_SIMD, CrossShape<D, KIND, FEW>::WAVES_SIMD)))
 void paged_cross_kernel(CrossArgs a) {
     typedef CrossShape<D, KIND, FEW> S;
-    constexpr bool F16 = KIND == kCodes, PRIVATE = S::PRIVATE, SPLIT = S::SPLIT, PIPE = S::PIPE;
-    constexpr int KP = S::KP, QP = S::QP, WAVES = S::WAVES, WK = S::WK, SUB = S::SUB, ROWS = S::ROWS, TK = S::TK, NB = S::NB, THREADS = 64 * WAVES;
+    constexpr bool F16 = KIND == kCodes, CONVERT = S::CONVERT, V16 = F16 || CONVERT, PRIVATE = S::PRIVATE, SPLIT = S::SPLIT, PIPE = S::PIPE;
+    constexpr int KP = S::KP, QP = S::QP, PP = S::PP, WAVES = S::WAVES, WK = S::WK, SUB = S::SUB, ROWS = S::ROWS, TK = S::TK, NB = S::NB, THREADS = 64 * WAVES;
     constexpr int KST = cross_k_stride(D), VST = cross_v_stride(D);
     constexpr int STAGED = PRIVATE ? 32 : TK;          // keys side by side
     constexpr int KPLANE = STAGED * KST, VPLANE = STAGED * VST, VAT = PRIVATE && SPLIT ? 0 : KP * KPLANE;      // a part's rows; where values begin
@@ -179,7 +188,12 @@ void paged_cross_kernel(CrossArgs a) {
     // Staging: a wave takes SH of the tile's 16-key halves of keys or values, WR rows a pass, LPR lanes
     // a row (a power of two: some idle where D / 8 is none), 8 elements a lane.
     constexpr int LPR = D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32, WR = 64 / LPR, NPH = 16 / WR;
-    constexpr int SH = 2 * TK / 16 / WAVES, NP = SH * NPH;
+    // (CONVERT with one half for each wave: eight rows of keys and eight of values instead, so that no wave has more
+    // to convert than another: 610 -> 592 us for 8192 states of 128)
+    constexpr int SH = 2 * TK / 16 / WAVES;
+    constexpr bool EIGHT = CONVERT && SH == 1;
+    constexpr int UNITS = EIGHT ? 2 : SH, UP = EIGHT ? NPH / 2 : NPH, NP = UNITS * UP;
+    static_assert(UP >= 1, "whole passes");
     static_assert(SH >= 1 && SH * WAVES * 16 == 2 * TK && (SH == 1 || SH % 2 == 0), "whole halves");
     constexpr int EXTRA = cross_extra(FEW);
     constexpr int kOnce = FEW ? kCrossStream : 0;
@@ -260,11 +274,12 @@ void paged_cross_kernel(CrossArgs a) {
     const int nsc = CODES ? D >> a.sg_log2 : 0;
     const int p_sc = p_in ? (lane / LPR * nsc + (8 * p_c >> a.sg_log2)) * 4 : kCrossNowhere;
 
-    // half j of this wave's: of values (else keys), and which of the tile's
-    auto of_values = [&](int j) __attribute__((always_inline)) { return SH == 1 ? wave >= WAVES / 2 : j >= SH / 2; };
-    auto half_of = [&](int j) __attribute__((always_inline)) { return SH == 1 ? wave % (WAVES / 2) : wave * (SH / 2) + j % (SH / 2); };
+    // half j of this wave's: of values (else keys), and which of the tile's; the first of its rows
+    auto of_values = [&](int j) __attribute__((always_inline)) { return UNITS == 1 ? wave >= WAVES / 2 : j >= UNITS / 2; };
+    auto half_of = [&](int j) __attribute__((always_inline)) { return EIGHT ? wave / 2 : SH == 1 ? wave % (WAVES / 2) : wave * (SH / 2) + j % (SH / 2); };
+    const int row0 = EIGHT ? 8 * (wave % 2) : 0;
 
-    const uint32_t ones = cross_ones<F16>();
+    const uint32_t ones = cross_ones();
     // A SIMD has waves i and i + 4 of a workgroup: the second goes first, so that the two get out of
     // phase and one's products run beside the other's arithmetic.
     if (WAVES == 8 && wave >= 4) __builtin_amdgcn_s_setprio(1);
@@ -326,7 +341,7 @@ void paged_cross_kernel(CrossArgs a) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         uint32_t p[QP];
-                        cross_parts<F16, QP>(x[2 * j], x[2 * j + 1], p);
+                        cross_parts<QP>(x[2 * j], x[2 * j + 1], p);
 #pragma unroll
                         for (int k = 0; k < QP; ++k) qf[k][s][2 * i + j] = p[k];
                     }
@@ -350,22 +365,29 @@ void paged_cross_kernel(CrossArgs a) {
                     qf[0][s][j] = cross_f16_pair(__uint_as_float(qf[0][s][j] << 16) * fq, __uint_as_float(qf[0][s][j] & 0xFFFF0000u) * fq);
         }
         cross_f32x16 acc[CT];
-#pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
         // Probabilities are held 2^(score - base), the base kDown above every score so far: 2^24 of
         // them sum to 1 at most, so that values near the largest float do too.  (f16 ones up to
-        // 2^15, so that they keep 11 bits down to 2^-25 of the largest; values are below 2^15 there.)
+        // 2^15, so that they keep 11 bits down to 2^-25 of the largest; values are below 2^16 there.)
         // A base is taken kSlack further up, so that it seldom changes: where a score passes lim.
-        constexpr float kDown = F16 ? -15.0f : 24.0f, kSlack = 4.0f, kFar = 0x1p20f;
-        float base = -INFINITY, lim = -INFINITY, l_run = 0.0f;
+        constexpr float kSlack = 4.0f, kFar = 0x1p20f;
+        float kDown, base, lim, l_run;
+        auto clear = [&](float down) __attribute__((always_inline)) {
+            kDown = down;
+            base = lim = -INFINITY;
+            l_run = 0.0f;
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
+        };
+        clear(V16 ? -15.0f : 24.0f);
 
         struct Raw {                                   // a tile on its way
             cross_u32x4 w[NP][KIND == kFloats ? 2 : 1];
             float s[CODES ? NP : 1];
         } raw, next;                                   // (next: kCodes with two buffers, a tile further ahead)
-        float fk = 1.0f, fk_next = 1.0f, fv = 0.0f, fv_next = 0.0f;    // kCodes: powers of two (0: no value yet)
+        float fk = 1.0f, fk_next = 1.0f, fv = 0.0f, fv_next = 0.0f;    // kCodes: powers of two (0: no value yet); CONVERT: fv
+        int counted = 0;                               // tiles whose table entries are (CONVERT comes twice)
         // lane h: the entry of a tile's half h, read a tile before it is needed, and its block
         int32_t entry = 0, window = -1;
         auto fetch = [&](int t) __attribute__((always_inline)) {
@@ -377,10 +399,11 @@ void paged_cross_kernel(CrossArgs a) {
             const bool there = t < tiles && lane < TK / 16 && key < sq.len, out = there && (entry < 0 || entry >= a.num_blocks);
             window = out || !there ? -1 : entry;
             // counted once: by the first block of rows at the first head
-            if (head == 0 && blk == 0 && wave == 0) {
+            if (head == 0 && blk == 0 && wave == 0 && (!CONVERT || t >= counted)) {
                 const int n = __popcll(__ballot(out && (key & ((1 << a.bs_log2) - 1)) == 0));
                 if (n && lane == 0) atomicAdd(a.errors, (unsigned long long)n);
             }
+            if (CONVERT && t >= counted) counted = t + 1;
             if (!PRIVATE && wave == 0 && lane < TK / 16) s_ok[t % 8][lane] = window >= 0;
             fetch(t + 1);
         };
@@ -393,22 +416,22 @@ void paged_cross_kernel(CrossArgs a) {
         };
         auto load_tile = [&](int t, Raw &raw, auto part) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < SH; ++j) {
+            for (int j = 0; j < UNITS; ++j) {
                 if (skip(j, part)) continue;
                 const int half = half_of(j);
                 const bool val = of_values(j);
                 const int32_t e = __builtin_amdgcn_readlane(window, half);
-                const int64_t rest = sq.len - (key0 + (int64_t)t * TK + 16 * half);
-                const int have = e < 0 || rest <= 0 ? 0 : rest < 16 ? (int)rest : 16;
-                const int64_t prow = (((int64_t)(e < 0 ? 0 : e) * a.heads + head) << a.bs_log2) + (16 * half & ((1 << a.bs_log2) - 1));
+                const int64_t rest = sq.len - (key0 + (int64_t)t * TK + 16 * half + row0);
+                const int have = e < 0 || rest <= 0 ? 0 : rest < 16 - row0 ? (int)rest : 16 - row0;
+                const int64_t prow = (((int64_t)(e < 0 ? 0 : e) * a.heads + head) << a.bs_log2) + (16 * half & ((1 << a.bs_log2) - 1)) + row0;
                 const uint8_t *pages = (const uint8_t *)(val ? a.v_pages : a.k_pages) + prow * (D * esize);
                 // rows past the sequence's end lie outside of the buffer: zeros
                 const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)pages, (short)0, have * D * esize, kCrossBuffer);
                 const float *scales = (val ? a.v_scales : a.k_scales) + prow * nsc;
                 const __amdgpu_buffer_rsrc_t ss = __builtin_amdgcn_make_buffer_rsrc((void *)scales, (short)0, have * nsc * 4, kCrossBuffer);
 #pragma unroll
-                for (int k = 0; k < NPH; ++k) {
-                    const int i = j * NPH + k;
+                for (int k = 0; k < UP; ++k) {
+                    const int i = j * UP + k;
                     if constexpr (KIND == kBf16 || KIND == kParts) {
                         raw.w[i][0] = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off + k * WR * D * 2, 0, kOnce));
                     } else if constexpr (CODES) {
@@ -434,7 +457,7 @@ void paged_cross_kernel(CrossArgs a) {
                 for (int i = 0; i < NP; ++i) {
                     const float x = __builtin_fabsf(raw.s[i]);
                     const float y = x < INFINITY && ((raw.w[i][0][0] | raw.w[i][0][1]) & sign) ? x : 0.0f;
-                    if (of_values(i / NPH)) v = fmaxf(v, y);
+                    if (of_values(i / UP)) v = fmaxf(v, y);
                     else k = fmaxf(k, y);
                 }
                 if (SH > 1 || !of_values(0)) k = cross_wave_max(k);
@@ -452,26 +475,53 @@ void paged_cross_kernel(CrossArgs a) {
             const float want = cross_pow2(3 - cross_exponent(v));
             fv_next = v == 0.0f ? fv_next : fv_next == 0.0f || fv_next > 4.0f * want ? want : fv_next;
         };
-        auto write_tile = [&](int t, const Raw &raw, auto part) __attribute__((always_inline)) {
+        // CONVERT: the values' power of two, from the largest of the first 64 * 8 of the slice's, which every wave
+        // reads for itself: 1 where that lies in [2^-2, 2^10), else what brings it to 2^9, and 0, no f16 values, where
+        // all are zeros.  f16 holds bf16's 8 bits from 2^-17 on, in steps of 2^-24 below (2^-22 of the largest and
+        // less), up to 2^16; a value beyond that is found at the block's end, which is then computed again (a call of such
+        // blocks alone takes 2.1 times as long, one of zeros first 1.2).
+        auto sample = [&]() __attribute__((always_inline)) {
+            const int32_t e = __builtin_amdgcn_readlane(window, 0);
+            const int64_t rest = sq.len - key0, prow = ((int64_t)(e < 0 ? 0 : e) * a.heads + head) << a.bs_log2;
+            const int have = e < 0 ? 0 : rest < 16 ? (int)rest : 16;
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((uint8_t *)a.v_pages + prow * (D * esize), (short)0, have * D * esize, kCrossBuffer);
+            const cross_u32x4 w = __builtin_bit_cast(cross_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, p_off, 0, 0));
+            float x = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                x = fmaxf(x, fmaxf(__builtin_fabsf(__uint_as_float(w[j] << 16)), __builtin_fabsf(__uint_as_float(w[j] & 0xFFFF0000u))));
+            x = cross_wave_max(x);
+            fv = x == 0.0f ? 0.0f : !(x < INFINITY) || (x >= 0x1p-2f && x < 0x1p10f) ? 1.0f : cross_pow2(9 - cross_exponent(x));
+        };
+        // (exact: values of bf16 pages as they are)
+        constexpr std::integral_constant<bool, !CONVERT> kFast{};
+        constexpr std::true_type kExact{};
+        auto write_tile = [&](int t, const Raw &raw, auto part, auto exact) __attribute__((always_inline)) {
             uint8_t *mem = PRIVATE ? s_mem + wave * S::REGION : s_mem + t % NB * S::TILE;
             if constexpr (F16 && !PRIVATE) {
                 keys_power(__uint_as_float(__builtin_amdgcn_readfirstlane(s_top[t % 3][0])));
                 values_power(__uint_as_float(__builtin_amdgcn_readfirstlane(s_top[t % 3][1])));
             }
             // (the type is asked for once a tile; kWide asks at each chunk: all of a tile's, twice over, do not fit the registers)
-            auto rows = [&](auto type) __attribute__((always_inline)) {
+            auto rows = [&](auto type, auto scaled) __attribute__((always_inline)) {
                 constexpr int DT = decltype(type)::value;
 #pragma unroll
                 for (int i = 0; i < NP; ++i) {
-                    if (skip(i / NPH, part)) continue;
-                    const bool val = of_values(i / NPH);
-                    const int at = 16 * (PRIVATE ? i / NPH % (SH > 1 ? SH / 2 : 1) : half_of(i / NPH)) + i % NPH * WR + lane / LPR;
+                    if (skip(i / UP, part)) continue;
+                    const bool val = of_values(i / UP);
+                    const int at = 16 * (PRIVATE ? i / UP % (SH > 1 ? SH / 2 : 1) : half_of(i / UP)) + row0 + i % UP * WR + lane / LPR;
                     const int chunk = val && cross_v_xor(D) ? p_c ^ ((at & 3) << 2) : p_c;
                     uint8_t *to = mem + (val ? VAT + at * VST : at * KST) + 16 * chunk;
                     const int plane = val ? VPLANE : KPLANE;
                     cross_u32x4 y[KP];
                     if constexpr (DT == AIR_KV_BF16) {
                         y[0] = raw.w[i][0];
+                        if (!decltype(exact)::value && val)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float lo = __uint_as_float(y[0][j] << 16), hi = __uint_as_float(y[0][j] & 0xFFFF0000u);
+                                y[0][j] = decltype(scaled)::value ? cross_f16_pair(lo * fv, hi * fv) : cross_f16_pair(lo, hi);
+                            }
                     } else {
                         float x[8];
                         if constexpr (DT == AIR_KV_F32) {
@@ -498,7 +548,7 @@ void paged_cross_kernel(CrossArgs a) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             uint32_t p[KP];
-                            cross_parts<F16, KP>(x[2 * j], x[2 * j + 1], p);
+                            cross_parts<KP>(x[2 * j], x[2 * j + 1], p);
 #pragma unroll
                             for (int k = 0; k < KP; ++k) y[k][j] = p[k];
                         }
@@ -510,16 +560,20 @@ void paged_cross_kernel(CrossArgs a) {
                     if constexpr (KP == 3) __builtin_amdgcn_sched_barrier(0);
                 }
             };
-            if constexpr (KIND == kBf16 || KIND == kParts) rows(std::integral_constant<int, AIR_KV_BF16>{});
-            else if constexpr (KIND == kFloats) rows(std::integral_constant<int, AIR_KV_F32>{});
-            else if (KIND == kCodes && a.dtype == AIR_KV_INT8) rows(std::integral_constant<int, AIR_KV_INT8>{});
-            else rows(std::integral_constant<int, AIR_KV_FP8>{});
+            constexpr std::false_type plain{};
+            if constexpr (KIND == kBf16 || KIND == kParts) {
+                constexpr std::integral_constant<int, AIR_KV_BF16> bf16{};
+                if (decltype(exact)::value || fv == 1.0f) rows(bf16, plain);
+                else rows(bf16, std::true_type{});
+            } else if constexpr (KIND == kFloats) rows(std::integral_constant<int, AIR_KV_F32>{}, plain);
+            else if (KIND == kCodes && a.dtype == AIR_KV_INT8) rows(std::integral_constant<int, AIR_KV_INT8>{}, plain);
+            else rows(std::integral_constant<int, AIR_KV_FP8>{}, plain);
         };
         float mk = 0.0f, mv = 0.0f;
         // Many rows: what comes between two tiles' products, t the one at hand: tile t + 1 into its
         // buffer, t + 2 on its way (kCodes with two buffers: t + 2 marked, t + 3 on its way).
-        auto stage = [&](int t) __attribute__((always_inline)) {
-            write_tile(t + 1, raw, kBoth);
+        auto stage = [&](int t, auto exact) __attribute__((always_inline)) {
+            write_tile(t + 1, raw, kBoth, exact);
             if (t + 2 >= tiles) return;
             if constexpr (F16 && NB >= 2) {
                 raw = next;
@@ -534,37 +588,44 @@ void paged_cross_kernel(CrossArgs a) {
             }
         };
 
-        fetch(0);
-        __syncthreads();                               // the buffers of the block before are free
-        look_up(0);
-        load_tile(0, raw, kBoth);
-        if constexpr (!PRIVATE) {
-            if (F16 && tid < 6) s_top[tid / 2][tid % 2] = 0;
-            if (F16 && NB >= 2 && 1 < tiles) {
-                look_up(1);
-                load_tile(1, next, kBoth);
+        auto begin = [&](auto exact) __attribute__((always_inline)) {
+            fetch(0);
+            __syncthreads();                               // the buffers of the block before are free
+            look_up(0);
+            load_tile(0, raw, kBoth);
+            if constexpr (!decltype(exact)::value) {
+                sample();
+                if (fv == 0.0f) return;
             }
-            if constexpr (F16) {
-                __syncthreads();
-                mark(0, raw, mk, mv);
-                __syncthreads();
-            }
-            write_tile(0, raw, kBoth);
-            if (1 < tiles) {
-                if constexpr (F16 && NB >= 2) {
-                    raw = next;
-                    if (2 < tiles) {
-                        look_up(2);
-                        load_tile(2, next, kBoth);
-                    }
-                    mark(1, raw, mk, mv);
-                } else {
+            if constexpr (!PRIVATE) {
+                if (F16 && tid < 6) s_top[tid / 2][tid % 2] = 0;
+                if (F16 && NB >= 2 && 1 < tiles) {
                     look_up(1);
-                    load_tile(1, raw, kBoth);
+                    load_tile(1, next, kBoth);
                 }
+                if constexpr (F16) {
+                    __syncthreads();
+                    mark(0, raw, mk, mv);
+                    __syncthreads();
+                }
+                write_tile(0, raw, kBoth, exact);
+                if (1 < tiles) {
+                    if constexpr (F16 && NB >= 2) {
+                        raw = next;
+                        if (2 < tiles) {
+                            look_up(2);
+                            load_tile(2, next, kBoth);
+                        }
+                        mark(1, raw, mk, mv);
+                    } else {
+                        look_up(1);
+                        load_tile(1, raw, kBoth);
+                    }
+                }
+                __syncthreads();
             }
-            __syncthreads();
-        }
+        };
+        begin(kFast);
         // ---- a step's parts: 32 keys, those of a buffer `mem` from row k0 on
 
         auto scores = [&](const uint8_t *mem, int k0, cross_f32x16 &sc) __attribute__((always_inline)) {
@@ -635,7 +696,8 @@ void paged_cross_kernel(CrossArgs a) {
             ft = a.scale_log2;
             if constexpr (F16) ft = fminf(fmaxf(__builtin_amdgcn_ldexpf(ft, -(qe + cross_exponent(fk))), 0x1p-126f), 0x1.fffffep127f);
         };
-        auto probabilities = [&](cross_f32x16 &sc, float ft, cross_u32x4 (&p)[QP][2]) __attribute__((always_inline)) {
+        auto probabilities = [&](cross_f32x16 &sc, float ft, auto &p) __attribute__((always_inline)) {
+            constexpr int P = std::extent_v<std::remove_reference_t<decltype(p)>>;
             const float from = base == -INFINITY ? 0.0f : base;
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], ft, -from));
@@ -643,12 +705,12 @@ void paged_cross_kernel(CrossArgs a) {
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    uint32_t x[QP];
-                    cross_parts<F16, QP>(sc[8 * s + 2 * j], sc[8 * s + 2 * j + 1], x);
+                    uint32_t x[P];
+                    cross_parts<P>(sc[8 * s + 2 * j], sc[8 * s + 2 * j + 1], x);
 #pragma unroll
-                    for (int k = 0; k < QP; ++k) p[k][s][j] = x[k];
-                    // (16-bit ones are summed as they were rounded)
-                    if constexpr (QP == 1) l_run = cross_add_pair<F16>(x[0], ones, l_run);
+                    for (int k = 0; k < P; ++k) p[k][s][j] = x[k];
+                    // (f16 ones are summed as they were rounded)
+                    if constexpr (P == 1) l_run = cross_add_pair(x[0], ones, l_run);
                     else l_run += sc[8 * s + 2 * j] + sc[8 * s + 2 * j + 1];
                 }
         };
@@ -656,7 +718,8 @@ void paged_cross_kernel(CrossArgs a) {
         // Within each 16-lane group, lane j of a transposing read receives element j % 4 of the 8
         // bytes that lanes 4 k + j / 4 address, k = 0 .. 3: lane i points at key i / 4 of the four
         // and columns 4 (i % 4) of the group's sixteen.
-        auto values = [&](const uint8_t *mem, int k0, const cross_u32x4 (&p)[QP][2]) __attribute__((always_inline)) {
+        auto values = [&](const uint8_t *mem, int k0, const auto &p) __attribute__((always_inline)) {
+            constexpr int P = std::extent_v<std::remove_reference_t<decltype(p)>>;
             int ln = lane;                             // (its addresses are not kept in registers from step to step)
             asm volatile("" : "+v"(ln));
             const int vr = 4 * (ln >> 5) + ((ln & 15) >> 2);
@@ -676,120 +739,160 @@ void paged_cross_kernel(CrossArgs a) {
                                                   (__attribute__((address_space(3))) s16x4 *)(v + 8 * VST)));
                         const cross_u32x4 vf = {x[0], x[1], y[0], y[1]};
 #pragma unroll
-                        for (int j = 0; j < QP; ++j)
-                            if (i + j < 3) acc[c] = cross_mfma<F16>(vf, p[j][s], acc[c]);
+                        for (int j = 0; j < P; ++j)
+                            if (i + j < 3) acc[c] = cross_mfma<P == 1>(vf, p[j][s], acc[c]);
                     }
         };
 
+        // Many rows, a step after the other.
+        auto walk = [&](auto exact) __attribute__((always_inline)) {
+            for (int t = 0; t < tiles; ++t) {
+                if constexpr (F16) {
+                    fk = fk_next;
+                    if (fv != fv_next) {
+                        scale_sums(fv == 0.0f ? 1.0f : fv_next / fv);
+                        fv = fv_next;
+                    }
+                    if (tid < 2) s_top[t % 3][tid] = 0;
+                }
+                if (NB >= 2 && t + 1 < tiles) stage(t, exact);
+                if (any) {
+                    const uint8_t *mem = s_mem + t % NB * S::TILE;
+#pragma unroll
+                    for (int sub = 0; sub < SUB; ++sub) {
+                        const int64_t rest = sq.len - (key0 + (int64_t)t * TK + 32 * sub);
+                        if (rest <= 0) continue;
+                        cross_f32x16 sc;
+                        cross_u32x4 p[CONVERT && decltype(exact)::value ? 2 : PP][2];
+                        float top, ft, alpha;
+                        scores(mem, 32 * sub, sc);
+                        tops(sc, top);
+                        hide(rest, __builtin_amdgcn_readfirstlane(s_ok[t % 8][2 * sub] + 2 * s_ok[t % 8][2 * sub + 1]), sc, top);
+                        factors(fk, ft);
+                        if (rebase(sc, top, ft, alpha)) scale_sums(alpha);
+                        probabilities(sc, ft, p);
+                        values(mem, 32 * sub, p);
+                    }
+                }
+                if (NB == 1 && t + 1 < tiles) mark(t + 1, raw, mk, mv);
+                __syncthreads();
+                if (NB == 1 && t + 1 < tiles) {
+                    stage(t, exact);
+                    __syncthreads();
+                }
+            }
+        };
         if constexpr (PIPE) {
             // A step's probabilities are computed beside the next step's scores and the one before's
             // values, so that products and arithmetic, about as much of either, run at once.  A tile is
             // two steps; the next tile is staged beside the first and there at a barrier before the second.
-            static_assert(QP == 1 && KP == 1 && KS == 2 * CT && NB == 3, "16-bit parts");
-            cross_f32x16 sa, sb;
-            cross_u32x4 pa[2], pb[2];
-            float top;
-            float fv_t = fv_next;                      // kCodes: of the tile whose values come next
-            // (this lane's places in a buffer: keys, values of four column tiles)
-            const int k_at = r32 * KST + 16 * hf, vr = 4 * hf + ((lane & 15) >> 2);
-            int v_at[4];
+            static_assert(PP == 1 && KP == 1 && KS == 2 * CT && NB == 3, "16-bit parts");
+            if (!CONVERT || fv != 0.0f) {
+                cross_f32x16 sa, sb;
+                cross_u32x4 pa[2], pb[2];
+                float top;
+                float fv_t = fv_next;                      // kCodes: of the tile whose values come next
+                // (this lane's places in a buffer: keys, values of four column tiles)
+                const int k_at = r32 * KST + 16 * hf, vr = 4 * hf + ((lane & 15) >> 2);
+                int v_at[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                v_at[c] = VAT + vr * VST + 32 * ((lane >> 4) & 1) + 8 * (lane & 3) + 64 * (cross_v_xor(D) ? c ^ (vr & 3) : c);
-            // A step from its scores in sc: p; the next step's scores, of the keys from row k0 of buffer kb, in
-            // sn; the sums of the step before, its probabilities q and the values from row v0 of buffer vb.
-            auto step = [&](cross_f32x16 &sc, cross_f32x16 &sn, cross_u32x4 (&p)[2], const cross_u32x4 (&q)[2], int kb, int k0, int vb,
-                            int v0, int64_t rest, int ok, float fk) __attribute__((always_inline)) {
-                hide(rest, ok, sc, top);
-                float ft, alpha;
-                factors(fk, ft);
-                const bool changed = rebase(sc, top, ft, alpha);
-                // what follows is in the order in which it shall run: a product, then arithmetic that is done
-                // while it runs, fragments read three products ahead
-                constexpr int AHEAD = 3, N = KS + 2 * CT;
-                typedef const __attribute__((address_space(3))) uint8_t *lds_t;
-                const lds_t k = (lds_t)s_mem + kb * S::TILE + k0 * KST + k_at;
-                lds_t v[CT < 4 ? CT : 4];
+                for (int c = 0; c < 4; ++c)
+                    v_at[c] = VAT + vr * VST + 32 * ((lane >> 4) & 1) + 8 * (lane & 3) + 64 * (cross_v_xor(D) ? c ^ (vr & 3) : c);
+                // A step from its scores in sc: p; the next step's scores, of the keys from row k0 of buffer kb, in
+                // sn; the sums of the step before, its probabilities q and the values from row v0 of buffer vb.
+                auto step = [&](cross_f32x16 &sc, cross_f32x16 &sn, cross_u32x4 (&p)[2], const cross_u32x4 (&q)[2], int kb, int k0, int vb,
+                                int v0, int64_t rest, int ok, float fk) __attribute__((always_inline)) {
+                    hide(rest, ok, sc, top);
+                    float ft, alpha;
+                    factors(fk, ft);
+                    const bool changed = rebase(sc, top, ft, alpha);
+                    // what follows is in the order in which it shall run: a product, then arithmetic that is done
+                    // while it runs, fragments read three products ahead
+                    constexpr int AHEAD = 3, N = KS + 2 * CT;
+                    typedef const __attribute__((address_space(3))) uint8_t *lds_t;
+                    const lds_t k = (lds_t)s_mem + kb * S::TILE + k0 * KST + k_at;
+                    lds_t v[CT < 4 ? CT : 4];
 #pragma unroll
-                for (int c = 0; c < CT && c < 4; ++c) v[c] = (lds_t)s_mem + vb * S::TILE + v0 * VST + v_at[c];
-                cross_u32x4 f[N];
-                auto read = [&](int i) __attribute__((always_inline)) {
-                    typedef short s16x4 __attribute__((ext_vector_type(4)));
-                    if (i < KS) {
-                        f[i] = *reinterpret_cast<const __attribute__((address_space(3))) cross_u32x4 *>(k + 32 * i);
-                    } else if (i < N) {
-                        const int c = (i - KS) / 2, at = 256 * (c / 4) + 16 * ((i - KS) % 2) * VST;
-                        const cross_u32x2 x = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                  (__attribute__((address_space(3))) s16x4 *)(v[c % 4] + at)));
-                        const cross_u32x2 y = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                  (__attribute__((address_space(3))) s16x4 *)(v[c % 4] + at + 8 * VST)));
-                        f[i] = cross_u32x4{x[0], x[1], y[0], y[1]};
-                    }
-                };
-                const float from = base == -INFINITY ? 0.0f : base;
-                auto pair = [&](int i) __attribute__((always_inline)) {
-                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * i], ft, -from));
-                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * i + 1], ft, -from));
-                    p[i / 4][i % 4] = F16 ? cross_f16_pair(x, y) : cross_bf16_pair(x, y);
-                    l_run = cross_add_pair<F16>(p[i / 4][i % 4], ones, l_run);
-                };
+                    for (int c = 0; c < CT && c < 4; ++c) v[c] = (lds_t)s_mem + vb * S::TILE + v0 * VST + v_at[c];
+                    cross_u32x4 f[N];
+                    auto read = [&](int i) __attribute__((always_inline)) {
+                        typedef short s16x4 __attribute__((ext_vector_type(4)));
+                        if (i < KS) {
+                            f[i] = *reinterpret_cast<const __attribute__((address_space(3))) cross_u32x4 *>(k + 32 * i);
+                        } else if (i < N) {
+                            const int c = (i - KS) / 2, at = 256 * (c / 4) + 16 * ((i - KS) % 2) * VST;
+                            const cross_u32x2 x = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                      (__attribute__((address_space(3))) s16x4 *)(v[c % 4] + at)));
+                            const cross_u32x2 y = __builtin_bit_cast(cross_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                      (__attribute__((address_space(3))) s16x4 *)(v[c % 4] + at + 8 * VST)));
+                            f[i] = cross_u32x4{x[0], x[1], y[0], y[1]};
+                        }
+                    };
+                    const float from = base == -INFINITY ? 0.0f : base;
+                    auto pair = [&](int i) __attribute__((always_inline)) {
+                        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * i], ft, -from));
+                        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * i + 1], ft, -from));
+                        p[i / 4][i % 4] = cross_f16_pair(x, y);
+                        l_run = cross_add_pair(p[i / 4][i % 4], ones, l_run);
+                    };
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sn[i] = 0.0f;
+                    for (int i = 0; i < 16; ++i) sn[i] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < AHEAD; ++i) read(i);
-                __builtin_amdgcn_sched_barrier(0);
-                int done = 0;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    read(i + AHEAD);
-                    if (i < KS) sn = cross_mfma<F16>(f[i], qf[0][i], sn);
-                    else acc[(i - KS) / 2] = cross_mfma<F16>(f[i], q[(i - KS) % 2], acc[(i - KS) / 2]);
-#pragma unroll
-                    for (; done < 8 * (i + 1) / N; ++done) pair(done);
+                    for (int i = 0; i < AHEAD; ++i) read(i);
                     __builtin_amdgcn_sched_barrier(0);
-                }
-                tops(sn, top);
-                // (here, and not where they are used: behind a branch)
-                asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(l_run));
-                if (__builtin_expect(changed, 0)) {
-                    asm volatile("");                  // (a branch: no products by 1)
-                    scale_sums(alpha);
-                }
-            };
-            auto in_pool = [&](int t, int half) __attribute__((always_inline)) {
-                return __builtin_amdgcn_readfirstlane(s_ok[t % 8][half] + 2 * s_ok[t % 8][half + 1]);
-            };
-            // (the step before the first: probabilities of 0, of values that are there)
-            pb[0] = pb[1] = cross_u32x4{0, 0, 0, 0};
-            scores(s_mem, 0, sa);
-            tops(sa, top);
-            int before = 0, at = 0;                    // buffers of tiles t - 1 and t
-            for (int t = 0; t < tiles; ++t) {
-                const int next = at == 2 ? 0 : at + 1;
-                const int64_t rest = sq.len - (key0 + (int64_t)t * TK);
-                step(sa, sb, pa, pb, at, 32, before, 32, rest, in_pool(t, 0), fk_next);
-                if constexpr (F16) {
-                    fk = fk_next;
-                    fv_t = fv_next;
-                    if (tid < 2) s_top[t % 3][tid] = 0;
-                }
-                if (t + 1 < tiles) stage(t);
-                __syncthreads();
-                if constexpr (F16) {
-                    // (a power of two that changes: the sums so far are brought under it)
-                    if (__builtin_expect(fv != fv_t, 0)) {
-                        scale_sums(fv == 0.0f ? 1.0f : fv_t / fv);
-                        fv = fv_t;
+                    int done = 0;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        read(i + AHEAD);
+                        if (i < KS) sn = cross_mfma<F16>(f[i], qf[0][i], sn);
+                        else acc[(i - KS) / 2] = cross_mfma<true>(f[i], q[(i - KS) % 2], acc[(i - KS) / 2]);
+#pragma unroll
+                        for (; done < 8 * (i + 1) / N; ++done) pair(done);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
+                    tops(sn, top);
+                    // (here, and not where they are used: behind a branch)
+                    asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(l_run));
+                    if (__builtin_expect(changed, 0)) {
+                        asm volatile("");                  // (a branch: no products by 1)
+                        scale_sums(alpha);
+                    }
+                };
+                auto in_pool = [&](int t, int half) __attribute__((always_inline)) {
+                    return __builtin_amdgcn_readfirstlane(s_ok[t % 8][half] + 2 * s_ok[t % 8][half + 1]);
+                };
+                // (the step before the first: probabilities of 0, of values that are there)
+                pb[0] = pb[1] = cross_u32x4{0, 0, 0, 0};
+                scores(s_mem, 0, sa);
+                tops(sa, top);
+                int before = 0, at = 0;                    // buffers of tiles t - 1 and t
+                for (int t = 0; t < tiles; ++t) {
+                    const int next = at == 2 ? 0 : at + 1;
+                    const int64_t rest = sq.len - (key0 + (int64_t)t * TK);
+                    step(sa, sb, pa, pb, at, 32, before, 32, rest, in_pool(t, 0), fk_next);
+                    if constexpr (F16) {
+                        fk = fk_next;
+                        fv_t = fv_next;
+                        if (tid < 2) s_top[t % 3][tid] = 0;
+                    }
+                    if (t + 1 < tiles) stage(t, kFast);
+                    __syncthreads();
+                    if constexpr (F16) {
+                        // (a power of two that changes: the sums so far are brought under it)
+                        if (__builtin_expect(fv != fv_t, 0)) {
+                            scale_sums(fv == 0.0f ? 1.0f : fv_t / fv);
+                            fv = fv_t;
+                        }
+                    }
+                    step(sb, sa, pb, pa, next, 0, at, 0, rest - 32, in_pool(t, 2), fk);
+                    before = at;
+                    at = next;
                 }
-                step(sb, sa, pb, pa, next, 0, at, 0, rest - 32, in_pool(t, 2), fk);
-                before = at;
-                at = next;
+                // (the last tile's second half)
+                cross_u32x4 p[PP][2] = {{pb[0], pb[1]}};
+                values(s_mem + before * S::TILE, 32, p);
+                __syncthreads();
             }
-            // (the last tile's second half)
-            cross_u32x4 p[QP][2] = {{pb[0], pb[1]}};
-            values(s_mem + before * S::TILE, 32, p);
-            __syncthreads();
         } else if constexpr (PRIVATE) {
             uint8_t *mem = s_mem + wave * S::REGION;
             // (a wave's LDS accesses are in order: what was there has been read)
@@ -801,7 +904,7 @@ void paged_cross_kernel(CrossArgs a) {
                 // whether this wave's halves are in the pool
                 const int ok = (__builtin_amdgcn_readlane(window, 2 * wave) >= 0 ? 1 : 0) | (__builtin_amdgcn_readlane(window, 2 * wave + 1) >= 0 ? 2 : 0);
                 const int64_t rest = sq.len - (key0 + (int64_t)t * TK + 32 * wave);
-                cross_u32x4 p[QP][2];
+                cross_u32x4 p[PP][2];
                 if constexpr (F16) {
                     mark(t, raw, mk, mv);
                     keys_power(mk);
@@ -814,7 +917,7 @@ void paged_cross_kernel(CrossArgs a) {
                 }
                 constexpr auto kFirst = std::conditional_t<SPLIT, decltype(kKeys), decltype(kBoth)>{};
                 ordered();
-                write_tile(t, raw, kFirst);
+                write_tile(t, raw, kFirst, kFast);
                 ordered();
                 if (t + 1 < tiles) {
                     look_up(t + 1);
@@ -832,53 +935,34 @@ void paged_cross_kernel(CrossArgs a) {
                 }
                 if constexpr (SPLIT) {
                     ordered();
-                    write_tile(t, raw, kValues);
+                    write_tile(t, raw, kValues, kFast);
                     ordered();
                     if (t + 1 < tiles) load_tile(t + 1, raw, kValues);
                 }
                 if (rest > 0) values(mem, 0, p);
             }
             __syncthreads();
-        } else {
-            for (int t = 0; t < tiles; ++t) {
-                if constexpr (F16) {
-                    fk = fk_next;
-                    if (fv != fv_next) {
-                        scale_sums(fv == 0.0f ? 1.0f : fv_next / fv);
-                        fv = fv_next;
-                    }
-                    if (tid < 2) s_top[t % 3][tid] = 0;
-                }
-                if (NB == 2 && t + 1 < tiles) stage(t);
-                if (any) {
-                    const uint8_t *mem = s_mem + t % NB * S::TILE;
+        } else if (!CONVERT || fv != 0.0f) {
+            walk(kFast);
+        }
+        if constexpr (CONVERT) {
+            // A row whose probabilities are finite and whose sums are not: a value was not, or beyond f16 (an
+            // infinity there).
+            float x = 0.0f;
 #pragma unroll
-                    for (int sub = 0; sub < SUB; ++sub) {
-                        const int64_t rest = sq.len - (key0 + (int64_t)t * TK + 32 * sub);
-                        if (rest <= 0) continue;
-                        cross_f32x16 sc;
-                        cross_u32x4 p[QP][2];
-                        float top, ft, alpha;
-                        scores(mem, 32 * sub, sc);
-                        tops(sc, top);
-                        hide(rest, __builtin_amdgcn_readfirstlane(s_ok[t % 8][2 * sub] + 2 * s_ok[t % 8][2 * sub + 1]), sc, top);
-                        factors(fk, ft);
-                        if (rebase(sc, top, ft, alpha)) scale_sums(alpha);
-                        probabilities(sc, ft, p);
-                        values(mem, 32 * sub, p);
-                    }
-                }
-                if (NB == 1 && t + 1 < tiles) mark(t + 1, raw, mk, mv);
-                __syncthreads();
-                if (NB == 1 && t + 1 < tiles) {
-                    stage(t);
-                    __syncthreads();
-                }
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x = __builtin_fmaf(acc[c][i], 0.0f, x);
+            if (__builtin_expect(__syncthreads_or(fv == 0.0f || (x != 0.0f && l_run < INFINITY)), 0)) {     // from values as they are
+                fv = 0.0f;
+                clear(24.0f);
+                begin(kExact);
+                walk(kExact);
             }
         }
 
         // lane (n, h): columns 32 c + 8 (i / 4) + 4 h + i % 4 of row n in acc[c][i]
-        float unit = F16 && fv != 0.0f ? 1.0f / fv : 1.0f;     // of the sums (pieces' stay under it)
+        float unit = V16 && fv != 0.0f ? 1.0f / fv : 1.0f;     // of the sums (pieces' stay under it)
         const int64_t slot = 2 * cell + (t0 == 0 ? 1 : 0);
         if constexpr (WK == 1) {
             const float l = sum_x32(l_run);
@@ -891,7 +975,7 @@ void paged_cross_kernel(CrossArgs a) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         cross_f32x4 x = cross_f32x4{acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]} * k;
-                        if (F16 && whole) x *= unit;
+                        if (V16 && whole) x *= unit;
                         const int col = 32 * c + 8 * i + 4 * hf;
                         if (whole) cross_store4(a, io + col, x);
                         else *reinterpret_cast<cross_f32x4 *>(a.part_o + prow * D + col) = x;

@@ -466,7 +466,11 @@ int air_paged_diff_prefill(air_kv_pool *pool, void *stream, const void *q, int32
  * be q itself where both have one type, and overlaps it nowhere else.
  *
  * Scores, sums and outputs are held in 32 bits.  bf16 queries with bf16 outputs on
- * BF16 pools round probabilities to bf16; on INT8 and FP8 pools they round
+ * BF16 pools keep 16 bits of probabilities where few rows share a workgroup's keys,
+ * and 11 where many do (no finer than 2^-35 of a row's largest), with values that
+ * are exact down to 2^-15 of the largest of the first ones read, and no finer than
+ * 2^-22 of it; where a value leaves that range upwards, or all of the first ones are
+ * zeros, they too keep 16 bits.  On INT8 and FP8 pools they round
  * probabilities, keys and values to 11 bits, and no finer than 2^-35 of a row's
  * largest probability, 2^-37 of the largest key among its 32 or 64 neighbours and
  * of the largest value so far.  Everything else keeps f32
