@@ -7,6 +7,22 @@ import torch
 import cross_precision
 
 
+def _parts(x, n):
+    """x (f32) as n bf16 parts, cut off."""
+    out = []
+    for _ in range(n):
+        p = (x.view(torch.int32) & -65536).view(torch.float32)
+        out.append(p)
+        x = x - p
+    return out
+
+
+def _product(a, b, parts):
+    """a @ b of f32 values in `parts` bf16 parts each, their products with i + j < parts."""
+    x, y = _parts(a, parts), _parts(b, parts)
+    return sum(x[i] @ y[j] for i in range(parts) for j in range(parts) if i + j < parts)
+
+
 def _rounded(x, bits):
     """x (64 bits) to `bits` significant ones."""
     m, e = torch.frexp(x)
@@ -16,6 +32,24 @@ def _rounded(x, bits):
 def _inputs(n, d, rows=64):
     g = torch.Generator().manual_seed(n + d)
     return [torch.randn(r, d, generator=g) for r in (rows, n, n)]
+
+
+def _exact(q, k, v):
+    return torch.softmax(q.double() @ k.double().t() / math.sqrt(q.shape[1]), -1) @ v.double()
+
+
+@pytest.mark.parametrize("n,d", [(333, 32), (2000, 64), (2000, 128), (333, 224), (9000, 256)])
+def test_f32_limit(n, d):
+    q, k, v = _inputs(n, d)
+    want = _exact(q, k, v)
+
+    def at(score, p=None, value=None):
+        s = _product(q, k.t().contiguous(), score) * (1.0 / math.sqrt(d))
+        p_ = torch.exp(s - s.amax(-1, keepdim=True))
+        w = p_.bfloat16().float() if p == "bf16" else p_
+        return cross_precision.off(_product(w, v, value or 3) / p_.sum(-1, keepdim=True), want)
+    assert at(3) <= cross_precision.F32 / 2
+    assert min(at(2), at(3, value=2), at(3, "bf16")) > 2 * cross_precision.F32
 
 
 @pytest.mark.parametrize("n,d", [(333, 32), (2000, 64), (2000, 128), (333, 224), (9000, 256)])

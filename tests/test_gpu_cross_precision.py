@@ -21,6 +21,16 @@ def test_16_bit_products(d, dtype, rows):
     assert got <= cross_precision.WITHIN * least
 
 
+@pytest.mark.parametrize("rows", ["few", "many"])
+@pytest.mark.parametrize("dtype,io", [(airkv.F32, "f32"), (airkv.BF16, "f32"), (airkv.INT8, "f32"), (airkv.FP8, "f32"), (airkv.BF16, "bf16")])
+@pytest.mark.parametrize("d", [32, 64, 128, 224])
+def test_f32_precision(d, dtype, io, rows):
+    c = Case(dtype, d, 2, 2, 16, [2000, 333], [3, 2] if rows == "few" else [150, 90], io, "f32", seed=d)
+    got = cross_precision.off(c.call(max_q_len=int(c.rows.max())).cpu(), c.want()[0])
+    print(f"2^{torch_mod().tensor(got).log2():.2f}")
+    assert got <= cross_precision.F32
+
+
 SIZES = {"tiny": lambda t: 1e-30, "small": lambda t: 1e-6, "large": lambda t: 1e5, "huge": lambda t: 1e30,
          # beyond f16 behind a first token's size, once and from there on; behind zeros; far below it
          "one": lambda t: 3e5 if t == 150 else 1.0, "grows": lambda t: 10.0 ** (t // 40), "zeros": lambda t: 0.0 if t < 100 else 1e8,
