@@ -519,7 +519,10 @@ class KvPool:
         return out
 
     def bind_cross(self, q, cu_q, block_tables, seq_lens, out, max_q_len=None, scale=None, workspace=None, stream=None):
-        """Validate once, return a zero-argument launcher of paged_cross."""
+        """Validate once, return a zero-argument launcher of paged_cross.  out is not q: the next launch would
+        attend with this one's result."""
+        if q.numel() and out.data_ptr() == q.data_ptr():
+            raise ValueError("a bound call needs an out of its own")
         args, ws = self._cross_args(q, cu_q, block_tables, seq_lens, out, max_q_len, scale, workspace, stream)
         fn = _lib.load().air_paged_cross
         _lib.check(fn(*args), "air_paged_cross")

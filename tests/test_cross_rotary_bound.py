@@ -1,0 +1,23 @@
+"""Bound launchers of cross attention and rotary appends: what they refuse, without a GPU."""
+import pytest
+import torch
+
+from test_cross_rotary_refusals import call  # noqa: F401 (a fixture)
+
+
+def test_bound_cross_attention_has_an_out_of_its_own(call):  # noqa: F811
+    """In place, a second launch would attend with what the first one gave as its queries."""
+    with pytest.raises(ValueError, match="out"):
+        call.pool.bind_cross(call.q, call.cu, call.tables, call.lens, call.q)
+    assert not call.launched
+    # once is fine
+    call.pool.paged_cross(call.q, call.cu, call.tables, call.lens, call.q)
+    assert len(call.launched) == 1
+
+
+def test_bound_cross_attention_without_rows(call):  # noqa: F811
+    """Tensors without elements have one address, 0, and are not each other's."""
+    q, out = torch.zeros(0, 4, 32), torch.zeros(0, 4, 32)
+    assert q.data_ptr() == out.data_ptr()
+    call.pool.bind_cross(q, call.cu, call.tables, call.lens, out)()
+    assert len(call.launched) == 2
