@@ -575,7 +575,7 @@ class KvPool:
     def bind_append_rotary(self, q, k, v, slot_mapping, positions, inv_freq, q_out, interleaved=False, magnitude=1.0,
                            stream=None):
         """Validate once, return a zero-argument launcher of append_rotary."""
-        if q is not None and (q_out is None or q_out.data_ptr() == q.data_ptr()):
+        if q is not None and (q_out is None or (q.numel() and q_out.data_ptr() == q.data_ptr())):
             raise ValueError("a bound append needs a q_out of its own")
         self.append_rotary(q, k, v, slot_mapping, positions, inv_freq, q_out, interleaved, magnitude, stream)
         args, _ = self._append_rotary_args(q, k, v, slot_mapping, positions, inv_freq, q_out, interleaved, magnitude, stream)

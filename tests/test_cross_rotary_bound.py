@@ -21,3 +21,11 @@ def test_bound_cross_attention_without_rows(call):  # noqa: F811
     assert q.data_ptr() == out.data_ptr()
     call.pool.bind_cross(q, call.cu, call.tables, call.lens, out)()
     assert len(call.launched) == 2
+
+
+def test_a_bound_append_without_rows(call):  # noqa: F811
+    """A step of no tokens binds like any other."""
+    q, out = torch.zeros(0, 4, 32), torch.zeros(0, 4, 32)
+    kv = torch.zeros(0, 4, 32).split([2, 2], dim=1)
+    call.pool.bind_append_rotary(q, *kv, call.slots[:0], call.lens[:0], call.f, out)()
+    assert len(call.launched) == 2
