@@ -4,12 +4,14 @@
 #include <algorithm>
 #include <cmath>
 
+#include "host/span.hpp"
 #include "host/status.hpp"
 #include "on_device.hpp"
 #include "pool.hpp"
 
 using airkv::fail;
 using airkv::OnDevice;
+using airkv::Span;
 
 namespace {
 
@@ -25,14 +27,6 @@ int check_rotary(const air_kv_pool *p, const float *inv_freq, int32_t rot_dim, i
         return fail(AIR_KV_E_INVALID_ARG, "unknown rotary layout %d", layout);
     return AIR_KV_OK;
 }
-
-// The bytes that n rows of `width` elements, `stride` apart, span.
-struct Span {
-    uintptr_t at, end;
-    Span(const void *p, int64_t n, int64_t stride, int64_t width, int64_t bytes)
-        : at((uintptr_t)p), end(at + (uintptr_t)(((n - 1) * stride + width) * bytes)) {}
-    bool meets(const Span &o) const { return at < o.end && o.at < end; }
-};
 
 }  // namespace
 
