@@ -3,12 +3,14 @@
 
 #include <cmath>
 
+#include "host/span.hpp"
 #include "host/status.hpp"
 #include "on_device.hpp"
 #include "pool.hpp"
 
 using airkv::fail;
 using airkv::OnDevice;
+using airkv::Span;
 
 namespace {
 
@@ -52,6 +54,9 @@ int air_paged_cross(air_kv_pool *p, void *stream, const void *q, int32_t q_dtype
         return fail(AIR_KV_E_INVALID_ARG, "total_q times the query heads of a K/V head exceeds int32");
     if ((int64_t)max_blocks * p->desc.block_size > INT32_MAX)
         return fail(AIR_KV_E_INVALID_ARG, "max_blocks * block_size exceeds int32");
+    const int64_t width = (int64_t)n_q_heads * p->desc.head_dim, in = q_dtype == AIR_KV_BF16 ? 2 : 4, res = out_dtype == AIR_KV_BF16 ? 2 : 4;
+    if (!(out == q && q_dtype == out_dtype) && Span(out, total_q, width, width, res).meets(Span(q, total_q, width, width, in)))
+        return fail(AIR_KV_E_INVALID_ARG, "out overlaps q (it may be q itself where both have one type)");
     const size_t needed = airkv::cross_workspace(*p);
     if (ws_bytes < needed) return fail(AIR_KV_E_INVALID_ARG, "workspace %zu bytes < %zu needed", ws_bytes, needed);
     const OnDevice on(p->device);

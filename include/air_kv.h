@@ -463,7 +463,7 @@ int air_paged_diff_prefill(air_kv_pool *pool, void *stream, const void *q, int32
  * zero-filled; rows of a sequence of length 0 are zeros; rows of no sequence stay as
  * they were.  Out-of-pool table entries are counted and their tokens left out (of
  * all of a sequence's: zeros).  Rows of different sequences must not overlap; out may
- * be q itself where both have one type, and overlaps it nowhere else.
+ * be q itself where both have one type, and any other overlap is refused.
  *
  * Scores, sums and outputs are held in 32 bits.  bf16 queries with bf16 outputs on
  * BF16 pools keep 16 bits of probabilities where few rows share a workgroup's keys,
