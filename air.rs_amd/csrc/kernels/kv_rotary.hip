@@ -84,6 +84,13 @@ __device__ __forceinline__ void store8(const float (&x)[8], void *pages, float *
     }
 }
 
+// A row's lanes have loaded what they turn before any of them stores: a wave runs in step, and neither the
+// compiler nor the memory moves an access over this.  (No instruction.)
+__device__ __forceinline__ void row_loaded() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // The 8 elements x from element e on of a row, turned; y their partners (half layout).
 __device__ __forceinline__ void turn8(float (&x)[8], const float (&y)[2][4], const Rotary &r, const float2 *cs, int e) {
 #pragma unroll
@@ -163,6 +170,7 @@ __global__ __launch_bounds__(kThreads) void append_rotary_kernel(AppendArgs a) {
                 }
                 turn8(x, y, a.r, s_cs, e);
             }
+            row_loaded();                              // (q_out may be q)
             if (kind == 0) {
                 const int64_t to = (t * a.q_heads + row) * d + e;
                 if constexpr (OUT16) store8<AIR_KV_BF16>(x, a.q_out, nullptr, to, 0, false, 1);
@@ -283,6 +291,7 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
                         if (e + 4 * p < a.r.rot) four(rotary_partner(e + 4 * p, half), y[p]);
                 }
                 turn8(x, y, a.r, s_cs + k * half, e);
+                row_loaded();
                 const int64_t sc = QUANT ? row * (d >> a.p.sg_log2) + (e >> a.p.sg_log2) : 0;
                 store8<DT>(x, a.p.k_pages, a.p.k_scales, row * d + e, sc, ((e >> 3) & (lanes - 1)) == 0, lanes);
             }
