@@ -46,6 +46,7 @@ int air_rotary_frequencies(int32_t rot_dim, double base, int32_t scaling, double
     if (scaling == AIR_ROTARY_BASE) {
         if (rot_dim == 2) return fail(AIR_KV_E_INVALID_ARG, "another base changes nothing at rot_dim 2");
         base *= std::pow(factor, rot_dim / (rot_dim - 2.0));
+        if (!(base < INFINITY)) return fail(AIR_KV_E_INVALID_ARG, "the base times a power of factor %g is not finite", factor);
     }
     const double two_pi = 6.283185307179586;
     auto turns = [&](double n) { return rot_dim * std::log(trained_len / (two_pi * n)) / (2.0 * std::log(base)); };

@@ -19,3 +19,12 @@ def test_each_scaling_has_its_own_default_of_high():
         # a low above the default is refused as a low above any high
         with pytest.raises(airkv.AirKvError):
             rotary.frequencies(128, 10000.0, scaling, 8.0, 4096.0, low=high)
+
+
+def test_a_base_past_the_largest_double_is_refused():
+    """base * factor^(rot_dim / (rot_dim - 2)): infinite, it gave the frequencies 1, 0, 0, ..."""
+    assert np.isfinite(rotary.frequencies(64, 1e6, "base", 1e250)[0]).all()
+    for rot, factor in ((4, 1e200), (64, 1e305)):
+        with pytest.raises(airkv.AirKvError) as e:
+            rotary.frequencies(rot, 1e6, "base", factor)
+        assert e.value.code == airkv.AIR_KV_E_INVALID_ARG
