@@ -181,6 +181,7 @@ void paged_cross_kernel(CrossArgs a) {
     typedef CrossShape<D, KIND, FEW> S;
     constexpr bool F16 = KIND == kCodes, CONVERT = S::CONVERT, V16 = F16 || CONVERT, PRIVATE = S::PRIVATE, SPLIT = S::SPLIT, PIPE = S::PIPE;
     constexpr int KP = S::KP, QP = S::QP, PP = S::PP, WAVES = S::WAVES, WK = S::WK, SUB = S::SUB, ROWS = S::ROWS, TK = S::TK, NB = S::NB, THREADS = 64 * WAVES;
+    static_assert(!F16 || PRIVATE || NB >= 2, "tiles' scales are looked through a tile before they are staged");
     constexpr int KST = cross_k_stride(D), VST = cross_v_stride(D);
     constexpr int STAGED = PRIVATE ? 32 : TK;          // keys side by side
     constexpr int KPLANE = STAGED * KST, VPLANE = STAGED * VST, VAT = PRIVATE && SPLIT ? 0 : KP * KPLANE;      // a part's rows; where values begin
@@ -385,7 +386,7 @@ void paged_cross_kernel(CrossArgs a) {
         struct Raw {                                   // a tile on its way
             cross_u32x4 w[NP][KIND == kFloats ? 2 : 1];
             float s[CODES ? NP : 1];
-        } raw, next;                                   // (next: kCodes with two buffers, a tile further ahead)
+        } raw, next;                                   // (next: kCodes, a tile further ahead)
         float fk = 1.0f, fk_next = 1.0f, fv = 0.0f, fv_next = 0.0f;    // kCodes: powers of two (0: no value yet); CONVERT: fv
         int counted = 0;                               // tiles whose table entries are (CONVERT comes twice)
         // lane h: the entry of a tile's half h, read a tile before it is needed, and its block
@@ -571,11 +572,11 @@ void paged_cross_kernel(CrossArgs a) {
         };
         float mk = 0.0f, mv = 0.0f;
         // Many rows: what comes between two tiles' products, t the one at hand: tile t + 1 into its
-        // buffer, t + 2 on its way (kCodes with two buffers: t + 2 marked, t + 3 on its way).
+        // buffer, t + 2 on its way (kCodes: t + 2 marked, t + 3 on its way).
         auto stage = [&](int t, auto exact) __attribute__((always_inline)) {
             write_tile(t + 1, raw, kBoth, exact);
             if (t + 2 >= tiles) return;
-            if constexpr (F16 && NB >= 2) {
+            if constexpr (F16) {
                 raw = next;
                 if (t + 3 < tiles) {
                     look_up(t + 3);
@@ -599,7 +600,7 @@ void paged_cross_kernel(CrossArgs a) {
             }
             if constexpr (!PRIVATE) {
                 if (F16 && tid < 6) s_top[tid / 2][tid % 2] = 0;
-                if (F16 && NB >= 2 && 1 < tiles) {
+                if (F16 && 1 < tiles) {
                     look_up(1);
                     load_tile(1, next, kBoth);
                 }
@@ -610,7 +611,7 @@ void paged_cross_kernel(CrossArgs a) {
                 }
                 write_tile(0, raw, kBoth, exact);
                 if (1 < tiles) {
-                    if constexpr (F16 && NB >= 2) {
+                    if constexpr (F16) {
                         raw = next;
                         if (2 < tiles) {
                             look_up(2);
@@ -774,7 +775,6 @@ void paged_cross_kernel(CrossArgs a) {
                         values(mem, 32 * sub, p);
                     }
                 }
-                if (NB == 1 && t + 1 < tiles) mark(t + 1, raw, mk, mv);
                 __syncthreads();
                 if (NB == 1 && t + 1 < tiles) {
                     stage(t, exact);
