@@ -349,7 +349,7 @@ void paged_cross_kernel(CrossArgs a) {
                 }
         }
         if constexpr (F16) {
-            // the row's largest element to [2^4, 2^5): bf16's 8 bits are exact in f16 down to 2^-11
+            // the row's largest element to [2^4, 2^5): bf16's 8 bits are exact in f16 down to 2^-17, 2^-21 of it
             float top = 0.0f;
 #pragma unroll
             for (int s = 0; s < KS; ++s)
@@ -469,7 +469,8 @@ void paged_cross_kernel(CrossArgs a) {
                 }
             }
         };
-        // codes are at most 448 (2^9): the largest value to 2^13 at most
+        // codes are at most 448 (2^9): the largest value to 2^13 at most (an int8 one, 127, to 2^10 to 2^11, f16's
+        // steps of 2^-24 being 2^-34 of it; an fp8 one to 2^11.8 to 2^12.8)
         auto keys_power = [&](float k) __attribute__((always_inline)) { fk_next = k == 0.0f ? 1.0f : cross_pow2(3 - cross_exponent(k)); };
         auto values_power = [&](float v) __attribute__((always_inline)) {
             // (kept as long as the largest stays below 2^15; it never grows)

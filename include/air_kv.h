@@ -470,13 +470,15 @@ int air_paged_diff_prefill(air_kv_pool *pool, void *stream, const void *q, int32
  * and 11 where many do (no finer than 2^-35 of a row's largest), with values that
  * are exact down to 2^-15 of the largest of the first ones read, and no finer than
  * 2^-22 of it; where a value leaves that range upwards, or all of the first ones are
- * zeros, they too keep 16 bits.  On INT8 and FP8 pools they round
- * probabilities, keys and values to 11 bits, and no finer than 2^-35 of a row's
- * largest probability, 2^-37 of the largest key among its 32 or 64 neighbours and
- * of the largest value so far.  Everything else keeps f32
- * precision, where what lies below 2^-133 of an f32 or 1-byte page's value is cut
- * off.  Probabilities below 2^-98 of a row's largest count as 0, and so may what
- * values below 2^-98 add.  Keys and values that are not finite give NaN where they reach.
+ * zeros, they too keep 16 bits.  On INT8 and FP8 pools they round probabilities, keys
+ * and values to 11 bits: probabilities no finer than 2^-35 of a row's largest, keys
+ * than 2^-34 (INT8) or 2^-36 (FP8) of the largest among their 32 or 64 neighbours,
+ * values than the same of the largest so far, where scales are those that appends
+ * make; queries are exact down to 2^-21 of their row's largest element, and no finer
+ * than 2^-28 of it.  Everything else keeps f32 precision, where what lies below
+ * 2^-133 of an f32 or 1-byte page's value is cut off.  Probabilities below 2^-98 of a
+ * row's largest count as 0, and so may what values below 2^-98 add.  Keys and values
+ * that are not finite give NaN where they reach, and so do those of a scale that is not.
  * The workspace (16-byte aligned, at least air_paged_cross_workspace_size bytes, no
  * initialisation needed) holds the parts of blocks of rows that several workgroups
  * share; calls that share one must be ordered (same stream). */
