@@ -513,7 +513,8 @@ class KvPool:
     def paged_cross(self, q, cu_q, block_tables, seq_lens, out, max_q_len=None, scale=None, workspace=None, stream=None):
         """Cross attention (air_paged_cross): each sequence's cu_q[b+1] - cu_q[b] rows of q [total_q][n_q][d] see
         all of its seq_lens[b] cached tokens.  max_q_len, the most rows of a sequence, is a hint (nothing is read
-        back without it)."""
+        back without it).  A workspace serves every call of the pool on its stream; without one a call takes one
+        of its own.  One row a sequence: paged_decode takes less time on most pools of head_dim 128."""
         args, _ws = self._cross_args(q, cu_q, block_tables, seq_lens, out, max_q_len, scale, workspace, stream)
         _lib.check(_lib.load().air_paged_cross(*args), "air_paged_cross")
         return out

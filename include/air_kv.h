@@ -454,7 +454,7 @@ int air_paged_diff_prefill(air_kv_pool *pool, void *stream, const void *q, int32
  *   out[r][h] = softmax(scale * q[r][h] . K[h / group]^T) . V[h / group]
  * whatever the number of rows (one token, a prompt, the beams of a sequence): there
  * is no order between rows and tokens.  Arguments, pools and refusals are those of
- * air_paged_prefill: q and out [total_q][n_q_heads][head_dim] as q_dtype and out_dtype
+ * air_paged_prefill, but the workspace is needed: q and out [total_q][n_q_heads][head_dim] as q_dtype and out_dtype
  * (16-byte aligned), any group, any head_dim of a pool; max_q_len is a hint (an upper
  * bound of a sequence's rows; 0: not known), under which few rows take their
  * sequence's keys side by side.  A sequence whose rows do not lie in [0, total_q] or
@@ -481,7 +481,10 @@ int air_paged_diff_prefill(air_kv_pool *pool, void *stream, const void *q, int32
  * that are not finite give NaN where they reach, and so do those of a scale that is not.
  * The workspace (16-byte aligned, at least air_paged_cross_workspace_size bytes, no
  * initialisation needed) holds the parts of blocks of rows that several workgroups
- * share; calls that share one must be ordered (same stream). */
+ * share; calls that share one must be ordered (same stream).  Its size is that of a
+ * pool's largest call, whatever the arguments, so that one serves all of them.
+ * One row a sequence is what air_paged_decode computes too, in less time on most
+ * pools of head_dim 128 (on 1-byte ones with values rounded to bf16). */
 int air_paged_cross_workspace_size(const air_kv_pool *pool, int32_t n_q_heads, int32_t batch, int32_t max_q_len,
                                    size_t *bytes);
 int air_paged_cross(air_kv_pool *pool, void *stream, const void *q, int32_t q_dtype, int32_t n_q_heads,
@@ -549,7 +552,7 @@ int air_kv_append_rotary(air_kv_pool *pool, void *stream, const void *q, int64_t
  * b, n of them for its n entries from[cu[b] .. cu[b + 1]) (int32, device), hold keys
  * turned for positions `from`, and leave turned for `to` (laid out alike; NULL: their
  * place in the sequence).  After air_kv_compact(..., keep, cu_keep, ...) that is
- * air_kv_rotate(..., keep, NULL, cu_keep, ...).  A key is read (1-byte pages:
+ * air_kv_rotate(..., keep, NULL, cu_keep, ...), if none of keep was skipped there.  A key is read (1-byte pages:
  * dequantized), turned by to - from, and stored again (1-byte pages: the scale groups
  * that hold a turned element are quantized anew); tokens with to == from keep their
  * bytes, and values are not touched.  cu is int32 [batch + 1] (device) over total
@@ -609,8 +612,10 @@ int air_kv_session_truncate_to(air_kv_session *s, int64_t pos);
  * (host memory, ascending, below the length, which every layer must share) in
  * every layer, as tokens 0 .. n_keep - 1, by air_kv_compact; blocks that another
  * sequence shares and that would be written are copied first, and the blocks past
- * the kept tokens are released.  Keys keep the rotation they were appended with.
- * An error before the first layer's rows move leaves the session as it was. */
+ * the kept tokens are released.  Keys keep the rotation they were appended with:
+ * air_kv_rotate over each layer's pool, with the sequence's new table, `from` = keep
+ * and cu = {0, n_keep}, turns them to their places (air_kv_session_compact has copied
+ * the blocks that are written then).  An error before the first layer's rows move leaves the session as it was. */
 int air_kv_session_compact(air_kv_session *s, void *stream, const int64_t *keep, int64_t n_keep);
 /* Bytes of device memory the session's blocks occupy over all its layers
  * (the paged form of memory_usage, src/kv_cache.rs:388-414). */
