@@ -590,15 +590,13 @@ void paged_cross_kernel(CrossArgs a) {
             }
         };
 
+        int again = 0;                                 // CONVERT: values as they are
         auto begin = [&](auto exact) __attribute__((always_inline)) {
             fetch(0);
             __syncthreads();                               // the buffers of the block before are free
             look_up(0);
             load_tile(0, raw, kBoth);
-            if constexpr (!decltype(exact)::value) {
-                sample();
-                if (fv == 0.0f) return;
-            }
+            if constexpr (!decltype(exact)::value) sample();
             if constexpr (!PRIVATE) {
                 if (F16 && tid < 6) s_top[tid / 2][tid % 2] = 0;
                 if (F16 && 1 < tiles) {
@@ -624,7 +622,9 @@ void paged_cross_kernel(CrossArgs a) {
                         load_tile(1, raw, kBoth);
                     }
                 }
-                __syncthreads();
+                // (a vote: whatever waves have read, all take the same way)
+                if constexpr (!decltype(exact)::value) again = __syncthreads_or(fv == 0.0f);
+                else __syncthreads();
             }
         };
         begin(kFast);
@@ -788,7 +788,7 @@ void paged_cross_kernel(CrossArgs a) {
             // values, so that products and arithmetic, about as much of either, run at once.  A tile is
             // two steps; the next tile is staged beside the first and there at a barrier before the second.
             static_assert(PP == 1 && KP == 1 && KS == 2 * CT && NB == 3, "16-bit parts");
-            if (!CONVERT || fv != 0.0f) {
+            if (!again) {
                 cross_f32x16 sa, sb;
                 cross_u32x4 pa[2], pb[2];
                 float top;
@@ -943,7 +943,7 @@ void paged_cross_kernel(CrossArgs a) {
                 if (rest > 0) values(mem, 0, p);
             }
             __syncthreads();
-        } else if (!CONVERT || fv != 0.0f) {
+        } else if (!again) {
             walk(kFast);
         }
         if constexpr (CONVERT) {
@@ -954,7 +954,8 @@ void paged_cross_kernel(CrossArgs a) {
             for (int c = 0; c < CT; ++c)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) x = __builtin_fmaf(acc[c][i], 0.0f, x);
-            if (__builtin_expect(__syncthreads_or(fv == 0.0f || (x != 0.0f && l_run < INFINITY)), 0)) {     // from values as they are
+            if (!again) again = __syncthreads_or(x != 0.0f && l_run < INFINITY);
+            if (__builtin_expect(again, 0)) {
                 fv = 0.0f;
                 clear(24.0f);
                 begin(kExact);
