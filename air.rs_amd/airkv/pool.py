@@ -76,17 +76,17 @@ def _dev_rows(t, dtype, what, shape):
     return t.data_ptr(), row if n > 1 else heads * d
 
 
-def _workspace(nbytes, stream):
-    """Device memory for calls on `stream` (None: the current one), of that stream's own: what
+def _workspace(nbytes, stream, device="cuda"):
+    """Memory of `device` ("cuda": the current one) for calls on `stream` (None: the current one), of that stream's own: what
     it is given out for next there runs after those calls, whenever the tensor is dropped.
     (The current stream's could be in use again while another stream's kernels still write it.)"""
     torch = _torch()
     if stream is None:
-        return torch.empty(max(nbytes, 16), dtype=torch.uint8, device="cuda")
+        return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
     if not isinstance(stream, torch.cuda.Stream):
         stream = torch.cuda.ExternalStream(stream.cuda_stream)
     with torch.cuda.stream(stream):
-        return torch.empty(max(nbytes, 16), dtype=torch.uint8, device="cuda")
+        return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
 
 
 def _launcher(fn, args, name, keep):
@@ -505,7 +505,7 @@ class KvPool:
         cu_at = _dev(cu_q, torch.int32, "cu_q", (batch + 1,))
         most = 0 if max_q_len is None else max_q_len
         if workspace is None:
-            workspace = self.new_cross_workspace(n_q, batch, most, stream)
+            workspace = _workspace(self.cross_workspace_size(n_q, batch, most), stream, q.device)
         ws_at = _dev(workspace, workspace.dtype, "workspace")
         return (self.handle, _stream_ptr(stream), q_at, qdt, n_q, cu_at, total_q, most, tables_at, lens_at, batch, max_blocks,
                 self._scale if scale is None else scale, ws_at, workspace.nbytes, out_at, odt), workspace

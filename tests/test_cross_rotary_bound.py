@@ -29,3 +29,15 @@ def test_a_bound_append_without_rows(call):  # noqa: F811
     kv = torch.zeros(0, 4, 32).split([2, 2], dim=1)
     call.pool.bind_append_rotary(q, *kv, call.slots[:0], call.lens[:0], call.f, out)()
     assert len(call.launched) == 2
+
+
+def test_a_calls_own_workspace_is_on_its_queries_device(call, monkeypatch):  # noqa: F811
+    """The kernel runs on the pool's device, whichever is current."""
+    devices, real = [], torch.empty
+
+    def empty(*shape, dtype=None, device=None):
+        devices.append(device)
+        return real(*shape, dtype=dtype)
+    monkeypatch.setattr(torch, "empty", empty)
+    call.pool.paged_cross(call.q, call.cu, call.tables, call.lens, call.out)
+    assert devices == [call.q.device]
